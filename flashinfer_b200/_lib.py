@@ -31,6 +31,7 @@ ERRORS = {
 NOALLOC_MAX_TOKENS = 4096
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
 OUT_BF16 = 0
 OUT_F32 = 1
 OUT_F16S = 2
@@ -49,13 +50,18 @@ GEMV_MAX_T = 2  # calls of at most this many tokens take the matrix-vector path 
  ROUTING_RENORMALIZE_NAIVE, ROUTING_TOPK) = range(6)
 STATUS_TIMEOUT_GEMM1 = 0x1
 STATUS_TIMEOUT_GEMM2 = 0x2
+STATUS_TIMEOUT_INT8 = 0x4
+GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = 0, 1, 2, 3
 
 EXPORTS = ("fmoe_workspace_size", "fmoe_workspace_layout", "fmoe_run", "fmoe_route",
            "fmoe_read_status", "fmoe_device_sm_count", "fmoe_version",
            "fmoe_route_permute_noalloc", "fmoe_quantize_activations", "fmoe_ep_layout",
            "fmoe_ep_alloc", "fmoe_ep_free", "fmoe_ipc_get_handle", "fmoe_ipc_open",
            "fmoe_ipc_close", "fmoe_ep_dispatch", "fmoe_ep_reduce", "fmoe_fp8_mma_peak",
-           "fmoe_debug_arm_timeout")
+           "fmoe_debug_arm_timeout", "fmoe_sort_size", "fmoe_sort_by_expert", "fmoe_sort_rows",
+           "fmoe_unsort_rows", "fmoe_unsort_rows_backward", "fmoe_quantize_int8",
+           "fmoe_int8_matmul", "fmoe_int8_expert_matmul", "fmoe_int8_status",
+           "fmoe_block_norm_workspace_size", "fmoe_block_norm", "fmoe_block_norm_backward")
 
 
 class FmoeArgs(Structure):
@@ -113,6 +119,25 @@ class FmoeLayout(Structure):
         ("num_blocks", c_int64)]
 
 
+class FmoeTokenOrder(Structure):
+    _fields_ = [("num_tokens", c_int32), ("top_k", c_int32), ("num_local_experts", c_int32),
+                ("num_rows", c_int64), ("expert_base", c_void_p), ("row_pick", c_void_p),
+                ("pick_row", c_void_p)]
+
+
+class FmoeBlockNormArgs(Structure):
+    _fields_ = [("num_tokens", c_int64), ("hidden_size", c_int32), ("dtype", c_int32)] + \
+        [(n, c_void_p) for n in ("branch", "residual", "post_weight", "gate", "pre_weight")] + \
+        [(n, c_int32) for n in ("post_weight_dtype", "gate_dtype", "pre_weight_dtype",
+                                "gate_kind")] + \
+        [("residual_scale", c_float), ("eps", c_float)] + \
+        [(n, c_void_p) for n in ("hidden", "normed", "normed_q", "normed_scale", "stats",
+                                 "grad_hidden", "grad_normed", "grad_branch", "grad_residual",
+                                 "grad_post_weight", "grad_gate", "grad_pre_weight",
+                                 "workspace")] + \
+        [("workspace_bytes", c_size_t)]
+
+
 _lib = None
 
 
@@ -153,6 +178,28 @@ def load() -> ctypes.CDLL:
                                    c_void_p, c_void_p]
     lib.fmoe_fp8_mma_peak.argtypes = [c_int32, c_void_p, POINTER(ctypes.c_double), c_void_p]
     lib.fmoe_debug_arm_timeout.argtypes = [c_int32, ctypes.c_uint64]
+    lib.fmoe_sort_size.argtypes = [c_int32, c_int32, c_int32, c_int32, POINTER(c_int64),
+                                   POINTER(c_size_t)]
+    lib.fmoe_sort_by_expert.argtypes = [c_void_p, c_int32, c_int32, POINTER(FmoeTokenOrder),
+                                        c_void_p, c_size_t, c_void_p]
+    lib.fmoe_sort_rows.argtypes = [c_void_p, c_int64, POINTER(FmoeTokenOrder), c_void_p, c_int32,
+                                   c_void_p]
+    lib.fmoe_unsort_rows.argtypes = [c_void_p, c_int32, c_int64, POINTER(FmoeTokenOrder), c_void_p,
+                                     c_void_p, c_void_p]
+    lib.fmoe_unsort_rows_backward.argtypes = [c_void_p, c_void_p, c_int32, c_int64,
+                                              POINTER(FmoeTokenOrder), c_void_p, c_void_p,
+                                              c_void_p, c_void_p]
+    lib.fmoe_quantize_int8.argtypes = [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p,
+                                       c_void_p]
+    lib.fmoe_int8_matmul.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                     c_int32, c_int32, c_void_p, c_int32, c_void_p]
+    lib.fmoe_int8_expert_matmul.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                            c_int64, c_int32, c_int32, c_int32, c_void_p, c_int32,
+                                            c_int32, c_void_p]
+    lib.fmoe_int8_status.argtypes = [POINTER(c_int32), c_void_p]
+    lib.fmoe_block_norm_workspace_size.argtypes = [c_int64, c_int32, POINTER(c_size_t)]
+    lib.fmoe_block_norm.argtypes = [POINTER(FmoeBlockNormArgs), c_void_p]
+    lib.fmoe_block_norm_backward.argtypes = [POINTER(FmoeBlockNormArgs), c_void_p]
     lib.fmoe_version.restype = c_char_p
     for name in EXPORTS:
         if name != "fmoe_version":

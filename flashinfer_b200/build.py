@@ -17,8 +17,9 @@ CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIBDIR, "libfmoe.so")
 SOURCES = ["fmoe_api.cu", "fmoe_kernels.cu", "fmoe_gemm.cu", "fmoe_gemv.cu", "fmoe_static.cu",
-           "fmoe_quant.cu", "fmoe_ep.cu", "fmoe_peak.cu"]
-HEADERS = ["fmoe_internal.h", "fmoe_ptx.cuh", "fmoe_gemm_common.cuh", "fmoe_route.cuh",
+           "fmoe_quant.cu", "fmoe_ep.cu", "fmoe_peak.cu", "fmoe_tokens.cu", "fmoe_int8.cu",
+           "fmoe_norm.cu", "fmoe_layer_api.cu"]
+HEADERS = ["fmoe_internal.h", "fmoe_elem.cuh", "fmoe_ptx.cuh", "fmoe_gemm_common.cuh", "fmoe_route.cuh",
            os.path.join("..", "..", "include", "fmoe.h")]
 
 NVCC_FLAGS = [

@@ -170,6 +170,21 @@ struct ArmedTimeout {
 thread_local ArmedTimeout g_armed;
 
 }  // namespace
+
+int device_sms(int* sms) {
+  DeviceInfo d;
+  const int rc = device_info(&d);
+  if (rc) return rc;
+  if (d.major != 10) return FMOE_ERR_DEVICE;
+  *sms = d.sms;
+  return FMOE_OK;
+}
+
+bool tensor_map_u8(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows,
+                   uint64_t row_stride, uint32_t box_cols, uint32_t box_rows) {
+  return make_tmap_u8(m, base, cols, rows, row_stride, box_cols, box_rows);
+}
+
 }  // namespace fmoe
 
 using namespace fmoe;

@@ -1,0 +1,653 @@
+// fmoe_int8.cu -- 8-bit integer products with one scale per token and one per output channel,
+// for one weight matrix or one per expert, and the quantisation of their activations.
+//
+//   q[t, k] = round_half_even(127 x[t, k] / amax_t),  a_scale[t] = amax_t / 127,
+//             amax_t = max(max_k |x[t, k]|, 1e-30)
+//   y[t, n] = a_scale[t] * w_scale[n] * sum_k a[t, k] * w[n, k] (+ bias[n])
+// The sum is exact in int32 (127 * 127 * K and -128 * -128 * K stay below 2^31 for K <= 131071);
+// the scaling is fp32 and rounded once to the output type.
+//
+// The weight rows are the M side of the MMA (128 per tile) and the tokens its N side (16..256 per
+// tile, the instruction's N chosen per tile): a decode step then fills the 128 MMA rows with
+// weights, which are all that costs, and a tile with few tokens issues a narrow MMA instead of
+// padding. A tile's accumulator has one weight row per TMEM lane, so each epilogue thread keeps
+// its channel's scale and bias in a register and a warp stores 32 neighbouring channels of a
+// token at a time.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "fmoe_elem.cuh"
+#include "fmoe_internal.h"
+#include "fmoe_ptx.cuh"
+
+namespace fmoe {
+namespace {
+
+// ------------------------------------------------------------------ quantisation
+// |x| as ordered integer bits: NaN ranks above infinity, so a row that holds one gets a NaN (or
+// infinite) scale and its products are NaN.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// One quotient: both operands scaled by 2^-8 (exact), so 127 * x stays finite. For 16-bit inputs
+// 127 * x is exact in fp32 and the distance of the true quotient from a rounding border is either
+// zero or far above fp32's rounding, so the result is the correctly rounded 127 x / amax.
+__device__ __forceinline__ int quant1(float v, float den) {
+  return __float2int_rn(__fdiv_rn(v * (127.0f / 256.0f), den));
+}
+
+// A row per G threads (32: a warp, 256: the block). Up to VPT groups of V elements per thread stay
+// in registers between the maximum and the rounding; longer rows are read a second time.
+template <typename T, int V, int G>
+__global__ void __launch_bounds__(256)
+    k_quantize_int8(const T* x, int64_t rows, int64_t K, int8_t* q, float* scale) {
+  pdl_begin_in_order();
+  constexpr int VPT = V > 1 ? 8 : 16;
+  __shared__ uint32_t part[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = G == 32 ? lane : static_cast<int>(threadIdx.x);
+  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
+  if (row >= rows) return;  // G = 32: whole warps; no block barrier follows
+  const int64_t nvec = K / V;
+  const T* xr = x + row * K;
+  int8_t* qr = q + row * K;
+  Pack<T, V> in[VPT];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int64_t v = g + static_cast<int64_t>(i) * G;
+    if (v < nvec) in[i] = load_pack<T, V>(xr + v * V);
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int64_t v = g + static_cast<int64_t>(i) * G;
+    if (v < nvec) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = max(m, abs_bits(to_f32(in[i].e[j])));
+    }
+  }
+  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < nvec; v += G) {
+    const Pack<T, V> p = load_pack<T, V>(xr + v * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = max(m, abs_bits(to_f32(p.e[j])));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (G == 256) {
+    if (lane == 0) part[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, part[i]);
+  }
+  m = max(m, __float_as_uint(1e-30f));
+  const float amax = __uint_as_float(m);
+  const float den = amax * (1.0f / 256.0f);
+  if (g == 0) scale[row] = __fdiv_rn(amax, 127.0f);
+  auto put = [&](const Pack<T, V>& p, int64_t v) {
+    uint8_t b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) b[j] = static_cast<uint8_t>(quant1(to_f32(p.e[j]), den));
+    if constexpr (V == 8) {
+      uint2 w;
+      memcpy(&w, b, 8);
+      *reinterpret_cast<uint2*>(qr + v * V) = w;
+    } else {
+      qr[v] = static_cast<int8_t>(b[0]);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int64_t v = g + static_cast<int64_t>(i) * G;
+    if (v < nvec) put(in[i], v);
+  }
+  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < nvec; v += G)
+    put(load_pack<T, V>(xr + v * V), v);
+}
+
+template <typename T, int V>
+cudaError_t quantize_rows(const void* x, int64_t rows, int64_t K, void* q, float* scale,
+                          cudaStream_t s) {
+  // a warp holds rows of up to 8 (16-byte groups) or 16 (single elements) units per lane
+  const int64_t nvec = K / V;
+  if (nvec <= 32 * (V > 1 ? 8 : 16))
+    return launch_pdl(k_quantize_int8<T, V, 32>, dim3(static_cast<unsigned>((rows + 7) / 8)),
+                      dim3(256), 0, s, static_cast<const T*>(x), rows, K, static_cast<int8_t*>(q),
+                      scale);
+  return launch_pdl(k_quantize_int8<T, V, 256>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s,
+                    static_cast<const T*>(x), rows, K, static_cast<int8_t*>(q), scale);
+}
+
+// ------------------------------------------------------------------ product
+constexpr int kI8Threads = 384;   // warps 0, 2, 3 load, warp 1 issues MMAs, 4..11 store
+constexpr int kI8Producers = 3;
+constexpr int kI8Epi0 = 4;
+constexpr int kI8EpiWarps = 8;
+constexpr int kWRows = 128;       // weight rows per tile (MMA M)
+constexpr int kKB = 128;          // K bytes per stage (one 128-byte swizzled row)
+constexpr int kI8MaxStages = 12;
+
+template <int BN>
+struct I8Cfg {
+  static constexpr int STAGE = (kWRows + BN) * kKB;
+  static constexpr int NS = BN == 16 ? 12 : BN == 64 ? 9 : BN == 128 ? 6 : 4;
+  static constexpr int BOX = BN == 16 ? 16 : 64;   // token rows per TMA box
+  static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;
+  static_assert(NS > kI8Producers && NS <= kI8MaxStages, "producer parity and barrier arrays");
+};
+
+struct alignas(16) I8Tail {
+  uint64_t full[kI8MaxStages];
+  uint64_t empty[kI8MaxStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int tiles;
+  int live;
+  int last_issue[kI8Producers][kI8MaxStages];
+  float a_scale[256];
+  int ebase[kMaxLocalExperts + 1];
+  int etile[kMaxLocalExperts + 1];  // token tiles before expert e
+};
+
+struct I8Args {
+  const float* a_scale;
+  const float* w_scale;
+  const float* bias;          // or null
+  const int32_t* expert_base; // or null: one matrix
+  void* out;
+  int64_t M;                  // token rows
+  int N, E, nkb, S;
+  int dtype;                  // output
+  int zero_tail;
+};
+
+template <int BN>
+constexpr size_t i8_smem_bytes() {
+  return static_cast<size_t>(I8Cfg<BN>::NS) * I8Cfg<BN>::STAGE + sizeof(I8Tail) + 1024;
+}
+static_assert(i8_smem_bytes<16>() <= 227 * 1024 && i8_smem_bytes<64>() <= 227 * 1024 &&
+                  i8_smem_bytes<128>() <= 227 * 1024 && i8_smem_bytes<256>() <= 227 * 1024,
+              "shared memory per CTA");
+
+// D[tmem] (+)= A[smem] * B[smem]^T, s8 x s8 -> s32.
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                       uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: D s32, A and B signed 8-bit, both K-major.
+__device__ __forceinline__ uint32_t idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+struct I8Tile {
+  int e, n0;         // expert, first weight row (channel)
+  int64_t row0;      // first token row
+  int rows, cols;    // tokens in the tile, and the MMA's N (a multiple of 16)
+};
+
+// Tile order: expert, weight tile, token tile (fastest), so CTAs that run side by side share
+// weight tiles. The tokens of an expert are cut into equal tiles of at most BN.
+template <int BN>
+__device__ __forceinline__ I8Tile decode_tile(int tile, int NT, const I8Tail* t, int E) {
+  int lo = 0, hi = E - 1;
+  while (lo < hi) {  // first expert e with tile < etile[e + 1] * NT
+    const int mid = (lo + hi) >> 1;
+    if (tile < t->etile[mid + 1] * NT)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  const int mt = t->etile[lo + 1] - t->etile[lo];
+  const int local = tile - t->etile[lo] * NT;
+  const int n = local / mt;
+  const int m = local - n * mt;
+  const int count = t->ebase[lo + 1] - t->ebase[lo];
+  // at most BN: count <= mt * BN, and BN is a multiple of 16
+  const int per = ((count + mt - 1) / mt + 15) / 16 * 16;
+  I8Tile r;
+  r.e = lo;
+  r.n0 = n * kWRows;
+  r.row0 = t->ebase[lo] + static_cast<int64_t>(m) * per;
+  r.rows = max(0, min(per, count - m * per));
+  r.cols = max(16, (r.rows + 15) / 16 * 16);
+  return r;
+}
+
+__device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                        bool park) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (park ? mbar_try_wait_sleep(bar, parity, 2000u) : mbar_test_wait(bar, parity)) return true;
+    if (park || (++spins & 255u) == 0) {
+      if (*abort_flag) return false;
+      if (global_timer_ns() - t0 > FMOE_WAIT_NS) return false;
+    }
+  }
+}
+
+// Set by a product whose bounded wait ran out, until take_int8_status reads it.
+__device__ int32_t g_int8_status;
+
+__device__ __forceinline__ void i8_abort(I8Tail* t) {
+  *reinterpret_cast<volatile int*>(&t->abort_flag) = 1;
+  atomicOr(&g_int8_status, FMOE_STATUS_TIMEOUT_INT8);
+}
+
+__device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float v) {
+  if (dtype == FMOE_DTYPE_BF16)
+    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  else if (dtype == FMOE_DTYPE_F16)
+    static_cast<__half*>(out)[i] = __float2half_rn(v);
+  else
+    static_cast<float*>(out)[i] = v;
+}
+
+__device__ __forceinline__ void zero_out(void* out, int dtype, int64_t i) {
+  if (dtype == FMOE_DTYPE_F32)
+    static_cast<float*>(out)[i] = 0.0f;
+  else
+    static_cast<uint16_t*>(out)[i] = 0;
+}
+
+__device__ __forceinline__ int4 ld_dsmem_int4(const void* p, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(remote)
+               : "memory");
+  return v;
+}
+
+// SPLIT: the cluster's S CTAs share one tile, each with a range of K; their int32 partial tiles
+// are added through distributed shared memory (exact, so the split changes no result).
+template <int BN, bool SPLIT>
+__global__ void __launch_bounds__(kI8Threads, 1)
+    k_int8_mm(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+              const I8Args args) {
+  using C = I8Cfg<BN>;
+  constexpr int NS = C::NS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  I8Tail* tail = reinterpret_cast<I8Tail*>(smem + NS * C::STAGE);
+  volatile int* abort_flag = &tail->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int E = args.E;
+  const int NT = (args.N + kWRows - 1) / kWRows;
+  const int S = SPLIT ? args.S : 1;
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&tail->full[s], 1);
+      mbar_init(&tail->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tail->tfull[b], 1);
+      mbar_init(&tail->tempty[b], kI8EpiWarps * 32);
+    }
+    mbar_init(&tail->drain, 1);
+    tail->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tail->tmem_base, C::COLS);
+    tmem_relinquish();
+  }
+  // everything this kernel reads may have been written by the previous grid
+  pdl_begin_in_order();
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
+    int64_t b = args.expert_base ? __ldcg(args.expert_base + e) : (e == 0 ? 0 : args.M);
+    tail->ebase[e] = static_cast<int>(b < 0 ? 0 : b > args.M ? args.M : b);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    // token tiles per expert and their running sum; a base that steps back counts as empty
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      int mt = 0;
+      if (e < E) {
+        const int count = max(0, tail->ebase[e + 1] - tail->ebase[e]);
+        mt = (count + BN - 1) / BN;
+      }
+      int incl = mt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      if (e < E) tail->etile[e] = carry + incl - mt;
+      carry += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+      tail->etile[E] = carry;
+      tail->tiles = carry * NT;
+      tail->live = tail->ebase[E];
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tail->tmem_base;
+  const int tiles = tail->tiles;
+  const int rank = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first = SPLIT ? blockIdx.x / S : blockIdx.x;
+  const int step = SPLIT ? gridDim.x / S : gridDim.x;  // SPLIT: at most one tile per cluster
+  const int kb0 = rank * args.nkb / S, kb1 = (rank + 1) * args.nkb / S;
+
+  if (warp == 0 || warp == 2 || warp == 3) {
+    // ---------------------------------------------------------------- TMA producers
+    const int pw = warp == 0 ? 0 : warp - 1;
+    if (lane == 0) {
+      const uint64_t pol_first = policy_evict_first();
+      const uint64_t pol_last = policy_evict_last();
+      for (int s = 0; s < NS; ++s) tail->last_issue[pw][s] = -1;
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const I8Tile u = decode_tile<BN>(tile, NT, tail, E);
+        const int boxes = (u.cols + C::BOX - 1) / C::BOX;
+        const uint32_t bytes = kWRows * kKB + boxes * C::BOX * kKB;
+        // a weight tile that several token tiles read stays in L2; one that is read once goes first
+        const uint64_t pol_w =
+            tail->etile[u.e + 1] - tail->etile[u.e] > 1 ? pol_last : pol_first;
+        const int wrow = u.e * args.N + u.n0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          if (it % kI8Producers != pw) continue;
+          const int s = it % NS, r = it / NS;
+          // This producer issued iteration it - kI8Producers after that stage's release, and the
+          // MMA warp releases in order, so with NS > kI8Producers the barrier is at most one
+          // phase behind and the parity wait is unambiguous.
+          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, true)) {
+            i8_abort(tail);
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * C::STAGE;
+          mbar_arrive_expect_tx(&tail->full[s], bytes);
+          tma_load_2d(st, &tm_w, &tail->full[s], kb * kKB, wrow, pol_w);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(st + (kWRows + b * C::BOX) * kKB, &tm_a, &tail->full[s], kb * kKB,
+                        static_cast<int>(u.row0) + b * C::BOX, pol_last);
+          tail->last_issue[pw][s] = r;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step, ++n) {
+        const I8Tile u = decode_tile<BN>(tile, NT, tail, E);
+        const uint32_t idesc = idesc_i8(kWRows, u.cols);
+        const int b = n & 1, rb = n >> 1;
+        const uint32_t d = tmem + b * BN;
+        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, false)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % NS, r = it / NS;
+          if (!i8_wait(&tail->full[s], r & 1, abort_flag, false)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * C::STAGE);
+          const uint64_t w_desc = smem_desc_k128(st);
+          const uint64_t a_desc = smem_desc_k128(st + kWRows * kKB);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_i8(d, w_desc + 2 * j, a_desc + 2 * j, idesc, kb > kb0 || j > 0 ? 1u : 0u);
+          mma_commit(&tail->empty[s]);
+        }
+        if (ok) mma_commit(&tail->tfull[b]);
+      }
+      if (!ok) i8_abort(tail);
+      mma_commit(&tail->drain);
+      (void)mbar_wait(&tail->drain, 0);
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    const int q = warp & 3;              // TMEM lane quarter of this warp
+    const int g = (warp - kI8Epi0) >> 2; // column groups of 16: even or odd
+    const int etid = threadIdx.x - kI8Epi0 * 32;
+    if (args.zero_tail) {
+      const int64_t total = (args.M - tail->live) * static_cast<int64_t>(args.N);
+      const int64_t i0 = tail->live * static_cast<int64_t>(args.N);
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kI8EpiWarps * 32) + etid; i < total;
+           i += static_cast<int64_t>(gridDim.x) * (kI8EpiWarps * 32))
+        zero_out(args.out, args.dtype, i0 + i);
+    }
+    int n = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles; tile += step, ++n) {
+      const I8Tile u = decode_tile<BN>(tile, NT, tail, E);
+      const int b = n & 1, rb = n >> 1;
+      const int ch = u.n0 + q * 32 + lane;
+      const bool live = ch < args.N;
+      const float ws = live ? __ldcg(args.w_scale + static_cast<int64_t>(u.e) * args.N + ch) : 0.0f;
+      const float bias = live && args.bias ? __ldcg(args.bias + ch) : 0.0f;
+      named_bar_sync(1, kI8EpiWarps * 32);  // the previous tile's a_scale is no longer read
+      if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
+      named_bar_sync(1, kI8EpiWarps * 32);
+      // after a wait that ran out, the warp still takes part in the barriers of later tiles
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, false));
+      if (!ok) {
+        if (lane == 0) i8_abort(tail);
+        continue;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * BN;
+      for (int c = g * 16; c < u.cols; c += 32) {
+        float v[16];
+        tmem_ld_32x32b_x16(taddr + c, v);
+        tmem_ld_wait16(v);
+        if constexpr (SPLIT) {
+          // every load of this CTA has landed and been read (the tile's MMAs are complete), so
+          // the stages hold the partial tile [token][128 channels]
+          int* part = reinterpret_cast<int*>(smem) + c * kWRows + q * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part[i * kWRows] = __float_as_int(v[i]);
+        } else if (live) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (c + i < u.rows)
+              store_out(args.out, args.dtype, (u.row0 + c + i) * args.N + ch,
+                        fmaf(static_cast<float>(__float_as_int(v[i])) * tail->a_scale[c + i], ws,
+                             bias));
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&tail->tempty[b]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // Never leave a bulk copy in flight into shared memory that is about to be released: after an
+  // abort, wait for each stage's latest issued round (without one the MMA warp has seen them all).
+  if (threadIdx.x == 0 && *abort_flag) {
+    for (int s = 0; s < NS; ++s) {
+      int r = -1;
+      for (int p = 0; p < kI8Producers; ++p) r = max(r, tail->last_issue[p][s]);
+      if (r >= 0) (void)mbar_wait(&tail->full[s], r & 1);
+    }
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::COLS);
+  }
+  if constexpr (SPLIT) {
+    cluster_arrive();
+    cluster_wait();
+    if (first < tiles) {
+      const I8Tile u = decode_tile<BN>(first, NT, tail, E);
+      // four neighbouring channels of a token per item, the items dealt out over the cluster
+      const int items = u.rows * (kWRows / 4);
+      for (int i = rank * kI8Threads + threadIdx.x; i < items; i += S * kI8Threads) {
+        const int tok = i / (kWRows / 4), c4 = (i % (kWRows / 4)) * 4;
+        const int* p = reinterpret_cast<const int*>(smem) + tok * kWRows + c4;
+        int sum[4] = {0, 0, 0, 0};
+        for (int r = 0; r < S; ++r) {
+          const int4 v = ld_dsmem_int4(p, r);
+          sum[0] += v.x;
+          sum[1] += v.y;
+          sum[2] += v.z;
+          sum[3] += v.w;
+        }
+        const float as = __ldcg(args.a_scale + u.row0 + tok);
+        for (int j = 0; j < 4; ++j) {
+          const int ch = u.n0 + c4 + j;
+          if (ch >= args.N) break;
+          const float ws = __ldcg(args.w_scale + static_cast<int64_t>(u.e) * args.N + ch);
+          const float bias = args.bias ? __ldcg(args.bias + ch) : 0.0f;
+          store_out(args.out, args.dtype, (u.row0 + tok) * args.N + ch,
+                    fmaf(static_cast<float>(sum[j]) * as, ws, bias));
+        }
+      }
+    }
+    // no CTA's shared memory goes away while another reads it
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
+template <int BN, bool SPLIT>
+cudaError_t launch_mm(const CUtensorMap& tm_a, const CUtensorMap& tm_w, const I8Args& a, int grid,
+                      cudaStream_t s) {
+  const size_t smem = i8_smem_bytes<BN>();
+  // per-device function attribute: set once per device (idempotent)
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        k_int8_mm<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
+  if constexpr (SPLIT)
+    return launch_pdl_cluster(k_int8_mm<BN, true>, dim3(grid), dim3(kI8Threads), smem, s, a.S, tm_a,
+                              tm_w, a);
+  else
+    return launch_pdl(k_int8_mm<BN, false>, dim3(grid), dim3(kI8Threads), smem, s, tm_a, tm_w, a);
+}
+
+struct I8Plan {
+  int bn, S;
+};
+
+// The tile width and K split with the shortest estimated pipeline: rounds of tiles over the SMs
+// times the K blocks of a tile, a K block costing the slower of its MMAs (2 cycles per token
+// column) and its fill of shared memory (about 79 bytes a cycle).
+I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms) {
+  const int64_t NT = (N + kWRows - 1) / kWRows;
+  const int64_t used = M < E ? M : E;
+  I8Plan best{256, 1};
+  double best_cost = 1e30;
+  for (const int bn : {16, 64, 128, 256}) {
+    const int64_t per = (M + used - 1) / used;           // tokens of an expert, evenly spread
+    const int64_t mt = (per + bn - 1) / bn;
+    const int64_t tiles = mt * used * NT;
+    const int64_t most = (grouped ? M / bn + used : mt) * NT;  // no spread has more tiles
+    const int64_t cols = ((per + mt - 1) / mt + 15) / 16 * 16;
+    const double kb = cols * 2.0 > (kWRows + cols) * kKB / 79.0 ? cols * 2.0
+                                                               : (kWRows + cols) * kKB / 79.0;
+    for (int S = 1; S <= 8; ++S) {
+      if (S > 1 && (bn > 128 || most * S > sms || nkb < 2 * S)) break;
+      const int64_t waves = S > 1 ? 1 : (tiles + sms - 1) / sms;
+      const double cost = waves * ((nkb + S - 1) / S) * kb + cols * 20.0 + (S > 1 ? 1500.0 : 0.0);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = I8Plan{bn, S};
+      }
+    }
+  }
+  return best;
+}
+
+template <int BN>
+cudaError_t run_mm(const Int8Product& p, int S, bool grouped, int sms, cudaStream_t s) {
+  CUtensorMap tm_a, tm_w;
+  if (!tensor_map_u8(&tm_a, p.a, p.K, p.M, p.K, kKB, I8Cfg<BN>::BOX) ||
+      !tensor_map_u8(&tm_w, p.w, p.K, static_cast<uint64_t>(p.E) * p.N, p.K, kKB, kWRows))
+    return cudaErrorInvalidValue;
+  I8Args a{};
+  a.a_scale = p.a_scale;
+  a.w_scale = p.w_scale;
+  a.bias = p.bias;
+  a.expert_base = p.expert_base;
+  a.out = p.out;
+  a.M = p.M;
+  a.N = p.N;
+  a.E = p.E;
+  a.nkb = (p.K + kKB - 1) / kKB;
+  a.S = S;
+  a.dtype = p.out_dtype;
+  a.zero_tail = p.zero_tail;
+  const int64_t NT = (p.N + kWRows - 1) / kWRows;
+  const int64_t used = p.M < p.E ? p.M : p.E;
+  int64_t most = (grouped ? p.M / BN + used : (p.M + BN - 1) / BN) * NT;
+  if constexpr (BN <= 128)
+    if (S > 1) return launch_mm<BN, true>(tm_a, tm_w, a, static_cast<int>(most * S), s);
+  if (most > sms) most = sms;
+  return launch_mm<BN, false>(tm_a, tm_w, a, static_cast<int>(most), s);
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, void* q,
+                                 float* scale, cudaStream_t s) {
+  const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0 &&
+                   (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  if (dtype == FMOE_DTYPE_BF16)
+    return vec ? quantize_rows<__nv_bfloat16, 8>(x, rows, K, q, scale, s)
+               : quantize_rows<__nv_bfloat16, 1>(x, rows, K, q, scale, s);
+  return vec ? quantize_rows<__half, 8>(x, rows, K, q, scale, s)
+             : quantize_rows<__half, 1>(x, rows, K, q, scale, s);
+}
+
+cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
+  const bool grouped = p.expert_base != nullptr;
+  const I8Plan plan = i8_plan(p.M, p.N, p.E, (p.K + kKB - 1) / kKB, grouped, sms);
+  switch (plan.bn) {
+    case 16:
+      return run_mm<16>(p, plan.S, grouped, sms, s);
+    case 64:
+      return run_mm<64>(p, plan.S, grouped, sms, s);
+    case 128:
+      return run_mm<128>(p, plan.S, grouped, sms, s);
+    default:
+      return run_mm<256>(p, plan.S, grouped, sms, s);
+  }
+}
+
+cudaError_t take_int8_status(int32_t* status, cudaStream_t s) {
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, g_int8_status);
+  if (e != cudaSuccess) return e;
+  e = cudaMemcpyAsync(status, p, sizeof(int32_t), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int32_t), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  return e;
+}
+
+}  // namespace fmoe

@@ -208,6 +208,70 @@ cudaError_t launch_route_permute(const void* logits, int logits_dtype, const voi
                                  int H, int I, int num_sms, const PermuteBuffers& b,
                                  cudaStream_t s);
 
+// ---------------------------------------------------------------- operators around the experts
+// (fmoe_tokens.cu, fmoe_int8.cu, fmoe_norm.cu; argument checks in fmoe_layer_api.cu)
+
+// SM count of the current device; FMOE_ERR_DEVICE unless it is an sm_100.
+int device_sms(int* sms);
+// 2-D tensor map over a row-major byte matrix, 128-byte-swizzled boxes.
+bool tensor_map_u8(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows,
+                   uint64_t row_stride, uint32_t box_cols, uint32_t box_rows);
+
+struct TokenOrder {
+  const int32_t* expert_base;  // [E + 1]
+  const int32_t* row_pick;     // [R]
+  const int32_t* pick_row;     // [T, K]
+  int T, K, E;
+  int64_t R;
+};
+constexpr int kMaxOrderExperts = 1024;
+size_t order_scratch_bytes(int64_t picks, int E);
+cudaError_t launch_order(const int32_t* ids, const TokenOrder& o, int offset, int align,
+                         int32_t* expert_base, int32_t* row_pick, int32_t* pick_row,
+                         int32_t* hist, cudaStream_t s);
+cudaError_t launch_sort_rows(const void* x, void* rows, const TokenOrder& o, int64_t row_bytes,
+                             int zero_tail, int num_sms, cudaStream_t s);
+cudaError_t launch_unsort_rows(const void* rows, const float* w, void* y, int dtype,
+                               const TokenOrder& o, int64_t H, cudaStream_t s);
+cudaError_t launch_unsort_back(const void* dy, const void* rows, const float* w, void* drows,
+                               float* dw, int dtype, const TokenOrder& o, int64_t H, int num_sms,
+                               cudaStream_t s);
+
+struct Int8Product {
+  const void* a;        // [M, K]
+  const void* w;        // [E * N, K]
+  const float* a_scale; // [M]
+  const float* w_scale; // [E * N]
+  const float* bias;    // [N] or null
+  const int32_t* expert_base;  // [E + 1], or null for one matrix (E = 1)
+  void* out;            // [M, N]
+  int64_t M;
+  int N, K, E;
+  int out_dtype;
+  int zero_tail;        // rows from expert_base[E] on are zeroed
+};
+cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, void* q,
+                                 float* scale, cudaStream_t s);
+cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s);
+cudaError_t take_int8_status(int32_t* status, cudaStream_t s);
+
+constexpr int kMaxNormBlocks = 296;  // blocks of the backward pass (two per SM of a 148-SM part)
+struct BlockNorm {
+  int dtype;
+  int64_t T;
+  int H;
+  const void *f, *x, *wp, *g, *wq;
+  int wp_dtype, g_dtype, wq_dtype, gate;
+  float s, eps;
+  void *h, *y, *q;
+  float *q_scale, *stats;
+  bool back;
+  const void *da, *dy;
+  void *df, *dx, *dwp, *dg, *dwq;
+  float* part;
+};
+cudaError_t launch_block_norm(const BlockNorm& p, int sms, cudaStream_t s);
+
 // ---------------------------------------------------------------- output stores
 // Eight fp32 values of an output row as bf16 (round to nearest even) or fp32; v counts groups of
 // eight columns.

@@ -1,0 +1,172 @@
+"""The RMS norms before and after a block, fused with the block's gate and the residual scale.
+
+One call sits between two blocks of a model: it normalises what the block returned, gates it, adds
+it to the scaled residual stream and normalises the sum for the next block; for an FP8 expert layer
+the result leaves as ``run``'s e4m3 input with its scales. Forward and backward are one pass each.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import FmoeBlockNormArgs
+from ._op import DTYPE_TAG, call, need, ptr, recording
+
+BLOCK = 128
+
+
+def _args(branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps):
+    a = FmoeBlockNormArgs()
+    a.num_tokens, a.hidden_size = residual.shape
+    a.dtype = DTYPE_TAG[residual.dtype]
+    a.branch, a.residual = ptr(branch), residual.data_ptr()
+    if post_weight is not None:
+        a.post_weight, a.post_weight_dtype = post_weight.data_ptr(), DTYPE_TAG[post_weight.dtype]
+    if gate is not None:
+        a.gate, a.gate_dtype, a.gate_kind = gate.data_ptr(), DTYPE_TAG[gate.dtype], kind
+    if pre_weight is not None:
+        a.pre_weight, a.pre_weight_dtype = pre_weight.data_ptr(), DTYPE_TAG[pre_weight.dtype]
+    a.residual_scale, a.eps = residual_scale, eps
+    return a
+
+
+def _forward(branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps, quantize,
+             hidden, want_stats):
+    a = _args(branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps)
+    T, H = residual.shape
+    device = residual.device
+    if hidden is None:
+        # without a block output and with scale 1 the residual stream is what it was
+        if branch is None and residual_scale == 1.0 and not want_stats:
+            hidden = residual
+        else:
+            hidden = torch.empty_like(residual)
+            a.hidden = hidden.data_ptr()
+    else:
+        a.hidden = hidden.data_ptr()
+    normed = stats = None
+    if quantize:
+        q = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=device)
+        scale = torch.empty((H // BLOCK, T), dtype=torch.float32, device=device)
+        a.normed_q, a.normed_scale = q.data_ptr(), scale.data_ptr()
+        normed = (q, scale)
+    elif pre_weight is not None:
+        normed = torch.empty_like(residual)
+        a.normed = normed.data_ptr()
+    if want_stats:
+        stats = torch.empty((T, 2), dtype=torch.float32, device=device)
+        a.stats = stats.data_ptr()
+    call("fmoe_block_norm", device, ctypes.byref(a))
+    return hidden, normed, stats
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps):
+        hidden, normed, stats = _forward(branch, residual, post_weight, gate, pre_weight, kind,
+                                         residual_scale, eps, False, None, True)
+        ctx.save_for_backward(branch, residual, post_weight, gate, pre_weight, stats)
+        ctx.rest = (kind, residual_scale, eps)
+        ctx.set_materialize_grads(False)
+        return hidden, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_hidden, grad_normed):
+        branch, residual, post_weight, gate, pre_weight, stats = ctx.saved_tensors
+        a = _args(branch, residual, post_weight, gate, pre_weight, *ctx.rest)
+        if grad_hidden is not None:
+            grad_hidden = grad_hidden.contiguous()
+            a.grad_hidden = grad_hidden.data_ptr()
+        if grad_normed is not None:
+            grad_normed = grad_normed.contiguous()
+            a.grad_normed = grad_normed.data_ptr()
+        a.stats = stats.data_ptr()
+        grads = [torch.empty_like(t) if t is not None and wanted else None
+                 for t, wanted in zip((branch, residual, post_weight, gate, pre_weight),
+                                      ctx.needs_input_grad)]
+        (a.grad_branch, a.grad_residual, a.grad_post_weight, a.grad_gate,
+         a.grad_pre_weight) = map(ptr, grads)
+        T, H = residual.shape
+        workspace = None
+        if grads[2] is not None or grads[3] is not None or grads[4] is not None:
+            size = ctypes.c_size_t()
+            _lib.check(_lib.load().fmoe_block_norm_workspace_size(T, H, ctypes.byref(size)),
+                       "fmoe_block_norm_workspace_size")
+            workspace = torch.empty(size.value, dtype=torch.uint8, device=residual.device)
+            a.workspace, a.workspace_bytes = ptr(workspace), size.value
+        call("fmoe_block_norm_backward", residual.device, ctypes.byref(a))
+        return (*grads, None, None, None)
+
+
+def block_norm(branch: Optional[torch.Tensor], residual: torch.Tensor, *,
+               post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+               residual_scale: float = 1.0, pre_weight: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, quantize: bool = False,
+               output: Optional[torch.Tensor] = None,
+               ) -> Tuple[torch.Tensor, Union[None, torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]]:
+    """``hidden = residual_scale * residual + gate * norm(branch) * post_weight`` and
+    ``normed = norm(hidden) * pre_weight``, with ``norm(v) = v / sqrt(mean(v^2) + eps)`` per token.
+
+    branch, residual [T, H] of one type (bf16, fp16, fp32), H up to 16384; branch None where no
+    block came before (``hidden`` is then the scaled residual). post_weight [H]: None for no norm
+    after the block. gate: one factor per token [T, 1], per channel [H] or per element [T, H], or
+    None. pre_weight [H]: None for no norm before the next block (``normed`` is then None). Weights
+    and gate are of the activations' type or fp32. hidden stays in fp32 between the two norms.
+
+    Returns ``(hidden, normed)``. With ``quantize`` (H a multiple of 128, 16-byte aligned tensors)
+    normed is the pair ``(e4m3 [T, H], fp32 scales [H/128, T])`` that ``run`` takes as
+    ``hidden_states`` and ``hidden_states_scale``; that form has no gradient. ``output`` receives
+    hidden and may be ``residual`` itself (no gradient either). Otherwise differentiable in every
+    tensor; weight gradients are summed over tokens in a fixed order.
+    """
+    if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
+        raise ValueError("residual must be a tensor of shape [T, H]")
+    need(residual, "residual", None, None, tuple(DTYPE_TAG))
+    T, H = residual.shape
+    if not 1 <= H <= 16384:
+        raise ValueError(f"the hidden size must be 1..16384, got {H}")
+    device, dtype = residual.device, residual.dtype
+    params = (dtype, torch.float32)
+    if branch is not None:
+        need(branch, "branch", device, (T, H), (dtype,))
+    elif post_weight is not None or gate is not None:
+        raise ValueError("post_weight and gate need a branch")
+    if post_weight is not None:
+        need(post_weight, "post_weight", device, (H,), params)
+    if pre_weight is not None:
+        need(pre_weight, "pre_weight", device, (H,), params)
+    kind = _lib.GATE_NONE
+    if gate is not None:
+        need(gate, "gate", device, None, params)
+        shape = tuple(gate.shape)
+        if shape == (H,):
+            kind = _lib.GATE_CHANNEL
+        elif shape == (T, 1):
+            kind = _lib.GATE_TOKEN
+        elif shape == (T, H):
+            kind = _lib.GATE_FULL
+        else:
+            raise ValueError(f"gate must have shape {(T, 1)}, {(H,)} or {(T, H)}, got {shape}")
+    if quantize:
+        if pre_weight is None:
+            raise ValueError("quantize needs a pre_weight")
+        if H % BLOCK:
+            raise ValueError(f"quantize needs a hidden size that is a multiple of {BLOCK}, got {H}")
+    if output is not None:
+        need(output, "output", device, (T, H), (dtype,))
+    residual_scale, eps = float(residual_scale), float(eps)
+    if recording(branch, residual, post_weight, gate, pre_weight, output):
+        if quantize:
+            raise ValueError("the quantised form has no gradient: call it under torch.no_grad()")
+        if output is not None:
+            raise ValueError("output cannot be given where gradients are recorded")
+        return _BlockNorm.apply(branch, residual, post_weight, gate, pre_weight, kind,
+                                residual_scale, eps)
+    hidden, normed, _ = _forward(branch, residual, post_weight, gate, pre_weight, kind,
+                                 residual_scale, eps, quantize, output, False)
+    return hidden, normed

@@ -1,0 +1,199 @@
+"""Tokens sorted by expert and back, with the routing weights applied, and the gradients.
+
+``sort_by_expert`` turns the routing's picks (``route``, or any top-k) into an ``ExpertOrder``;
+``sort_tokens`` copies token rows into expert order, where one product per expert (for instance
+``int8_expert_matmul`` with ``order.expert_base``) can run over them; ``unsort_tokens`` adds the
+experts' output rows back up per token, each times its routing weight. The tables stay on the
+device and nothing waits for it, so the whole run can be captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import FmoeTokenOrder
+from ._op import DTYPE_TAG, call, need, ptr, recording
+
+
+class ExpertOrder:
+    """The row of every pick, and back. Made by ``sort_by_expert``; all tensors on one device.
+
+    ``expert_base`` int32 [E+1]: first row of each local expert (a multiple of ``align``); the
+    last entry is where the rows end. ``row_pick`` int32 [num_rows]: the flat pick ``t * top_k + k``
+    of each row, -1 for a row without one (padding, and every row from ``expert_base[E]`` on).
+    ``pick_row`` int32 [T, top_k]: the row of each pick, -1 if its expert is not local. Rows are
+    ordered by expert, within an expert by pick.
+    """
+
+    __slots__ = ("expert_base", "row_pick", "pick_row", "num_tokens", "top_k", "num_rows",
+                 "device", "_c", "_ref")
+
+    def __init__(self, expert_base, row_pick, pick_row):
+        self.expert_base, self.row_pick, self.pick_row = expert_base, row_pick, pick_row
+        self.num_tokens, self.top_k = pick_row.shape
+        self.num_rows = row_pick.shape[0]
+        self.device = pick_row.device
+        self._c = FmoeTokenOrder(self.num_tokens, self.top_k, expert_base.shape[0] - 1,
+                                 self.num_rows, expert_base.data_ptr(), row_pick.data_ptr(),
+                                 pick_row.data_ptr())
+        self._ref = ctypes.byref(self._c)
+
+
+@torch.no_grad()
+def sort_by_expert(topk_ids: torch.Tensor, num_local_experts: int, local_expert_offset: int = 0,
+                   *, align: int = 1) -> ExpertOrder:
+    """The expert order of int32 picks ``topk_ids`` [T, top_k].
+
+    Local are the experts [local_expert_offset, local_expert_offset + num_local_experts); picks of
+    other ids (-1 = no pick) get no row. Every expert's rows start at a multiple of ``align``
+    (1..1024). A token may pick the same expert twice: each pick has its own row. Stable: equal
+    inputs give equal tables.
+    """
+    if not isinstance(topk_ids, torch.Tensor) or topk_ids.dim() != 2:
+        raise ValueError("topk_ids must be a tensor of shape [T, top_k]")
+    need(topk_ids, "topk_ids", None, None, (torch.int32,))
+    T, K = topk_ids.shape
+    if K < 1:
+        raise ValueError("topk_ids needs at least one pick per token")
+    if not 1 <= num_local_experts <= 1024:
+        raise ValueError(f"num_local_experts must be 1..1024, got {num_local_experts}")
+    if local_expert_offset < 0:
+        raise ValueError(f"local_expert_offset must not be negative, got {local_expert_offset}")
+    if not 1 <= align <= 1024:
+        raise ValueError(f"align must be 1..1024, got {align}")
+    rows, scratch_bytes = ctypes.c_int64(), ctypes.c_size_t()
+    _lib.check(_lib.load().fmoe_sort_size(T, K, num_local_experts, align, ctypes.byref(rows),
+                                          ctypes.byref(scratch_bytes)), "fmoe_sort_size")
+    device = topk_ids.device
+    order = ExpertOrder(
+        torch.empty(num_local_experts + 1, dtype=torch.int32, device=device),
+        torch.empty(rows.value, dtype=torch.int32, device=device),
+        torch.empty((T, K), dtype=torch.int32, device=device))
+    scratch = None
+    if scratch_bytes.value:
+        scratch = torch.empty(scratch_bytes.value, dtype=torch.uint8, device=device)
+    call("fmoe_sort_by_expert", device, topk_ids.data_ptr(), local_expert_offset, align,
+         order._ref, ptr(scratch), scratch_bytes.value)
+    return order
+
+
+def _rows_shape(x: torch.Tensor, n: int):
+    return (n,) if x.dim() == 1 else (n, x.shape[1])
+
+
+def _sort(x: torch.Tensor, order: ExpertOrder, output: Optional[torch.Tensor]) -> torch.Tensor:
+    zero_tail = output is None
+    if output is None:
+        output = torch.empty(_rows_shape(x, order.num_rows), dtype=x.dtype, device=x.device)
+    row_bytes = x.element_size() * (1 if x.dim() == 1 else x.shape[1])
+    call("fmoe_sort_rows", order.device, x.data_ptr(), row_bytes, order._ref, output.data_ptr(),
+         int(zero_tail))
+    return output
+
+
+def _unsort(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor],
+            output: Optional[torch.Tensor]) -> torch.Tensor:
+    if output is None:
+        output = torch.empty(_rows_shape(rows, order.num_tokens), dtype=rows.dtype,
+                             device=rows.device)
+    call("fmoe_unsort_rows", order.device, rows.data_ptr(), DTYPE_TAG[rows.dtype],
+         1 if rows.dim() == 1 else rows.shape[1], order._ref, ptr(weights), output.data_ptr())
+    return output
+
+
+class _SortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, order):
+        ctx.order = order
+        return _sort(x, order, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_rows):
+        return _unsort(grad_rows.contiguous(), ctx.order, None, None), None
+
+
+class _UnsortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, order):
+        ctx.order = order
+        ctx.weighted = weights is not None
+        # the rows are needed again only for the weights' gradient
+        keep = rows if ctx.weighted and ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(keep, weights)
+        return _unsort(rows, order, weights, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        rows, weights = ctx.saved_tensors
+        order = ctx.order
+        grad_y = grad_y.contiguous()
+        grad_rows = grad_weights = None
+        if ctx.needs_input_grad[0]:
+            grad_rows = torch.empty(_rows_shape(grad_y, order.num_rows), dtype=grad_y.dtype,
+                                    device=grad_y.device)
+        if ctx.weighted and ctx.needs_input_grad[1]:
+            grad_weights = torch.empty_like(weights)
+        call("fmoe_unsort_rows_backward", order.device, grad_y.data_ptr(), ptr(rows),
+             DTYPE_TAG[grad_y.dtype], 1 if grad_y.dim() == 1 else grad_y.shape[1], order._ref,
+             ptr(weights), ptr(grad_rows), ptr(grad_weights))
+        return grad_rows, grad_weights, None
+
+
+def _check(t, name: str, order, n: int) -> None:
+    if not isinstance(order, ExpertOrder):
+        raise TypeError("order must be an ExpertOrder (sort_by_expert)")
+    need(t, name, order.device)
+    if t.dim() not in (1, 2) or t.shape[0] != n or (t.dim() == 2 and t.shape[1] < 1):
+        raise ValueError(f"{name} must have shape [{n}] or [{n}, H], got {tuple(t.shape)}")
+
+
+def sort_tokens(x: torch.Tensor, order: ExpertOrder, *,
+                output: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Token rows ``x`` [T, H] (or one value per token, [T]) in expert order: [num_rows, H].
+
+    Any element type (int8 and e4m3 rows and fp32 scales among them). Padding rows inside an
+    expert's range are zero. Rows from ``order.expert_base[E]`` on are zero in a new tensor and
+    left as they were in a given ``output``. Differentiable for bf16, fp16 and fp32 ``x`` (without
+    ``output``): a token's gradient is the sum of its rows' gradients in fp32, rounded once.
+    """
+    _check(x, "x", order, order.num_tokens if isinstance(order, ExpertOrder) else 0)
+    if output is not None:
+        need(output, "output", order.device, _rows_shape(x, order.num_rows), (x.dtype,))
+    if recording(x, output):
+        if output is not None:
+            raise ValueError("output cannot be given where gradients are recorded")
+        if x.dtype not in DTYPE_TAG:
+            raise TypeError(f"no gradient for {x.dtype} rows")
+        return _SortTokens.apply(x, order)
+    return _sort(x, order, output)
+
+
+def unsort_tokens(rows: torch.Tensor, order: ExpertOrder,
+                  topk_weights: Optional[torch.Tensor] = None, *,
+                  output: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Expert rows back per token: ``y[t] = sum_k topk_weights[t, k] * rows[pick_row[t, k]]``.
+
+    ``rows`` [num_rows, H] (or [num_rows]) bf16, fp16 or fp32, ``topk_weights`` fp32 [T, top_k] or
+    None for ones. Sums in fp32 in pick order, rounded once; picks without a row add nothing,
+    whatever their weight, and rows without a pick are not read. Differentiable in ``rows`` and
+    ``topk_weights`` (without ``output``); rows without a pick get a zero gradient.
+    """
+    _check(rows, "rows", order, order.num_rows if isinstance(order, ExpertOrder) else 0)
+    if rows.dtype not in DTYPE_TAG:
+        raise TypeError(f"rows must be bfloat16, float16 or float32, got {rows.dtype}")
+    if topk_weights is not None:
+        need(topk_weights, "topk_weights", order.device, (order.num_tokens, order.top_k),
+             (torch.float32,))
+    if output is not None:
+        need(output, "output", order.device, _rows_shape(rows, order.num_tokens), (rows.dtype,))
+    if recording(rows, topk_weights, output):
+        if output is not None:
+            raise ValueError("output cannot be given where gradients are recorded")
+        return _UnsortTokens.apply(rows, topk_weights, order)
+    return _unsort(rows, order, topk_weights, output)

@@ -48,6 +48,7 @@ extern "C" {
 /* Device status word bits (fmoe_read_status): set by a kernel whose bounded wait ran out. */
 #define FMOE_STATUS_TIMEOUT_GEMM1  0x1
 #define FMOE_STATUS_TIMEOUT_GEMM2  0x2
+#define FMOE_STATUS_TIMEOUT_INT8   0x4  /* fmoe_int8_status */
 
 /* output dtypes */
 #define FMOE_OUT_BF16    0
@@ -63,6 +64,7 @@ extern "C" {
 /* dtype tags for the routing inputs */
 #define FMOE_DTYPE_F32   0
 #define FMOE_DTYPE_BF16  1
+#define FMOE_DTYPE_F16   2   /* the operators around the experts (below) only */
 
 /* Routing methods (FmoeArgs.routing_method). DeepSeek-V3 is the hot path of kernel.py:371-457
  * and the zero value; the others are the same definition family's routing references
@@ -331,6 +333,145 @@ FMOE_API int fmoe_read_status(const void* workspace, void* cuda_stream, int32_t*
  * word *status. k_blocks: 1..500000. */
 FMOE_API int fmoe_fp8_mma_peak(int32_t k_blocks, int32_t* status, double* flops,
                                void* cuda_stream);
+
+/* ---------------------------------------------------------------- around the experts
+ * Operators next to the fused layer, for models whose experts are not its FP8 ones, for training
+ * and for the layers around it. No counterpart in the reference. Same conventions: device
+ * pointers, the caller's stream, no allocation, no host synchronisation, graph-capturable.
+ * `dtype` is FMOE_DTYPE_BF16, _F16 or _F32; tensors are row-major and contiguous, aligned to their
+ * element (16-byte alignment and rows of a multiple of 16 bytes take the fast path). Outputs may
+ * not overlap inputs unless a function says so. */
+
+/* Tokens sorted by expert. Pick p = t * top_k + k of topk_ids [T, top_k] is local if its expert
+ * e = topk_ids[p] - local_expert_offset lies in [0, num_local_experts); other ids (-1 among them)
+ * have no row. Rows are ordered by expert, within an expert by pick; expert e's start at
+ * expert_base[e], a multiple of `align`. fmoe_sort_size gives the rows R = P + min(P, E) *
+ * (align - 1), P = T * top_k, that always suffice, and the scratch bytes of fmoe_sort_by_expert
+ * (may be 0).
+ *   expert_base int32 [E + 1]   row_pick int32 [R] (-1 = no pick)   pick_row int32 [T, top_k]
+ * num_local_experts: 1..1024, align: 1..1024. */
+typedef struct FmoeTokenOrder {
+  int32_t num_tokens;
+  int32_t top_k;
+  int32_t num_local_experts;
+  int64_t num_rows;
+  int32_t* expert_base;
+  int32_t* row_pick;
+  int32_t* pick_row;
+} FmoeTokenOrder;
+
+FMOE_API int fmoe_sort_size(int32_t num_tokens, int32_t top_k, int32_t num_local_experts,
+                            int32_t align, int64_t* num_rows, size_t* scratch_bytes);
+
+FMOE_API int fmoe_sort_by_expert(const int32_t* topk_ids, int32_t local_expert_offset,
+                                 int32_t align, const FmoeTokenOrder* order, void* scratch,
+                                 size_t scratch_bytes, void* cuda_stream);
+
+/* rows[r] = x[row_pick[r] / top_k] for rows of row_bytes bytes (any element type); a padding row
+ * inside an expert's range is zeroed, and so are the rows from expert_base[E] on if zero_tail is
+ * set (else they are left as they were). */
+FMOE_API int fmoe_sort_rows(const void* x, int64_t row_bytes, const FmoeTokenOrder* order,
+                            void* rows, int32_t zero_tail, void* cuda_stream);
+
+/* y[t] = sum over k of weights[t, k] * rows[pick_row[t, k]] in fp32, k ascending, rounded once.
+ * weights fp32 [T, top_k], or NULL for ones; weights of picks without a row are not used. With
+ * NULL weights this is also the gradient of fmoe_sort_rows. */
+FMOE_API int fmoe_unsort_rows(const void* rows, int32_t dtype, int64_t hidden_size,
+                              const FmoeTokenOrder* order, const float* weights, void* y,
+                              void* cuda_stream);
+
+/* Gradients of fmoe_unsort_rows: grad_rows[r] = weight * grad_y[t] (all R rows written, zero where
+ * there is no pick), grad_weights[t, k] = <grad_y[t], rows[pick_row[t, k]]> in fp32 (0 where there
+ * is no row). Either output may be NULL; rows may be NULL without grad_weights. */
+FMOE_API int fmoe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtype,
+                                       int64_t hidden_size, const FmoeTokenOrder* order,
+                                       const float* weights, void* grad_rows, float* grad_weights,
+                                       void* cuda_stream);
+
+/* Symmetric int8 quantisation per row: amax = max(max |x|, 1e-30), scale[r] = amax / 127,
+ * q = round half to even of 127 x / amax. x [R, K] bf16 or fp16. A row that holds a NaN or an
+ * infinity has a NaN or infinite scale, so its products are NaN. */
+FMOE_API int fmoe_quantize_int8(const void* x, int32_t dtype, int64_t num_rows, int64_t k,
+                                void* q, float* scale, void* cuda_stream);
+
+/* out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] * b[n, k] (+ bias[n]): a int8 [M, K],
+ * b int8 [N, K], scales and bias fp32 (bias may be NULL), out [M, N] of out_dtype. The sum is exact
+ * (int32), the rest fp32, rounded once. K: a multiple of 16 up to 131056; a and b 16-byte
+ * aligned. */
+FMOE_API int fmoe_int8_matmul(const void* a, const void* b, const float* a_scale,
+                              const float* b_scale, const float* bias, int64_t m, int32_t n,
+                              int32_t k, void* out, int32_t out_dtype, void* cuda_stream);
+
+/* The same with one matrix per expert: rows expert_base[e] .. expert_base[e + 1] of `rows`
+ * int8 [R, K] are multiplied with weights[e] (int8 [E, N, K], scales [E, N]); expert_base int32
+ * [E + 1] stays on the device. Bases outside [0, R] are clamped. Rows from expert_base[E] on are
+ * zeroed if zero_tail is set and left as they were otherwise. num_local_experts: 1..256. */
+FMOE_API int fmoe_int8_expert_matmul(const void* rows, const void* weights, const float* row_scale,
+                                     const float* weight_scale, const int32_t* expert_base,
+                                     int64_t num_rows, int32_t num_local_experts, int32_t n,
+                                     int32_t k, void* out, int32_t out_dtype, int32_t zero_tail,
+                                     void* cuda_stream);
+
+/* FMOE_STATUS_TIMEOUT_INT8 if a wait of an int8 product on the current device ran out since the
+ * last call (its output is not valid), else 0; synchronises the stream and clears the word. */
+FMOE_API int fmoe_int8_status(int32_t* status, void* cuda_stream);
+
+/* The norms before and after a block, with its gate and the residual scale. Per token:
+ *   n = post_weight ? branch * rsqrt(mean(branch^2) + eps) * post_weight : branch
+ *   hidden = residual_scale * residual + gate * n
+ *   normed = hidden * rsqrt(mean(hidden^2) + eps) * pre_weight
+ * hidden is kept in fp32 between the two and rounded once for output. branch NULL: hidden =
+ * residual_scale * residual (then no post_weight and no gate). pre_weight NULL: no normed.
+ * gate_kind: FMOE_GATE_*; a gate per token [T], per channel [H] or per element [T, H].
+ * Weights and gate are of `dtype` or fp32, each tagged. normed leaves as `dtype`, or with normed_q
+ * set as e4m3 [T, H] with fp32 scales [H/128, T] (scale = max(amax, 1e-30) / 448), the layout of
+ * FmoeArgs.hidden_states; H is then a multiple of 128 and every pointer 16-byte aligned.
+ * hidden may be NULL, and may be residual itself. hidden_size: 1..16384. stats fp32 [T, 2], or
+ * NULL: what the backward pass needs.
+ * Backward: the forward's inputs and stats, grad_hidden and grad_normed (either may be NULL: zero)
+ * and the wanted gradients (NULL: not wanted), each of its input's type; workspace of
+ * fmoe_block_norm_workspace_size bytes where a weight's or a channel gate's gradient is wanted.
+ * Sums over tokens run in a fixed order. */
+#define FMOE_GATE_NONE     0
+#define FMOE_GATE_TOKEN    1
+#define FMOE_GATE_CHANNEL  2
+#define FMOE_GATE_FULL     3
+
+typedef struct FmoeBlockNormArgs {
+  int64_t num_tokens;
+  int32_t hidden_size;
+  int32_t dtype;
+  const void* branch;
+  const void* residual;
+  const void* post_weight;
+  const void* gate;
+  const void* pre_weight;
+  int32_t post_weight_dtype;
+  int32_t gate_dtype;
+  int32_t pre_weight_dtype;
+  int32_t gate_kind;
+  float residual_scale;
+  float eps;
+  void* hidden;
+  void* normed;
+  void* normed_q;
+  float* normed_scale;
+  float* stats;
+  const void* grad_hidden;
+  const void* grad_normed;
+  void* grad_branch;
+  void* grad_residual;
+  void* grad_post_weight;
+  void* grad_gate;
+  void* grad_pre_weight;
+  void* workspace;
+  size_t workspace_bytes;
+} FmoeBlockNormArgs;
+
+FMOE_API int fmoe_block_norm_workspace_size(int64_t num_tokens, int32_t hidden_size,
+                                            size_t* bytes);
+FMOE_API int fmoe_block_norm(const FmoeBlockNormArgs* args, void* cuda_stream);
+FMOE_API int fmoe_block_norm_backward(const FmoeBlockNormArgs* args, void* cuda_stream);
 
 /* Number of SMs the persistent GEMM kernels size their grid for on the current device. */
 FMOE_API int fmoe_device_sm_count(int32_t* sms);
