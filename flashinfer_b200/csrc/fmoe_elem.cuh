@@ -45,15 +45,50 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return r;
 }
 
+// Two neighbouring 16-bit elements as one word, first element low.
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16*, float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &p, 4);
+  return w;
+}
+__device__ __forceinline__ uint32_t pack2(__half*, float lo, float hi) {
+  const __half2 p = __floats2half2_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &p, 4);
+  return w;
+}
+__device__ __forceinline__ float2 unpack2(__nv_bfloat16*, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(__half*, uint32_t w) {
+  __half2 p;
+  memcpy(&p, &w, 4);
+  return __half22float2(p);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> pack(const float (&v)[V]) {
+  Pack<T, V> r;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = pack2(static_cast<T*>(nullptr), v[2 * i], v[2 * i + 1]);
+    memcpy(&r, w, sizeof(r));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) from_f32(v[i], &r.e[i]);
+  }
+  return r;
+}
+
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
-  Pack<T, V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) from_f32(v[i], &r.e[i]);
+  const Pack<T, V> r = pack<T, V>(v);
   if constexpr (V * sizeof(T) == 16) {
-    uint32_t w[4];
-    memcpy(w, &r, 16);
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    uint4 w;
+    memcpy(&w, &r, 16);
+    *reinterpret_cast<uint4*>(p) = w;
   } else {
     *p = r.e[0];
   }
@@ -61,8 +96,19 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
 
 template <typename T, int V>
 __device__ __forceinline__ void unpack(const Pack<T, V>& r, float (&v)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    uint32_t w[V / 2];
+    memcpy(w, &r, sizeof(r));
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = to_f32(r.e[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 f = unpack2(static_cast<T*>(nullptr), w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32(r.e[i]);
+  }
 }
 
 __device__ __forceinline__ float warp_sum_f32(float v) {

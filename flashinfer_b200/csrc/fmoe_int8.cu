@@ -29,66 +29,79 @@ namespace {
 // infinite) scale and its products are NaN.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// One quotient: both operands scaled by 2^-8 (exact), so 127 * x stays finite. For 16-bit inputs
-// 127 * x is exact in fp32 and the distance of the true quotient from a rounding border is either
-// zero or far above fp32's rounding, so the result is the correctly rounded 127 x / amax.
-__device__ __forceinline__ int quant1(float v, float den) {
-  return __float2int_rn(__fdiv_rn(v * (127.0f / 256.0f), den));
+// 127 x / amax rounded to the nearest integer, ties to even, as a signed byte. With both operands
+// scaled by 2^-8, p = 127 x and den = amax are exact for 16-bit inputs and stay finite. p * inv is
+// within 2^-22 of the true quotient (relative), while a quotient that is no tie is at least 2^-18
+// (relative) away from every rounding border, since x and amax have at most 11 bits: only a true
+// tie can come out on either side. p - n * den is exact, tells a tie, and the odd neighbour then
+// steps to the even one. Against one IEEE division per element: quantising 8192 x 7168 took
+// 84.9 us with it.
+__device__ __forceinline__ uint32_t quant1(float v, float den, float inv) {
+  const float p = v * (127.0f / 256.0f);
+  const float m = fmaf(p, inv, 12582912.0f);   // 1.5 * 2^23: the sum's low bits are the integer
+  const float n = m - 12582912.0f;
+  uint32_t b = __float_as_uint(m);
+  const float d = fmaf(-n, den, p);
+  if (fabsf(d + d) == den && (b & 1u)) b += d > 0.0f ? 1u : ~0u;
+  return b & 0xffu;
 }
 
-// A row per G threads (32: a warp, 256: the block). Up to VPT groups of V elements per thread stay
-// in registers between the maximum and the rounding; longer rows are read a second time.
-template <typename T, int V, int G>
+// A row per G threads: a warp (WARP, eight rows per block) or the block. Up to VPT groups of V
+// elements per thread stay in registers between the maximum and the rounding; what a longer row
+// has beyond them is read a second time.
+template <typename T, int V, int VPT, bool WARP>
 __global__ void __launch_bounds__(256)
     k_quantize_int8(const T* x, int64_t rows, int64_t K, int8_t* q, float* scale) {
   pdl_begin_in_order();
-  constexpr int VPT = V > 1 ? 8 : 16;
   __shared__ uint32_t part[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = G == 32 ? lane : static_cast<int>(threadIdx.x);
-  const int64_t row = G == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
-  if (row >= rows) return;  // G = 32: whole warps; no block barrier follows
+  const int G = WARP ? 32 : blockDim.x;
+  const int g = WARP ? lane : static_cast<int>(threadIdx.x);
+  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
+  if (row >= rows) return;  // WARP: whole warps; no block barrier follows
   const int64_t nvec = K / V;
   const T* xr = x + row * K;
   int8_t* qr = q + row * K;
   Pack<T, V> in[VPT];
   uint32_t m = 0;
+  auto maximum = [&](const Pack<T, V>& p) {
+    float f[V];
+    unpack(p, f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = max(m, abs_bits(f[j]));
+  };
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int64_t v = g + static_cast<int64_t>(i) * G;
     if (v < nvec) in[i] = load_pack<T, V>(xr + v * V);
   }
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int64_t v = g + static_cast<int64_t>(i) * G;
-    if (v < nvec) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) m = max(m, abs_bits(to_f32(in[i].e[j])));
-    }
-  }
-  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < nvec; v += G) {
-    const Pack<T, V> p = load_pack<T, V>(xr + v * V);
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = max(m, abs_bits(to_f32(p.e[j])));
-  }
+  for (int i = 0; i < VPT; ++i)
+    if (g + static_cast<int64_t>(i) * G < nvec) maximum(in[i]);
+  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < nvec; v += G)
+    maximum(load_pack<T, V>(xr + v * V));
   m = __reduce_max_sync(0xffffffffu, m);
-  if (G == 256) {
+  if (!WARP) {
     if (lane == 0) part[warp] = m;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, part[i]);
+    for (int i = 0; i < (G >> 5); ++i) m = max(m, part[i]);
   }
   m = max(m, __float_as_uint(1e-30f));
   const float amax = __uint_as_float(m);
-  const float den = amax * (1.0f / 256.0f);
   if (g == 0) scale[row] = __fdiv_rn(amax, 127.0f);
+  const bool finite = m < 0x7f800000u;  // else the row's values are zeros
+  const float den = amax * (1.0f / 256.0f);
+  const float inv = 1.0f / den;
   auto put = [&](const Pack<T, V>& p, int64_t v) {
-    uint8_t b[V];
+    float f[V];
+    unpack(p, f);
+    uint32_t b[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) b[j] = static_cast<uint8_t>(quant1(to_f32(p.e[j]), den));
+    for (int j = 0; j < V; ++j) b[j] = finite ? quant1(f[j], den, inv) : 0u;
     if constexpr (V == 8) {
       uint2 w;
-      memcpy(&w, b, 8);
+      w.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+      w.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
       *reinterpret_cast<uint2*>(qr + v * V) = w;
     } else {
       qr[v] = static_cast<int8_t>(b[0]);
@@ -106,14 +119,18 @@ __global__ void __launch_bounds__(256)
 template <typename T, int V>
 cudaError_t quantize_rows(const void* x, int64_t rows, int64_t K, void* q, float* scale,
                           cudaStream_t s) {
-  // a warp holds rows of up to 8 (16-byte groups) or 16 (single elements) units per lane
+  // a row of up to four units per lane is a warp's; a longer one a block's, with as few threads
+  // as hold four units each
   const int64_t nvec = K / V;
-  if (nvec <= 32 * (V > 1 ? 8 : 16))
-    return launch_pdl(k_quantize_int8<T, V, 32>, dim3(static_cast<unsigned>((rows + 7) / 8)),
-                      dim3(256), 0, s, static_cast<const T*>(x), rows, K, static_cast<int8_t*>(q),
-                      scale);
-  return launch_pdl(k_quantize_int8<T, V, 256>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, s,
-                    static_cast<const T*>(x), rows, K, static_cast<int8_t*>(q), scale);
+  const T* xt = static_cast<const T*>(x);
+  int8_t* qt = static_cast<int8_t*>(q);
+  if (nvec <= 32 * 4)
+    return launch_pdl(k_quantize_int8<T, V, 4, true>, dim3(static_cast<unsigned>((rows + 7) / 8)),
+                      dim3(256), 0, s, xt, rows, K, qt, scale);
+  int64_t threads = (nvec + 127) / 128 * 32;
+  if (threads > 256) threads = 256;
+  return launch_pdl(k_quantize_int8<T, V, 4, false>, dim3(static_cast<unsigned>(rows)),
+                    dim3(static_cast<unsigned>(threads)), 0, s, xt, rows, K, qt, scale);
 }
 
 // ------------------------------------------------------------------ product

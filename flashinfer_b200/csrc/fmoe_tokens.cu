@@ -248,22 +248,26 @@ __global__ void __launch_bounds__(256)
        v < a.nvec; v += step) {
     float acc[V] = {};
     for (int k0 = 0; k0 < a.K; k0 += 8) {
+      // eight picks at a time: their rows and weights, then all eight loads, then the sums
       Pack<T, V> in[8];
-      int64_t r[8];
+      int r[8];
+      float f[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         r[j] = k0 + j < a.K ? __ldcg(pr + k0 + j) : -1;
+        f[j] = w && k0 + j < a.K ? __ldcg(w + t * a.K + k0 + j) : 1.0f;
         if (r[j] >= a.R) r[j] = -1;
-        if (r[j] >= 0) in[j] = load_pack<T, V>(rows + r[j] * H + v * V);
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (r[j] >= 0) in[j] = load_pack<T, V>(rows + r[j] * H + v * V);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (r[j] < 0) continue;
-        const float f = w ? __ldcg(w + t * a.K + k0 + j) : 1.0f;
         float e[V];
         unpack(in[j], e);
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(f, e[i], acc[i]);
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(f[j], e[i], acc[i]);
       }
     }
     store_pack<T, V>(y + t * H + v * V, acc);
@@ -289,13 +293,13 @@ __global__ void __launch_bounds__(256)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarp = blockDim.x >> 5;
   const int32_t* pr = a.pick_row + t * a.K;
   for (int k0 = 0; k0 < a.K; k0 += 8) {
-    int64_t r[8];
+    int r[8];
     float f[8], dot[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       r[j] = k0 + j < a.K ? __ldcg(pr + k0 + j) : -1;
+      f[j] = w && k0 + j < a.K ? __ldcg(w + t * a.K + k0 + j) : 1.0f;
       if (r[j] >= a.R) r[j] = -1;
-      f[j] = w && r[j] >= 0 ? __ldcg(w + t * a.K + k0 + j) : 1.0f;
       dot[j] = 0.0f;
     }
     for (int64_t v = threadIdx.x; v < a.nvec; v += blockDim.x) {
