@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t quant1(float v, float den, float inv) {
 // elements per thread stay in registers between the maximum and the rounding; what a longer row
 // has beyond them is read a second time.
 template <typename T, int V, int VPT, bool WARP>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
     k_quantize_int8(const T* x, int64_t rows, int64_t K, int8_t* q, float* scale) {
   pdl_begin_in_order();
   __shared__ uint32_t part[8];

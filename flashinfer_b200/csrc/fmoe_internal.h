@@ -255,7 +255,7 @@ cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t
 cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s);
 cudaError_t take_int8_status(int32_t* status, cudaStream_t s);
 
-constexpr int kMaxNormBlocks = 296;  // blocks of the backward pass (two per SM of a 148-SM part)
+constexpr int kMaxNormBlocks = 160;  // blocks of the norm's backward pass, at most one per SM
 struct BlockNorm {
   int dtype;
   int64_t T;

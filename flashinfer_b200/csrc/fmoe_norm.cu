@@ -17,6 +17,8 @@
 // so one pass over the row collects all three sums before anything is written.
 // All sums and statistics are fp32; the sums over rows run in a fixed order (rows of a block
 // ascending, then blocks ascending).
+#include <atomic>
+
 #include "fmoe_elem.cuh"
 #include "fmoe_internal.h"
 #include "fmoe_ptx.cuh"
@@ -77,7 +79,17 @@ __device__ __forceinline__ void load_param(const void* p, int f32, int64_t i, fl
       v[0] = *s;
     }
   } else {
-    const Pack<T, V> r = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(p) + i);
+    const T* s = static_cast<const T*>(p) + i;
+    Pack<T, V> r;
+    if constexpr (V > 1) {
+      const uint4 w = *reinterpret_cast<const uint4*>(s);
+      r.w[0] = w.x;
+      r.w[1] = w.y;
+      r.w[2] = w.z;
+      r.w[3] = w.w;
+    } else {
+      r.e = *s;
+    }
     unpack(r, v);
   }
 }
@@ -85,7 +97,7 @@ __device__ __forceinline__ void load_param(const void* p, int f32, int64_t i, fl
 template <typename T>
 __device__ __forceinline__ float load_scalar(const void* p, int f32, int64_t i) {
   return f32 ? __ldcg(static_cast<const float*>(p) + i)
-             : to_f32(load_pack<T, 1>(static_cast<const T*>(p) + i).e[0]);
+             : to_f32(load_pack<T, 1>(static_cast<const T*>(p) + i).e);
 }
 
 // The gate of V columns starting at col of row t (token gates are passed in).
@@ -100,6 +112,22 @@ __device__ __forceinline__ void load_gate(const NormGeom& a, const void* g, floa
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = g_tok;
   }
+}
+
+// V (4 or 8) values over their block's scale as e4m3.
+template <int V>
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&y)[V], float scale) {
+  uint32_t w[V / 4];
+#pragma unroll
+  for (int j = 0; j < V; j += 4)
+    w[j / 4] = static_cast<uint32_t>(pack_e4m3x2(__fdiv_rn(y[j], scale), __fdiv_rn(y[j + 1], scale))) |
+               static_cast<uint32_t>(pack_e4m3x2(__fdiv_rn(y[j + 2], scale),
+                                                 __fdiv_rn(y[j + 3], scale)))
+                   << 16;
+  if constexpr (V == 8)
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
 // Sums of N values over the block, the same in every thread. buf: [32][N], one per call site in
@@ -119,7 +147,10 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float* buf) {
   for (int i = 0; i < N; ++i) v[i] = warp_sum_f32(lane < nwarp ? buf[lane * N + i] : 0.0f);
 }
 
-// One row per block; a thread holds VPT groups of V columns.
+// ------------------------------------------------------------------ direct kernels
+// Rows whose tensors do not start on 16-byte boundaries (V = 1: single elements), or that are too
+// long for the ring of the kernels below (V: a 16-byte group): VPT groups per thread, one row per
+// block at a time, parameters read from global memory. Only V > 1 can leave as e4m3.
 template <typename T, int V, int VPT, int MAXT>
 __global__ void __launch_bounds__(MAXT)
     k_block_norm(const NormGeom a, const NormIn in, const NormOut out) {
@@ -209,11 +240,7 @@ __global__ void __launch_bounds__(MAXT)
           amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         const float scale = __fdiv_rn(fmaxf(amax, 1e-30f), 448.0f);
         if (live) {
-          uint16_t b[V / 2];
-#pragma unroll
-          for (int j = 0; j < V; j += 2)
-            b[j / 2] = pack_e4m3x2(__fdiv_rn(w[j], scale), __fdiv_rn(w[j + 1], scale));
-          memcpy(out.q + row + col, b, V);
+          store_e4m3<V>(out.q + row + col, w, scale);
           if (col % kBlock == 0) out.q_scale[(col / kBlock) * a.T + t] = scale;
         }
         continue;
@@ -370,6 +397,590 @@ __global__ void __launch_bounds__(MAXT)
   }
 }
 
+// ------------------------------------------------------------------ ring kernels
+// A group of G threads owns a row at a time; every thread copies the 16-byte granules that it will
+// use itself into a ring of `stages` rows in shared memory (cp.async), so rows arrive while earlier
+// ones are computed and no barrier guards the ring. A block holds gpb groups.
+//
+// The first form of these kernels was bound by its instructions (42 per element forward, 86
+// backward, at half the copy bandwidth). What depends on the column alone is therefore combined
+// once per block: wg = wp * (channel gate) and wq, in fp32, in registers (forward) or each thread's
+// own part of shared memory (backward); the arithmetic runs in packed pairs (fma.f32x2); and the
+// sums over rows need one accumulator for wp and the channel gate together, since
+// dwp = g * C and dg = wp * C with C = sum over rows of dh * f * r1 (the factor of a token or
+// element gate inside).
+//
+// A row of H elements starts at a multiple of H, which for odd H is no multiple of 16 bytes. Its
+// offset in its first granule, shift = (t * H) mod V, repeats every P = V / gcd(V, H) rows, so
+// block b takes rows t = b mod P only: shift, and with it the columns of every thread, are the
+// same for all its rows, and the sums over rows stay in registers. Elements of a neighbouring row
+// in the first granule are read as zero; the last granule's copy stops at the row's end.
+constexpr int kRingThreads = 512;
+
+struct RingGeom {
+  int G;          // threads per row, a multiple of 32
+  int gpb;        // rows in flight per block and stage
+  int P;          // row classes
+  int stages;
+  int slots;      // granules of one row in the ring: G * VPT
+  int row_step;   // between a group's rows
+  int narr;       // row tensors in the ring
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+// All but the latest `later` groups of this thread have landed.
+__device__ __forceinline__ void cp_async_wait(int later) {
+  if (later >= 2)
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (later == 1)
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Sums of N values over the G threads of a group, the same in each. buf: [N][16] of the group
+// (zero beyond its warps), and another one at the next call (one barrier each). After the barrier
+// every thread adds the warps' sums itself: four 16-byte reads and 15 additions are sooner done
+// than five shuffles.
+template <int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float* buf, int group, int G) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum_f32(v[i]);
+  if (G == 32) return;
+  const int lane = threadIdx.x & 31, w = (threadIdx.x - group * G) >> 5;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) buf[i * 16 + w] = v[i];
+  }
+  named_bar_sync(1 + group, G);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 q = *reinterpret_cast<const float4*>(buf + i * 16 + 4 * j);
+      sum += (q.x + q.y) + (q.z + q.w);
+    }
+    v[i] = sum;
+  }
+}
+
+template <typename T>
+constexpr int kV = 16 / static_cast<int>(sizeof(T));
+
+// A granule's values in fp32, as pairs for the packed instructions.
+template <typename T>
+struct Gran {
+  static constexpr int N = kV<T> / 2;
+  float2 p[N];
+};
+
+template <typename T>
+__device__ __forceinline__ void zero(Gran<T>& v) {
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) v.p[i] = make_float2(0.0f, 0.0f);
+}
+// a * b, a * s, a * b + c, a * s + c, element by element
+template <typename T>
+__device__ __forceinline__ Gran<T> mul(const Gran<T>& a, const Gran<T>& b) {
+  Gran<T> r;
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) r.p[i] = __fmul2_rn(a.p[i], b.p[i]);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Gran<T> mul(const Gran<T>& a, float s) {
+  Gran<T> r;
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) r.p[i] = __fmul2_rn(a.p[i], make_float2(s, s));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Gran<T> fma(const Gran<T>& a, const Gran<T>& b, const Gran<T>& c) {
+  Gran<T> r;
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) r.p[i] = __ffma2_rn(a.p[i], b.p[i], c.p[i]);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Gran<T> fma(const Gran<T>& a, float s, const Gran<T>& c) {
+  Gran<T> r;
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i)
+    r.p[i] = __ffma2_rn(a.p[i], make_float2(s, s), c.p[i]);
+  return r;
+}
+// acc += a * b, in two interleaved sums
+template <typename T>
+__device__ __forceinline__ void dot(float2& acc, const Gran<T>& a, const Gran<T>& b) {
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) acc = __ffma2_rn(a.p[i], b.p[i], acc);
+}
+
+// One granule from shared memory; element j < skip (a neighbouring row's) reads as zero.
+template <typename T>
+__device__ __forceinline__ Gran<T> read_granule(const uint4* p, int skip) {
+  Gran<T> r;
+  const uint4 q = *p;
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) {
+    if constexpr (sizeof(T) == 4)
+      r.p[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else
+      r.p[i] = unpack2(static_cast<T*>(nullptr), w[i]);
+  }
+  if (skip > 0) {
+#pragma unroll
+    for (int i = 0; i < Gran<T>::N; ++i) {
+      if (2 * i < skip) r.p[i].x = 0.0f;
+      if (2 * i + 1 < skip) r.p[i].y = 0.0f;
+    }
+  }
+  return r;
+}
+
+// V columns of a parameter (of T or fp32) from global memory, zero outside the row.
+template <typename T, bool ODD>
+__device__ __forceinline__ Gran<T> global_param(const void* p, int f32, int col0, int H) {
+  float v[kV<T>];
+  if (!ODD || (f32 && col0 >= 0 && col0 + kV<T> <= H && col0 % 4 == 0 &&
+               (reinterpret_cast<uintptr_t>(p) & 15u) == 0)) {
+    load_param<T, kV<T>>(p, f32, col0, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j)
+      v[j] = col0 + j >= 0 && col0 + j < H ? load_scalar<T>(p, f32, col0 + j) : 0.0f;
+  }
+  Gran<T> r;
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) r.p[i] = make_float2(v[2 * i], v[2 * i + 1]);
+  return r;
+}
+
+// wp * channel gate of V columns, ones where there is neither (zero outside the row, so that what
+// a thread computes there is zero too).
+template <typename T, bool ODD>
+__device__ __forceinline__ Gran<T> branch_weight(const NormGeom& a, const NormIn& in, int col0) {
+  Gran<T> r;
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; ++i) {
+    const int c = col0 + 2 * i;
+    r.p[i] = make_float2(c >= 0 && c < a.H ? 1.0f : 0.0f, c >= -1 && c + 1 < a.H ? 1.0f : 0.0f);
+  }
+  if (in.wp) r = global_param<T, ODD>(in.wp, a.wp_f32, col0, a.H);
+  if (a.gate == FMOE_GATE_CHANNEL) r = mul(r, global_param<T, ODD>(in.g, a.g_f32, col0, a.H));
+  return r;
+}
+
+// A granule of fp32 values in a thread's own part of shared memory: 16-byte pieces `stride` threads
+// apart, so neighbouring threads' pieces are neighbours.
+template <typename T>
+__device__ __forceinline__ void put_own(float4* p, int stride, const Gran<T>& v) {
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; i += 2)
+    p[(i / 2) * stride] = make_float4(v.p[i].x, v.p[i].y, v.p[i + 1].x, v.p[i + 1].y);
+}
+template <typename T>
+__device__ __forceinline__ Gran<T> get_own(const float4* p, int stride) {
+  Gran<T> r;
+#pragma unroll
+  for (int i = 0; i < Gran<T>::N; i += 2) {
+    const float4 q = p[(i / 2) * stride];
+    r.p[i] = make_float2(q.x, q.y);
+    r.p[i + 1] = make_float2(q.z, q.w);
+  }
+  return r;
+}
+
+// V columns starting at col0 of a row whose first element is row[0]; columns outside stay. A
+// granule across the row's edge goes element by element, by way of the thread's `edge` slot.
+template <typename T, bool ODD>
+__device__ __forceinline__ void store_granule(T* row, int col0, int H, const Gran<T>& g,
+                                              uint4* edge) {
+  uint4 w;
+  if constexpr (sizeof(T) == 4) {
+    w = make_uint4(__float_as_uint(g.p[0].x), __float_as_uint(g.p[0].y),
+                   __float_as_uint(g.p[1].x), __float_as_uint(g.p[1].y));
+  } else {
+    T* type = nullptr;
+    w = make_uint4(pack2(type, g.p[0].x, g.p[0].y), pack2(type, g.p[1].x, g.p[1].y),
+                   pack2(type, g.p[2].x, g.p[2].y), pack2(type, g.p[3].x, g.p[3].y));
+  }
+  if (!ODD || (col0 >= 0 && col0 + kV<T> <= H)) {
+    *reinterpret_cast<uint4*>(row + col0) = w;
+  } else {
+    *edge = w;
+    const int hi = H - col0 < kV<T> ? H - col0 : kV<T>;
+#pragma unroll 1
+    for (int j = col0 < 0 ? -col0 : 0; j < hi; ++j)
+      row[col0 + j] = reinterpret_cast<const T*>(edge)[j];
+  }
+}
+
+// Where a thread stands: its group, its rows and its shift.
+template <typename T, bool ODD>
+struct RowWalk {
+  int group, g, shift;
+  int64_t t;
+  __device__ RowWalk(const NormGeom& a, const RingGeom& r) {
+    group = threadIdx.x / r.G;
+    g = threadIdx.x - group * r.G;
+    const int cls = ODD ? blockIdx.x % r.P : 0;
+    shift = ODD ? static_cast<int>((static_cast<int64_t>(cls) * a.H) % kV<T>) : 0;
+    t = cls + static_cast<int64_t>(r.P) * ((blockIdx.x / r.P) * r.gpb + group);
+  }
+};
+
+// Copies the thread's granules of row t of one tensor into its ring slots.
+template <typename T, int VPT, bool ODD>
+__device__ __forceinline__ void fetch_row(uint32_t dst, const void* src, int64_t t, int H, int g,
+                                          int G, int shift) {
+  const T* row = static_cast<const T*>(src) + t * H - shift;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = g + i * G;
+    const int left = H + shift - v * kV<T>;  // elements from the granule's start to the row's end
+    if (left > 0)
+      cp_async16(dst + v * 16, row + v * kV<T>,
+                 ODD && left < kV<T> ? left * static_cast<int>(sizeof(T)) : 16);
+  }
+}
+
+template <typename T, int VPT, bool ODD>
+__global__ void __launch_bounds__(kRingThreads, 2)
+    k_norm_ring(const NormGeom a, const RingGeom r, const NormIn in, const NormOut out) {
+  constexpr int V = kV<T>;
+  extern __shared__ uint4 ring[];   // [stages][gpb][narr][slots], then wg and wq per thread
+  __shared__ float4 sums[4][kRingThreads / 64][4];  // [row parity and call site][group]
+  __shared__ uint4 edge[ODD ? kRingThreads : 1];
+  const RowWalk<T, ODD> w(a, r);
+  const int H = a.H;
+  const bool full = a.gate == FMOE_GATE_FULL;
+  const int per_row = r.narr * r.slots;
+  float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * per_row) +
+                threadIdx.x;
+  const int own_step = blockDim.x * (V / 4);
+  uint4* my_edge = &edge[ODD ? threadIdx.x : 0];
+  for (int i = threadIdx.x; i < static_cast<int>(sizeof(sums) / 16); i += blockDim.x)
+    (&sums[0][0][0])[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __syncthreads();
+  const int xa = in.f ? 1 : 0, ga = xa + 1;  // ring order: f, x, gate
+  auto slot = [&](int s) { return ring + (static_cast<size_t>(s) * r.gpb + w.group) * per_row; };
+  auto fetch = [&](int s, int64_t t) {
+    if (t < a.T) {
+      const uint32_t d = smem_u32(slot(s));
+      if (in.f) fetch_row<T, VPT, ODD>(d, in.f, t, H, w.g, r.G, w.shift);
+      fetch_row<T, VPT, ODD>(d + xa * r.slots * 16, in.x, t, H, w.g, r.G, w.shift);
+      if (full) fetch_row<T, VPT, ODD>(d + ga * r.slots * 16, in.g, t, H, w.g, r.G, w.shift);
+    }
+    cp_async_commit();
+  };
+  pdl_begin_in_order();
+  int64_t ahead = w.t;
+  for (int s = 0; s < r.stages; ++s, ahead += r.row_step) fetch(s, ahead);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = w.g + i * r.G;
+    if (v * V < H + w.shift) {
+      if (in.f) put_own(own + i * own_step, blockDim.x, branch_weight<T, ODD>(a, in, v * V - w.shift));
+      if (in.wq)
+        put_own(own + (VPT + i) * own_step, blockDim.x,
+                global_param<T, ODD>(in.wq, a.wq_f32, v * V - w.shift, H));
+    }
+  }
+  const float inv_h = 1.0f / H;
+  const int gr = r.G == 32 ? 0 : w.group;
+  const bool tok = a.gate == FMOE_GATE_TOKEN;
+  // a token's gate is loaded a row ahead
+  float g_next = tok && w.t < a.T ? load_scalar<T>(in.g, a.g_f32, w.t) : 1.0f;
+  int s = 0, flip = 0;
+  for (int64_t t = w.t; t < a.T;
+       t += r.row_step, s = s + 1 == r.stages ? 0 : s + 1, flip ^= 2) {
+    const float g_tok = g_next;
+    if (tok && t + r.row_step < a.T) g_next = load_scalar<T>(in.g, a.g_f32, t + r.row_step);
+    cp_async_wait(r.stages - 1);
+    const uint4* row = slot(s);
+    Gran<T> h[VPT];
+    float r1 = 1.0f;
+    if (in.f) {
+      float2 sq = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = w.g + i * r.G;
+        zero(h[i]);
+        if (v * V < H + w.shift) h[i] = read_granule<T>(row + v, ODD && v == 0 ? w.shift : 0);
+        dot(sq, h[i], h[i]);
+      }
+      if (in.wp) {
+        float sum[1] = {sq.x + sq.y};
+        group_sum<1>(sum, &sums[flip][gr][0].x, w.group, r.G);
+        r1 = rsqrtf(fmaf(sum[0], inv_h, a.eps));
+      }
+    }
+    const float rg = r1 * g_tok;
+    float2 sq = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = w.g + i * r.G;
+      if (v * V < H + w.shift) {
+        const int skip = ODD && v == 0 ? w.shift : 0;
+        const Gran<T> x = mul(read_granule<T>(row + xa * r.slots + v, skip), a.s);
+        if (in.f) {
+          h[i] = mul(h[i], rg);
+          if (full) h[i] = mul(h[i], read_granule<T>(row + ga * r.slots + v, skip));
+          h[i] = fma(h[i], get_own<T>(own + i * own_step, blockDim.x), x);
+        } else {
+          h[i] = x;
+        }
+        if (out.h)
+          store_granule<T, ODD>(static_cast<T*>(out.h) + t * H, v * V - w.shift, H, h[i], my_edge);
+        dot(sq, h[i], h[i]);
+      }
+    }
+    fetch(s, ahead);  // the row's tensors are in registers now
+    ahead += r.row_step;
+    if (!in.wq) {
+      if (out.stats && w.g == 0) out.stats[2 * t] = r1;
+      continue;
+    }
+    float sum[1] = {sq.x + sq.y};
+    group_sum<1>(sum, &sums[flip + 1][gr][0].x, w.group, r.G);
+    const float r2 = rsqrtf(fmaf(sum[0], inv_h, a.eps));
+    if (out.stats && w.g == 0) {
+      out.stats[2 * t] = r1;
+      out.stats[2 * t + 1] = r2;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = w.g + i * r.G;
+      // whole warps keep going for the e4m3 maximum: 128 columns are 128 / V neighbouring lanes
+      const bool live = v * V < H + w.shift;
+      const int col = v * V - w.shift;
+      if (live) h[i] = mul(mul(h[i], r2), get_own<T>(own + (VPT + i) * own_step, blockDim.x));
+      if constexpr (!ODD) {
+        if (out.q) {
+          float y[V];
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            y[2 * j] = live ? h[i].p[j].x : 0.0f;
+            y[2 * j + 1] = live ? h[i].p[j].y : 0.0f;
+          }
+          float amax = 0.0f;
+#pragma unroll
+          for (int j = 0; j < V; ++j) amax = fmaxf(amax, fabsf(y[j]));
+#pragma unroll
+          for (int o = kBlock / V / 2; o > 0; o >>= 1)
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          const float scale = __fdiv_rn(fmaxf(amax, 1e-30f), 448.0f);
+          if (live) {
+            store_e4m3<V>(out.q + t * H + col, y, scale);
+            if (col % kBlock == 0) out.q_scale[static_cast<int64_t>(col / kBlock) * a.T + t] = scale;
+          }
+          continue;
+        }
+      }
+      if (live) store_granule<T, ODD>(static_cast<T*>(out.y) + t * H, col, H, h[i], my_edge);
+    }
+  }
+  cp_async_wait(0);
+}
+
+// The gradients of a group's rows; this block's share of the sums over rows stays in registers and
+// goes to part at the end, the groups added in order.
+template <typename T, int VPT, bool ODD>
+__global__ void __launch_bounds__(kRingThreads, 1)
+    k_norm_back_ring(const NormGeom a, const RingGeom r, const NormIn in, const NormGrad d) {
+  constexpr int V = kV<T>;
+  extern __shared__ uint4 ring[];   // [stages][gpb][narr][slots], then wg and wq per thread
+  __shared__ float4 sums[2][kRingThreads / 64][3 * 4];  // [row parity][group][sum]
+  __shared__ uint4 edge[ODD ? kRingThreads : 1];
+  const RowWalk<T, ODD> w(a, r);
+  const int H = a.H;
+  const bool tok = a.gate == FMOE_GATE_TOKEN, full = a.gate == FMOE_GATE_FULL;
+  const int per_row = r.narr * r.slots;
+  // piece p of granule i of parameter q of this thread: own[((q * VPT + i) * (V / 4) + p) * blockDim]
+  float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * per_row) +
+                threadIdx.x;
+  const int own_step = blockDim.x * (V / 4);
+  uint4* my_edge = &edge[ODD ? threadIdx.x : 0];
+  for (int i = threadIdx.x; i < static_cast<int>(sizeof(sums) / 16); i += blockDim.x)
+    (&sums[0][0][0])[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __syncthreads();
+  const int gr = r.G == 32 ? 0 : w.group;
+  // ring order: x, f, da, dy, gate
+  const int fa = 1, da = fa + (in.f ? 1 : 0), ya = da + (d.da ? 1 : 0), ga = ya + (d.dy ? 1 : 0);
+  auto slot = [&](int s) { return ring + (static_cast<size_t>(s) * r.gpb + w.group) * per_row; };
+  // a row in two parts: what the first pass over it reads alone, and what both read
+  auto fetch_first = [&](int s, int64_t t) {
+    if (t < a.T) {
+      const uint32_t p = smem_u32(slot(s));
+      fetch_row<T, VPT, ODD>(p, in.x, t, H, w.g, r.G, w.shift);
+      if (d.da) fetch_row<T, VPT, ODD>(p + da * r.slots * 16, d.da, t, H, w.g, r.G, w.shift);
+      if (d.dy) fetch_row<T, VPT, ODD>(p + ya * r.slots * 16, d.dy, t, H, w.g, r.G, w.shift);
+    }
+  };
+  auto fetch_rest = [&](int s, int64_t t) {
+    if (t < a.T) {
+      const uint32_t p = smem_u32(slot(s));
+      if (in.f) fetch_row<T, VPT, ODD>(p + fa * r.slots * 16, in.f, t, H, w.g, r.G, w.shift);
+      if (full) fetch_row<T, VPT, ODD>(p + ga * r.slots * 16, in.g, t, H, w.g, r.G, w.shift);
+    }
+    cp_async_commit();
+  };
+  pdl_begin_in_order();
+  int64_t ahead = w.t;
+  for (int s = 0; s < r.stages; ++s, ahead += r.row_step) {
+    fetch_first(s, ahead);
+    fetch_rest(s, ahead);
+  }
+  Gran<T> C[VPT], Q[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = w.g + i * r.G;
+    zero(C[i]);
+    zero(Q[i]);
+    if (v * V < H + w.shift) {
+      if (in.f) put_own(own + i * own_step, blockDim.x, branch_weight<T, ODD>(a, in, v * V - w.shift));
+      if (d.dy)
+        put_own(own + (VPT + i) * own_step, blockDim.x,
+                global_param<T, ODD>(in.wq, a.wq_f32, v * V - w.shift, H));
+    }
+  }
+  const float inv_h = 1.0f / H;
+  // a row's statistics and token gate are loaded a row ahead
+  float r1_next = 1.0f, r2_next = 0.0f, g_next = 1.0f;
+  auto scalars = [&](int64_t t) {
+    if (t >= a.T) return;
+    if (in.wp) r1_next = __ldcg(d.stats + 2 * t);
+    if (d.dy) r2_next = __ldcg(d.stats + 2 * t + 1);
+    if (tok) g_next = load_scalar<T>(in.g, a.g_f32, t);
+  };
+  scalars(w.t);
+  int s = 0, flip = 0;
+  for (int64_t t = w.t; t < a.T;
+       t += r.row_step, s = s + 1 == r.stages ? 0 : s + 1, flip ^= 1) {
+    const float r1 = r1_next, r2 = r2_next, g_tok = g_next, rg = r1 * g_tok;
+    scalars(t + r.row_step);
+    cp_async_wait(r.stages - 1);
+    const uint4* row = slot(s);
+    Gran<T> h[VPT], tt[VPT];
+    float2 s0 = make_float2(0.0f, 0.0f), s1 = s0, s2 = s0;  // u h; m t; m h (no token gate in m)
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = w.g + i * r.G;
+      if (v * V < H + w.shift) {
+        const int skip = ODD && v == 0 ? w.shift : 0;
+        h[i] = mul(read_granule<T>(row + v, skip), a.s);
+        Gran<T> m;
+        zero(m);
+        if (in.f) {
+          m = mul(read_granule<T>(row + fa * r.slots + v, skip), get_own<T>(own + i * own_step, blockDim.x));
+          if (full) m = mul(m, read_granule<T>(row + ga * r.slots + v, skip));
+          h[i] = fma(m, rg, h[i]);
+        }
+        zero(tt[i]);
+        if (d.da) tt[i] = read_granule<T>(row + da * r.slots + v, skip);
+        if (d.dy) {
+          const Gran<T> dy = read_granule<T>(row + ya * r.slots + v, skip);
+          const Gran<T> b = get_own<T>(own + (VPT + i) * own_step, blockDim.x);
+          const Gran<T> p = mul(dy, h[i]);
+          dot(s0, p, b);
+          Q[i] = fma(p, r2, Q[i]);
+          tt[i] = fma(mul(dy, b), r2, tt[i]);
+        }
+        dot(s1, m, tt[i]);
+        dot(s2, m, h[i]);
+      }
+    }
+    fetch_first(s, ahead);  // x, da and dy are in registers now, as h and t
+    float sum[3] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y};
+    group_sum<3>(sum, &sums[flip][gr][0].x, w.group, r.G);
+    const float c = r2 * r2 * r2 * (sum[0] * inv_h);
+    const float gm = sum[1] - c * sum[2];
+    if (tok && d.dg_row && w.g == 0) {
+      if (a.g_f32)
+        static_cast<float*>(d.dg_row)[t] = r1 * gm;
+      else
+        from_f32(r1 * gm, static_cast<T*>(d.dg_row) + t);
+    }
+    const float k1 = in.wp ? r1 * r1 * r1 * (g_tok * gm * inv_h) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = w.g + i * r.G;
+      if (v * V < H + w.shift) {
+        const int skip = ODD && v == 0 ? w.shift : 0;
+        const int col = v * V - w.shift;
+        const Gran<T> dh = fma(h[i], -c, tt[i]);
+        if (d.dx)
+          store_granule<T, ODD>(static_cast<T*>(d.dx) + t * H, col, H,
+                                a.s == 1.0f ? dh : mul(dh, a.s), my_edge);
+        if (in.f) {
+          const Gran<T> f = read_granule<T>(row + fa * r.slots + v, skip);
+          const Gran<T> wg = get_own<T>(own + i * own_step, blockDim.x);
+          Gran<T> gd = mul(dh, rg);     // r1 * gate * dh, without a channel gate
+          if (full) {
+            if (d.dg_row)
+              store_granule<T, ODD>(static_cast<T*>(d.dg_row) + t * H, col, H,
+                                    mul(mul(f, wg), mul(dh, r1)), my_edge);
+            gd = mul(gd, read_granule<T>(row + ga * r.slots + v, skip));
+          }
+          C[i] = fma(gd, f, C[i]);
+          if (d.df)
+            store_granule<T, ODD>(static_cast<T*>(d.df) + t * H, col, H,
+                                  fma(f, -k1, mul(gd, wg)), my_edge);
+        }
+      }
+    }
+    fetch_rest(s, ahead);
+    ahead += r.row_step;
+  }
+  cp_async_wait(0);
+  // the ring is free: group by group the sums of a parameter's gradient meet there
+  const int64_t plane = static_cast<int64_t>(gridDim.x) * H;
+  float* acc = reinterpret_cast<float*>(ring);  // [slots * V]
+  for (int which = 0; which < 2; ++which) {
+    if (!(which == 0 ? d.want_wp || d.want_gc : d.want_wq)) continue;
+    float* dst = d.part + static_cast<int64_t>(blockIdx.x) * H;
+    for (int grp = 0; grp < r.gpb; ++grp) {
+      __syncthreads();
+      if (w.group != grp) continue;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = w.g + i * r.G;
+        if (v * V < H + w.shift) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float2 e = which == 0 ? C[i].p[j / 2] : Q[i].p[j / 2];
+            float x = j & 1 ? e.y : e.x;
+            if (grp > 0) x += acc[v * V + j];
+            const int col = v * V + j - w.shift;
+            if (grp + 1 < r.gpb) {
+              acc[v * V + j] = x;
+            } else if (!ODD || (col >= 0 && col < H)) {
+              if (which == 1) {
+                dst[plane + col] = x;
+              } else {
+                // C times the other factor of n: the channel gate for wp, wp for the gate
+                if (d.want_wp)
+                  dst[col] = a.gate == FMOE_GATE_CHANNEL ? x * load_scalar<T>(in.g, a.g_f32, col) : x;
+                if (d.want_gc)
+                  dst[2 * plane + col] = in.wp ? x * load_scalar<T>(in.wp, a.wp_f32, col) : x;
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
 // out[c] = sum over blocks of part[b][c], eight interleaved runs of blocks added in order.
 struct ColumnSums {
   void* out[3];
@@ -418,21 +1029,11 @@ NormGeom geom(const BlockNorm& p, int V) {
 }
 
 int back_blocks(const BlockNorm& p, int sms) {
-  int b = 2 * sms < kMaxNormBlocks ? 2 * sms : kMaxNormBlocks;
+  const int b = sms < kMaxNormBlocks ? sms : kMaxNormBlocks;
   return static_cast<int>(p.T < b ? p.T : b);
 }
 
-template <typename T, int V, int VPT, int MAXT>
-cudaError_t norm_one(const BlockNorm& p, int sms, cudaStream_t s) {
-  const NormGeom a = geom(p, V);
-  const NormIn in{p.f, p.x, p.wp, p.g, p.wq};
-  int threads = (a.nvec + VPT - 1) / VPT;
-  threads = (threads + 31) / 32 * 32;
-  if (!p.back) {
-    const NormOut out{p.h, p.y, static_cast<uint8_t*>(p.q), p.q_scale, p.stats};
-    return launch_pdl(k_block_norm<T, V, VPT, MAXT>, dim3(static_cast<unsigned>(p.T)),
-                      dim3(threads), 0, s, a, in, out);
-  }
+NormGrad grads(const BlockNorm& p) {
   NormGrad d{};
   d.da = p.da;
   d.dy = p.dy;
@@ -445,10 +1046,14 @@ cudaError_t norm_one(const BlockNorm& p, int sms, cudaStream_t s) {
   d.want_wp = p.dwp != nullptr;
   d.want_wq = p.dwq != nullptr;
   d.want_gc = channel && p.dg != nullptr;
-  const int blocks = back_blocks(p, sms);
-  cudaError_t e = launch_pdl(k_block_norm_back<T, V, VPT, MAXT>, dim3(blocks), dim3(threads), 0, s,
-                             a, in, d);
-  if (e != cudaSuccess || !(d.want_wp || d.want_wq || d.want_gc)) return e;
+  return d;
+}
+
+// The sums over the blocks' shares, if any are wanted.
+template <typename T>
+cudaError_t column_sums(const BlockNorm& p, const NormGeom& a, const NormGrad& d, int blocks,
+                        cudaStream_t s) {
+  if (!(d.want_wp || d.want_wq || d.want_gc)) return cudaSuccess;
   ColumnSums o{};
   o.out[0] = p.dwp;
   o.out[1] = p.dwq;
@@ -460,24 +1065,133 @@ cudaError_t norm_one(const BlockNorm& p, int sms, cudaStream_t s) {
                     static_cast<const float*>(p.part), blocks, p.H, o);
 }
 
+template <typename T, int V, int VPT, int MAXT>
+cudaError_t norm_direct(const BlockNorm& p, int sms, cudaStream_t s) {
+  if (V == 1 && p.q) return cudaErrorInvalidValue;  // the caller checks the alignment
+  const NormGeom a = geom(p, V);
+  const NormIn in{p.f, p.x, p.wp, p.g, p.wq};
+  int threads = (a.nvec + VPT - 1) / VPT;
+  threads = (threads + 31) / 32 * 32;
+  if (!p.back) {
+    const NormOut out{p.h, p.y, static_cast<uint8_t*>(p.q), p.q_scale, p.stats};
+    return launch_pdl(k_block_norm<T, V, VPT, MAXT>, dim3(static_cast<unsigned>(p.T)),
+                      dim3(threads), 0, s, a, in, out);
+  }
+  const NormGrad d = grads(p);
+  const int blocks = back_blocks(p, sms);
+  const cudaError_t e = launch_pdl(k_block_norm_back<T, V, VPT, MAXT>, dim3(blocks), dim3(threads),
+                                   0, s, a, in, d);
+  return e != cudaSuccess ? e : column_sums<T>(p, a, d, blocks, s);
+}
+
+// Dynamic shared memory of a block: two blocks per SM in the forward pass, whose barriers each
+// other's work hides, and one in the backward pass, which holds its sums over rows in registers.
+// Static shared memory (sums, edges) comes on top.
+constexpr int kNormSmem = 212 * 1024;
+
+// The ring's shape for rows of ng granules, or stages = 0 if not even one stage fits.
+template <typename T>
+RingGeom ring_geom(const BlockNorm& p, int vpt, int ng, int cps, size_t* smem) {
+  RingGeom r{};
+  r.G = ((ng + vpt - 1) / vpt + 31) / 32 * 32;
+  r.gpb = kRingThreads / r.G;  // at most 8 where groups need their named barriers (1 .. 8)
+  r.slots = r.G * vpt;
+  r.narr = 1 + (p.f ? 1 : 0) + (p.gate == FMOE_GATE_FULL ? 1 : 0) + (p.back && p.da ? 1 : 0) +
+           (p.back && p.dy ? 1 : 0);
+  // fewer rows at a time where the ring would not fit beside two parameters per thread; the
+  // backward pass has, at its end, the fp32 sums of a row where the ring was
+  for (; r.gpb >= 1; --r.gpb) {
+    const size_t row = static_cast<size_t>(r.slots) * kV<T> * 4;
+    const size_t stage = static_cast<size_t>(r.gpb) * r.narr * r.slots * 16;
+    for (r.stages = 3; r.stages >= 1; --r.stages) {
+      size_t bytes = r.stages * stage;
+      if (p.back && bytes < row) bytes = row;
+      bytes += 2 * r.gpb * row;
+      if (bytes <= static_cast<size_t>(kNormSmem / cps)) {
+        *smem = bytes;
+        return r;
+      }
+    }
+  }
+  r.stages = 0;
+  return r;
+}
+
+template <typename T, int VPT, bool ODD>
+cudaError_t norm_ring(const BlockNorm& p, RingGeom r, size_t smem, int cps, int sms,
+                      cudaStream_t s) {
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(k_norm_ring<T, VPT, ODD>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_norm_back_ring<T, VPT, ODD>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem);
+    if (e != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
+  const NormGeom a = geom(p, kV<T>);
+  const NormIn in{p.f, p.x, p.wp, p.g, p.wq};
+  r.P = 1;
+  if (ODD)
+    for (r.P = 2; (r.P * p.H) % kV<T> != 0;) r.P *= 2;
+  int limit = cps * sms;
+  if (p.back && limit > kMaxNormBlocks) limit = kMaxNormBlocks;
+  limit = limit / r.P * r.P;
+  r.row_step = limit * r.gpb;
+  // block b's first row is b % P + P * gpb * (b / P), increasing in b: those that have one
+  const int64_t per = static_cast<int64_t>(r.P) * r.gpb;
+  int64_t blocks = p.T / per * r.P + (p.T % per < r.P ? p.T % per : r.P);
+  if (blocks > limit) blocks = limit;
+  const dim3 grid(static_cast<unsigned>(blocks)), block(r.G * r.gpb);
+  if (!p.back) {
+    const NormOut out{p.h, p.y, static_cast<uint8_t*>(p.q), p.q_scale, p.stats};
+    return launch_pdl(k_norm_ring<T, VPT, ODD>, grid, block, smem, s, a, r, in, out);
+  }
+  const NormGrad d = grads(p);
+  const cudaError_t e =
+      launch_pdl(k_norm_back_ring<T, VPT, ODD>, grid, block, smem, s, a, r, in, d);
+  return e != cudaSuccess ? e : column_sums<T>(p, a, d, static_cast<int>(blocks), s);
+}
+
 template <typename T>
 cudaError_t norm_typed(const BlockNorm& p, int sms, cudaStream_t s) {
-  constexpr int V = 16 / static_cast<int>(sizeof(T));
-  bool vec = p.H % V == 0;
-  for (const void* q : {p.f, p.x, p.wp, p.g, p.wq, p.da, p.dy, static_cast<const void*>(p.h),
+  constexpr int V = kV<T>;
+  const bool odd = p.H % V != 0;
+  bool rows16 = true, params16 = true;  // on 16-byte boundaries
+  for (const void* q : {p.f, p.x, p.da, p.dy, static_cast<const void*>(p.h),
                         static_cast<const void*>(p.y), static_cast<const void*>(p.df),
-                        static_cast<const void*>(p.dx), static_cast<const void*>(p.dg)})
-    vec = vec && aligned16_or_null(q);
-  if (vec) {
-    const int nvec = p.H / V;
-    if (nvec <= 512) return norm_one<T, V, 1, 512>(p, sms, s);
-    if (nvec <= 1024) return norm_one<T, V, 2, 512>(p, sms, s);
-    if (nvec <= 2048) return norm_one<T, V, 4, 512>(p, sms, s);
-    return norm_one<T, V, 4, 1024>(p, sms, s);  // fp32 rows of more than 8192 columns
+                        static_cast<const void*>(p.dx)})
+    rows16 = rows16 && aligned16_or_null(q);
+  if (p.gate == FMOE_GATE_FULL) rows16 = rows16 && aligned16_or_null(p.g) && aligned16_or_null(p.dg);
+  for (const void* q : {p.wp, p.wq, p.g}) params16 = params16 && aligned16_or_null(q);
+  // parameters are staged in 16-byte pieces unless the rows are shifted
+  const bool ring = rows16 && (odd || params16) &&
+                    (p.gate != FMOE_GATE_FULL || p.g_dtype == p.dtype);
+  if (ring) {
+    // granules of a row at the largest shift
+    const int ng = (p.H + V - 1) / V + (odd ? 1 : 0);
+    if (ng <= 2048) {
+      const int vpt = ng <= 32 ? 1 : ng <= 2 * kRingThreads ? 2 : 4;
+      size_t smem = 0;
+      int cps = p.back ? 1 : 2;
+      RingGeom r = ring_geom<T>(p, vpt, ng, cps, &smem);
+      if (r.stages == 0 && cps == 2) r = ring_geom<T>(p, vpt, ng, cps = 1, &smem);
+      if (r.stages > 0) {
+#define RUN(VPT) (odd ? norm_ring<T, VPT, true>(p, r, smem, cps, sms, s) \
+                      : norm_ring<T, VPT, false>(p, r, smem, cps, sms, s))
+        return vpt == 1 ? RUN(1) : vpt == 2 ? RUN(2) : RUN(4);
+#undef RUN
+      }
+    }
   }
-  if (p.H <= 512) return norm_one<T, 1, 1, 512>(p, sms, s);
-  if (p.H <= 2048) return norm_one<T, 1, 4, 512>(p, sms, s);
-  return norm_one<T, 1, 16, 1024>(p, sms, s);
+  // 16384 columns are 2048 (16-bit) or 4096 (fp32) groups
+  if (rows16 && params16 && !odd) return norm_direct<T, V, 4, sizeof(T) == 2 ? 512 : 1024>(p, sms, s);
+  if (p.H <= 512) return norm_direct<T, 1, 1, 512>(p, sms, s);
+  if (p.H <= 2048) return norm_direct<T, 1, 4, 512>(p, sms, s);
+  return norm_direct<T, 1, 16, 1024>(p, sms, s);
 }
 
 }  // namespace

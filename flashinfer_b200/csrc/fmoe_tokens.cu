@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(256) k_sort_rows(const U* x, U* rows, const Ro
 
 // y[t] = sum_k w[t, k] * rows[pick_row[t, k]] (w null: 1), k ascending, in fp32.
 template <typename T, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
     k_unsort_rows(const T* rows, const float* w, T* y, const RowsArgs a) {
   pdl_begin_in_order();
   const int64_t t = static_cast<int64_t>(blockIdx.x / a.chunks) * blockDim.y + threadIdx.y;
