@@ -599,10 +599,10 @@ __device__ __forceinline__ Gran<T> get_own(const float4* p, int stride) {
   return r;
 }
 
-// V columns starting at col0 of a row whose first element is row[0]; columns outside stay. A
-// granule across the row's edge goes element by element, by way of the thread's `edge` slot.
+// V columns from column col0 on, whose place is p; columns outside the row stay. A granule across
+// the row's edge goes element by element, by way of the thread's `edge` slot.
 template <typename T, bool ODD>
-__device__ __forceinline__ void store_granule(T* row, int col0, int H, const Gran<T>& g,
+__device__ __forceinline__ void store_granule(T* p, int col0, int H, const Gran<T>& g,
                                               uint4* edge) {
   uint4 w;
   if constexpr (sizeof(T) == 4) {
@@ -614,113 +614,127 @@ __device__ __forceinline__ void store_granule(T* row, int col0, int H, const Gra
                    pack2(type, g.p[2].x, g.p[2].y), pack2(type, g.p[3].x, g.p[3].y));
   }
   if (!ODD || (col0 >= 0 && col0 + kV<T> <= H)) {
-    *reinterpret_cast<uint4*>(row + col0) = w;
+    *reinterpret_cast<uint4*>(p) = w;
   } else {
     *edge = w;
     const int hi = H - col0 < kV<T> ? H - col0 : kV<T>;
 #pragma unroll 1
     for (int j = col0 < 0 ? -col0 : 0; j < hi; ++j)
-      row[col0 + j] = reinterpret_cast<const T*>(edge)[j];
+      p[j] = reinterpret_cast<const T*>(edge)[j];
   }
 }
 
-// Where a thread stands: its group, its rows and its shift.
-template <typename T, bool ODD>
+// Where a thread stands: its group, its columns (granule i starts at col0 + i * step, of which the
+// first `live` lie in the row) and its rows (t, then every row_step).
+template <typename T, int VPT, bool ODD>
 struct RowWalk {
-  int group, g, shift;
+  int group, g, shift, col0, step, live;
   int64_t t;
   __device__ RowWalk(const NormGeom& a, const RingGeom& r) {
+    constexpr int V = kV<T>;
     group = threadIdx.x / r.G;
     g = threadIdx.x - group * r.G;
     const int cls = ODD ? blockIdx.x % r.P : 0;
-    shift = ODD ? static_cast<int>((static_cast<int64_t>(cls) * a.H) % kV<T>) : 0;
+    shift = ODD ? static_cast<int>((static_cast<int64_t>(cls) * a.H) % V) : 0;
+    col0 = g * V - shift;
+    step = r.G * V;
+    live = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) live += col0 + i * step < a.H ? 1 : 0;
     t = cls + static_cast<int64_t>(r.P) * ((blockIdx.x / r.P) * r.gpb + group);
   }
+  // elements of a neighbouring row at the start of granule i
+  __device__ int skip(int i) const { return ODD && i == 0 && col0 < 0 ? shift : 0; }
 };
 
-// Copies the thread's granules of row t of one tensor into its ring slots.
+// Copies the thread's granules of one tensor's row into its ring slots; off: the row's first
+// element plus col0.
 template <typename T, int VPT, bool ODD>
-__device__ __forceinline__ void fetch_row(uint32_t dst, const void* src, int64_t t, int H, int g,
-                                          int G, int shift) {
-  const T* row = static_cast<const T*>(src) + t * H - shift;
+__device__ __forceinline__ void fetch_row(uint32_t dst, const void* src, int64_t off, int H,
+                                          const RowWalk<T, VPT, ODD>& w, int G) {
+  const T* p = static_cast<const T*>(src) + off;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = g + i * G;
-    const int left = H + shift - v * kV<T>;  // elements from the granule's start to the row's end
-    if (left > 0)
-      cp_async16(dst + v * 16, row + v * kV<T>,
+    if (i < w.live) {
+      const int left = H - w.col0 - i * w.step;  // elements from the granule's start to the row's end
+      cp_async16(dst + i * G * 16, p + i * w.step,
                  ODD && left < kV<T> ? left * static_cast<int>(sizeof(T)) : 16);
+    }
   }
 }
 
-template <typename T, int VPT, bool ODD>
+// COMMON: a block output, no gate per element, and both results wanted (forward) or both gradients
+// given (backward); what is not common is decided at run time.
+template <typename T, int VPT, bool ODD, bool COMMON>
 __global__ void __launch_bounds__(kRingThreads, 2)
     k_norm_ring(const NormGeom a, const RingGeom r, const NormIn in, const NormOut out) {
   constexpr int V = kV<T>;
   extern __shared__ uint4 ring[];   // [stages][gpb][narr][slots], then wg and wq per thread
   __shared__ float4 sums[4][kRingThreads / 64][4];  // [row parity and call site][group]
   __shared__ uint4 edge[ODD ? kRingThreads : 1];
-  const RowWalk<T, ODD> w(a, r);
-  const int H = a.H;
-  const bool full = a.gate == FMOE_GATE_FULL;
-  const int per_row = r.narr * r.slots;
-  float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * per_row) +
+  const RowWalk<T, VPT, ODD> w(a, r);
+  const int H = a.H, G = r.G;
+  const bool has_f = COMMON || in.f != nullptr, has_wq = COMMON || in.wq != nullptr;
+  const bool has_h = COMMON || out.h != nullptr, full = !COMMON && a.gate == FMOE_GATE_FULL;
+  float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * r.narr * r.slots) +
                 threadIdx.x;
   const int own_step = blockDim.x * (V / 4);
   uint4* my_edge = &edge[ODD ? threadIdx.x : 0];
   for (int i = threadIdx.x; i < static_cast<int>(sizeof(sums) / 16); i += blockDim.x)
     (&sums[0][0][0])[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   __syncthreads();
-  const int xa = in.f ? 1 : 0, ga = xa + 1;  // ring order: f, x, gate
-  auto slot = [&](int s) { return ring + (static_cast<size_t>(s) * r.gpb + w.group) * per_row; };
-  auto fetch = [&](int s, int64_t t) {
+  // ring order: x, f, gate
+  const int arr = r.slots, stage = r.gpb * r.narr * arr;
+  const uint4* mine = ring + w.group * r.narr * arr + w.g;
+  const uint32_t mine32 = smem_u32(mine);
+  auto fetch = [&](int s, int64_t t, int64_t off) {
     if (t < a.T) {
-      const uint32_t d = smem_u32(slot(s));
-      if (in.f) fetch_row<T, VPT, ODD>(d, in.f, t, H, w.g, r.G, w.shift);
-      fetch_row<T, VPT, ODD>(d + xa * r.slots * 16, in.x, t, H, w.g, r.G, w.shift);
-      if (full) fetch_row<T, VPT, ODD>(d + ga * r.slots * 16, in.g, t, H, w.g, r.G, w.shift);
+      const uint32_t d = mine32 + s * stage * 16;
+      fetch_row<T, VPT, ODD>(d, in.x, off, H, w, G);
+      if (has_f) fetch_row<T, VPT, ODD>(d + arr * 16, in.f, off, H, w, G);
+      if (full) fetch_row<T, VPT, ODD>(d + 2 * arr * 16, in.g, off, H, w, G);
     }
     cp_async_commit();
   };
   pdl_begin_in_order();
-  int64_t ahead = w.t;
-  for (int s = 0; s < r.stages; ++s, ahead += r.row_step) fetch(s, ahead);
+  const int64_t off_step = static_cast<int64_t>(r.row_step) * H;
+  int64_t ahead = w.t, off = w.t * H + w.col0, off_ahead = off;
+  for (int s = 0; s < r.stages; ++s, ahead += r.row_step, off_ahead += off_step)
+    fetch(s, ahead, off_ahead);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = w.g + i * r.G;
-    if (v * V < H + w.shift) {
-      if (in.f) put_own(own + i * own_step, blockDim.x, branch_weight<T, ODD>(a, in, v * V - w.shift));
-      if (in.wq)
+    if (i < w.live) {
+      const int col = w.col0 + i * w.step;
+      if (has_f) put_own(own + i * own_step, blockDim.x, branch_weight<T, ODD>(a, in, col));
+      if (has_wq)
         put_own(own + (VPT + i) * own_step, blockDim.x,
-                global_param<T, ODD>(in.wq, a.wq_f32, v * V - w.shift, H));
+                global_param<T, ODD>(in.wq, a.wq_f32, col, H));
     }
   }
   const float inv_h = 1.0f / H;
-  const int gr = r.G == 32 ? 0 : w.group;
+  const int gr = G == 32 ? 0 : w.group;
   const bool tok = a.gate == FMOE_GATE_TOKEN;
   // a token's gate is loaded a row ahead
   float g_next = tok && w.t < a.T ? load_scalar<T>(in.g, a.g_f32, w.t) : 1.0f;
   int s = 0, flip = 0;
-  for (int64_t t = w.t; t < a.T;
-       t += r.row_step, s = s + 1 == r.stages ? 0 : s + 1, flip ^= 2) {
+  for (int64_t t = w.t; t < a.T; t += r.row_step, off += off_step, flip ^= 2) {
     const float g_tok = g_next;
     if (tok && t + r.row_step < a.T) g_next = load_scalar<T>(in.g, a.g_f32, t + r.row_step);
     cp_async_wait(r.stages - 1);
-    const uint4* row = slot(s);
+    const uint4* row = mine + s * stage;
     Gran<T> h[VPT];
     float r1 = 1.0f;
-    if (in.f) {
+    if (has_f) {
       float2 sq = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int v = w.g + i * r.G;
         zero(h[i]);
-        if (v * V < H + w.shift) h[i] = read_granule<T>(row + v, ODD && v == 0 ? w.shift : 0);
+        if (i < w.live) h[i] = read_granule<T>(row + arr + i * G, w.skip(i));
         dot(sq, h[i], h[i]);
       }
       if (in.wp) {
         float sum[1] = {sq.x + sq.y};
-        group_sum<1>(sum, &sums[flip][gr][0].x, w.group, r.G);
+        group_sum<1>(sum, &sums[flip][gr][0].x, w.group, G);
         r1 = rsqrtf(fmaf(sum[0], inv_h, a.eps));
       }
     }
@@ -728,30 +742,31 @@ __global__ void __launch_bounds__(kRingThreads, 2)
     float2 sq = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = w.g + i * r.G;
-      if (v * V < H + w.shift) {
-        const int skip = ODD && v == 0 ? w.shift : 0;
-        const Gran<T> x = mul(read_granule<T>(row + xa * r.slots + v, skip), a.s);
-        if (in.f) {
+      if (i < w.live) {
+        const Gran<T> x = mul(read_granule<T>(row + i * G, w.skip(i)), a.s);
+        if (has_f) {
           h[i] = mul(h[i], rg);
-          if (full) h[i] = mul(h[i], read_granule<T>(row + ga * r.slots + v, skip));
+          if (full) h[i] = mul(h[i], read_granule<T>(row + 2 * arr + i * G, w.skip(i)));
           h[i] = fma(h[i], get_own<T>(own + i * own_step, blockDim.x), x);
         } else {
           h[i] = x;
         }
-        if (out.h)
-          store_granule<T, ODD>(static_cast<T*>(out.h) + t * H, v * V - w.shift, H, h[i], my_edge);
+        if (has_h)
+          store_granule<T, ODD>(static_cast<T*>(out.h) + off + i * w.step, w.col0 + i * w.step, H,
+                                h[i], my_edge);
         dot(sq, h[i], h[i]);
       }
     }
-    fetch(s, ahead);  // the row's tensors are in registers now
+    fetch(s, ahead, off_ahead);  // the row's tensors are in registers now
     ahead += r.row_step;
-    if (!in.wq) {
+    off_ahead += off_step;
+    s = s + 1 == r.stages ? 0 : s + 1;
+    if (!has_wq) {
       if (out.stats && w.g == 0) out.stats[2 * t] = r1;
       continue;
     }
     float sum[1] = {sq.x + sq.y};
-    group_sum<1>(sum, &sums[flip + 1][gr][0].x, w.group, r.G);
+    group_sum<1>(sum, &sums[flip + 1][gr][0].x, w.group, G);
     const float r2 = rsqrtf(fmaf(sum[0], inv_h, a.eps));
     if (out.stats && w.g == 0) {
       out.stats[2 * t] = r1;
@@ -759,10 +774,9 @@ __global__ void __launch_bounds__(kRingThreads, 2)
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = w.g + i * r.G;
       // whole warps keep going for the e4m3 maximum: 128 columns are 128 / V neighbouring lanes
-      const bool live = v * V < H + w.shift;
-      const int col = v * V - w.shift;
+      const bool live = i < w.live;
+      const int col = w.col0 + i * w.step;
       if (live) h[i] = mul(mul(h[i], r2), get_own<T>(own + (VPT + i) * own_step, blockDim.x));
       if constexpr (!ODD) {
         if (out.q) {
@@ -780,13 +794,14 @@ __global__ void __launch_bounds__(kRingThreads, 2)
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
           const float scale = __fdiv_rn(fmaxf(amax, 1e-30f), 448.0f);
           if (live) {
-            store_e4m3<V>(out.q + t * H + col, y, scale);
+            store_e4m3<V>(out.q + off + i * w.step, y, scale);
             if (col % kBlock == 0) out.q_scale[static_cast<int64_t>(col / kBlock) * a.T + t] = scale;
           }
           continue;
         }
       }
-      if (live) store_granule<T, ODD>(static_cast<T*>(out.y) + t * H, col, H, h[i], my_edge);
+      if (live)
+        store_granule<T, ODD>(static_cast<T*>(out.y) + off + i * w.step, col, H, h[i], my_edge);
     }
   }
   cp_async_wait(0);
@@ -794,63 +809,68 @@ __global__ void __launch_bounds__(kRingThreads, 2)
 
 // The gradients of a group's rows; this block's share of the sums over rows stays in registers and
 // goes to part at the end, the groups added in order.
-template <typename T, int VPT, bool ODD>
+template <typename T, int VPT, bool ODD, bool COMMON>
 __global__ void __launch_bounds__(kRingThreads, 1)
     k_norm_back_ring(const NormGeom a, const RingGeom r, const NormIn in, const NormGrad d) {
   constexpr int V = kV<T>;
   extern __shared__ uint4 ring[];   // [stages][gpb][narr][slots], then wg and wq per thread
   __shared__ float4 sums[2][kRingThreads / 64][3 * 4];  // [row parity][group][sum]
   __shared__ uint4 edge[ODD ? kRingThreads : 1];
-  const RowWalk<T, ODD> w(a, r);
-  const int H = a.H;
-  const bool tok = a.gate == FMOE_GATE_TOKEN, full = a.gate == FMOE_GATE_FULL;
-  const int per_row = r.narr * r.slots;
+  const RowWalk<T, VPT, ODD> w(a, r);
+  const int H = a.H, G = r.G;
+  const bool has_f = COMMON || in.f != nullptr;
+  const bool has_da = COMMON || d.da != nullptr, has_dy = COMMON || d.dy != nullptr;
+  const bool tok = a.gate == FMOE_GATE_TOKEN, full = !COMMON && a.gate == FMOE_GATE_FULL;
   // piece p of granule i of parameter q of this thread: own[((q * VPT + i) * (V / 4) + p) * blockDim]
-  float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * per_row) +
+  float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * r.narr * r.slots) +
                 threadIdx.x;
   const int own_step = blockDim.x * (V / 4);
   uint4* my_edge = &edge[ODD ? threadIdx.x : 0];
   for (int i = threadIdx.x; i < static_cast<int>(sizeof(sums) / 16); i += blockDim.x)
     (&sums[0][0][0])[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   __syncthreads();
-  const int gr = r.G == 32 ? 0 : w.group;
-  // ring order: x, f, da, dy, gate
-  const int fa = 1, da = fa + (in.f ? 1 : 0), ya = da + (d.da ? 1 : 0), ga = ya + (d.dy ? 1 : 0);
-  auto slot = [&](int s) { return ring + (static_cast<size_t>(s) * r.gpb + w.group) * per_row; };
+  const int gr = G == 32 ? 0 : w.group;
+  // ring order: x, f, da, dy, gate, without those that are not there
+  const int arr = r.slots, stage = r.gpb * r.narr * arr;
+  const int fa = arr, da = fa + (has_f ? arr : 0), ya = da + (has_da ? arr : 0);
+  const int ga = ya + (has_dy ? arr : 0);
+  const uint4* mine = ring + w.group * r.narr * arr + w.g;
+  const uint32_t mine32 = smem_u32(mine);
   // a row in two parts: what the first pass over it reads alone, and what both read
-  auto fetch_first = [&](int s, int64_t t) {
+  auto fetch_first = [&](int s, int64_t t, int64_t off) {
     if (t < a.T) {
-      const uint32_t p = smem_u32(slot(s));
-      fetch_row<T, VPT, ODD>(p, in.x, t, H, w.g, r.G, w.shift);
-      if (d.da) fetch_row<T, VPT, ODD>(p + da * r.slots * 16, d.da, t, H, w.g, r.G, w.shift);
-      if (d.dy) fetch_row<T, VPT, ODD>(p + ya * r.slots * 16, d.dy, t, H, w.g, r.G, w.shift);
+      const uint32_t p = mine32 + s * stage * 16;
+      fetch_row<T, VPT, ODD>(p, in.x, off, H, w, G);
+      if (has_da) fetch_row<T, VPT, ODD>(p + da * 16, d.da, off, H, w, G);
+      if (has_dy) fetch_row<T, VPT, ODD>(p + ya * 16, d.dy, off, H, w, G);
     }
   };
-  auto fetch_rest = [&](int s, int64_t t) {
+  auto fetch_rest = [&](int s, int64_t t, int64_t off) {
     if (t < a.T) {
-      const uint32_t p = smem_u32(slot(s));
-      if (in.f) fetch_row<T, VPT, ODD>(p + fa * r.slots * 16, in.f, t, H, w.g, r.G, w.shift);
-      if (full) fetch_row<T, VPT, ODD>(p + ga * r.slots * 16, in.g, t, H, w.g, r.G, w.shift);
+      const uint32_t p = mine32 + s * stage * 16;
+      if (has_f) fetch_row<T, VPT, ODD>(p + fa * 16, in.f, off, H, w, G);
+      if (full) fetch_row<T, VPT, ODD>(p + ga * 16, in.g, off, H, w, G);
     }
     cp_async_commit();
   };
   pdl_begin_in_order();
-  int64_t ahead = w.t;
-  for (int s = 0; s < r.stages; ++s, ahead += r.row_step) {
-    fetch_first(s, ahead);
-    fetch_rest(s, ahead);
+  const int64_t off_step = static_cast<int64_t>(r.row_step) * H;
+  int64_t ahead = w.t, off = w.t * H + w.col0, off_ahead = off;
+  for (int s = 0; s < r.stages; ++s, ahead += r.row_step, off_ahead += off_step) {
+    fetch_first(s, ahead, off_ahead);
+    fetch_rest(s, ahead, off_ahead);
   }
   Gran<T> C[VPT], Q[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = w.g + i * r.G;
     zero(C[i]);
     zero(Q[i]);
-    if (v * V < H + w.shift) {
-      if (in.f) put_own(own + i * own_step, blockDim.x, branch_weight<T, ODD>(a, in, v * V - w.shift));
-      if (d.dy)
+    if (i < w.live) {
+      const int col = w.col0 + i * w.step;
+      if (has_f) put_own(own + i * own_step, blockDim.x, branch_weight<T, ODD>(a, in, col));
+      if (has_dy)
         put_own(own + (VPT + i) * own_step, blockDim.x,
-                global_param<T, ODD>(in.wq, a.wq_f32, v * V - w.shift, H));
+                global_param<T, ODD>(in.wq, a.wq_f32, col, H));
     }
   }
   const float inv_h = 1.0f / H;
@@ -859,36 +879,34 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   auto scalars = [&](int64_t t) {
     if (t >= a.T) return;
     if (in.wp) r1_next = __ldcg(d.stats + 2 * t);
-    if (d.dy) r2_next = __ldcg(d.stats + 2 * t + 1);
+    if (has_dy) r2_next = __ldcg(d.stats + 2 * t + 1);
     if (tok) g_next = load_scalar<T>(in.g, a.g_f32, t);
   };
   scalars(w.t);
   int s = 0, flip = 0;
-  for (int64_t t = w.t; t < a.T;
-       t += r.row_step, s = s + 1 == r.stages ? 0 : s + 1, flip ^= 1) {
+  for (int64_t t = w.t; t < a.T; t += r.row_step, off += off_step, flip ^= 1) {
     const float r1 = r1_next, r2 = r2_next, g_tok = g_next, rg = r1 * g_tok;
     scalars(t + r.row_step);
     cp_async_wait(r.stages - 1);
-    const uint4* row = slot(s);
+    const uint4* row = mine + s * stage;
     Gran<T> h[VPT], tt[VPT];
     float2 s0 = make_float2(0.0f, 0.0f), s1 = s0, s2 = s0;  // u h; m t; m h (no token gate in m)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = w.g + i * r.G;
-      if (v * V < H + w.shift) {
-        const int skip = ODD && v == 0 ? w.shift : 0;
-        h[i] = mul(read_granule<T>(row + v, skip), a.s);
+      if (i < w.live) {
+        h[i] = mul(read_granule<T>(row + i * G, w.skip(i)), a.s);
         Gran<T> m;
         zero(m);
-        if (in.f) {
-          m = mul(read_granule<T>(row + fa * r.slots + v, skip), get_own<T>(own + i * own_step, blockDim.x));
-          if (full) m = mul(m, read_granule<T>(row + ga * r.slots + v, skip));
+        if (has_f) {
+          m = mul(read_granule<T>(row + fa + i * G, w.skip(i)),
+                  get_own<T>(own + i * own_step, blockDim.x));
+          if (full) m = mul(m, read_granule<T>(row + ga + i * G, w.skip(i)));
           h[i] = fma(m, rg, h[i]);
         }
         zero(tt[i]);
-        if (d.da) tt[i] = read_granule<T>(row + da * r.slots + v, skip);
-        if (d.dy) {
-          const Gran<T> dy = read_granule<T>(row + ya * r.slots + v, skip);
+        if (has_da) tt[i] = read_granule<T>(row + da + i * G, w.skip(i));
+        if (has_dy) {
+          const Gran<T> dy = read_granule<T>(row + ya + i * G, w.skip(i));
           const Gran<T> b = get_own<T>(own + (VPT + i) * own_step, blockDim.x);
           const Gran<T> p = mul(dy, h[i]);
           dot(s0, p, b);
@@ -899,9 +917,9 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         dot(s2, m, h[i]);
       }
     }
-    fetch_first(s, ahead);  // x, da and dy are in registers now, as h and t
+    fetch_first(s, ahead, off_ahead);  // x, da and dy are in registers now, as h and t
     float sum[3] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y};
-    group_sum<3>(sum, &sums[flip][gr][0].x, w.group, r.G);
+    group_sum<3>(sum, &sums[flip][gr][0].x, w.group, G);
     const float c = r2 * r2 * r2 * (sum[0] * inv_h);
     const float gm = sum[1] - c * sum[2];
     if (tok && d.dg_row && w.g == 0) {
@@ -913,78 +931,71 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     const float k1 = in.wp ? r1 * r1 * r1 * (g_tok * gm * inv_h) : 0.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = w.g + i * r.G;
-      if (v * V < H + w.shift) {
-        const int skip = ODD && v == 0 ? w.shift : 0;
-        const int col = v * V - w.shift;
+      if (i < w.live) {
+        const int col = w.col0 + i * w.step;
+        const int64_t at = off + i * w.step;
         const Gran<T> dh = fma(h[i], -c, tt[i]);
         if (d.dx)
-          store_granule<T, ODD>(static_cast<T*>(d.dx) + t * H, col, H,
+          store_granule<T, ODD>(static_cast<T*>(d.dx) + at, col, H,
                                 a.s == 1.0f ? dh : mul(dh, a.s), my_edge);
-        if (in.f) {
-          const Gran<T> f = read_granule<T>(row + fa * r.slots + v, skip);
+        if (has_f) {
+          const Gran<T> f = read_granule<T>(row + fa + i * G, w.skip(i));
           const Gran<T> wg = get_own<T>(own + i * own_step, blockDim.x);
           Gran<T> gd = mul(dh, rg);     // r1 * gate * dh, without a channel gate
           if (full) {
             if (d.dg_row)
-              store_granule<T, ODD>(static_cast<T*>(d.dg_row) + t * H, col, H,
+              store_granule<T, ODD>(static_cast<T*>(d.dg_row) + at, col, H,
                                     mul(mul(f, wg), mul(dh, r1)), my_edge);
-            gd = mul(gd, read_granule<T>(row + ga * r.slots + v, skip));
+            gd = mul(gd, read_granule<T>(row + ga + i * G, w.skip(i)));
           }
           C[i] = fma(gd, f, C[i]);
           if (d.df)
-            store_granule<T, ODD>(static_cast<T*>(d.df) + t * H, col, H,
-                                  fma(f, -k1, mul(gd, wg)), my_edge);
+            store_granule<T, ODD>(static_cast<T*>(d.df) + at, col, H, fma(f, -k1, mul(gd, wg)),
+                                  my_edge);
         }
       }
     }
-    fetch_rest(s, ahead);
+    fetch_rest(s, ahead, off_ahead);
     ahead += r.row_step;
+    off_ahead += off_step;
+    s = s + 1 == r.stages ? 0 : s + 1;
   }
   cp_async_wait(0);
-  // the ring is free: group by group the sums of a parameter's gradient meet there
+  // the ring is free: the groups' sums meet there, and are added in order
   const int64_t plane = static_cast<int64_t>(gridDim.x) * H;
-  float* acc = reinterpret_cast<float*>(ring);  // [slots * V]
+  float* acc = reinterpret_cast<float*>(ring);  // [gpb][slots * V]
   for (int which = 0; which < 2; ++which) {
     if (!(which == 0 ? d.want_wp || d.want_gc : d.want_wq)) continue;
-    float* dst = d.part + static_cast<int64_t>(blockIdx.x) * H;
-    for (int grp = 0; grp < r.gpb; ++grp) {
-      __syncthreads();
-      if (w.group != grp) continue;
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = w.g + i * r.G;
-        if (v * V < H + w.shift) {
+    for (int i = 0; i < VPT; ++i) {
+      float4* dst = reinterpret_cast<float4*>(acc) + (w.group * arr + w.g + i * G) * (V / 4);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float2 e = which == 0 ? C[i].p[j / 2] : Q[i].p[j / 2];
-            float x = j & 1 ? e.y : e.x;
-            if (grp > 0) x += acc[v * V + j];
-            const int col = v * V + j - w.shift;
-            if (grp + 1 < r.gpb) {
-              acc[v * V + j] = x;
-            } else if (!ODD || (col >= 0 && col < H)) {
-              if (which == 1) {
-                dst[plane + col] = x;
-              } else {
-                // C times the other factor of n: the channel gate for wp, wp for the gate
-                if (d.want_wp)
-                  dst[col] = a.gate == FMOE_GATE_CHANNEL ? x * load_scalar<T>(in.g, a.g_f32, col) : x;
-                if (d.want_gc)
-                  dst[2 * plane + col] = in.wp ? x * load_scalar<T>(in.wp, a.wp_f32, col) : x;
-              }
-            }
-          }
-        }
+      for (int j = 0; j < V / 2; j += 2) {
+        const float2 x = which == 0 ? C[i].p[j] : Q[i].p[j];
+        const float2 y = which == 0 ? C[i].p[j + 1] : Q[i].p[j + 1];
+        dst[j / 2] = make_float4(x.x, x.y, y.x, y.y);
       }
+    }
+    __syncthreads();
+    float* dst = d.part + which * plane + static_cast<int64_t>(blockIdx.x) * H;
+    for (int c = threadIdx.x; c < H; c += blockDim.x) {
+      float x = acc[c + w.shift];
+      for (int grp = 1; grp < r.gpb; ++grp) x += acc[grp * arr * V + c + w.shift];
+      dst[c] = x;
     }
   }
 }
 
-// out[c] = sum over blocks of part[b][c], eight interleaved runs of blocks added in order.
+// Sums over the blocks' shares, eight interleaved runs of blocks added in order. Plane 0 holds the
+// sums behind the post norm's weight and a channel gate: C of the ring kernels (dwp = g * C, dg =
+// wp * C), plane 1 dwq. The direct kernels store dwp, dwq and dg as they are, in three planes.
 struct ColumnSums {
-  void* out[3];
+  void* out[3];          // dwp, dwq, dg
   int f32[3];
+  const void* factor[3]; // what the plane is multiplied with, or null
+  int factor_f32[3];
+  int plane[3];
 };
 
 template <typename T>
@@ -995,16 +1006,23 @@ __global__ void __launch_bounds__(256)
   const int which = blockIdx.y;
   if (!o.out[which]) return;
   const int c = blockIdx.x * 32 + threadIdx.x;
-  const float* p = part + static_cast<int64_t>(which) * blocks * H;
+  const float* p = part + static_cast<int64_t>(o.plane[which]) * blocks * H;
   float sum = 0.0f;
   if (c < H) {
-#pragma unroll 4
-    for (int b = threadIdx.y; b < blocks; b += 8) sum += __ldcg(p + static_cast<int64_t>(b) * H + c);
+    for (int b0 = threadIdx.y; b0 < blocks; b0 += 64) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = b0 + 8 * i < blocks ? __ldcg(p + static_cast<int64_t>(b0 + 8 * i) * H + c) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += v[i];
+    }
   }
   buf[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
   if (threadIdx.y == 0 && c < H) {
     for (int i = 1; i < 8; ++i) sum += buf[i][threadIdx.x];
+    if (o.factor[which]) sum *= load_scalar<T>(o.factor[which], o.factor_f32[which], c);
     if (o.f32[which])
       static_cast<float*>(o.out[which])[c] = sum;
     else
@@ -1052,7 +1070,7 @@ NormGrad grads(const BlockNorm& p) {
 // The sums over the blocks' shares, if any are wanted.
 template <typename T>
 cudaError_t column_sums(const BlockNorm& p, const NormGeom& a, const NormGrad& d, int blocks,
-                        cudaStream_t s) {
+                        bool ring, cudaStream_t s) {
   if (!(d.want_wp || d.want_wq || d.want_gc)) return cudaSuccess;
   ColumnSums o{};
   o.out[0] = p.dwp;
@@ -1061,6 +1079,14 @@ cudaError_t column_sums(const BlockNorm& p, const NormGeom& a, const NormGrad& d
   o.f32[0] = a.wp_f32;
   o.f32[1] = a.wq_f32;
   o.f32[2] = a.g_f32;
+  o.plane[1] = 1;
+  o.plane[2] = ring ? 0 : 2;
+  if (ring && p.gate == FMOE_GATE_CHANNEL) {
+    o.factor[0] = p.g;
+    o.factor_f32[0] = a.g_f32;
+    o.factor[2] = p.wp;
+    o.factor_f32[2] = a.wp_f32;
+  }
   return launch_pdl(k_column_sums<T>, dim3((p.H + 31) / 32, 3), dim3(32, 8), 0, s,
                     static_cast<const float*>(p.part), blocks, p.H, o);
 }
@@ -1081,7 +1107,7 @@ cudaError_t norm_direct(const BlockNorm& p, int sms, cudaStream_t s) {
   const int blocks = back_blocks(p, sms);
   const cudaError_t e = launch_pdl(k_block_norm_back<T, V, VPT, MAXT>, dim3(blocks), dim3(threads),
                                    0, s, a, in, d);
-  return e != cudaSuccess ? e : column_sums<T>(p, a, d, blocks, s);
+  return e != cudaSuccess ? e : column_sums<T>(p, a, d, blocks, false, s);
 }
 
 // Dynamic shared memory of a block: two blocks per SM in the forward pass, whose barriers each
@@ -1105,7 +1131,7 @@ RingGeom ring_geom(const BlockNorm& p, int vpt, int ng, int cps, size_t* smem) {
     const size_t stage = static_cast<size_t>(r.gpb) * r.narr * r.slots * 16;
     for (r.stages = 3; r.stages >= 1; --r.stages) {
       size_t bytes = r.stages * stage;
-      if (p.back && bytes < row) bytes = row;
+      if (p.back && bytes < r.gpb * row) bytes = r.gpb * row;
       bytes += 2 * r.gpb * row;
       if (bytes <= static_cast<size_t>(kNormSmem / cps)) {
         *smem = bytes;
@@ -1117,17 +1143,17 @@ RingGeom ring_geom(const BlockNorm& p, int vpt, int ng, int cps, size_t* smem) {
   return r;
 }
 
-template <typename T, int VPT, bool ODD>
+template <typename T, int VPT, bool ODD, bool COMMON>
 cudaError_t norm_ring(const BlockNorm& p, RingGeom r, size_t smem, int cps, int sms,
                       cudaStream_t s) {
   static std::atomic<bool> configured[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(k_norm_ring<T, VPT, ODD>,
+    cudaError_t e = cudaFuncSetAttribute(k_norm_ring<T, VPT, ODD, COMMON>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k_norm_back_ring<T, VPT, ODD>,
+      e = cudaFuncSetAttribute(k_norm_back_ring<T, VPT, ODD, COMMON>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem);
     if (e != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
@@ -1148,12 +1174,12 @@ cudaError_t norm_ring(const BlockNorm& p, RingGeom r, size_t smem, int cps, int 
   const dim3 grid(static_cast<unsigned>(blocks)), block(r.G * r.gpb);
   if (!p.back) {
     const NormOut out{p.h, p.y, static_cast<uint8_t*>(p.q), p.q_scale, p.stats};
-    return launch_pdl(k_norm_ring<T, VPT, ODD>, grid, block, smem, s, a, r, in, out);
+    return launch_pdl(k_norm_ring<T, VPT, ODD, COMMON>, grid, block, smem, s, a, r, in, out);
   }
   const NormGrad d = grads(p);
   const cudaError_t e =
-      launch_pdl(k_norm_back_ring<T, VPT, ODD>, grid, block, smem, s, a, r, in, d);
-  return e != cudaSuccess ? e : column_sums<T>(p, a, d, static_cast<int>(blocks), s);
+      launch_pdl(k_norm_back_ring<T, VPT, ODD, COMMON>, grid, block, smem, s, a, r, in, d);
+  return e != cudaSuccess ? e : column_sums<T>(p, a, d, static_cast<int>(blocks), true, s);
 }
 
 template <typename T>
@@ -1180,9 +1206,14 @@ cudaError_t norm_typed(const BlockNorm& p, int sms, cudaStream_t s) {
       RingGeom r = ring_geom<T>(p, vpt, ng, cps, &smem);
       if (r.stages == 0 && cps == 2) r = ring_geom<T>(p, vpt, ng, cps = 1, &smem);
       if (r.stages > 0) {
-#define RUN(VPT) (odd ? norm_ring<T, VPT, true>(p, r, smem, cps, sms, s) \
-                      : norm_ring<T, VPT, false>(p, r, smem, cps, sms, s))
-        return vpt == 1 ? RUN(1) : vpt == 2 ? RUN(2) : RUN(4);
+        // rows of more than 8192 16-bit columns do not have a variant of their own for the common case
+        const bool common = vpt < 4 && p.f && p.gate != FMOE_GATE_FULL &&
+                            (p.back ? p.da && p.dy : p.h && p.wq);
+#define RUN(VPT, COMMON)                                                  \
+  (odd ? norm_ring<T, VPT, true, COMMON>(p, r, smem, cps, sms, s)         \
+       : norm_ring<T, VPT, false, COMMON>(p, r, smem, cps, sms, s))
+        if (common) return vpt == 1 ? RUN(1, true) : RUN(2, true);
+        return vpt == 1 ? RUN(1, false) : vpt == 2 ? RUN(2, false) : RUN(4, false);
 #undef RUN
       }
     }
