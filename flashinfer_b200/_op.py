@@ -1,48 +1,78 @@
-"""What the operators around the experts share: tensor checks and the call into the library."""
+"""What the operators around the experts share: tensor checks and the call into the library.
+
+The calls of one decode step take a few microseconds on the device, so the checks test everything
+in one expression per tensor and look for the reason only when it fails.
+"""
 from __future__ import annotations
 
 from typing import Optional
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
 
 from . import _lib
 
 DTYPE_TAG = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
              torch.float16: _lib.DTYPE_F16}
+I8 = (torch.int8,)
+I32 = (torch.int32,)
+F32 = (torch.float32,)
+FLOATS = tuple(DTYPE_TAG)
 
 
-def need(t, name: str, device: Optional[torch.device], shape=None, dtypes=None) -> None:
-    """A contiguous CUDA tensor (on ``device`` if given) of one of ``dtypes`` and of ``shape``."""
+def _refuse(t, name: str, index: Optional[int], shape, dtypes) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
     if dtypes is not None and t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if index is not None and t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    raise ValueError(f"{name} must be contiguous")
+
+
+def first(t, name: str, dtypes, dim: int) -> int:
+    """The device index of a call's first tensor: CUDA, contiguous, ``dim`` axes, of ``dtypes``."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dim() != dim:
+        raise ValueError(f"{name} must be a tensor of {dim} axes, got shape {tuple(t.shape)}")
+    if not (t.is_cuda and t.dtype in dtypes and t.is_contiguous()):
+        _refuse(t, name, None, None, dtypes)
+    return t.get_device()
+
+
+def need(t, name: str, index: int, shape, dtypes) -> None:
+    """A contiguous tensor on CUDA device ``index``, of ``shape`` and one of ``dtypes`` (None: any)."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == index
+            and (shape is None or t.shape == shape) and (dtypes is None or t.dtype in dtypes)
+            and t.is_contiguous()):
+        _refuse(t, name, index, shape, dtypes)
 
 
 def ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def call(name: str, device: torch.device, *args) -> None:
-    """One library call on ``device`` and its current stream; raises on an error code."""
+def call(name: str, index: int, *args) -> None:
+    """One library call on CUDA device ``index`` and its current stream; raises on an error code."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
 
 def recording(*tensors) -> bool:
     """Whether autograd records a call on these tensors (None among them allowed)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False

@@ -12,13 +12,11 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._op import DTYPE_TAG, call, need, ptr
+from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, call, first, need, ptr
 
-_I8 = (torch.int8,)
-_F32 = (torch.float32,)
+_HALVES = (torch.bfloat16, torch.float16)
 
 
-@torch.no_grad()
 def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """bf16 or fp16 rows [R, K] -> (int8 [R, K], fp32 scales [R]), symmetric per row.
 
@@ -27,13 +25,13 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     ``amax / 127``. A row with a NaN or an infinity gets a NaN or infinite scale: its products are
     NaN. Weights [N, K] are quantised per output channel by the same call.
     """
-    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError("x must be a tensor of shape [R, K]")
-    need(x, "x", None, None, (torch.bfloat16, torch.float16))
+    index = first(x, "x", _HALVES, 2)
     R, K = x.shape
-    q = torch.empty((R, K), dtype=torch.int8, device=x.device)
-    scale = torch.empty(R, dtype=torch.float32, device=x.device)
-    call("fmoe_quantize_int8", x.device, x.data_ptr(), DTYPE_TAG[x.dtype], R, K, q.data_ptr(),
+    if K < 1:
+        raise ValueError("x needs at least one column")
+    q = x.new_empty((R, K), dtype=torch.int8)
+    scale = x.new_empty(R, dtype=torch.float32)
+    call("fmoe_quantize_int8", index, x.data_ptr(), DTYPE_TAG[x.dtype], R, K, q.data_ptr(),
          scale.data_ptr())
     return q, scale
 
@@ -43,16 +41,15 @@ def _check_depth(K: int) -> None:
         raise ValueError(f"the depth K must be a multiple of 16 from 16 to 131056, got {K}")
 
 
-def _output(output, out_dtype, device, shape):
+def _output(output, out_dtype, a, index, shape):
     if output is None:
         if out_dtype not in DTYPE_TAG:
             raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-        return torch.empty(shape, dtype=out_dtype, device=device)
-    need(output, "output", device, shape, tuple(DTYPE_TAG))
+        return a.new_empty(shape, dtype=out_dtype)
+    need(output, "output", index, shape, FLOATS)
     return output
 
 
-@torch.no_grad()
 def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, *, out_dtype: torch.dtype = torch.bfloat16,
                 output: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -62,25 +59,23 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
     multiple of 16. The result is [M, N] of ``out_dtype`` (bf16, fp16 or fp32), or is written to
     ``output`` in that tensor's type.
     """
-    need(a, "a", None, None, _I8)
-    need(b, "b", a.device, None, _I8)
-    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1] or b.shape[0] < 1:
+    index = first(a, "a", I8, 2)
+    need(b, "b", index, None, I8)
+    if b.dim() != 2 or a.shape[1] != b.shape[1] or b.shape[0] < 1:
         raise ValueError(f"a [M, K] and b [N, K] do not fit: {tuple(a.shape)}, {tuple(b.shape)}")
     M, K = a.shape
     N = b.shape[0]
     _check_depth(K)
-    device = a.device
-    need(a_scale, "a_scale", device, (M,), _F32)
-    need(b_scale, "b_scale", device, (N,), _F32)
+    need(a_scale, "a_scale", index, (M,), F32)
+    need(b_scale, "b_scale", index, (N,), F32)
     if bias is not None:
-        need(bias, "bias", device, (N,), _F32)
-    output = _output(output, out_dtype, device, (M, N))
-    call("fmoe_int8_matmul", device, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(),
+        need(bias, "bias", index, (N,), F32)
+    output = _output(output, out_dtype, a, index, (M, N))
+    call("fmoe_int8_matmul", index, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(),
          b_scale.data_ptr(), ptr(bias), M, N, K, output.data_ptr(), DTYPE_TAG[output.dtype])
     return output
 
 
-@torch.no_grad()
 def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: torch.Tensor,
                        weight_scale: torch.Tensor, expert_base: torch.Tensor, *,
                        out_dtype: torch.dtype = torch.bfloat16,
@@ -92,10 +87,9 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
     device. Returns [R, N]; rows from ``expert_base[E]`` on are zero in a new tensor and left as
     they were in a given ``output``.
     """
-    need(rows, "rows", None, None, _I8)
-    need(weights, "weights", rows.device, None, _I8)
-    if (rows.dim() != 2 or weights.dim() != 3 or rows.shape[1] != weights.shape[2]
-            or weights.shape[1] < 1):
+    index = first(rows, "rows", I8, 2)
+    need(weights, "weights", index, None, I8)
+    if weights.dim() != 3 or rows.shape[1] != weights.shape[2] or weights.shape[1] < 1:
         raise ValueError(f"rows [R, K] and weights [E, N, K] do not fit: {tuple(rows.shape)}, "
                          f"{tuple(weights.shape)}")
     R, K = rows.shape
@@ -103,13 +97,12 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
     if not 1 <= E <= 256:
         raise ValueError(f"weights must hold 1..256 experts, got {E}")
     _check_depth(K)
-    device = rows.device
-    need(row_scale, "row_scale", device, (R,), _F32)
-    need(weight_scale, "weight_scale", device, (E, N), _F32)
-    need(expert_base, "expert_base", device, (E + 1,), (torch.int32,))
+    need(row_scale, "row_scale", index, (R,), F32)
+    need(weight_scale, "weight_scale", index, (E, N), F32)
+    need(expert_base, "expert_base", index, (E + 1,), I32)
     zero_tail = output is None
-    output = _output(output, out_dtype, device, (R, N))
-    call("fmoe_int8_expert_matmul", device, rows.data_ptr(), weights.data_ptr(),
+    output = _output(output, out_dtype, rows, index, (R, N))
+    call("fmoe_int8_expert_matmul", index, rows.data_ptr(), weights.data_ptr(),
          row_scale.data_ptr(), weight_scale.data_ptr(), expert_base.data_ptr(), R, E, N, K,
          output.data_ptr(), DTYPE_TAG[output.dtype], int(zero_tail))
     return output
@@ -118,9 +111,9 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
 def int8_status(device: Optional[torch.device] = None) -> int:
     """``_lib.STATUS_TIMEOUT_INT8`` if a wait inside an int8 product on the device ran out since the
     last call (its output is not valid), else 0. Synchronises the current stream."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
+    index = None if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
     status = ctypes.c_int32(0)
-    call("fmoe_int8_status", device, ctypes.byref(status))
+    call("fmoe_int8_status", index, ctypes.byref(status))
     return status.value

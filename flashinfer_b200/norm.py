@@ -7,6 +7,7 @@ the result leaves as ``run``'s e4m3 input with its scales. Forward and backward 
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
@@ -14,54 +15,59 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import FmoeBlockNormArgs
-from ._op import DTYPE_TAG, call, need, ptr, recording
+from ._op import DTYPE_TAG, FLOATS, call, first, need, ptr, recording
 
 BLOCK = 128
 
 
+_PARAMS = {t: (t, torch.float32) for t in FLOATS}
+_ONE = {t: (t,) for t in FLOATS}
+
+
+def _tag(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else DTYPE_TAG[t.dtype]
+
+
 def _args(branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps):
-    a = FmoeBlockNormArgs()
-    a.num_tokens, a.hidden_size = residual.shape
-    a.dtype = DTYPE_TAG[residual.dtype]
-    a.branch, a.residual = ptr(branch), residual.data_ptr()
-    if post_weight is not None:
-        a.post_weight, a.post_weight_dtype = post_weight.data_ptr(), DTYPE_TAG[post_weight.dtype]
-    if gate is not None:
-        a.gate, a.gate_dtype, a.gate_kind = gate.data_ptr(), DTYPE_TAG[gate.dtype], kind
-    if pre_weight is not None:
-        a.pre_weight, a.pre_weight_dtype = pre_weight.data_ptr(), DTYPE_TAG[pre_weight.dtype]
-    a.residual_scale, a.eps = residual_scale, eps
-    return a
+    T, H = residual.shape
+    return FmoeBlockNormArgs(T, H, DTYPE_TAG[residual.dtype], ptr(branch), residual.data_ptr(),
+                             ptr(post_weight), ptr(gate), ptr(pre_weight), _tag(post_weight),
+                             _tag(gate), _tag(pre_weight), kind, residual_scale, eps)
 
 
 def _forward(branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps, quantize,
              hidden, want_stats):
     a = _args(branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps)
     T, H = residual.shape
-    device = residual.device
-    if hidden is None:
-        # without a block output and with scale 1 the residual stream is what it was
-        if branch is None and residual_scale == 1.0 and not want_stats:
-            hidden = residual
-        else:
-            hidden = torch.empty_like(residual)
-            a.hidden = hidden.data_ptr()
+    if hidden is not None:
+        a.hidden = hidden.data_ptr()
+    elif branch is None and residual_scale == 1.0 and not want_stats:
+        hidden = residual  # without a block output and with scale 1 it is what it was
     else:
+        hidden = torch.empty_like(residual)
         a.hidden = hidden.data_ptr()
     normed = stats = None
     if quantize:
-        q = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=device)
-        scale = torch.empty((H // BLOCK, T), dtype=torch.float32, device=device)
+        q = residual.new_empty((T, H), dtype=torch.float8_e4m3fn)
+        scale = residual.new_empty((H // BLOCK, T), dtype=torch.float32)
         a.normed_q, a.normed_scale = q.data_ptr(), scale.data_ptr()
         normed = (q, scale)
     elif pre_weight is not None:
         normed = torch.empty_like(residual)
         a.normed = normed.data_ptr()
     if want_stats:
-        stats = torch.empty((T, 2), dtype=torch.float32, device=device)
+        stats = residual.new_empty((T, 2), dtype=torch.float32)
         a.stats = stats.data_ptr()
-    call("fmoe_block_norm", device, ctypes.byref(a))
+    call("fmoe_block_norm", residual.get_device(), ctypes.byref(a))
     return hidden, normed, stats
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(T: int, H: int) -> int:
+    size = ctypes.c_size_t()
+    _lib.check(_lib.load().fmoe_block_norm_workspace_size(T, H, ctypes.byref(size)),
+               "fmoe_block_norm_workspace_size")
+    return size.value
 
 
 class _BlockNorm(torch.autograd.Function):
@@ -94,12 +100,10 @@ class _BlockNorm(torch.autograd.Function):
         T, H = residual.shape
         workspace = None
         if grads[2] is not None or grads[3] is not None or grads[4] is not None:
-            size = ctypes.c_size_t()
-            _lib.check(_lib.load().fmoe_block_norm_workspace_size(T, H, ctypes.byref(size)),
-                       "fmoe_block_norm_workspace_size")
-            workspace = torch.empty(size.value, dtype=torch.uint8, device=residual.device)
-            a.workspace, a.workspace_bytes = ptr(workspace), size.value
-        call("fmoe_block_norm_backward", residual.device, ctypes.byref(a))
+            size = _workspace_bytes(T, H)
+            workspace = residual.new_empty(size // 4, dtype=torch.float32)
+            a.workspace, a.workspace_bytes = ptr(workspace), size
+        call("fmoe_block_norm_backward", residual.get_device(), ctypes.byref(a))
         return (*grads, None, None, None)
 
 
@@ -124,41 +128,38 @@ def block_norm(branch: Optional[torch.Tensor], residual: torch.Tensor, *,
     hidden and may be ``residual`` itself (no gradient either). Otherwise differentiable in every
     tensor; weight gradients are summed over tokens in a fixed order.
     """
-    if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
-        raise ValueError("residual must be a tensor of shape [T, H]")
-    need(residual, "residual", None, None, tuple(DTYPE_TAG))
-    T, H = residual.shape
+    index = first(residual, "residual", FLOATS, 2)
+    T, H = shape = residual.shape
     if not 1 <= H <= 16384:
         raise ValueError(f"the hidden size must be 1..16384, got {H}")
-    device, dtype = residual.device, residual.dtype
-    params = (dtype, torch.float32)
+    same, params = _ONE[residual.dtype], _PARAMS[residual.dtype]
     if branch is not None:
-        need(branch, "branch", device, (T, H), (dtype,))
+        need(branch, "branch", index, shape, same)
     elif post_weight is not None or gate is not None:
         raise ValueError("post_weight and gate need a branch")
     if post_weight is not None:
-        need(post_weight, "post_weight", device, (H,), params)
+        need(post_weight, "post_weight", index, (H,), params)
     if pre_weight is not None:
-        need(pre_weight, "pre_weight", device, (H,), params)
+        need(pre_weight, "pre_weight", index, (H,), params)
     kind = _lib.GATE_NONE
     if gate is not None:
-        need(gate, "gate", device, None, params)
-        shape = tuple(gate.shape)
-        if shape == (H,):
+        need(gate, "gate", index, None, params)
+        if gate.shape == (H,):
             kind = _lib.GATE_CHANNEL
-        elif shape == (T, 1):
+        elif gate.shape == (T, 1):
             kind = _lib.GATE_TOKEN
-        elif shape == (T, H):
+        elif gate.shape == shape:
             kind = _lib.GATE_FULL
         else:
-            raise ValueError(f"gate must have shape {(T, 1)}, {(H,)} or {(T, H)}, got {shape}")
+            raise ValueError(f"gate must have shape {(T, 1)}, {(H,)} or {(T, H)}, "
+                             f"got {tuple(gate.shape)}")
     if quantize:
         if pre_weight is None:
             raise ValueError("quantize needs a pre_weight")
         if H % BLOCK:
             raise ValueError(f"quantize needs a hidden size that is a multiple of {BLOCK}, got {H}")
     if output is not None:
-        need(output, "output", device, (T, H), (dtype,))
+        need(output, "output", index, shape, same)
     residual_scale, eps = float(residual_scale), float(eps)
     if recording(branch, residual, post_weight, gate, pre_weight, output):
         if quantize:

@@ -9,14 +9,15 @@ device and nothing waits for it, so the whole run can be captured in a CUDA grap
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from functools import lru_cache
+from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import FmoeTokenOrder
-from ._op import DTYPE_TAG, call, need, ptr, recording
+from ._op import DTYPE_TAG, F32, I32, call, first, need, ptr, recording
 
 
 class ExpertOrder:
@@ -30,20 +31,29 @@ class ExpertOrder:
     """
 
     __slots__ = ("expert_base", "row_pick", "pick_row", "num_tokens", "top_k", "num_rows",
-                 "device", "_c", "_ref")
+                 "device", "_index", "_c", "_ref")
 
     def __init__(self, expert_base, row_pick, pick_row):
         self.expert_base, self.row_pick, self.pick_row = expert_base, row_pick, pick_row
         self.num_tokens, self.top_k = pick_row.shape
         self.num_rows = row_pick.shape[0]
         self.device = pick_row.device
+        self._index = pick_row.get_device()
         self._c = FmoeTokenOrder(self.num_tokens, self.top_k, expert_base.shape[0] - 1,
                                  self.num_rows, expert_base.data_ptr(), row_pick.data_ptr(),
                                  pick_row.data_ptr())
         self._ref = ctypes.byref(self._c)
 
 
-@torch.no_grad()
+@lru_cache(maxsize=1024)
+def _sizes(T: int, K: int, E: int, align: int) -> Tuple[int, int]:
+    """Rows and scratch bytes of an order of these sizes."""
+    rows, scratch = ctypes.c_int64(), ctypes.c_size_t()
+    _lib.check(_lib.load().fmoe_sort_size(T, K, E, align, ctypes.byref(rows),
+                                          ctypes.byref(scratch)), "fmoe_sort_size")
+    return rows.value, scratch.value
+
+
 def sort_by_expert(topk_ids: torch.Tensor, num_local_experts: int, local_expert_offset: int = 0,
                    *, align: int = 1) -> ExpertOrder:
     """The expert order of int32 picks ``topk_ids`` [T, top_k].
@@ -53,9 +63,7 @@ def sort_by_expert(topk_ids: torch.Tensor, num_local_experts: int, local_expert_
     (1..1024). A token may pick the same expert twice: each pick has its own row. Stable: equal
     inputs give equal tables.
     """
-    if not isinstance(topk_ids, torch.Tensor) or topk_ids.dim() != 2:
-        raise ValueError("topk_ids must be a tensor of shape [T, top_k]")
-    need(topk_ids, "topk_ids", None, None, (torch.int32,))
+    index = first(topk_ids, "topk_ids", I32, 2)
     T, K = topk_ids.shape
     if K < 1:
         raise ValueError("topk_ids needs at least one pick per token")
@@ -65,19 +73,12 @@ def sort_by_expert(topk_ids: torch.Tensor, num_local_experts: int, local_expert_
         raise ValueError(f"local_expert_offset must not be negative, got {local_expert_offset}")
     if not 1 <= align <= 1024:
         raise ValueError(f"align must be 1..1024, got {align}")
-    rows, scratch_bytes = ctypes.c_int64(), ctypes.c_size_t()
-    _lib.check(_lib.load().fmoe_sort_size(T, K, num_local_experts, align, ctypes.byref(rows),
-                                          ctypes.byref(scratch_bytes)), "fmoe_sort_size")
-    device = topk_ids.device
-    order = ExpertOrder(
-        torch.empty(num_local_experts + 1, dtype=torch.int32, device=device),
-        torch.empty(rows.value, dtype=torch.int32, device=device),
-        torch.empty((T, K), dtype=torch.int32, device=device))
-    scratch = None
-    if scratch_bytes.value:
-        scratch = torch.empty(scratch_bytes.value, dtype=torch.uint8, device=device)
-    call("fmoe_sort_by_expert", device, topk_ids.data_ptr(), local_expert_offset, align,
-         order._ref, ptr(scratch), scratch_bytes.value)
+    rows, scratch_bytes = _sizes(T, K, num_local_experts, align)
+    order = ExpertOrder(topk_ids.new_empty(num_local_experts + 1), topk_ids.new_empty(rows),
+                        topk_ids.new_empty((T, K)))
+    scratch = topk_ids.new_empty(scratch_bytes // 4) if scratch_bytes else None
+    call("fmoe_sort_by_expert", index, topk_ids.data_ptr(), local_expert_offset, align, order._ref,
+         ptr(scratch), scratch_bytes)
     return order
 
 
@@ -88,9 +89,9 @@ def _rows_shape(x: torch.Tensor, n: int):
 def _sort(x: torch.Tensor, order: ExpertOrder, output: Optional[torch.Tensor]) -> torch.Tensor:
     zero_tail = output is None
     if output is None:
-        output = torch.empty(_rows_shape(x, order.num_rows), dtype=x.dtype, device=x.device)
+        output = x.new_empty(_rows_shape(x, order.num_rows))
     row_bytes = x.element_size() * (1 if x.dim() == 1 else x.shape[1])
-    call("fmoe_sort_rows", order.device, x.data_ptr(), row_bytes, order._ref, output.data_ptr(),
+    call("fmoe_sort_rows", order._index, x.data_ptr(), row_bytes, order._ref, output.data_ptr(),
          int(zero_tail))
     return output
 
@@ -98,9 +99,8 @@ def _sort(x: torch.Tensor, order: ExpertOrder, output: Optional[torch.Tensor]) -
 def _unsort(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor],
             output: Optional[torch.Tensor]) -> torch.Tensor:
     if output is None:
-        output = torch.empty(_rows_shape(rows, order.num_tokens), dtype=rows.dtype,
-                             device=rows.device)
-    call("fmoe_unsort_rows", order.device, rows.data_ptr(), DTYPE_TAG[rows.dtype],
+        output = rows.new_empty(_rows_shape(rows, order.num_tokens))
+    call("fmoe_unsort_rows", order._index, rows.data_ptr(), DTYPE_TAG[rows.dtype],
          1 if rows.dim() == 1 else rows.shape[1], order._ref, ptr(weights), output.data_ptr())
     return output
 
@@ -135,11 +135,10 @@ class _UnsortTokens(torch.autograd.Function):
         grad_y = grad_y.contiguous()
         grad_rows = grad_weights = None
         if ctx.needs_input_grad[0]:
-            grad_rows = torch.empty(_rows_shape(grad_y, order.num_rows), dtype=grad_y.dtype,
-                                    device=grad_y.device)
+            grad_rows = grad_y.new_empty(_rows_shape(grad_y, order.num_rows))
         if ctx.weighted and ctx.needs_input_grad[1]:
             grad_weights = torch.empty_like(weights)
-        call("fmoe_unsort_rows_backward", order.device, grad_y.data_ptr(), ptr(rows),
+        call("fmoe_unsort_rows_backward", order._index, grad_y.data_ptr(), ptr(rows),
              DTYPE_TAG[grad_y.dtype], 1 if grad_y.dim() == 1 else grad_y.shape[1], order._ref,
              ptr(weights), ptr(grad_rows), ptr(grad_weights))
         return grad_rows, grad_weights, None
@@ -148,7 +147,7 @@ class _UnsortTokens(torch.autograd.Function):
 def _check(t, name: str, order, n: int) -> None:
     if not isinstance(order, ExpertOrder):
         raise TypeError("order must be an ExpertOrder (sort_by_expert)")
-    need(t, name, order.device)
+    need(t, name, order._index, None, None)
     if t.dim() not in (1, 2) or t.shape[0] != n or (t.dim() == 2 and t.shape[1] < 1):
         raise ValueError(f"{name} must have shape [{n}] or [{n}, H], got {tuple(t.shape)}")
 
@@ -164,7 +163,7 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder, *,
     """
     _check(x, "x", order, order.num_tokens if isinstance(order, ExpertOrder) else 0)
     if output is not None:
-        need(output, "output", order.device, _rows_shape(x, order.num_rows), (x.dtype,))
+        need(output, "output", order._index, _rows_shape(x, order.num_rows), (x.dtype,))
     if recording(x, output):
         if output is not None:
             raise ValueError("output cannot be given where gradients are recorded")
@@ -188,10 +187,9 @@ def unsort_tokens(rows: torch.Tensor, order: ExpertOrder,
     if rows.dtype not in DTYPE_TAG:
         raise TypeError(f"rows must be bfloat16, float16 or float32, got {rows.dtype}")
     if topk_weights is not None:
-        need(topk_weights, "topk_weights", order.device, (order.num_tokens, order.top_k),
-             (torch.float32,))
+        need(topk_weights, "topk_weights", order._index, (order.num_tokens, order.top_k), F32)
     if output is not None:
-        need(output, "output", order.device, _rows_shape(rows, order.num_tokens), (rows.dtype,))
+        need(output, "output", order._index, _rows_shape(rows, order.num_tokens), (rows.dtype,))
     if recording(rows, topk_weights, output):
         if output is not None:
             raise ValueError("output cannot be given where gradients are recorded")
