@@ -16,6 +16,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "fmoe_elem.cuh"
 #include "fmoe_internal.h"
@@ -25,61 +26,77 @@ namespace fmoe {
 namespace {
 
 // ------------------------------------------------------------------ quantisation
-// |x| as ordered integer bits: NaN ranks above infinity, so a row that holds one gets a NaN (or
-// infinite) scale and its products are NaN.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-// 127 x / amax rounded to the nearest integer, ties to even, as a signed byte. With both operands
-// scaled by 2^-8, p = 127 x and den = amax are exact for 16-bit inputs and stay finite. p * inv is
-// within 2^-22 of the true quotient (relative), while a quotient that is no tie is at least 2^-18
-// (relative) away from every rounding border, since x and amax have at most 11 bits: only a true
-// tie can come out on either side. p - n * den is exact, tells a tie, and the odd neighbour then
-// steps to the even one. Against one IEEE division per element: quantising 8192 x 7168 took
-// 84.9 us with it.
-__device__ __forceinline__ uint32_t quant1(float v, float den, float inv) {
-  const float p = v * (127.0f / 256.0f);
-  const float m = fmaf(p, inv, 12582912.0f);   // 1.5 * 2^23: the sum's low bits are the integer
-  const float n = m - 12582912.0f;
-  uint32_t b = __float_as_uint(m);
-  const float d = fmaf(-n, den, p);
-  if (fabsf(d + d) == den && (b & 1u)) b += d > 0.0f ? 1u : ~0u;
-  return b & 0xffu;
+// Elementwise maximum of absolute values of 16-bit pairs; a NaN stays.
+__device__ __forceinline__ uint32_t abs_max2(__nv_bfloat16*, uint32_t a, uint32_t b) {
+  b &= 0x7fff7fffu;
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t abs_max2(__half*, uint32_t a, uint32_t b) {
+  b &= 0x7fff7fffu;
+  const __half2 m =
+      __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
 }
 
-// A row per G threads: a warp (WARP, eight rows per block) or the block. Up to VPT groups of V
-// elements per thread stay in registers between the maximum and the rounding; what a longer row
-// has beyond them is read a second time.
-template <typename T, int V, int VPT, bool WARP>
+// Two values as 127 x / amax rounded to the nearest integer, ties to even; the integers are the low
+// bytes of the result. With both operands scaled by 2^-8, p = 127 x and den = amax are exact for
+// 16-bit inputs and stay finite. v = p * inv is within two units of the quotient and p - v * den is
+// exact, so the corrected v is the rounded quotient: a quotient halfway between integers comes out
+// as that, and any other is 2^-18 (relative) or more away from halfway, x and amax having at most
+// 11 bits. Adding 1.5 * 2^23 then rounds to the even integer. Against one IEEE division per
+// element, quantising 8192 x 7168 took 84.9 us with it.
+__device__ __forceinline__ uint2 quant2(float2 x, float den, float inv) {
+  const float2 c = make_float2(127.0f / 256.0f, 127.0f / 256.0f);
+  const float2 i2 = make_float2(inv, inv), d2 = make_float2(-den, -den);
+  const float2 p = __fmul2_rn(x, c);
+  float2 v = __fmul2_rn(p, i2);
+  v = __ffma2_rn(__ffma2_rn(v, d2, p), i2, v);
+  v = __fadd2_rn(v, make_float2(12582912.0f, 12582912.0f));
+  return make_uint2(__float_as_uint(v.x), __float_as_uint(v.y));
+}
+
+// A row per G threads: a warp (WARP, eight rows per block) or the block. Up to VPT 16-byte granules
+// (VEC; else single elements) per thread stay in registers between the maximum and the rounding;
+// what a longer row has beyond them is read a second time.
+template <typename T, bool VEC, int VPT, bool WARP>
 __global__ void __launch_bounds__(256, 6)
     k_quantize_int8(const T* x, int64_t rows, int64_t K, int8_t* q, float* scale) {
   pdl_begin_in_order();
+  using Unit = typename std::conditional<VEC, uint4, uint16_t>::type;
   __shared__ uint32_t part[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = WARP ? 32 : blockDim.x;
   const int g = WARP ? lane : static_cast<int>(threadIdx.x);
   const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
   if (row >= rows) return;  // WARP: whole warps; no block barrier follows
-  const int64_t nvec = K / V;
-  const T* xr = x + row * K;
+  T* type = nullptr;
+  const int64_t n = VEC ? K / 8 : K;
+  const Unit* xr = reinterpret_cast<const Unit*>(x) + row * n;
   int8_t* qr = q + row * K;
-  Pack<T, V> in[VPT];
-  uint32_t m = 0;
-  auto maximum = [&](const Pack<T, V>& p) {
-    float f[V];
-    unpack(p, f);
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = max(m, abs_bits(f[j]));
+  Unit in[VPT];
+  uint32_t m2 = 0;
+  auto maximum = [&](const Unit& u) {
+    if constexpr (VEC) {
+      m2 = abs_max2(type, m2, u.x);
+      m2 = abs_max2(type, m2, u.y);
+      m2 = abs_max2(type, m2, u.z);
+      m2 = abs_max2(type, m2, u.w);
+    } else {
+      m2 = abs_max2(type, m2, u);
+    }
   };
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int64_t v = g + static_cast<int64_t>(i) * G;
-    if (v < nvec) in[i] = load_pack<T, V>(xr + v * V);
-  }
+  for (int i = 0; i < VPT; ++i)
+    if (g + static_cast<int64_t>(i) * G < n) in[i] = __ldcg(xr + g + static_cast<int64_t>(i) * G);
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
-    if (g + static_cast<int64_t>(i) * G < nvec) maximum(in[i]);
-  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < nvec; v += G)
-    maximum(load_pack<T, V>(xr + v * V));
+    if (g + static_cast<int64_t>(i) * G < n) maximum(in[i]);
+  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < n; v += G) maximum(__ldcg(xr + v));
+  // as ordered integers the bits of non-negative floats keep their order, NaN above infinity
+  const float2 halves = unpack2(type, m2);
+  uint32_t m = max(__float_as_uint(halves.x), __float_as_uint(halves.y)) & 0x7fffffffu;
   m = __reduce_max_sync(0xffffffffu, m);
   if (!WARP) {
     if (lane == 0) part[warp] = m;
@@ -92,44 +109,38 @@ __global__ void __launch_bounds__(256, 6)
   const bool finite = m < 0x7f800000u;  // else the row's values are zeros
   const float den = amax * (1.0f / 256.0f);
   const float inv = 1.0f / den;
-  auto put = [&](const Pack<T, V>& p, int64_t v) {
-    float f[V];
-    unpack(p, f);
-    uint32_t b[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) b[j] = finite ? quant1(f[j], den, inv) : 0u;
-    if constexpr (V == 8) {
+  auto put = [&](const Unit& u, int64_t v) {
+    if constexpr (VEC) {
+      const uint2 a = quant2(unpack2(type, u.x), den, inv), b = quant2(unpack2(type, u.y), den, inv);
+      const uint2 c = quant2(unpack2(type, u.z), den, inv), d = quant2(unpack2(type, u.w), den, inv);
       uint2 w;
-      w.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-      w.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
-      *reinterpret_cast<uint2*>(qr + v * V) = w;
+      w.x = __byte_perm(__byte_perm(a.x, a.y, 0x0040), __byte_perm(b.x, b.y, 0x0040), 0x5410);
+      w.y = __byte_perm(__byte_perm(c.x, c.y, 0x0040), __byte_perm(d.x, d.y, 0x0040), 0x5410);
+      reinterpret_cast<uint2*>(qr)[v] = finite ? w : make_uint2(0u, 0u);
     } else {
-      qr[v] = static_cast<int8_t>(b[0]);
+      qr[v] = finite ? static_cast<int8_t>(quant2(unpack2(type, u), den, inv).x) : int8_t{0};
     }
   };
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int64_t v = g + static_cast<int64_t>(i) * G;
-    if (v < nvec) put(in[i], v);
-  }
-  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < nvec; v += G)
-    put(load_pack<T, V>(xr + v * V), v);
+  for (int i = 0; i < VPT; ++i)
+    if (g + static_cast<int64_t>(i) * G < n) put(in[i], g + static_cast<int64_t>(i) * G);
+  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < n; v += G) put(__ldcg(xr + v), v);
 }
 
-template <typename T, int V>
+template <typename T, bool VEC>
 cudaError_t quantize_rows(const void* x, int64_t rows, int64_t K, void* q, float* scale,
                           cudaStream_t s) {
   // a row of up to four units per lane is a warp's; a longer one a block's, with as few threads
   // as hold four units each
-  const int64_t nvec = K / V;
+  const int64_t n = VEC ? K / 8 : K;
   const T* xt = static_cast<const T*>(x);
   int8_t* qt = static_cast<int8_t*>(q);
-  if (nvec <= 32 * 4)
-    return launch_pdl(k_quantize_int8<T, V, 4, true>, dim3(static_cast<unsigned>((rows + 7) / 8)),
+  if (n <= 32 * 4)
+    return launch_pdl(k_quantize_int8<T, VEC, 4, true>, dim3(static_cast<unsigned>((rows + 7) / 8)),
                       dim3(256), 0, s, xt, rows, K, qt, scale);
-  int64_t threads = (nvec + 127) / 128 * 32;
+  int64_t threads = (n + 127) / 128 * 32;
   if (threads > 256) threads = 256;
-  return launch_pdl(k_quantize_int8<T, V, 4, false>, dim3(static_cast<unsigned>(rows)),
+  return launch_pdl(k_quantize_int8<T, VEC, 4, false>, dim3(static_cast<unsigned>(rows)),
                     dim3(static_cast<unsigned>(threads)), 0, s, xt, rows, K, qt, scale);
 }
 
@@ -636,10 +647,10 @@ cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t
   const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0 &&
                    (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
   if (dtype == FMOE_DTYPE_BF16)
-    return vec ? quantize_rows<__nv_bfloat16, 8>(x, rows, K, q, scale, s)
-               : quantize_rows<__nv_bfloat16, 1>(x, rows, K, q, scale, s);
-  return vec ? quantize_rows<__half, 8>(x, rows, K, q, scale, s)
-             : quantize_rows<__half, 1>(x, rows, K, q, scale, s);
+    return vec ? quantize_rows<__nv_bfloat16, true>(x, rows, K, q, scale, s)
+               : quantize_rows<__nv_bfloat16, false>(x, rows, K, q, scale, s);
+  return vec ? quantize_rows<__half, true>(x, rows, K, q, scale, s)
+             : quantize_rows<__half, false>(x, rows, K, q, scale, s);
 }
 
 cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {

@@ -471,71 +471,10 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* buf, int group, 
   }
 }
 
-template <typename T>
-constexpr int kV = 16 / static_cast<int>(sizeof(T));
-
-// A granule's values in fp32, as pairs for the packed instructions.
-template <typename T>
-struct Gran {
-  static constexpr int N = kV<T> / 2;
-  float2 p[N];
-};
-
-template <typename T>
-__device__ __forceinline__ void zero(Gran<T>& v) {
-#pragma unroll
-  for (int i = 0; i < Gran<T>::N; ++i) v.p[i] = make_float2(0.0f, 0.0f);
-}
-// a * b, a * s, a * b + c, a * s + c, element by element
-template <typename T>
-__device__ __forceinline__ Gran<T> mul(const Gran<T>& a, const Gran<T>& b) {
-  Gran<T> r;
-#pragma unroll
-  for (int i = 0; i < Gran<T>::N; ++i) r.p[i] = __fmul2_rn(a.p[i], b.p[i]);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ Gran<T> mul(const Gran<T>& a, float s) {
-  Gran<T> r;
-#pragma unroll
-  for (int i = 0; i < Gran<T>::N; ++i) r.p[i] = __fmul2_rn(a.p[i], make_float2(s, s));
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ Gran<T> fma(const Gran<T>& a, const Gran<T>& b, const Gran<T>& c) {
-  Gran<T> r;
-#pragma unroll
-  for (int i = 0; i < Gran<T>::N; ++i) r.p[i] = __ffma2_rn(a.p[i], b.p[i], c.p[i]);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ Gran<T> fma(const Gran<T>& a, float s, const Gran<T>& c) {
-  Gran<T> r;
-#pragma unroll
-  for (int i = 0; i < Gran<T>::N; ++i)
-    r.p[i] = __ffma2_rn(a.p[i], make_float2(s, s), c.p[i]);
-  return r;
-}
-// acc += a * b, in two interleaved sums
-template <typename T>
-__device__ __forceinline__ void dot(float2& acc, const Gran<T>& a, const Gran<T>& b) {
-#pragma unroll
-  for (int i = 0; i < Gran<T>::N; ++i) acc = __ffma2_rn(a.p[i], b.p[i], acc);
-}
-
 // One granule from shared memory; element j < skip (a neighbouring row's) reads as zero.
 template <typename T>
 __device__ __forceinline__ Gran<T> read_granule(const uint4* p, int skip) {
-  Gran<T> r;
-  const uint4 q = *p;
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < Gran<T>::N; ++i) {
-    if constexpr (sizeof(T) == 4)
-      r.p[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-    else
-      r.p[i] = unpack2(static_cast<T*>(nullptr), w[i]);
-  }
+  Gran<T> r = gran_of<T>(*p);
   if (skip > 0) {
 #pragma unroll
     for (int i = 0; i < Gran<T>::N; ++i) {
@@ -604,15 +543,7 @@ __device__ __forceinline__ Gran<T> get_own(const float4* p, int stride) {
 template <typename T, bool ODD>
 __device__ __forceinline__ void store_granule(T* p, int col0, int H, const Gran<T>& g,
                                               uint4* edge) {
-  uint4 w;
-  if constexpr (sizeof(T) == 4) {
-    w = make_uint4(__float_as_uint(g.p[0].x), __float_as_uint(g.p[0].y),
-                   __float_as_uint(g.p[1].x), __float_as_uint(g.p[1].y));
-  } else {
-    T* type = nullptr;
-    w = make_uint4(pack2(type, g.p[0].x, g.p[0].y), pack2(type, g.p[1].x, g.p[1].y),
-                   pack2(type, g.p[2].x, g.p[2].y), pack2(type, g.p[3].x, g.p[3].y));
-  }
+  const uint4 w = words_of(g);
   if (!ODD || (col0 >= 0 && col0 + kV<T> <= H)) {
     *reinterpret_cast<uint4*>(p) = w;
   } else {

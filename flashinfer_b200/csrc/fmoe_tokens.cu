@@ -234,112 +234,220 @@ __global__ void __launch_bounds__(256) k_sort_rows(const U* x, U* rows, const Ro
   }
 }
 
-// y[t] = sum_k w[t, k] * rows[pick_row[t, k]] (w null: 1), k ascending, in fp32.
-template <typename T, int V>
-__global__ void __launch_bounds__(256, 4)
-    k_unsort_rows(const T* rows, const float* w, T* y, const RowsArgs a) {
+// Up to eight picks of a token from k0 on: their rows (-1: none) and weights.
+struct Picks {
+  int r[8];
+  float f[8];
+};
+
+__device__ __forceinline__ Picks load_picks(const RowsArgs& a, const float* w, int64_t t, int k0) {
+  Picks p;
+  const int64_t at = t * a.K + k0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool has = k0 + j < a.K;
+    p.r[j] = has ? __ldcg(a.pick_row + at + j) : -1;
+    p.f[j] = has && w ? __ldcg(w + at + j) : 1.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (p.r[j] >= a.R) p.r[j] = -1;
+    if (p.r[j] < 0) p.f[j] = 0.0f;  // a weight without a row is not used, whatever it holds
+  }
+  return p;
+}
+
+// The picks k0 .. k0 + 31 of one token, one per lane (a warp works on one token at a time).
+struct LanePick {
+  int r;    // row, -1: none
+  float f;  // weight, 0 without a row, whatever the weight holds
+};
+
+__device__ __forceinline__ LanePick lane_pick(const RowsArgs& a, const float* w, int64_t t, int k0) {
+  const int k = k0 + (threadIdx.x & 31);
+  LanePick p{-1, 0.0f};
+  if (t < a.T && k < a.K) {
+    p.r = __ldcg(a.pick_row + t * a.K + k);
+    if (p.r >= a.R) p.r = -1;
+    if (p.r >= 0) p.f = w ? __ldcg(w + t * a.K + k) : 1.0f;
+  }
+  return p;
+}
+
+// y[t] = sum_k w[t, k] * rows[pick_row[t, k]] (w null: 1), k ascending, in fp32. Eight rows' loads
+// are in flight per thread; a pick without a row adds 0 * 0, so the sums have no branches. With
+// single conversions and a branch per pick the kernel issued 75 instructions per row and granule.
+template <typename T>
+__global__ void __launch_bounds__(256, 3)
+    k_unsort_granules(const T* rows, const float* w, T* y, const RowsArgs a) {
   pdl_begin_in_order();
   const int64_t t = static_cast<int64_t>(blockIdx.x / a.chunks) * blockDim.y + threadIdx.y;
   const int64_t step = static_cast<int64_t>(a.chunks) * blockDim.x;
   if (t >= a.T) return;
-  const int32_t* pr = a.pick_row + t * a.K;
-  const int64_t H = a.nvec * V;
+  const uint4* in = reinterpret_cast<const uint4*>(rows);
   for (int64_t v = static_cast<int64_t>(blockIdx.x % a.chunks) * blockDim.x + threadIdx.x;
        v < a.nvec; v += step) {
-    float acc[V] = {};
+    Gran<T> acc;
+    zero(acc);
     for (int k0 = 0; k0 < a.K; k0 += 8) {
-      // eight picks at a time: their rows and weights, then all eight loads, then the sums
-      Pack<T, V> in[8];
-      int r[8];
-      float f[8];
+      const Picks p = load_picks(a, w, t, k0);
+      uint4 q[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        r[j] = k0 + j < a.K ? __ldcg(pr + k0 + j) : -1;
-        f[j] = w && k0 + j < a.K ? __ldcg(w + t * a.K + k0 + j) : 1.0f;
-        if (r[j] >= a.R) r[j] = -1;
+        q[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (p.r[j] >= 0) q[j] = __ldcg(in + p.r[j] * a.nvec + v);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (r[j] >= 0) in[j] = load_pack<T, V>(rows + r[j] * H + v * V);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (r[j] < 0) continue;
-        float e[V];
-        unpack(in[j], e);
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(f[j], e[i], acc[i]);
-      }
+      for (int j = 0; j < 8; ++j) acc = fma(gran_of<T>(q[j]), p.f[j], acc);
     }
-    store_pack<T, V>(y + t * H + v * V, acc);
+    reinterpret_cast<uint4*>(y)[t * a.nvec + v] = words_of(acc);
   }
 }
 
-// One block per token: drows[pick_row[t, k]] = w[t, k] * dy[t]; dw[t, k] = <dy[t], rows[..]>
-// (dw null: rows are not read; drows null: not written). Eight picks at a time; the sums over the row are in a fixed
-// order (thread, lane tree, warps ascending).
-template <typename T, int V>
+// The same by single elements, for rows that are no multiple of 16 bytes.
+template <typename T>
 __global__ void __launch_bounds__(256)
-    k_unsort_back(const T* dy, const T* rows, const float* w, T* drows, float* dw,
-                  const RowsArgs a) {
+    k_unsort_elements(const T* rows, const float* w, T* y, const RowsArgs a) {
+  pdl_begin_in_order();
+  const int64_t t = static_cast<int64_t>(blockIdx.x / a.chunks) * blockDim.y + threadIdx.y;
+  const int64_t step = static_cast<int64_t>(a.chunks) * blockDim.x;
+  if (t >= a.T) return;
+  for (int64_t v = static_cast<int64_t>(blockIdx.x % a.chunks) * blockDim.x + threadIdx.x;
+       v < a.nvec; v += step) {
+    float acc = 0.0f;
+    for (int k0 = 0; k0 < a.K; k0 += 8) {
+      const Picks p = load_picks(a, w, t, k0);
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        e[j] = p.r[j] >= 0 ? to_f32(load_pack<T, 1>(rows + p.r[j] * a.nvec + v).e) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc = fmaf(p.f[j], e[j], acc);
+    }
+    from_f32(acc, y + t * a.nvec + v);
+  }
+}
+
+// The eight sums of a block's threads, added in a fixed order (lane tree, warps ascending), to
+// dw[t, k0 ..]. One barrier: the next call uses another `part`.
+__device__ __forceinline__ void store_dots(float (&dot)[8], float* dw, int64_t t, int k0, int K,
+                                           float (*part)[8]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarp = blockDim.x >> 5;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float s = warp_sum_f32(dot[j]);
+    if (lane == 0) part[warp][j] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x < 8 && k0 + static_cast<int>(threadIdx.x) < K) {
+    float s = 0.0f;
+    for (int i = 0; i < nwarp; ++i) s += part[i][threadIdx.x];
+    dw[t * K + k0 + threadIdx.x] = s;
+  }
+}
+
+// One block per token at a time: drows[pick_row[t, k]] = w[t, k] * dy[t]; dw[t, k] =
+// <dy[t], rows[..]> (dw null: rows are not read; drows null: not written). Eight picks at a time.
+template <typename T>
+__global__ void __launch_bounds__(256, 3)
+    k_unsort_back_granules(const T* dy, const T* rows, const float* w, T* drows, float* dw,
+                           const RowsArgs a) {
   pdl_begin_in_order();
   if (static_cast<int>(blockIdx.x) >= a.copy_blocks) {
-    zero_rows(reinterpret_cast<Pack<T, V>*>(drows), a.row_pick, zero_limit(a), a.nvec,
+    zero_rows(reinterpret_cast<uint4*>(drows), a.row_pick, zero_limit(a), a.nvec,
               blockIdx.x - a.copy_blocks, gridDim.x - a.copy_blocks);
     return;
   }
-  __shared__ float part[8][8];
-  const int64_t t = blockIdx.x;
-  const int64_t H = a.nvec * V;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarp = blockDim.x >> 5;
-  const int32_t* pr = a.pick_row + t * a.K;
-  for (int k0 = 0; k0 < a.K; k0 += 8) {
-    int r[8];
-    float f[8], dot[8];
+  __shared__ float part[2][8][8];
+  const int nvec = static_cast<int>(a.nvec);
+  const uint4* in = reinterpret_cast<const uint4*>(rows);
+  uint4* out = reinterpret_cast<uint4*>(drows);
+  int flip = 0;
+  int64_t t = blockIdx.x;
+  LanePick next = lane_pick(a, w, t, 0);
+  for (; t < a.T; t += a.copy_blocks) {
+    const uint4* g_in = reinterpret_cast<const uint4*>(dy) + t * nvec;
+    LanePick p = next;
+    next = lane_pick(a, w, t + a.copy_blocks, 0);
+    for (int k0 = 0; k0 < a.K; k0 += 8) {
+      const int k = k0 & 31;
+      if (k0 > 0 && k == 0) p = lane_pick(a, w, t, k0);
+      float2 dot2[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      r[j] = k0 + j < a.K ? __ldcg(pr + k0 + j) : -1;
-      f[j] = w && k0 + j < a.K ? __ldcg(w + t * a.K + k0 + j) : 1.0f;
-      if (r[j] >= a.R) r[j] = -1;
-      dot[j] = 0.0f;
+      for (int j = 0; j < 8; ++j) dot2[j] = make_float2(0.0f, 0.0f);
+      // whole warps keep going for the shuffles
+      for (int v0 = 0; v0 < nvec; v0 += blockDim.x) {
+        const int v = v0 + threadIdx.x;
+        uint4 gq = make_uint4(0u, 0u, 0u, 0u), q[8];
+        if (v < nvec) gq = __ldcg(g_in + v);
+        if (dw) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = __shfl_sync(0xffffffffu, p.r, k + j);
+            q[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (r >= 0 && v < nvec) q[j] = __ldcg(in + static_cast<int64_t>(r) * nvec + v);
+          }
+        }
+        const Gran<T> g = gran_of<T>(gq);
+        if (drows) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = __shfl_sync(0xffffffffu, p.r, k + j);
+            const float f = __shfl_sync(0xffffffffu, p.f, k + j);
+            if (r >= 0 && v < nvec) out[static_cast<int64_t>(r) * nvec + v] = words_of(mul(g, f));
+          }
+        }
+        if (dw) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const Gran<T> e = gran_of<T>(q[j]);
+#pragma unroll
+            for (int i = 0; i < Gran<T>::N; ++i) dot2[j] = __ffma2_rn(g.p[i], e.p[i], dot2[j]);
+          }
+        }
+      }
+      if (dw) {
+        float dot[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)  // a gradient that is no number stays out of absent picks
+          dot[j] = __shfl_sync(0xffffffffu, p.r, k + j) >= 0 ? dot2[j].x + dot2[j].y : 0.0f;
+        store_dots(dot, dw, t, k0, a.K, part[flip]);
+        flip ^= 1;
+      }
     }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_unsort_back_elements(const T* dy, const T* rows, const float* w, T* drows, float* dw,
+                           const RowsArgs a) {
+  pdl_begin_in_order();
+  if (static_cast<int>(blockIdx.x) >= a.copy_blocks) {
+    zero_rows(reinterpret_cast<Pack<T, 1>*>(drows), a.row_pick, zero_limit(a), a.nvec,
+              blockIdx.x - a.copy_blocks, gridDim.x - a.copy_blocks);
+    return;
+  }
+  __shared__ float part[2][8][8];
+  const int64_t t = blockIdx.x;
+  for (int k0 = 0; k0 < a.K; k0 += 8) {
+    const Picks p = load_picks(a, w, t, k0);
+    float dot[8] = {};
     for (int64_t v = threadIdx.x; v < a.nvec; v += blockDim.x) {
-      float g[V];
-      unpack(load_pack<T, V>(dy + t * H + v * V), g);
-      Pack<T, V> in[8];
+      const float g = to_f32(load_pack<T, 1>(dy + t * a.nvec + v).e);
+      float e[8];
       if (dw) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (r[j] >= 0) in[j] = load_pack<T, V>(rows + r[j] * H + v * V);
+          e[j] = p.r[j] >= 0 ? to_f32(load_pack<T, 1>(rows + p.r[j] * a.nvec + v).e) : 0.0f;
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (r[j] < 0) continue;
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = f[j] * g[i];
-        if (drows) store_pack<T, V>(drows + r[j] * H + v * V, o);
-        if (dw) {
-          float e[V];
-          unpack(in[j], e);
-#pragma unroll
-          for (int i = 0; i < V; ++i) dot[j] = fmaf(g[i], e[i], dot[j]);
-        }
+        if (drows && p.r[j] >= 0) from_f32(p.f[j] * g, drows + p.r[j] * a.nvec + v);
+        if (dw && p.r[j] >= 0) dot[j] = fmaf(g, e[j], dot[j]);
       }
     }
-    if (dw) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float s = warp_sum_f32(dot[j]);
-        if (lane == 0) part[warp][j] = s;
-      }
-      __syncthreads();
-      if (threadIdx.x < 8 && k0 + static_cast<int>(threadIdx.x) < a.K) {
-        float s = 0.0f;
-        for (int i = 0; i < nwarp; ++i) s += part[i][threadIdx.x];
-        dw[t * a.K + k0 + threadIdx.x] = s;
-      }
-      __syncthreads();
-    }
+    if (dw) store_dots(dot, dw, t, k0, a.K, part[(k0 >> 3) & 1]);
   }
 }
 
@@ -401,28 +509,32 @@ cudaError_t sort_rows(const void* x, void* rows, const TokenOrder& o, int64_t ro
                     g.block, 0, s, static_cast<const U*>(x), static_cast<U*>(rows), a);
 }
 
-template <typename T, int V>
+template <typename T>
 cudaError_t unsort_rows(const void* rows, const float* w, void* y, const TokenOrder& o, int64_t H,
-                        cudaStream_t s) {
-  RowsArgs a = rows_args(o, H / V);
-  const RowGrid g = row_grid(o.T, a.nvec, V > 1 ? 1 : 4);
+                        bool vec, cudaStream_t s) {
+  RowsArgs a = rows_args(o, vec ? H / kV<T> : H);
+  const RowGrid g = row_grid(o.T, a.nvec, vec ? 1 : 4);
   a.chunks = g.chunks;
-  return launch_pdl(k_unsort_rows<T, V>, dim3(static_cast<unsigned>(g.blocks)), g.block, 0, s,
+  return launch_pdl(vec ? k_unsort_granules<T> : k_unsort_elements<T>,
+                    dim3(static_cast<unsigned>(g.blocks)), g.block, 0, s,
                     static_cast<const T*>(rows), w, static_cast<T*>(y), a);
 }
 
-template <typename T, int V>
+template <typename T>
 cudaError_t unsort_back(const void* dy, const void* rows, const float* w, void* drows, float* dw,
-                        const TokenOrder& o, int64_t H, int num_sms, cudaStream_t s) {
-  RowsArgs a = rows_args(o, H / V);
-  a.copy_blocks = o.T;
-  a.zero_tail = 1;
-  const int64_t blocks = o.T + (drows ? zero_blocks(o.R, num_sms) : 0);
+                        const TokenOrder& o, int64_t H, bool vec, int num_sms, cudaStream_t s) {
+  RowsArgs a = rows_args(o, vec ? H / kV<T> : H);
   int64_t threads = (a.nvec + 31) / 32 * 32;
   if (threads > 256) threads = 256;
-  return launch_pdl(k_unsort_back<T, V>, dim3(static_cast<unsigned>(blocks)),
-                    dim3(static_cast<unsigned>(threads)), 0, s, static_cast<const T*>(dy),
-                    static_cast<const T*>(rows), w, static_cast<T*>(drows), dw, a);
+  a.copy_blocks = o.T;
+  const int64_t most = static_cast<int64_t>(num_sms) * (768 / threads);
+  if (vec && a.copy_blocks > most) a.copy_blocks = static_cast<int>(most);
+  a.zero_tail = 1;
+  const int64_t blocks = a.copy_blocks + (drows ? zero_blocks(o.R, num_sms) : 0);
+  return launch_pdl(vec ? k_unsort_back_granules<T> : k_unsort_back_elements<T>,
+                    dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), 0, s,
+                    static_cast<const T*>(dy), static_cast<const T*>(rows), w,
+                    static_cast<T*>(drows), dw, a);
 }
 
 }  // namespace
@@ -459,23 +571,18 @@ cudaError_t launch_sort_rows(const void* x, void* rows, const TokenOrder& o, int
   return sort_rows<uint8_t>(x, rows, o, row_bytes, zero_tail, num_sms, s);
 }
 
-#define FMOE_BY_TYPE(dtype, vec, CALL)                              \
-  switch (dtype) {                                                  \
-    case FMOE_DTYPE_F32:                                            \
-      return vec ? CALL(float, 4) : CALL(float, 1);                 \
-    case FMOE_DTYPE_BF16:                                           \
-      return vec ? CALL(__nv_bfloat16, 8) : CALL(__nv_bfloat16, 1); \
-    default:                                                        \
-      return vec ? CALL(__half, 8) : CALL(__half, 1);               \
-  }
-
 cudaError_t launch_unsort_rows(const void* rows, const float* w, void* y, int dtype,
                                const TokenOrder& o, int64_t H, cudaStream_t s) {
   const int64_t bytes = H * (dtype == FMOE_DTYPE_F32 ? 4 : 2);
   const bool vec = bytes % 16 == 0 && aligned(rows, 16) && aligned(y, 16);
-#define CALL(T, V) unsort_rows<T, V>(rows, w, y, o, H, s)
-  FMOE_BY_TYPE(dtype, vec, CALL)
-#undef CALL
+  switch (dtype) {
+    case FMOE_DTYPE_F32:
+      return unsort_rows<float>(rows, w, y, o, H, vec, s);
+    case FMOE_DTYPE_BF16:
+      return unsort_rows<__nv_bfloat16>(rows, w, y, o, H, vec, s);
+    default:
+      return unsort_rows<__half>(rows, w, y, o, H, vec, s);
+  }
 }
 
 cudaError_t launch_unsort_back(const void* dy, const void* rows, const float* w, void* drows,
@@ -484,9 +591,14 @@ cudaError_t launch_unsort_back(const void* dy, const void* rows, const float* w,
   const int64_t bytes = H * (dtype == FMOE_DTYPE_F32 ? 4 : 2);
   const bool vec = bytes % 16 == 0 && aligned(dy, 16) && aligned(drows, 16) &&
                    (!dw || aligned(rows, 16));
-#define CALL(T, V) unsort_back<T, V>(dy, rows, w, drows, dw, o, H, num_sms, s)
-  FMOE_BY_TYPE(dtype, vec, CALL)
-#undef CALL
+  switch (dtype) {
+    case FMOE_DTYPE_F32:
+      return unsort_back<float>(dy, rows, w, drows, dw, o, H, vec, num_sms, s);
+    case FMOE_DTYPE_BF16:
+      return unsort_back<__nv_bfloat16>(dy, rows, w, drows, dw, o, H, vec, num_sms, s);
+    default:
+      return unsort_back<__half>(dy, rows, w, drows, dw, o, H, vec, num_sms, s);
+  }
 }
 
 }  // namespace fmoe
