@@ -156,7 +156,7 @@ constexpr int kI8MaxStages = 12;
 template <int BN>
 struct I8Cfg {
   static constexpr int STAGE = (kWRows + BN) * kKB;
-  static constexpr int NS = BN == 16 ? 12 : BN == 64 ? 9 : BN == 128 ? 6 : 4;
+  static constexpr int NS = BN == 16 ? 12 : BN == 64 ? 9 : 6;
   static constexpr int BOX = BN == 16 ? 16 : 64;   // token rows per TMA box
   static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;
   static_assert(NS > kI8Producers && NS <= kI8MaxStages, "producer parity and barrier arrays");
@@ -173,7 +173,7 @@ struct alignas(16) I8Tail {
   int tiles;
   int live;
   int last_issue[kI8Producers][kI8MaxStages];
-  float a_scale[256];
+  float a_scale[128];
   int ebase[kMaxLocalExperts + 1];
   int etile[kMaxLocalExperts + 1];  // token tiles before expert e
 };
@@ -195,7 +195,7 @@ constexpr size_t i8_smem_bytes() {
   return static_cast<size_t>(I8Cfg<BN>::NS) * I8Cfg<BN>::STAGE + sizeof(I8Tail) + 1024;
 }
 static_assert(i8_smem_bytes<16>() <= 227 * 1024 && i8_smem_bytes<64>() <= 227 * 1024 &&
-                  i8_smem_bytes<128>() <= 227 * 1024 && i8_smem_bytes<256>() <= 227 * 1024,
+                  i8_smem_bytes<128>() <= 227 * 1024,
               "shared memory per CTA");
 
 // D[tmem] (+)= A[smem] * B[smem]^T, s8 x s8 -> s32.
@@ -558,6 +558,323 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   }
 }
 
+// ------------------------------------------------------------------ CTA pairs
+// For many tokens: two CTAs share a tile of 256 weight rows x up to 256 tokens. One MMA
+// (cta_group::2, M = 256) reads both CTAs' shared memory: each holds its own 128 weight rows and
+// half of the tokens, so a K block costs an SM 32 KB of shared-memory fill instead of 48 for the same
+// 128 x 256 outputs. One CTA per tile was bound by that fill: about 53 bytes a cycle per SM, 192 us
+// for 8192 x 4096 x 7168.
+//
+// Both CTAs load into their own stages and count on the leader's (rank 0's) barrier; the leader
+// issues the MMAs and commits to the barriers of both. Each CTA stores its own weight rows' outputs.
+constexpr int kPairTokens = 256;
+constexpr int kPairStage = (kWRows + kPairTokens / 2) * kKB;  // 32 KB
+constexpr int kPairStages = 6;
+constexpr int kPairBox = 32;                                  // token rows per TMA box
+
+struct alignas(16) PairTail {
+  uint64_t full[kPairStages];   // the leader's are used: one arrival and both CTAs' bytes
+  uint64_t empty[kPairStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];           // the leader's: every epilogue warp of both CTAs
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int tiles;
+  int live;
+  float a_scale[kPairTokens];
+  int ebase[kMaxLocalExperts + 1];
+  int etile[kMaxLocalExperts + 1];
+};
+constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStage + sizeof(PairTail) + 1024;
+static_assert(kPairSmem <= 227 * 1024 && kPairStages > kI8Producers, "pair shared memory, parity");
+
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+
+// Loads a box into this CTA's shared memory, its bytes counted on a barrier of the pair.
+__device__ __forceinline__ void tma_load_pair(void* dst, const void* tmap, uint32_t bar, int32_t c0,
+                                              int32_t c1, uint64_t hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile"
+      ".mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "l"(hint)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrives on the barrier at `bar`'s place in both CTAs when the issued MMAs have finished.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Tiles of 256 weight rows, otherwise as decode_tile: expert, weight tile, token tile (fastest);
+// the tokens of a tile are cut in two halves of a multiple of 16.
+__device__ __forceinline__ I8Tile decode_pair(int tile, int NT, const PairTail* t, int E) {
+  int lo = 0, hi = E - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (tile < t->etile[mid + 1] * NT)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  const int mt = t->etile[lo + 1] - t->etile[lo];
+  const int local = tile - t->etile[lo] * NT;
+  const int n = local / mt;
+  const int m = local - n * mt;
+  const int count = t->ebase[lo + 1] - t->ebase[lo];
+  const int per = ((count + mt - 1) / mt + 31) / 32 * 32;  // at most 256
+  I8Tile r;
+  r.e = lo;
+  r.n0 = n * 2 * kWRows;
+  r.row0 = t->ebase[lo] + static_cast<int64_t>(m) * per;
+  r.rows = max(0, min(per, count - m * per));
+  r.cols = max(32, (r.rows + 31) / 32 * 32);
+  return r;
+}
+
+__device__ __forceinline__ void pair_abort(PairTail* t) {
+  *reinterpret_cast<volatile int*>(&t->abort_flag) = 1;
+  atomicOr(&g_int8_status, FMOE_STATUS_TIMEOUT_INT8);
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
+    k_int8_pair(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                const I8Args args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  PairTail* tail = reinterpret_cast<PairTail*>(smem + kPairStages * kPairStage);
+  volatile int* abort_flag = &tail->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int E = args.E;
+  const int NT = (args.N + 2 * kWRows - 1) / (2 * kWRows);
+  const int rank = static_cast<int>(cluster_ctarank());
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&tail->full[s], 1);
+      mbar_init(&tail->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tail->tfull[b], 1);
+      mbar_init(&tail->tempty[b], 2 * kI8EpiWarps);
+    }
+    mbar_init(&tail->drain, 1);
+    tail->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tail->tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  pdl_begin_in_order();
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
+    int64_t b = args.expert_base ? __ldcg(args.expert_base + e) : (e == 0 ? 0 : args.M);
+    tail->ebase[e] = static_cast<int>(b < 0 ? 0 : b > args.M ? args.M : b);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      int mt = 0;
+      if (e < E) mt = (max(0, tail->ebase[e + 1] - tail->ebase[e]) + kPairTokens - 1) / kPairTokens;
+      int incl = mt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      if (e < E) tail->etile[e] = carry + incl - mt;
+      carry += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+      tail->etile[E] = carry;
+      tail->tiles = carry * NT;
+      tail->live = tail->ebase[E];
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  // both CTAs' barriers are initialised and both have their tensor memory
+  cluster_arrive();
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem = tail->tmem_base;
+  const int tiles = tail->tiles;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0 || warp == 2 || warp == 3) {
+    // ---------------------------------------------------------------- TMA producers
+    const int pw = warp == 0 ? 0 : warp - 1;
+    if (lane == 0) {
+      const uint64_t pol_first = policy_evict_first();
+      const uint64_t pol_last = policy_evict_last();
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const I8Tile u = decode_pair(tile, NT, tail, E);
+        const int half = u.cols / 2;
+        const int boxes = (half + kPairBox - 1) / kPairBox;
+        const uint32_t bytes = 2 * (kWRows + boxes * kPairBox) * kKB;
+        const uint64_t pol_w =
+            tail->etile[u.e + 1] - tail->etile[u.e] > 1 ? pol_last : pol_first;
+        const int wrow = u.e * args.N + u.n0 + rank * kWRows;
+        const int arow = static_cast<int>(u.row0) + rank * half;
+        for (int kb = 0; kb < args.nkb; ++kb, ++it) {
+          if (it % kI8Producers != pw) continue;
+          const int s = it % kPairStages, r = it / kPairStages;
+          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, true)) {
+            pair_abort(tail);
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * kPairStage;
+          if (rank == 0) mbar_arrive_expect_tx(&tail->full[s], bytes);
+          const uint32_t bar = at_rank(&tail->full[s], 0);
+          tma_load_pair(st, &tm_w, bar, kb * kKB, wrow, pol_w);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_pair(st + (kWRows + b * kPairBox) * kKB, &tm_a, bar, kb * kKB,
+                          arow + b * kPairBox, pol_last);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer (the leader's)
+    if (rank == 0 && lane == 0) {
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step, ++n) {
+        const I8Tile u = decode_pair(tile, NT, tail, E);
+        const uint32_t idesc = idesc_i8(2 * kWRows, u.cols);
+        const int b = n & 1, rb = n >> 1;
+        const uint32_t d = tmem + b * kPairTokens;
+        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, false)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < args.nkb; ++kb, ++it) {
+          const int s = it % kPairStages, r = it / kPairStages;
+          if (!i8_wait(&tail->full[s], r & 1, abort_flag, false)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * kPairStage);
+          const uint64_t w_desc = smem_desc_k128(st);
+          const uint64_t a_desc = smem_desc_k128(st + kWRows * kKB);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_i8_pair(d, w_desc + 2 * j, a_desc + 2 * j, idesc, kb > 0 || j > 0 ? 1u : 0u);
+          commit_pair(&tail->empty[s]);
+        }
+        if (ok) commit_pair(&tail->tfull[b]);
+      }
+      if (!ok) pair_abort(tail);
+      commit_pair(&tail->drain);
+    }
+    if (lane == 0) (void)mbar_wait(&tail->drain, 0);
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    const int q = warp & 3;
+    const int g = (warp - kI8Epi0) >> 2;
+    const int etid = threadIdx.x - kI8Epi0 * 32;
+    const uint32_t tempty[2] = {at_rank(&tail->tempty[0], 0), at_rank(&tail->tempty[1], 0)};
+    if (args.zero_tail) {
+      const int64_t total = (args.M - tail->live) * static_cast<int64_t>(args.N);
+      const int64_t i0 = tail->live * static_cast<int64_t>(args.N);
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kI8EpiWarps * 32) + etid; i < total;
+           i += static_cast<int64_t>(gridDim.x) * (kI8EpiWarps * 32))
+        zero_out(args.out, args.dtype, i0 + i);
+    }
+    int n = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles; tile += step, ++n) {
+      const I8Tile u = decode_pair(tile, NT, tail, E);
+      const int b = n & 1, rb = n >> 1;
+      const int ch = u.n0 + rank * kWRows + q * 32 + lane;
+      const bool live = ch < args.N;
+      const float ws = live ? __ldcg(args.w_scale + static_cast<int64_t>(u.e) * args.N + ch) : 0.0f;
+      const float bias = live && args.bias ? __ldcg(args.bias + ch) : 0.0f;
+      named_bar_sync(1, kI8EpiWarps * 32);  // the previous tile's a_scale is no longer read
+      if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
+      named_bar_sync(1, kI8EpiWarps * 32);
+      // after a wait that ran out, the warp still takes part in the barriers of later tiles
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, false));
+      if (!ok) {
+        if (lane == 0) pair_abort(tail);
+        continue;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kPairTokens;
+      for (int c = g * 16; c < u.cols; c += 32) {
+        float v[16];
+        tmem_ld_32x32b_x16(taddr + c, v);
+        tmem_ld_wait16(v);
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (c + i < u.rows)
+              store_out(args.out, args.dtype, (u.row0 + c + i) * args.N + ch,
+                        fmaf(static_cast<float>(__float_as_int(v[i])) * tail->a_scale[c + i], ws,
+                             bias));
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(tempty[b]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // Never leave a bulk copy in flight into shared memory that is about to be released. Without an
+  // abort the leader's MMAs have waited for all of them; after one, two milliseconds pass, far
+  // beyond any copy's time.
+  if (threadIdx.x == 0 && *abort_flag) {
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) {
+    }
+  }
+  // neither CTA's memory or barriers go away while the other may still use them
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+}
+
 template <int BN, bool SPLIT>
 cudaError_t launch_mm(const CUtensorMap& tm_a, const CUtensorMap& tm_w, const I8Args& a, int grid,
                       cudaStream_t s) {
@@ -580,28 +897,30 @@ cudaError_t launch_mm(const CUtensorMap& tm_a, const CUtensorMap& tm_w, const I8
 }
 
 struct I8Plan {
-  int bn, S;
+  int bn, S;  // bn 256: CTA pairs
 };
 
 // The tile width and K split with the shortest estimated pipeline: rounds of tiles over the SMs
-// times the K blocks of a tile, a K block costing the slower of its MMAs (2 cycles per token
-// column) and its fill of shared memory (about 79 bytes a cycle).
+// times the K blocks of a tile, a K block costing the slower of its MMAs (2 cycles per token column,
+// for 128 weight rows per SM) and its fill of shared memory (about 53 bytes a cycle).
 I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms) {
-  const int64_t NT = (N + kWRows - 1) / kWRows;
   const int64_t used = M < E ? M : E;
+  const int64_t per = (M + used - 1) / used;  // tokens of an expert, evenly spread
   I8Plan best{256, 1};
   double best_cost = 1e30;
   for (const int bn : {16, 64, 128, 256}) {
-    const int64_t per = (M + used - 1) / used;           // tokens of an expert, evenly spread
+    const bool pair = bn == 256;
+    const int64_t NT = (N + (pair ? 2 : 1) * kWRows - 1) / ((pair ? 2 : 1) * kWRows);
+    const int64_t units = pair ? sms / 2 : sms;
     const int64_t mt = (per + bn - 1) / bn;
     const int64_t tiles = mt * used * NT;
     const int64_t most = (grouped ? M / bn + used : mt) * NT;  // no spread has more tiles
     const int64_t cols = ((per + mt - 1) / mt + 15) / 16 * 16;
-    const double kb = cols * 2.0 > (kWRows + cols) * kKB / 79.0 ? cols * 2.0
-                                                               : (kWRows + cols) * kKB / 79.0;
-    for (int S = 1; S <= 8; ++S) {
-      if (S > 1 && (bn > 128 || most * S > sms || nkb < 2 * S)) break;
-      const int64_t waves = S > 1 ? 1 : (tiles + sms - 1) / sms;
+    const double fill = (kWRows + (pair ? cols / 2 : cols)) * kKB / 53.0;
+    const double kb = cols * 2.0 > fill ? cols * 2.0 : fill;
+    for (int S = 1; S <= 4; S *= 2) {
+      if (S > 1 && (pair || most * S > units || nkb < 2 * S)) break;
+      const int64_t waves = S > 1 ? 1 : (tiles + units - 1) / units;
       const double cost = waves * ((nkb + S - 1) / S) * kb + cols * 20.0 + (S > 1 ? 1500.0 : 0.0);
       if (cost < best_cost) {
         best_cost = cost;
@@ -612,12 +931,7 @@ I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms) {
   return best;
 }
 
-template <int BN>
-cudaError_t run_mm(const Int8Product& p, int S, bool grouped, int sms, cudaStream_t s) {
-  CUtensorMap tm_a, tm_w;
-  if (!tensor_map_u8(&tm_a, p.a, p.K, p.M, p.K, kKB, I8Cfg<BN>::BOX) ||
-      !tensor_map_u8(&tm_w, p.w, p.K, static_cast<uint64_t>(p.E) * p.N, p.K, kKB, kWRows))
-    return cudaErrorInvalidValue;
+I8Args i8_args(const Int8Product& p, int S) {
   I8Args a{};
   a.a_scale = p.a_scale;
   a.w_scale = p.w_scale;
@@ -631,13 +945,47 @@ cudaError_t run_mm(const Int8Product& p, int S, bool grouped, int sms, cudaStrea
   a.S = S;
   a.dtype = p.out_dtype;
   a.zero_tail = p.zero_tail;
-  const int64_t NT = (p.N + kWRows - 1) / kWRows;
+  return a;
+}
+
+bool i8_maps(const Int8Product& p, int box, CUtensorMap* tm_a, CUtensorMap* tm_w) {
+  return tensor_map_u8(tm_a, p.a, p.K, p.M, p.K, kKB, box) &&
+         tensor_map_u8(tm_w, p.w, p.K, static_cast<uint64_t>(p.E) * p.N, p.K, kKB, kWRows);
+}
+
+// The most tiles of bn tokens that any spread of the rows over the experts has, per weight tile.
+int64_t most_token_tiles(const Int8Product& p, int bn) {
   const int64_t used = p.M < p.E ? p.M : p.E;
-  int64_t most = (grouped ? p.M / BN + used : (p.M + BN - 1) / BN) * NT;
-  if constexpr (BN <= 128)
-    if (S > 1) return launch_mm<BN, true>(tm_a, tm_w, a, static_cast<int>(most * S), s);
+  return p.expert_base ? p.M / bn + used : (p.M + bn - 1) / bn;
+}
+
+template <int BN>
+cudaError_t run_mm(const Int8Product& p, int S, int sms, cudaStream_t s) {
+  CUtensorMap tm_a, tm_w;
+  if (!i8_maps(p, I8Cfg<BN>::BOX, &tm_a, &tm_w)) return cudaErrorInvalidValue;
+  const I8Args a = i8_args(p, S);
+  int64_t most = most_token_tiles(p, BN) * ((p.N + kWRows - 1) / kWRows);
+  if (S > 1) return launch_mm<BN, true>(tm_a, tm_w, a, static_cast<int>(most * S), s);
   if (most > sms) most = sms;
   return launch_mm<BN, false>(tm_a, tm_w, a, static_cast<int>(most), s);
+}
+
+cudaError_t run_pair(const Int8Product& p, int sms, cudaStream_t s) {
+  CUtensorMap tm_a, tm_w;
+  if (!i8_maps(p, kPairBox, &tm_a, &tm_w)) return cudaErrorInvalidValue;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        k_int8_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
+    if (e != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
+  int64_t pairs = most_token_tiles(p, kPairTokens) * ((p.N + 2 * kWRows - 1) / (2 * kWRows));
+  if (pairs > sms / 2) pairs = sms / 2;
+  return launch_pdl(k_int8_pair, dim3(static_cast<unsigned>(2 * pairs)), dim3(kI8Threads), kPairSmem,
+                    s, tm_a, tm_w, i8_args(p, 1));
 }
 
 }  // namespace
@@ -654,17 +1002,17 @@ cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t
 }
 
 cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
-  const bool grouped = p.expert_base != nullptr;
-  const I8Plan plan = i8_plan(p.M, p.N, p.E, (p.K + kKB - 1) / kKB, grouped, sms);
+  const I8Plan plan =
+      i8_plan(p.M, p.N, p.E, (p.K + kKB - 1) / kKB, p.expert_base != nullptr, sms);
   switch (plan.bn) {
     case 16:
-      return run_mm<16>(p, plan.S, grouped, sms, s);
+      return run_mm<16>(p, plan.S, sms, s);
     case 64:
-      return run_mm<64>(p, plan.S, grouped, sms, s);
+      return run_mm<64>(p, plan.S, sms, s);
     case 128:
-      return run_mm<128>(p, plan.S, grouped, sms, s);
+      return run_mm<128>(p, plan.S, sms, s);
     default:
-      return run_mm<256>(p, plan.S, grouped, sms, s);
+      return run_pair(p, sms, s);
   }
 }
 
