@@ -173,7 +173,7 @@ struct alignas(16) I8Tail {
   int tiles;
   int live;
   int last_issue[kI8Producers][kI8MaxStages];
-  float a_scale[128];
+  alignas(16) float a_scale[128];
   int ebase[kMaxLocalExperts + 1];
   int etile[kMaxLocalExperts + 1];  // token tiles before expert e
 };
@@ -296,6 +296,81 @@ __device__ __forceinline__ int4 ld_dsmem_int4(const void* p, uint32_t rank) {
                : "r"(remote)
                : "memory");
   return v;
+}
+
+// The epilogue of one warp: its 32 channels (one per lane) of the tile's columns c0, c0 + 16, ... in
+// steps of c_step, from the accumulator at taddr; out is the element of the tile's first token at
+// this warp's first channel. `live` channels of the 32 exist.
+// PAIRS (16-bit outputs at 4-byte boundaries): neighbouring lanes exchange halves of their tokens,
+// so a lane stores two channels at once and a warp two tokens' 64 bytes. Single 16-bit stores with
+// the type decided per element took 100 us for 8192 x 7168 outputs, whatever K.
+template <typename O, bool PAIRS>
+__device__ __forceinline__ void store_columns(uint32_t taddr, int c0, int c_step, int cols, int rows,
+                                              const float* a_scale, float ws, float bias, O* out,
+                                              int N, int live) {
+  const int lane = threadIdx.x & 31;
+  const bool odd = lane & 1;
+  O* mine = out + (PAIRS ? lane & ~1 : lane);
+  const bool writes = lane < live;  // N is even with PAIRS, so both channels of a pair exist
+  for (int c = c0; c < cols; c += c_step) {
+    float v[16];
+    tmem_ld_32x32b_x16(taddr + c, v);
+    tmem_ld_wait16(v);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(a_scale + c + i);
+      v[i] = fmaf(static_cast<float>(__float_as_int(v[i])) * s.x, ws, bias);
+      v[i + 1] = fmaf(static_cast<float>(__float_as_int(v[i + 1])) * s.y, ws, bias);
+      v[i + 2] = fmaf(static_cast<float>(__float_as_int(v[i + 2])) * s.z, ws, bias);
+      v[i + 3] = fmaf(static_cast<float>(__float_as_int(v[i + 3])) * s.w, ws, bias);
+    }
+    if constexpr (PAIRS) {
+      // even lanes take tokens c .. c + 7, odd lanes c + 8 .. c + 15
+      O* p = mine + static_cast<int64_t>(c + (odd ? 8 : 0)) * N;
+      const int left = rows - c - (odd ? 8 : 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 8], 1);
+        const uint32_t w = odd ? pack2(static_cast<O*>(nullptr), other, v[i + 8])
+                               : pack2(static_cast<O*>(nullptr), v[i], other);
+        if (writes && i < left) *reinterpret_cast<uint32_t*>(p + static_cast<int64_t>(i) * N) = w;
+      }
+    } else {
+      O* p = mine + static_cast<int64_t>(c) * N;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (writes && c + i < rows) from_f32(v[i], p + static_cast<int64_t>(i) * N);
+    }
+  }
+}
+
+// The same for the call's output type.
+__device__ __forceinline__ void store_columns(const I8Args& a, uint32_t taddr, int c0, int c_step,
+                                              const I8Tile& u, int n0, const float* a_scale,
+                                              float ws, float bias) {
+  const int64_t at = u.row0 * a.N + n0;
+  const int live = a.N - n0;
+  const bool pairs = (a.N & 1) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3u) == 0;
+  if (a.dtype == FMOE_DTYPE_F32) {
+    store_columns<float, false>(taddr, c0, c_step, u.cols, u.rows, a_scale, ws, bias,
+                                static_cast<float*>(a.out) + at, a.N, live);
+  } else if (a.dtype == FMOE_DTYPE_BF16) {
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
+    if (pairs)
+      store_columns<__nv_bfloat16, true>(taddr, c0, c_step, u.cols, u.rows, a_scale, ws, bias, o,
+                                         a.N, live);
+    else
+      store_columns<__nv_bfloat16, false>(taddr, c0, c_step, u.cols, u.rows, a_scale, ws, bias, o,
+                                          a.N, live);
+  } else {
+    __half* o = static_cast<__half*>(a.out) + at;
+    if (pairs)
+      store_columns<__half, true>(taddr, c0, c_step, u.cols, u.rows, a_scale, ws, bias, o, a.N,
+                                  live);
+    else
+      store_columns<__half, false>(taddr, c0, c_step, u.cols, u.rows, a_scale, ws, bias, o, a.N,
+                                   live);
+  }
 }
 
 // SPLIT: the cluster's S CTAs share one tile, each with a range of K; their int32 partial tiles
@@ -482,25 +557,19 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       }
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * BN;
-      for (int c = g * 16; c < u.cols; c += 32) {
-        float v[16];
-        tmem_ld_32x32b_x16(taddr + c, v);
-        tmem_ld_wait16(v);
-        if constexpr (SPLIT) {
+      if constexpr (SPLIT) {
+        for (int c = g * 16; c < u.cols; c += 32) {
+          float v[16];
+          tmem_ld_32x32b_x16(taddr + c, v);
+          tmem_ld_wait16(v);
           // every load of this CTA has landed and been read (the tile's MMAs are complete), so
           // the stages hold the partial tile [token][128 channels]
           int* part = reinterpret_cast<int*>(smem) + c * kWRows + q * 32 + lane;
 #pragma unroll
           for (int i = 0; i < 16; ++i) part[i * kWRows] = __float_as_int(v[i]);
-        } else if (live) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (c + i < u.rows)
-              store_out(args.out, args.dtype, (u.row0 + c + i) * args.N + ch,
-                        fmaf(static_cast<float>(__float_as_int(v[i])) * tail->a_scale[c + i], ws,
-                             bias));
-          }
         }
+      } else {
+        store_columns(args, taddr, g * 16, 32, u, u.n0 + q * 32, tail->a_scale, ws, bias);
       }
       tc_fence_before();
       mbar_arrive(&tail->tempty[b]);
@@ -582,7 +651,7 @@ struct alignas(16) PairTail {
   int abort_flag;
   int tiles;
   int live;
-  float a_scale[kPairTokens];
+  alignas(16) float a_scale[kPairTokens];
   int ebase[kMaxLocalExperts + 1];
   int etile[kMaxLocalExperts + 1];
 };
@@ -835,20 +904,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
       }
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kPairTokens;
-      for (int c = g * 16; c < u.cols; c += 32) {
-        float v[16];
-        tmem_ld_32x32b_x16(taddr + c, v);
-        tmem_ld_wait16(v);
-        if (live) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (c + i < u.rows)
-              store_out(args.out, args.dtype, (u.row0 + c + i) * args.N + ch,
-                        fmaf(static_cast<float>(__float_as_int(v[i])) * tail->a_scale[c + i], ws,
-                             bias));
-          }
-        }
-      }
+      store_columns(args, taddr, g * 16, 32, u, u.n0 + rank * kWRows + q * 32, tail->a_scale, ws,
+                    bias);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(tempty[b]);
