@@ -145,10 +145,11 @@ cudaError_t quantize_rows(const void* x, int64_t rows, int64_t K, void* q, float
 }
 
 // ------------------------------------------------------------------ product
-constexpr int kI8Threads = 384;   // warps 0, 2, 3 load, warp 1 issues MMAs, 4..11 store
+constexpr int kI8Threads = 640;   // warps 0, 2, 3 load, warp 1 issues MMAs, 4..19 store
 constexpr int kI8Producers = 3;
 constexpr int kI8Epi0 = 4;
-constexpr int kI8EpiWarps = 8;
+constexpr int kI8EpiWarps = 16;   // with 8 the stores of 8192 x 7168 outputs took 70 us at any K
+constexpr int kI8EpiCols = kI8EpiWarps / 4 * 16;  // columns that the warps take at a time
 constexpr int kWRows = 128;       // weight rows per tile (MMA M)
 constexpr int kKB = 128;          // K bytes per stage (one 128-byte swizzled row)
 constexpr int kI8MaxStages = 12;
@@ -249,16 +250,20 @@ __device__ __forceinline__ I8Tile decode_tile(int tile, int NT, const I8Tail* t,
   return r;
 }
 
+// Waits for the phase with the given parity; gives up after FMOE_WAIT_NS, or when another role of
+// this CTA has (both looked at every few hundred polls). park: each poll may suspend the thread for
+// a while.
 __device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                         bool park) {
-  if (mbar_test_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  uint32_t spins = 0;
-  while (true) {
+  uint64_t t0 = 0;
+  const uint32_t often = park ? 15u : 511u;
+  for (uint32_t polls = 1;; ++polls) {
     if (park ? mbar_try_wait_sleep(bar, parity, 2000u) : mbar_test_wait(bar, parity)) return true;
-    if (park || (++spins & 255u) == 0) {
+    if ((polls & often) == 0) {
       if (*abort_flag) return false;
-      if (global_timer_ns() - t0 > FMOE_WAIT_NS) return false;
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > FMOE_WAIT_NS) return false;
     }
   }
 }
@@ -285,17 +290,6 @@ __device__ __forceinline__ void zero_out(void* out, int dtype, int64_t i) {
     static_cast<float*>(out)[i] = 0.0f;
   else
     static_cast<uint16_t*>(out)[i] = 0;
-}
-
-__device__ __forceinline__ int4 ld_dsmem_int4(const void* p, uint32_t rank) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(remote)
-               : "memory");
-  return v;
 }
 
 // The epilogue of one warp: its 32 channels (one per lane) of the tile's columns c0, c0 + 16, ... in
@@ -326,20 +320,36 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int c0, int c_step
     }
     if constexpr (PAIRS) {
       // even lanes take tokens c .. c + 7, odd lanes c + 8 .. c + 15
-      O* p = mine + static_cast<int64_t>(c + (odd ? 8 : 0)) * N;
-      const int left = rows - c - (odd ? 8 : 0);
+      uint32_t w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 8], 1);
-        const uint32_t w = odd ? pack2(static_cast<O*>(nullptr), other, v[i + 8])
-                               : pack2(static_cast<O*>(nullptr), v[i], other);
-        if (writes && i < left) *reinterpret_cast<uint32_t*>(p + static_cast<int64_t>(i) * N) = w;
+        w[i] = odd ? pack2(static_cast<O*>(nullptr), other, v[i + 8])
+                   : pack2(static_cast<O*>(nullptr), v[i], other);
+      }
+      if (!writes) continue;
+      O* p = mine + static_cast<int64_t>(c + (odd ? 8 : 0)) * N;
+      const int left = rows - c - (odd ? 8 : 0);
+      if (left >= 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i, p += N) *reinterpret_cast<uint32_t*>(p) = w[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i, p += N)
+          if (i < left) *reinterpret_cast<uint32_t*>(p) = w[i];
       }
     } else {
+      if (!writes) continue;
       O* p = mine + static_cast<int64_t>(c) * N;
+      const int left = rows - c;
+      if (left >= 16) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (writes && c + i < rows) from_f32(v[i], p + static_cast<int64_t>(i) * N);
+        for (int i = 0; i < 16; ++i, p += N) from_f32(v[i], p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i, p += N)
+          if (i < left) from_f32(v[i], p);
+      }
     }
   }
 }
@@ -370,6 +380,93 @@ __device__ __forceinline__ void store_columns(const I8Args& a, uint32_t taddr, i
     else
       store_columns<__half, false>(taddr, c0, c_step, u.cols, u.rows, a_scale, ws, bias, o, a.N,
                                    live);
+  }
+}
+
+// Tokens of one of S shares of a tile: whole groups of 16, so a group has one receiver.
+__device__ __forceinline__ int split_share(int rows, int S) {
+  return ((rows + S - 1) / S + 15) / 16 * 16;
+}
+
+// The address in CTA `rank`'s shared memory of what this CTA has at p.
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+
+// The end of a tile whose K range was split over S CTAs of the cluster, ranks rank0 + r * rank_step.
+// Every CTA sends each token's 128 int32 partial sums to the CTA that finishes that token (share
+// number token / per, per = tokens of a share, a multiple of 16): [sender][token of the share][128] in the receiver's
+// stages, which are free once all of the tile's MMAs are done (a cluster barrier before). After
+// another barrier each CTA adds its senders' sums (exact, so the split changes no result) and stores
+// them. Sent rather than fetched: reads of the others' shared memory, one after the other, took
+// 11 us for 256 tokens.
+__device__ __forceinline__ void send_partials(uint32_t taddr, int g, const I8Tile& u, int per,
+                                              uint8_t* part, int mine, int rank0, int rank_step,
+                                              int channel) {
+  for (int c = g * 16; c < u.cols; c += kI8EpiCols) {
+    float v[16];
+    tmem_ld_32x32b_x16(taddr + c, v);
+    tmem_ld_wait16(v);
+    const int share = c / per;  // of all 16 columns
+    const uint32_t to = at_rank(part + ((mine * per + c - share * per) * kWRows + channel) * 4,
+                                rank0 + share * rank_step);
+    const int left = u.rows - c;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < left)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + i * kWRows * 4), "f"(v[i])
+                     : "memory");
+  }
+}
+
+__device__ __forceinline__ void finish_split(const I8Args& a, const I8Tile& u, int n0, int per,
+                                             const uint8_t* part, int S, int mine) {
+  const bool pairs = (a.N & 1) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3u) == 0;
+  const int first = mine * per;
+  const int tokens = min(per, u.rows - first);
+  const float* wsp = a.w_scale + static_cast<int64_t>(u.e) * a.N;
+  // a thread keeps its four channels: the block is a multiple of the 32 groups of a token
+  const int c4 = (threadIdx.x % (kWRows / 4)) * 4;
+  const int ch = n0 + c4;
+  const int live = a.N - ch < 4 ? a.N - ch : 4;
+  if (live <= 0) return;
+  float ws[4], bias[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ws[j] = j < live ? __ldcg(wsp + ch + j) : 0.0f;
+    bias[j] = j < live && a.bias ? __ldcg(a.bias + ch + j) : 0.0f;
+  }
+  for (int t = threadIdx.x / (kWRows / 4); t < tokens; t += kI8Threads / (kWRows / 4)) {
+    int sum[4] = {0, 0, 0, 0};
+    for (int r = 0; r < S; ++r) {
+      const int4 v = *reinterpret_cast<const int4*>(part + ((r * per + t) * kWRows + c4) * 4);
+      sum[0] += v.x;
+      sum[1] += v.y;
+      sum[2] += v.z;
+      sum[3] += v.w;
+    }
+    const int64_t row = u.row0 + first + t;
+    const float as = __ldcg(a.a_scale + row);
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = fmaf(static_cast<float>(sum[j]) * as, ws[j], bias[j]);
+    const int64_t at = row * a.N + ch;
+    if (pairs && live == 4 && a.dtype != FMOE_DTYPE_F32) {
+      uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at);
+      if (a.dtype == FMOE_DTYPE_BF16) {
+        o[0] = pack2(static_cast<__nv_bfloat16*>(nullptr), y[0], y[1]);
+        o[1] = pack2(static_cast<__nv_bfloat16*>(nullptr), y[2], y[3]);
+      } else {
+        o[0] = pack2(static_cast<__half*>(nullptr), y[0], y[1]);
+        o[1] = pack2(static_cast<__half*>(nullptr), y[2], y[3]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < live) store_out(a.out, a.dtype, at + j, y[j]);
+    }
   }
 }
 
@@ -528,7 +625,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   } else {
     // ---------------------------------------------------------------- epilogue
     const int q = warp & 3;              // TMEM lane quarter of this warp
-    const int g = (warp - kI8Epi0) >> 2; // column groups of 16: even or odd
+    const int g = (warp - kI8Epi0) >> 2; // which 16 of kI8EpiCols columns
     const int etid = threadIdx.x - kI8Epi0 * 32;
     if (args.zero_tail) {
       const int64_t total = (args.M - tail->live) * static_cast<int64_t>(args.N);
@@ -557,20 +654,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       }
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * BN;
-      if constexpr (SPLIT) {
-        for (int c = g * 16; c < u.cols; c += 32) {
-          float v[16];
-          tmem_ld_32x32b_x16(taddr + c, v);
-          tmem_ld_wait16(v);
-          // every load of this CTA has landed and been read (the tile's MMAs are complete), so
-          // the stages hold the partial tile [token][128 channels]
-          int* part = reinterpret_cast<int*>(smem) + c * kWRows + q * 32 + lane;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) part[i * kWRows] = __float_as_int(v[i]);
-        }
-      } else {
-        store_columns(args, taddr, g * 16, 32, u, u.n0 + q * 32, tail->a_scale, ws, bias);
-      }
+      if constexpr (!SPLIT)
+        store_columns(args, taddr, g * 16, kI8EpiCols, u, u.n0 + q * 32, tail->a_scale, ws, bias);
       tc_fence_before();
       mbar_arrive(&tail->tempty[b]);
     }
@@ -587,43 +672,24 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (r >= 0) (void)mbar_wait(&tail->full[s], r & 1);
     }
   }
+  if constexpr (SPLIT) {
+    const I8Tile u = first < tiles ? decode_tile<BN>(first, NT, tail, E) : I8Tile{};
+    const int per = split_share(u.rows, S);
+    cluster_arrive();  // every CTA's MMAs are done, their stages free
+    cluster_wait();
+    tc_fence_after();
+    if (warp >= kI8Epi0 && u.rows > 0)
+      send_partials(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), (warp - kI8Epi0) >> 2, u,
+                    per, smem, rank, 0, 1, (warp & 3) * 32 + lane);
+    tc_fence_before();
+    cluster_arrive();
+    cluster_wait();
+    if (u.rows > 0) finish_split(args, u, u.n0, per, smem, S, rank);
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, C::COLS);
-  }
-  if constexpr (SPLIT) {
-    cluster_arrive();
-    cluster_wait();
-    if (first < tiles) {
-      const I8Tile u = decode_tile<BN>(first, NT, tail, E);
-      // four neighbouring channels of a token per item, the items dealt out over the cluster
-      const int items = u.rows * (kWRows / 4);
-      for (int i = rank * kI8Threads + threadIdx.x; i < items; i += S * kI8Threads) {
-        const int tok = i / (kWRows / 4), c4 = (i % (kWRows / 4)) * 4;
-        const int* p = reinterpret_cast<const int*>(smem) + tok * kWRows + c4;
-        int sum[4] = {0, 0, 0, 0};
-        for (int r = 0; r < S; ++r) {
-          const int4 v = ld_dsmem_int4(p, r);
-          sum[0] += v.x;
-          sum[1] += v.y;
-          sum[2] += v.z;
-          sum[3] += v.w;
-        }
-        const float as = __ldcg(args.a_scale + u.row0 + tok);
-        for (int j = 0; j < 4; ++j) {
-          const int ch = u.n0 + c4 + j;
-          if (ch >= args.N) break;
-          const float ws = __ldcg(args.w_scale + static_cast<int64_t>(u.e) * args.N + ch);
-          const float bias = args.bias ? __ldcg(args.bias + ch) : 0.0f;
-          store_out(args.out, args.dtype, (u.row0 + tok) * args.N + ch,
-                    fmaf(static_cast<float>(sum[j]) * as, ws, bias));
-        }
-      }
-    }
-    // no CTA's shared memory goes away while another reads it
-    cluster_arrive();
-    cluster_wait();
   }
 }
 
@@ -656,13 +722,9 @@ struct alignas(16) PairTail {
   int etile[kMaxLocalExperts + 1];
 };
 constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStage + sizeof(PairTail) + 1024;
+static_assert((kPairTokens + 4 * 15) * kWRows * 4 <= kPairStages * kPairStage,
+              "four shares of a tile's partial sums fit the stages");
 static_assert(kPairSmem <= 227 * 1024 && kPairStages > kI8Producers, "pair shared memory, parity");
-
-__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
 
 // Loads a box into this CTA's shared memory, its bytes counted on a barrier of the pair.
 __device__ __forceinline__ void tma_load_pair(void* dst, const void* tmap, uint32_t bar, int32_t c0,
@@ -685,12 +747,13 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, ui
       : "memory");
 }
 
-// Arrives on the barrier at `bar`'s place in both CTAs when the issued MMAs have finished.
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+// Arrives on the barrier at `bar`'s place in both CTAs of the pair when the issued MMAs have
+// finished.
+__device__ __forceinline__ void commit_pair(uint64_t* bar, int lead) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
       "[%0], %1;" ::"r"(smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
+      "h"(static_cast<uint16_t>(3 << lead))
       : "memory");
 }
 
@@ -729,7 +792,9 @@ __device__ __forceinline__ void pair_abort(PairTail* t) {
   atomicOr(&g_int8_status, FMOE_STATUS_TIMEOUT_INT8);
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
+// SPLIT: the S pairs of a cluster share one tile, each with a range of K.
+template <bool SPLIT>
+__global__ void __launch_bounds__(kI8Threads, 1)
     k_int8_pair(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                 const I8Args args) {
   extern __shared__ uint8_t smem_raw[];
@@ -739,7 +804,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int E = args.E;
   const int NT = (args.N + 2 * kWRows - 1) / (2 * kWRows);
-  const int rank = static_cast<int>(cluster_ctarank());
+  const int S = SPLIT ? args.S : 1;
+  const int cta = static_cast<int>(cluster_ctarank());
+  const int rank = cta & 1, lead = cta & ~1;  // in the pair; the pair's leader in the cluster
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < kPairStages; ++s) {
@@ -798,7 +865,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   tc_fence_after();
   const uint32_t tmem = tail->tmem_base;
   const int tiles = tail->tiles;
-  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  // SPLIT: at most one tile per cluster
+  const int first = SPLIT ? blockIdx.x / (2 * S) : blockIdx.x >> 1;
+  const int step = SPLIT ? gridDim.x / (2 * S) : gridDim.x >> 1;
+  const int kb0 = (cta >> 1) * args.nkb / S, kb1 = ((cta >> 1) + 1) * args.nkb / S;
 
   if (warp == 0 || warp == 2 || warp == 3) {
     // ---------------------------------------------------------------- TMA producers
@@ -817,7 +887,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
             tail->etile[u.e + 1] - tail->etile[u.e] > 1 ? pol_last : pol_first;
         const int wrow = u.e * args.N + u.n0 + rank * kWRows;
         const int arow = static_cast<int>(u.row0) + rank * half;
-        for (int kb = 0; kb < args.nkb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           if (it % kI8Producers != pw) continue;
           const int s = it % kPairStages, r = it / kPairStages;
           if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, true)) {
@@ -827,7 +897,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
           }
           uint8_t* st = smem + s * kPairStage;
           if (rank == 0) mbar_arrive_expect_tx(&tail->full[s], bytes);
-          const uint32_t bar = at_rank(&tail->full[s], 0);
+          const uint32_t bar = at_rank(&tail->full[s], lead);
           tma_load_pair(st, &tm_w, bar, kb * kKB, wrow, pol_w);
           for (int b = 0; b < boxes; ++b)
             tma_load_pair(st + (kWRows + b * kPairBox) * kKB, &tm_a, bar, kb * kKB,
@@ -850,7 +920,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
           break;
         }
         tc_fence_after();
-        for (int kb = 0; kb < args.nkb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % kPairStages, r = it / kPairStages;
           if (!i8_wait(&tail->full[s], r & 1, abort_flag, false)) {
             ok = false;
@@ -862,13 +932,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
           const uint64_t a_desc = smem_desc_k128(st + kWRows * kKB);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            mma_i8_pair(d, w_desc + 2 * j, a_desc + 2 * j, idesc, kb > 0 || j > 0 ? 1u : 0u);
-          commit_pair(&tail->empty[s]);
+            mma_i8_pair(d, w_desc + 2 * j, a_desc + 2 * j, idesc, kb > kb0 || j > 0 ? 1u : 0u);
+          commit_pair(&tail->empty[s], lead);
         }
-        if (ok) commit_pair(&tail->tfull[b]);
+        if (ok) commit_pair(&tail->tfull[b], lead);
       }
       if (!ok) pair_abort(tail);
-      commit_pair(&tail->drain);
+      commit_pair(&tail->drain, lead);
     }
     if (lane == 0) (void)mbar_wait(&tail->drain, 0);
   } else {
@@ -876,7 +946,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
     const int q = warp & 3;
     const int g = (warp - kI8Epi0) >> 2;
     const int etid = threadIdx.x - kI8Epi0 * 32;
-    const uint32_t tempty[2] = {at_rank(&tail->tempty[0], 0), at_rank(&tail->tempty[1], 0)};
+    const uint32_t tempty[2] = {at_rank(&tail->tempty[0], lead), at_rank(&tail->tempty[1], lead)};
     if (args.zero_tail) {
       const int64_t total = (args.M - tail->live) * static_cast<int64_t>(args.N);
       const int64_t i0 = tail->live * static_cast<int64_t>(args.N);
@@ -904,8 +974,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
       }
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kPairTokens;
-      store_columns(args, taddr, g * 16, 32, u, u.n0 + rank * kWRows + q * 32, tail->a_scale, ws,
-                    bias);
+      if constexpr (!SPLIT)
+        store_columns(args, taddr, g * 16, kI8EpiCols, u, u.n0 + rank * kWRows + q * 32,
+                      tail->a_scale, ws, bias);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(tempty[b]);
@@ -922,7 +993,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
     while (global_timer_ns() - t0 < 2000000ull) {
     }
   }
-  // neither CTA's memory or barriers go away while the other may still use them
+  if constexpr (SPLIT) {
+    const I8Tile u = first < tiles ? decode_pair(first, NT, tail, E) : I8Tile{};
+    const int per = split_share(u.rows, S);
+    cluster_arrive();  // every pair's MMAs are done, their stages free
+    cluster_wait();
+    tc_fence_after();
+    if (warp >= kI8Epi0 && u.rows > 0)
+      send_partials(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), (warp - kI8Epi0) >> 2, u,
+                    per, smem, cta >> 1, rank, 2, (warp & 3) * 32 + lane);
+    tc_fence_before();
+    cluster_arrive();
+    cluster_wait();
+    if (u.rows > 0) finish_split(args, u, u.n0 + rank * kWRows, per, smem, S, cta >> 1);
+  }
+  // no CTA's memory or barriers go away while another may still use them
   cluster_arrive();
   cluster_wait();
   if (warp == 1) {
@@ -936,16 +1021,6 @@ template <int BN, bool SPLIT>
 cudaError_t launch_mm(const CUtensorMap& tm_a, const CUtensorMap& tm_w, const I8Args& a, int grid,
                       cudaStream_t s) {
   const size_t smem = i8_smem_bytes<BN>();
-  // per-device function attribute: set once per device (idempotent)
-  static std::atomic<bool> configured[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        k_int8_mm<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-    configured[dev].store(true, std::memory_order_release);
-  }
   if constexpr (SPLIT)
     return launch_pdl_cluster(k_int8_mm<BN, true>, dim3(grid), dim3(kI8Threads), smem, s, a.S, tm_a,
                               tm_w, a);
@@ -953,32 +1028,60 @@ cudaError_t launch_mm(const CUtensorMap& tm_a, const CUtensorMap& tm_w, const I8
     return launch_pdl(k_int8_mm<BN, false>, dim3(grid), dim3(kI8Threads), smem, s, tm_a, tm_w, a);
 }
 
+// How many clusters of `size` CTAs, one CTA per SM, run at a time on the current device: fewer than
+// SMs / size, by the sizes of its SM groups (33 of 4, 22 of 6, 15 of 8 where 148 SMs are in use).
+// Asked once per device and size.
+int max_clusters(int size, int dev) {
+  static std::atomic<int> known[64][9];
+  int n = known[dev][size].load(std::memory_order_acquire);
+  if (n > 0) return n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size * 64);
+  cfg.blockDim = dim3(kI8Threads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, k_int8_pair<true>, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = 1;
+  }
+  known[dev][size].store(n, std::memory_order_release);
+  return n;
+}
+
 struct I8Plan {
   int bn, S;  // bn 256: CTA pairs
 };
 
-// The tile width and K split with the shortest estimated pipeline: rounds of tiles over the SMs
-// times the K blocks of a tile, a K block costing the slower of its MMAs (2 cycles per token column,
-// for 128 weight rows per SM) and its fill of shared memory (about 53 bytes a cycle).
-I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms) {
+// The tile width and K split with the shortest estimated time in cycles: rounds of tiles over the
+// SMs times the K blocks of a tile, a K block costing the slower of its MMAs (2.7 cycles per token
+// column, for 128 weight rows per SM) and its fill of shared memory (about 53 bytes a cycle). A
+// split adds the exchange of partial tiles (20 cycles a column, measured about 2 us for 192) and
+// the cluster's barriers.
+I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms, int dev) {
   const int64_t used = M < E ? M : E;
   const int64_t per = (M + used - 1) / used;  // tokens of an expert, evenly spread
   I8Plan best{256, 1};
   double best_cost = 1e30;
   for (const int bn : {16, 64, 128, 256}) {
-    const bool pair = bn == 256;
-    const int64_t NT = (N + (pair ? 2 : 1) * kWRows - 1) / ((pair ? 2 : 1) * kWRows);
-    const int64_t units = pair ? sms / 2 : sms;
+    const int ctas = bn == 256 ? 2 : 1;
+    const int64_t NT = (N + ctas * kWRows - 1) / (ctas * kWRows);
     const int64_t mt = (per + bn - 1) / bn;
     const int64_t tiles = mt * used * NT;
     const int64_t most = (grouped ? M / bn + used : mt) * NT;  // no spread has more tiles
     const int64_t cols = ((per + mt - 1) / mt + 15) / 16 * 16;
-    const double fill = (kWRows + (pair ? cols / 2 : cols)) * kKB / 53.0;
-    const double kb = cols * 2.0 > fill ? cols * 2.0 : fill;
-    for (int S = 1; S <= 4; S *= 2) {
-      if (S > 1 && (pair || most * S > units || nkb < 2 * S)) break;
-      const int64_t waves = S > 1 ? 1 : (tiles + units - 1) / units;
-      const double cost = waves * ((nkb + S - 1) / S) * kb + cols * 20.0 + (S > 1 ? 1500.0 : 0.0);
+    const double fill = (kWRows + cols / ctas) * kKB / 53.0;
+    const double kb = cols * 2.7 > fill ? cols * 2.7 : fill;
+    for (int S = 1; S <= 4; ++S) {
+      if (S > 1 && (nkb < 2 * S || most > max_clusters(S * ctas, dev))) break;
+      const int64_t waves = S > 1 ? 1 : (tiles + sms / ctas - 1) / (sms / ctas);
+      const double cost = waves * ((nkb + S - 1) / S) * kb + cols * 20.0 +
+                          (S > 1 ? cols * 20.0 + 1500.0 : 0.0);
       if (cost < best_cost) {
         best_cost = cost;
         best = I8Plan{bn, S};
@@ -1027,22 +1130,33 @@ cudaError_t run_mm(const Int8Product& p, int S, int sms, cudaStream_t s) {
   return launch_mm<BN, false>(tm_a, tm_w, a, static_cast<int>(most), s);
 }
 
-cudaError_t run_pair(const Int8Product& p, int sms, cudaStream_t s) {
+template <bool SPLIT>
+cudaError_t launch_pair(const Int8Product& p, int S, int sms, cudaStream_t s) {
   CUtensorMap tm_a, tm_w;
   if (!i8_maps(p, kPairBox, &tm_a, &tm_w)) return cudaErrorInvalidValue;
-  static std::atomic<bool> configured[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        k_int8_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
-    if (e != cudaSuccess) return e;
-    configured[dev].store(true, std::memory_order_release);
-  }
-  int64_t pairs = most_token_tiles(p, kPairTokens) * ((p.N + 2 * kWRows - 1) / (2 * kWRows));
-  if (pairs > sms / 2) pairs = sms / 2;
-  return launch_pdl(k_int8_pair, dim3(static_cast<unsigned>(2 * pairs)), dim3(kI8Threads), kPairSmem,
-                    s, tm_a, tm_w, i8_args(p, 1));
+  const int64_t tiles = most_token_tiles(p, kPairTokens) * ((p.N + 2 * kWRows - 1) / (2 * kWRows));
+  const int64_t clusters = SPLIT || tiles < sms / 2 ? tiles : sms / 2;
+  return launch_pdl_cluster(k_int8_pair<SPLIT>, dim3(static_cast<unsigned>(2 * S * clusters)),
+                            dim3(kI8Threads), kPairSmem, s, 2 * S, tm_a, tm_w, i8_args(p, S));
+}
+
+// The shared-memory opt-in of every kernel, once per device (idempotent).
+cudaError_t configure(int dev) {
+  static std::atomic<bool> done[64];
+  if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  const auto set = [](const void* f, size_t bytes) {
+    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(bytes));
+  };
+  cudaError_t e = set(reinterpret_cast<const void*>(k_int8_pair<false>), kPairSmem);
+  if (e == cudaSuccess) e = set(reinterpret_cast<const void*>(k_int8_pair<true>), kPairSmem);
+#define SET(BN, SPLIT) \
+  if (e == cudaSuccess) \
+    e = set(reinterpret_cast<const void*>(k_int8_mm<BN, SPLIT>), i8_smem_bytes<BN>());
+  SET(16, false) SET(16, true) SET(64, false) SET(64, true) SET(128, false) SET(128, true)
+#undef SET
+  if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+  return e;
 }
 
 }  // namespace
@@ -1059,8 +1173,12 @@ cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t
 }
 
 cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  const cudaError_t e = configure(dev);
+  if (e != cudaSuccess) return e;
   const I8Plan plan =
-      i8_plan(p.M, p.N, p.E, (p.K + kKB - 1) / kKB, p.expert_base != nullptr, sms);
+      i8_plan(p.M, p.N, p.E, (p.K + kKB - 1) / kKB, p.expert_base != nullptr, sms, dev);
   switch (plan.bn) {
     case 16:
       return run_mm<16>(p, plan.S, sms, s);
@@ -1069,7 +1187,8 @@ cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
     case 128:
       return run_mm<128>(p, plan.S, sms, s);
     default:
-      return run_pair(p, sms, s);
+      return plan.S > 1 ? launch_pair<true>(p, plan.S, sms, s)
+                        : launch_pair<false>(p, 1, sms, s);
   }
 }
 
