@@ -9,6 +9,8 @@
 //   unsort   y[t] = sum over k ascending of w[t, k] * rows[pick_row[t, k]], fp32, one rounding
 //   backward of sort: unsort without weights; backward of unsort: drows[r] = w * dy[t] and
 //   dw[t, k] = <dy[t], rows[pick_row[t, k]]> in fp32
+#include <initializer_list>
+
 #include "fmoe_elem.cuh"
 #include "fmoe_internal.h"
 
@@ -174,21 +176,28 @@ __global__ void __launch_bounds__(1024)
     row_pick[r] = -1;
 }
 
-// Zeroes the rows without a pick among [0, limit): blocks b of nb, a warp looks at 32 rows at a
-// time. U: the access unit, nvec of them per row.
-template <typename U>
-__device__ __forceinline__ void zero_rows(U* rows, const int32_t* row_pick, int64_t limit,
-                                          int64_t nvec, int b, int nb) {
+// Zeroes the rows without a pick among [0, limit): blocks b of nb, a warp looks at four rows at a
+// time. Whatever the rows' size, all but their ends goes in 16-byte stores.
+__device__ __forceinline__ void zero_rows(void* rows, const int32_t* row_pick, int64_t limit,
+                                          int64_t row_bytes, int b, int nb) {
   const int tid = threadIdx.y * blockDim.x + threadIdx.x;
   const int nwarp = (blockDim.x * blockDim.y) >> 5, warp = tid >> 5, lane = tid & 31;
-  const int64_t step = static_cast<int64_t>(nb) * nwarp * 32;
-  for (int64_t r0 = (static_cast<int64_t>(b) * nwarp + warp) * 32; r0 < limit; r0 += step) {
-    const bool none = r0 + lane < limit && __ldcg(row_pick + r0 + lane) < 0;
+  const int64_t step = static_cast<int64_t>(nb) * nwarp * 4;
+  for (int64_t r0 = (static_cast<int64_t>(b) * nwarp + warp) * 4; r0 < limit; r0 += step) {
+    const bool none = lane < 4 && r0 + lane < limit && __ldcg(row_pick + r0 + lane) < 0;
     unsigned todo = __ballot_sync(0xffffffffu, none);
     while (todo) {
       const int64_t r = r0 + __ffs(todo) - 1;
       todo &= todo - 1;
-      for (int64_t v = lane; v < nvec; v += 32) rows[r * nvec + v] = U{};
+      uint8_t* p = static_cast<uint8_t*>(rows) + r * row_bytes;
+      int64_t head = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15;
+      if (head > row_bytes) head = row_bytes;
+      if (lane < head) p[lane] = 0;
+      const int64_t n = (row_bytes - head) / 16;
+      uint4* q = reinterpret_cast<uint4*>(p + head);
+      for (int64_t v = lane; v < n; v += 32) q[v] = make_uint4(0u, 0u, 0u, 0u);
+      const int64_t done = head + n * 16;
+      if (lane < row_bytes - done) p[done + lane] = 0;
     }
   }
 }
@@ -200,6 +209,7 @@ struct RowsArgs {
   int T, K, E;
   int64_t R;
   int64_t nvec;     // access units per row
+  int64_t bytes;    // per row
   int chunks;       // blocks along a row
   int copy_blocks;  // blocks that take tokens; the others zero rows
   int zero_tail;    // rows from expert_base[E] on are zeroed too
@@ -216,7 +226,7 @@ template <typename U>
 __global__ void __launch_bounds__(256) k_sort_rows(const U* x, U* rows, const RowsArgs a) {
   pdl_begin_in_order();
   if (static_cast<int>(blockIdx.x) >= a.copy_blocks) {
-    zero_rows(rows, a.row_pick, zero_limit(a), a.nvec, blockIdx.x - a.copy_blocks,
+    zero_rows(rows, a.row_pick, zero_limit(a), a.bytes, blockIdx.x - a.copy_blocks,
               gridDim.x - a.copy_blocks);
     return;
   }
@@ -226,10 +236,14 @@ __global__ void __launch_bounds__(256) k_sort_rows(const U* x, U* rows, const Ro
   const int32_t* pr = a.pick_row + t * a.K;
   for (int64_t v = static_cast<int64_t>(blockIdx.x % a.chunks) * blockDim.x + threadIdx.x;
        v < a.nvec; v += step) {
-    const U val = x[t * a.nvec + v];
-    for (int k = 0; k < a.K; ++k) {
-      const int64_t r = __ldcg(pr + k);
-      if (r >= 0 && r < a.R) rows[r * a.nvec + v] = val;
+    const U val = __ldcg(x + t * a.nvec + v);
+    for (int k0 = 0; k0 < a.K; k0 += 8) {
+      int r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = k0 + j < a.K ? __ldcg(pr + k0 + j) : -1;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (r[j] >= 0 && r[j] < a.R) rows[r[j] * a.nvec + v] = val;
     }
   }
 }
@@ -354,7 +368,7 @@ __global__ void __launch_bounds__(256, 3)
                            const RowsArgs a) {
   pdl_begin_in_order();
   if (static_cast<int>(blockIdx.x) >= a.copy_blocks) {
-    zero_rows(reinterpret_cast<uint4*>(drows), a.row_pick, zero_limit(a), a.nvec,
+    zero_rows(drows, a.row_pick, zero_limit(a), a.bytes,
               blockIdx.x - a.copy_blocks, gridDim.x - a.copy_blocks);
     return;
   }
@@ -424,7 +438,7 @@ __global__ void __launch_bounds__(256)
                            const RowsArgs a) {
   pdl_begin_in_order();
   if (static_cast<int>(blockIdx.x) >= a.copy_blocks) {
-    zero_rows(reinterpret_cast<Pack<T, 1>*>(drows), a.row_pick, zero_limit(a), a.nvec,
+    zero_rows(drows, a.row_pick, zero_limit(a), a.bytes,
               blockIdx.x - a.copy_blocks, gridDim.x - a.copy_blocks);
     return;
   }
@@ -448,6 +462,239 @@ __global__ void __launch_bounds__(256)
       }
     }
     if (dw) store_dots(dot, dw, t, k0, a.K, part[(k0 >> 3) & 1]);
+  }
+}
+
+// ------------------------------------------------------------------ rows of any size
+// Rows that are no multiple of 16 bytes, in tensors that start on a 16-byte boundary: all accesses
+// still go by aligned 16-byte granules. A row's granules are those that hold a byte of it; the
+// first and last may hold bytes of its neighbours. Moving a row to one with another offset in its
+// granules shifts two neighbouring granules against each other. Single-element accesses took 70 us
+// to sort 4096 x 2047 (bf16, top 8), granules take 25 us for 2048.
+
+// Granule g of a tensor of `total` bytes; bytes outside the tensor read as zero.
+__device__ __forceinline__ uint4 granule(const uint8_t* base, int64_t g, int64_t total) {
+  uint4 q = make_uint4(0u, 0u, 0u, 0u);
+  if (g >= 0 && g * 16 + 16 <= total) {
+    q = __ldcg(reinterpret_cast<const uint4*>(base) + g);
+  } else if (g >= 0 && g * 16 < total) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    const int n = static_cast<int>(total - g * 16);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < n) w[i / 4] |= static_cast<uint32_t>(__ldcg(base + g * 16 + i)) << (8 * (i % 4));
+    q = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return q;
+}
+
+// Bytes [by, by + 16) of the 32 bytes lo, hi (0 <= by < 16).
+__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int by) {
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (by & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (by & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const int bits = (by & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// Stores the bytes [lo, hi) of q to the granule at p (element size E).
+template <int E>
+__device__ __forceinline__ void store_part(uint8_t* p, const uint4& q, int lo, int hi) {
+  if (lo <= 0 && hi >= 16) {
+    *reinterpret_cast<uint4*>(p) = q;
+    return;
+  }
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 16; i += E) {
+    if (i < lo || i >= hi) continue;
+    if constexpr (E == 4)
+      *reinterpret_cast<uint32_t*>(p + i) = w[i / 4];
+    else if constexpr (E == 2)
+      *reinterpret_cast<uint16_t*>(p + i) = static_cast<uint16_t>(w[i / 4] >> (8 * (i % 4)));
+    else
+      p[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+__device__ __forceinline__ uint4 shfl_granule(const uint4& q, int from) {
+  return make_uint4(__shfl_sync(0xffffffffu, q.x, from), __shfl_sync(0xffffffffu, q.y, from),
+                    __shfl_sync(0xffffffffu, q.z, from), __shfl_sync(0xffffffffu, q.w, from));
+}
+
+// A granule of a token's row and its two neighbours, for shifting it to any other offset. Lanes hold
+// consecutive granules; only the outer lanes load their missing neighbour.
+struct Granules3 {
+  uint4 before, at, after;
+};
+
+__device__ __forceinline__ Granules3 load3(const uint8_t* base, int64_t g, int64_t total) {
+  const int lane = threadIdx.x & 31;
+  Granules3 t;
+  t.at = granule(base, g, total);
+  t.before = shfl_granule(t.at, lane - 1 < 0 ? 0 : lane - 1);
+  t.after = shfl_granule(t.at, lane + 1 > 31 ? 31 : lane + 1);
+  if (lane == 0) t.before = granule(base, g - 1, total);
+  if (lane == 31) t.after = granule(base, g + 1, total);
+  return t;
+}
+
+// The token's bytes for the granule of a row at the same index: `from` and `to` are the offsets of
+// the two rows in their first granules.
+__device__ __forceinline__ uint4 move(const Granules3& t, int from, int to) {
+  const int by = from - to;  // > -16 and < 16
+  return by >= 0 ? shifted(t.at, t.after, by) : shifted(t.before, t.at, by + 16);
+}
+
+// rows[pick_row[t, k]] = x[t], element size E.
+template <int E>
+__global__ void __launch_bounds__(256)
+    k_sort_shifted(const uint8_t* x, uint8_t* rows, const RowsArgs a) {
+  pdl_begin_in_order();
+  if (static_cast<int>(blockIdx.x) >= a.copy_blocks) {
+    zero_rows(rows, a.row_pick, zero_limit(a), a.bytes, blockIdx.x - a.copy_blocks,
+              gridDim.x - a.copy_blocks);
+    return;
+  }
+  const int64_t t = blockIdx.x / a.chunks;
+  // whole warps take part in the exchange of neighbours
+  const int64_t v = static_cast<int64_t>(blockIdx.x % a.chunks) * blockDim.x + threadIdx.x;
+  const int64_t start = t * a.bytes;
+  const int from = static_cast<int>(start & 15);
+  const Granules3 g = load3(x, start / 16 + v, a.T * a.bytes);
+  const int32_t* pr = a.pick_row + t * a.K;
+  for (int k0 = 0; k0 < a.K; k0 += 8) {
+    int picks[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) picks[j] = k0 + j < a.K ? __ldcg(pr + k0 + j) : -1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t r = picks[j];
+      if (r < 0 || r >= a.R) continue;
+      const int to = static_cast<int>((r * a.bytes) & 15);
+      const int64_t lo = to - v * 16, hi = to + a.bytes - v * 16;  // the row's bytes in this granule
+      if (hi <= 0) continue;
+      store_part<E>(rows + (r * a.bytes - to) + v * 16, move(g, from, to),
+                    static_cast<int>(lo < 0 ? 0 : lo), static_cast<int>(hi > 16 ? 16 : hi));
+    }
+  }
+}
+
+// As k_unsort_granules. Each of the eight rows is read at this token's offset: a granule and its
+// neighbour, which the next lane has.
+template <typename T>
+__global__ void __launch_bounds__(256, 2)
+    k_unsort_shifted(const T* rows, const float* w, T* y, const RowsArgs a) {
+  pdl_begin_in_order();
+  const int64_t t = blockIdx.x / a.chunks;
+  const int64_t v = static_cast<int64_t>(blockIdx.x % a.chunks) * blockDim.x + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  const uint8_t* in = reinterpret_cast<const uint8_t*>(rows);
+  const int64_t start = t * a.bytes, total = a.R * a.bytes;
+  const int to = static_cast<int>(start & 15);
+  Gran<T> acc;
+  zero(acc);
+  for (int k0 = 0; k0 < a.K; k0 += 8) {
+    const Picks p = load_picks(a, w, t, k0);
+    uint4 q[8], last[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      q[j] = last[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (p.r[j] >= 0) {
+        // this granule's bytes lie at row start + v * 16 - to
+        const int64_t at = p.r[j] * a.bytes + v * 16 - to;
+        const int64_t g = at >= 0 ? at / 16 : -1;  // at > -16
+        q[j] = granule(in, g, total);
+        if (lane == 31) last[j] = granule(in, g + 1, total);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint4 next = shfl_granule(q[j], lane + 1 > 31 ? 31 : lane + 1);
+      if (lane == 31) next = last[j];
+      if (p.r[j] < 0) continue;
+      const int by = static_cast<int>((p.r[j] * a.bytes + 16 - to) & 15);
+      acc = fma(gran_of<T>(shifted(q[j], next, by)), p.f[j], acc);
+    }
+  }
+  const int64_t lo = to - v * 16, hi = to + a.bytes - v * 16;
+  if (hi > 0)
+    store_part<sizeof(T)>(reinterpret_cast<uint8_t*>(y) + (start - to) + v * 16, words_of(acc),
+                          static_cast<int>(lo < 0 ? 0 : lo), static_cast<int>(hi > 16 ? 16 : hi));
+}
+
+// As k_unsort_back_granules: dy is shifted to each row's offset; bytes of neighbouring rows count
+// as zero in the sums.
+template <typename T>
+__global__ void __launch_bounds__(256, 2)
+    k_unsort_back_shifted(const T* dy, const T* rows, const float* w, T* drows, float* dw,
+                          const RowsArgs a) {
+  pdl_begin_in_order();
+  if (static_cast<int>(blockIdx.x) >= a.copy_blocks) {
+    zero_rows(drows, a.row_pick, zero_limit(a), a.bytes, blockIdx.x - a.copy_blocks,
+              gridDim.x - a.copy_blocks);
+    return;
+  }
+  __shared__ float part[2][8][8];
+  const int64_t t = blockIdx.x;
+  const int64_t start = t * a.bytes, total = a.R * a.bytes;
+  const int from = static_cast<int>(start & 15);
+  const uint8_t* in = reinterpret_cast<const uint8_t*>(rows);
+  for (int k0 = 0; k0 < a.K; k0 += 8) {
+    const Picks p = load_picks(a, w, t, k0);
+    float2 dot2[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dot2[j] = make_float2(0.0f, 0.0f);
+    for (int64_t v0 = 0; v0 < a.nvec; v0 += blockDim.x) {
+      const int64_t v = v0 + threadIdx.x;
+      uint4 q[8];
+      if (dw) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          q[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (p.r[j] >= 0 && v < a.nvec) q[j] = granule(in, p.r[j] * a.bytes / 16 + v, total);
+        }
+      }
+      const Granules3 g3 = load3(reinterpret_cast<const uint8_t*>(dy), start / 16 + v, a.T * a.bytes);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (p.r[j] < 0) continue;
+        const int to = static_cast<int>((p.r[j] * a.bytes) & 15);
+        const int64_t lo64 = to - v * 16, hi64 = to + a.bytes - v * 16;
+        if (hi64 <= 0) continue;
+        const int lo = static_cast<int>(lo64 < 0 ? 0 : lo64), hi = static_cast<int>(hi64 > 16 ? 16 : hi64);
+        Gran<T> g = gran_of<T>(move(g3, from, to));
+        if (drows)
+          store_part<sizeof(T)>(reinterpret_cast<uint8_t*>(drows) + (p.r[j] * a.bytes - to) + v * 16,
+                                words_of(mul(g, p.f[j])), lo, hi);
+        if (dw) {
+          Gran<T> e = gran_of<T>(q[j]);
+          if (lo > 0 || hi < 16) {
+            constexpr int S = sizeof(T);
+#pragma unroll
+            for (int i = 0; i < Gran<T>::N; ++i) {
+              if (2 * i * S < lo || 2 * i * S >= hi) g.p[i].x = e.p[i].x = 0.0f;
+              if ((2 * i + 1) * S < lo || (2 * i + 1) * S >= hi) g.p[i].y = e.p[i].y = 0.0f;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < Gran<T>::N; ++i) dot2[j] = __ffma2_rn(g.p[i], e.p[i], dot2[j]);
+        }
+      }
+    }
+    if (dw) {
+      float dot[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot[j] = p.r[j] >= 0 ? dot2[j].x + dot2[j].y : 0.0f;
+      store_dots(dot, dw, t, k0, a.K, part[(k0 >> 3) & 1]);
+    }
   }
 }
 
@@ -479,8 +726,9 @@ RowGrid row_grid(int64_t T, int64_t nvec, int per_thread) {
   return g;
 }
 
-RowsArgs rows_args(const TokenOrder& o, int64_t nvec) {
+RowsArgs rows_args(const TokenOrder& o, int64_t nvec, int64_t bytes) {
   RowsArgs a{};
+  a.bytes = bytes;
   a.expert_base = o.expert_base;
   a.row_pick = o.row_pick;
   a.pick_row = o.pick_row;
@@ -493,14 +741,14 @@ RowsArgs rows_args(const TokenOrder& o, int64_t nvec) {
 }
 
 int zero_blocks(int64_t R, int num_sms) {
-  const int64_t b = (R + 255) / 256;
+  const int64_t b = (R + 31) / 32;  // four rows per warp
   return static_cast<int>(b < 2 * num_sms ? b : 2 * num_sms);
 }
 
 template <typename U>
 cudaError_t sort_rows(const void* x, void* rows, const TokenOrder& o, int64_t row_bytes,
                       int zero_tail, int num_sms, cudaStream_t s) {
-  RowsArgs a = rows_args(o, row_bytes / static_cast<int64_t>(sizeof(U)));
+  RowsArgs a = rows_args(o, row_bytes / static_cast<int64_t>(sizeof(U)), row_bytes);
   const RowGrid g = row_grid(o.T, a.nvec, sizeof(U) == 16 ? 1 : 4);
   a.chunks = g.chunks;
   a.copy_blocks = static_cast<int>(g.blocks);
@@ -509,29 +757,71 @@ cudaError_t sort_rows(const void* x, void* rows, const TokenOrder& o, int64_t ro
                     g.block, 0, s, static_cast<const U*>(x), static_cast<U*>(rows), a);
 }
 
+// Rows from 512 bytes on, of any size, go by granules (a warp holds 32 of one row); shorter rows
+// that are no multiple of 16 bytes go by elements.
+enum RowPath { kGranules, kShifted, kElements };
+
+RowPath row_path(int64_t bytes, std::initializer_list<const void*> tensors) {
+  for (const void* p : tensors)
+    if (!aligned(p, 16)) return kElements;
+  return bytes % 16 == 0 ? kGranules : bytes >= 512 ? kShifted : kElements;
+}
+
+// Blocks along the granules of a shifted row (at most two more than its size gives).
+RowGrid shifted_grid(int64_t T, int64_t bytes) {
+  const int64_t n = bytes / 16 + 2;
+  RowGrid g{};
+  g.chunks = static_cast<int>((n + 255) / 256);
+  g.block = dim3(static_cast<unsigned>(((n + g.chunks - 1) / g.chunks + 31) / 32 * 32), 1);
+  g.blocks = T * g.chunks;
+  return g;
+}
+
+template <int E>
+cudaError_t sort_shifted(const void* x, void* rows, const TokenOrder& o, int64_t row_bytes,
+                         int zero_tail, int num_sms, cudaStream_t s) {
+  RowsArgs a = rows_args(o, 0, row_bytes);
+  const RowGrid g = shifted_grid(o.T, row_bytes);
+  a.chunks = g.chunks;
+  a.copy_blocks = static_cast<int>(g.blocks);
+  a.zero_tail = zero_tail;
+  return launch_pdl(k_sort_shifted<E>, dim3(static_cast<unsigned>(g.blocks + zero_blocks(o.R, num_sms))),
+                    g.block, 0, s, static_cast<const uint8_t*>(x), static_cast<uint8_t*>(rows), a);
+}
+
 template <typename T>
 cudaError_t unsort_rows(const void* rows, const float* w, void* y, const TokenOrder& o, int64_t H,
-                        bool vec, cudaStream_t s) {
-  RowsArgs a = rows_args(o, vec ? H / kV<T> : H);
-  const RowGrid g = row_grid(o.T, a.nvec, vec ? 1 : 4);
+                        cudaStream_t s) {
+  const int64_t bytes = H * static_cast<int64_t>(sizeof(T));
+  const RowPath path = row_path(bytes, {rows, y});
+  RowsArgs a = rows_args(o, path == kGranules ? H / kV<T> : H, bytes);
+  const RowGrid g = path == kShifted ? shifted_grid(o.T, bytes)
+                                     : row_grid(o.T, a.nvec, path == kGranules ? 1 : 4);
   a.chunks = g.chunks;
-  return launch_pdl(vec ? k_unsort_granules<T> : k_unsort_elements<T>,
+  return launch_pdl(path == kGranules  ? k_unsort_granules<T>
+                    : path == kShifted ? k_unsort_shifted<T>
+                                       : k_unsort_elements<T>,
                     dim3(static_cast<unsigned>(g.blocks)), g.block, 0, s,
                     static_cast<const T*>(rows), w, static_cast<T*>(y), a);
 }
 
 template <typename T>
 cudaError_t unsort_back(const void* dy, const void* rows, const float* w, void* drows, float* dw,
-                        const TokenOrder& o, int64_t H, bool vec, int num_sms, cudaStream_t s) {
-  RowsArgs a = rows_args(o, vec ? H / kV<T> : H);
-  int64_t threads = (a.nvec + 31) / 32 * 32;
-  if (threads > 256) threads = 256;
+                        const TokenOrder& o, int64_t H, int num_sms, cudaStream_t s) {
+  const int64_t bytes = H * static_cast<int64_t>(sizeof(T));
+  const RowPath path = row_path(bytes, {dy, dw ? rows : nullptr, drows});
+  RowsArgs a = rows_args(o, path == kGranules ? H / kV<T> : path == kShifted ? bytes / 16 + 2 : H, bytes);
+  // passes of equal length along the row
+  const int64_t passes = (a.nvec + 255) / 256;
+  const int64_t threads = ((a.nvec + passes - 1) / passes + 31) / 32 * 32;
   a.copy_blocks = o.T;
   const int64_t most = static_cast<int64_t>(num_sms) * (768 / threads);
-  if (vec && a.copy_blocks > most) a.copy_blocks = static_cast<int>(most);
+  if (path == kGranules && a.copy_blocks > most) a.copy_blocks = static_cast<int>(most);
   a.zero_tail = 1;
   const int64_t blocks = a.copy_blocks + (drows ? zero_blocks(o.R, num_sms) : 0);
-  return launch_pdl(vec ? k_unsort_back_granules<T> : k_unsort_back_elements<T>,
+  return launch_pdl(path == kGranules  ? k_unsort_back_granules<T>
+                    : path == kShifted ? k_unsort_back_shifted<T>
+                                       : k_unsort_back_elements<T>,
                     dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), 0, s,
                     static_cast<const T*>(dy), static_cast<const T*>(rows), w,
                     static_cast<T*>(drows), dw, a);
@@ -565,39 +855,40 @@ cudaError_t launch_sort_rows(const void* x, void* rows, const TokenOrder& o, int
   const auto fits = [&](int64_t n) {
     return row_bytes % n == 0 && aligned(x, n) && aligned(rows, n);
   };
+  const bool shift = row_path(row_bytes, {x, rows}) == kShifted;
   if (fits(16)) return sort_rows<uint4>(x, rows, o, row_bytes, zero_tail, num_sms, s);
-  if (fits(4)) return sort_rows<uint32_t>(x, rows, o, row_bytes, zero_tail, num_sms, s);
-  if (fits(2)) return sort_rows<uint16_t>(x, rows, o, row_bytes, zero_tail, num_sms, s);
-  return sort_rows<uint8_t>(x, rows, o, row_bytes, zero_tail, num_sms, s);
+  if (fits(4))
+    return shift ? sort_shifted<4>(x, rows, o, row_bytes, zero_tail, num_sms, s)
+                 : sort_rows<uint32_t>(x, rows, o, row_bytes, zero_tail, num_sms, s);
+  if (fits(2))
+    return shift ? sort_shifted<2>(x, rows, o, row_bytes, zero_tail, num_sms, s)
+                 : sort_rows<uint16_t>(x, rows, o, row_bytes, zero_tail, num_sms, s);
+  return shift ? sort_shifted<1>(x, rows, o, row_bytes, zero_tail, num_sms, s)
+               : sort_rows<uint8_t>(x, rows, o, row_bytes, zero_tail, num_sms, s);
 }
 
 cudaError_t launch_unsort_rows(const void* rows, const float* w, void* y, int dtype,
                                const TokenOrder& o, int64_t H, cudaStream_t s) {
-  const int64_t bytes = H * (dtype == FMOE_DTYPE_F32 ? 4 : 2);
-  const bool vec = bytes % 16 == 0 && aligned(rows, 16) && aligned(y, 16);
   switch (dtype) {
     case FMOE_DTYPE_F32:
-      return unsort_rows<float>(rows, w, y, o, H, vec, s);
+      return unsort_rows<float>(rows, w, y, o, H, s);
     case FMOE_DTYPE_BF16:
-      return unsort_rows<__nv_bfloat16>(rows, w, y, o, H, vec, s);
+      return unsort_rows<__nv_bfloat16>(rows, w, y, o, H, s);
     default:
-      return unsort_rows<__half>(rows, w, y, o, H, vec, s);
+      return unsort_rows<__half>(rows, w, y, o, H, s);
   }
 }
 
 cudaError_t launch_unsort_back(const void* dy, const void* rows, const float* w, void* drows,
                                float* dw, int dtype, const TokenOrder& o, int64_t H, int num_sms,
                                cudaStream_t s) {
-  const int64_t bytes = H * (dtype == FMOE_DTYPE_F32 ? 4 : 2);
-  const bool vec = bytes % 16 == 0 && aligned(dy, 16) && aligned(drows, 16) &&
-                   (!dw || aligned(rows, 16));
   switch (dtype) {
     case FMOE_DTYPE_F32:
-      return unsort_back<float>(dy, rows, w, drows, dw, o, H, vec, num_sms, s);
+      return unsort_back<float>(dy, rows, w, drows, dw, o, H, num_sms, s);
     case FMOE_DTYPE_BF16:
-      return unsort_back<__nv_bfloat16>(dy, rows, w, drows, dw, o, H, vec, num_sms, s);
+      return unsort_back<__nv_bfloat16>(dy, rows, w, drows, dw, o, H, num_sms, s);
     default:
-      return unsort_back<__half>(dy, rows, w, drows, dw, o, H, vec, num_sms, s);
+      return unsort_back<__half>(dy, rows, w, drows, dw, o, H, num_sms, s);
   }
 }
 

@@ -72,6 +72,8 @@ ROWS = [
     (5, 8, 8, 4, -2, 16, 16, 24),
     (37, 2, 4, 0, 0, 4, 1, 1),
     (64, 9, 16, 0, 0, 16, 1, 1407),    # more than eight picks, odd rows
+    (67, 3, 7, 1, 0, 9, 4, 2047),      # odd rows of several blocks, some picks not local
+    (13, 2, 3, 0, 0, 3, 1, 8209),
     (130, 6, 20, 40, 0, 160, 128, 514),
     (700, 8, 32, 0, 0, 256, 1, 256),
 ]
@@ -153,6 +155,7 @@ def test_gradients_against_differences():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,H", [(torch.int8, 7168), (torch.int8, 33), (torch.uint8, 1),
+                                     (torch.int8, 1001), (torch.uint8, 5003),
                                      (torch.float8_e4m3fn, 130), (torch.float32, 0),
                                      (torch.int64, 3)])
 def test_sort_any_element_type(dtype, H):
@@ -171,11 +174,11 @@ def test_sort_any_element_type(dtype, H):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shift", [0, 1])
-def test_given_output_keeps_the_rows_behind(shift):
+@pytest.mark.parametrize("shift,H", [(0, 64), (1, 64), (0, 333), (1, 333)])
+def test_given_output_keeps_the_rows_behind(shift, H):
     """Rows from expert_base[E] on stay as they were, padding rows inside are zeroed; a tensor that
     starts off a 16-byte boundary gives the same rows."""
-    T, K, E, H = 21, 2, 3, 64
+    T, K, E = 21, 2, 3
     ids = _ids(T, K, E, 0, 6, 8)
     base, row_pick, pick_row = R.order(ids, 0, E, 16)
     o = fb.sort_by_expert(ids.cuda(), E, align=16)
