@@ -20,6 +20,9 @@ F32 = (torch.float32,)
 FLOATS = tuple(DTYPE_TAG)
 
 
+_FUNCTIONS = {}  # the library's entry points by name
+
+
 def _refuse(t, name: str, index: Optional[int], shape, dtypes) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -59,7 +62,9 @@ def ptr(t: Optional[torch.Tensor]):
 
 def call(name: str, index: int, *args) -> None:
     """One library call on CUDA device ``index`` and its current stream; raises on an error code."""
-    fn = getattr(_lib.load(), name)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_lib.load(), name)
     if index == torch.cuda.current_device():
         rc = fn(*args, _raw_stream(index))
     else:
@@ -67,6 +72,13 @@ def call(name: str, index: int, *args) -> None:
             rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
+
+
+def first_order_only() -> None:
+    """Called in a backward pass: refuses to be recorded itself (``create_graph=True``), since the
+    library's gradients have no gradient of their own."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("this operator has no second derivative (create_graph=True)")
 
 
 def recording(*tensors) -> bool:

@@ -11,11 +11,10 @@ from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import FmoeBlockNormArgs
-from ._op import DTYPE_TAG, FLOATS, call, first, need, ptr, recording
+from ._op import DTYPE_TAG, FLOATS, call, first, first_order_only, need, ptr, recording
 
 BLOCK = 128
 
@@ -81,8 +80,8 @@ class _BlockNorm(torch.autograd.Function):
         return hidden, normed
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_hidden, grad_normed):
+        first_order_only()
         branch, residual, post_weight, gate, pre_weight, stats = ctx.saved_tensors
         a = _args(branch, residual, post_weight, gate, pre_weight, *ctx.rest)
         if grad_hidden is not None:
@@ -92,19 +91,29 @@ class _BlockNorm(torch.autograd.Function):
             grad_normed = grad_normed.contiguous()
             a.grad_normed = grad_normed.data_ptr()
         a.stats = stats.data_ptr()
-        grads = [torch.empty_like(t) if t is not None and wanted else None
-                 for t, wanted in zip((branch, residual, post_weight, gate, pre_weight),
-                                      ctx.needs_input_grad)]
-        (a.grad_branch, a.grad_residual, a.grad_post_weight, a.grad_gate,
-         a.grad_pre_weight) = map(ptr, grads)
-        T, H = residual.shape
-        workspace = None
-        if grads[2] is not None or grads[3] is not None or grads[4] is not None:
-            size = _workspace_bytes(T, H)
-            workspace = residual.new_empty(size // 4, dtype=torch.float32)
+        need_f, need_x, need_wp, need_g, need_wq = ctx.needs_input_grad[:5]
+        d_f = d_x = d_wp = d_g = d_wq = workspace = None
+        if need_f:
+            d_f = torch.empty_like(branch)
+            a.grad_branch = d_f.data_ptr()
+        if need_x:
+            d_x = torch.empty_like(residual)
+            a.grad_residual = d_x.data_ptr()
+        if need_wp:
+            d_wp = torch.empty_like(post_weight)
+            a.grad_post_weight = d_wp.data_ptr()
+        if need_g:
+            d_g = torch.empty_like(gate)
+            a.grad_gate = d_g.data_ptr()
+        if need_wq:
+            d_wq = torch.empty_like(pre_weight)
+            a.grad_pre_weight = d_wq.data_ptr()
+        if need_wp or need_g or need_wq:
+            size = _workspace_bytes(*residual.shape)
+            workspace = stats.new_empty(size // 4)
             a.workspace, a.workspace_bytes = ptr(workspace), size
         call("fmoe_block_norm_backward", residual.get_device(), ctypes.byref(a))
-        return (*grads, None, None, None)
+        return d_f, d_x, d_wp, d_g, d_wq, None, None, None
 
 
 def block_norm(branch: Optional[torch.Tensor], residual: torch.Tensor, *,

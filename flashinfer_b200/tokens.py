@@ -13,11 +13,10 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import FmoeTokenOrder
-from ._op import DTYPE_TAG, F32, I32, call, first, need, ptr, recording
+from ._op import DTYPE_TAG, F32, I32, call, first, first_order_only, need, ptr, recording
 
 
 class ExpertOrder:
@@ -112,8 +111,8 @@ class _SortTokens(torch.autograd.Function):
         return _sort(x, order, None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_rows):
+        first_order_only()
         return _unsort(grad_rows.contiguous(), ctx.order, None, None), None
 
 
@@ -128,8 +127,8 @@ class _UnsortTokens(torch.autograd.Function):
         return _unsort(rows, order, weights, None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
+        first_order_only()
         rows, weights = ctx.saved_tensors
         order = ctx.order
         grad_y = grad_y.contiguous()

@@ -295,3 +295,12 @@ def test_refusals_on_the_host():
     assert run(back, grad_post_weight=6 << 20, stats=8 << 20) == -5
     assert run(back, grad_gate=6 << 20, stats=8 << 20) == -1
     assert run(back, grad_residual=2 << 20, stats=8 << 20) == -2
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    t = [v.requires_grad_() for v in _inputs(3, 32, torch.float32, True, "none", True)
+         if v is not None]
+    h, _ = fb.block_norm(t[0], t[1], post_weight=t[2], pre_weight=t[3])
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(h.sum(), t[0], create_graph=True)
