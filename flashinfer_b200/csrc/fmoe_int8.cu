@@ -57,90 +57,108 @@ __device__ __forceinline__ uint2 quant2(float2 x, float den, float inv) {
   return make_uint2(__float_as_uint(v.x), __float_as_uint(v.y));
 }
 
-// A row per G threads: a warp (WARP, eight rows per block) or the block. Up to VPT 16-byte granules
-// (VEC; else single elements) per thread stay in registers between the maximum and the rounding;
-// what a longer row has beyond them is read a second time.
+// A group (a warp with WARP, eight groups per block; else the block) takes rows first, first + step,
+// .... Up to VPT 16-byte granules (VEC; else single elements) of a row per thread stay in registers
+// between the maximum and the rounding, and the next row's are on their way meanwhile; what a longer
+// row has beyond them is read a second time. One row per block, without the next row's loads:
+// 8192 x 7168 took 44.7 us.
 template <typename T, bool VEC, int VPT, bool WARP>
-__global__ void __launch_bounds__(256, 6)
+__global__ void __launch_bounds__(256, 4)
     k_quantize_int8(const T* x, int64_t rows, int64_t K, int8_t* q, float* scale) {
   pdl_begin_in_order();
   using Unit = typename std::conditional<VEC, uint4, uint16_t>::type;
-  __shared__ uint32_t part[8];
+  __shared__ uint32_t part[2][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = WARP ? 32 : blockDim.x;
   const int g = WARP ? lane : static_cast<int>(threadIdx.x);
-  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
-  if (row >= rows) return;  // WARP: whole warps; no block barrier follows
   T* type = nullptr;
   const int64_t n = VEC ? K / 8 : K;
-  const Unit* xr = reinterpret_cast<const Unit*>(x) + row * n;
-  int8_t* qr = q + row * K;
-  Unit in[VPT];
-  uint32_t m2 = 0;
-  auto maximum = [&](const Unit& u) {
-    if constexpr (VEC) {
-      m2 = abs_max2(type, m2, u.x);
-      m2 = abs_max2(type, m2, u.y);
-      m2 = abs_max2(type, m2, u.z);
-      m2 = abs_max2(type, m2, u.w);
-    } else {
-      m2 = abs_max2(type, m2, u);
-    }
+  const Unit* xu = reinterpret_cast<const Unit*>(x);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? 8 : 1);
+  int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
+  Unit next[VPT];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (r < rows && g + i * G < n) next[i] = __ldcg(xu + r * n + g + i * G);
   };
+  fetch(row);
+  int flip = 0;
+  for (; row < rows; row += step, flip ^= 1) {
+    Unit in[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (g + static_cast<int64_t>(i) * G < n) in[i] = __ldcg(xr + g + static_cast<int64_t>(i) * G);
+    for (int i = 0; i < VPT; ++i) in[i] = next[i];
+    fetch(row + step);
+    const Unit* xr = xu + row * n;
+    int8_t* qr = q + row * K;
+    uint32_t m2 = 0;
+    auto maximum = [&](const Unit& u) {
+      if constexpr (VEC) {
+        m2 = abs_max2(type, m2, u.x);
+        m2 = abs_max2(type, m2, u.y);
+        m2 = abs_max2(type, m2, u.z);
+        m2 = abs_max2(type, m2, u.w);
+      } else {
+        m2 = abs_max2(type, m2, u);
+      }
+    };
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (g + static_cast<int64_t>(i) * G < n) maximum(in[i]);
-  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < n; v += G) maximum(__ldcg(xr + v));
-  // as ordered integers the bits of non-negative floats keep their order, NaN above infinity
-  const float2 halves = unpack2(type, m2);
-  uint32_t m = max(__float_as_uint(halves.x), __float_as_uint(halves.y)) & 0x7fffffffu;
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (!WARP) {
-    if (lane == 0) part[warp] = m;
-    __syncthreads();
-    for (int i = 0; i < (G >> 5); ++i) m = max(m, part[i]);
+    for (int i = 0; i < VPT; ++i)
+      if (g + i * G < n) maximum(in[i]);
+    for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < n; v += G) maximum(__ldcg(xr + v));
+    // as ordered integers the bits of non-negative floats keep their order, NaN above infinity
+    const float2 halves = unpack2(type, m2);
+    uint32_t m = max(__float_as_uint(halves.x), __float_as_uint(halves.y)) & 0x7fffffffu;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (!WARP) {  // one barrier: the next row uses the other buffer
+      if (lane == 0) part[flip][warp] = m;
+      __syncthreads();
+      for (int i = 0; i < (G >> 5); ++i) m = max(m, part[flip][i]);
+    }
+    m = max(m, __float_as_uint(1e-30f));
+    const float amax = __uint_as_float(m);
+    if (g == 0) scale[row] = __fdiv_rn(amax, 127.0f);
+    const bool finite = m < 0x7f800000u;  // else the row's values are zeros
+    const float den = amax * (1.0f / 256.0f);
+    const float inv = 1.0f / den;
+    auto put = [&](const Unit& u, int64_t v) {
+      if constexpr (VEC) {
+        const uint2 a = quant2(unpack2(type, u.x), den, inv), b = quant2(unpack2(type, u.y), den, inv);
+        const uint2 c = quant2(unpack2(type, u.z), den, inv), d = quant2(unpack2(type, u.w), den, inv);
+        uint2 w;
+        w.x = __byte_perm(__byte_perm(a.x, a.y, 0x0040), __byte_perm(b.x, b.y, 0x0040), 0x5410);
+        w.y = __byte_perm(__byte_perm(c.x, c.y, 0x0040), __byte_perm(d.x, d.y, 0x0040), 0x5410);
+        reinterpret_cast<uint2*>(qr)[v] = finite ? w : make_uint2(0u, 0u);
+      } else {
+        qr[v] = finite ? static_cast<int8_t>(quant2(unpack2(type, u), den, inv).x) : int8_t{0};
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (g + i * G < n) put(in[i], g + i * G);
+    for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < n; v += G) put(__ldcg(xr + v), v);
   }
-  m = max(m, __float_as_uint(1e-30f));
-  const float amax = __uint_as_float(m);
-  if (g == 0) scale[row] = __fdiv_rn(amax, 127.0f);
-  const bool finite = m < 0x7f800000u;  // else the row's values are zeros
-  const float den = amax * (1.0f / 256.0f);
-  const float inv = 1.0f / den;
-  auto put = [&](const Unit& u, int64_t v) {
-    if constexpr (VEC) {
-      const uint2 a = quant2(unpack2(type, u.x), den, inv), b = quant2(unpack2(type, u.y), den, inv);
-      const uint2 c = quant2(unpack2(type, u.z), den, inv), d = quant2(unpack2(type, u.w), den, inv);
-      uint2 w;
-      w.x = __byte_perm(__byte_perm(a.x, a.y, 0x0040), __byte_perm(b.x, b.y, 0x0040), 0x5410);
-      w.y = __byte_perm(__byte_perm(c.x, c.y, 0x0040), __byte_perm(d.x, d.y, 0x0040), 0x5410);
-      reinterpret_cast<uint2*>(qr)[v] = finite ? w : make_uint2(0u, 0u);
-    } else {
-      qr[v] = finite ? static_cast<int8_t>(quant2(unpack2(type, u), den, inv).x) : int8_t{0};
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (g + static_cast<int64_t>(i) * G < n) put(in[i], g + static_cast<int64_t>(i) * G);
-  for (int64_t v = g + static_cast<int64_t>(VPT) * G; v < n; v += G) put(__ldcg(xr + v), v);
 }
 
 template <typename T, bool VEC>
-cudaError_t quantize_rows(const void* x, int64_t rows, int64_t K, void* q, float* scale,
+cudaError_t quantize_rows(const void* x, int64_t rows, int64_t K, void* q, float* scale, int sms,
                           cudaStream_t s) {
   // a row of up to four units per lane is a warp's; a longer one a block's, with as few threads
-  // as hold four units each
+  // as hold four units each; as many blocks as run at a time (64 registers per thread)
   const int64_t n = VEC ? K / 8 : K;
   const T* xt = static_cast<const T*>(x);
   int8_t* qt = static_cast<int8_t*>(q);
-  if (n <= 32 * 4)
-    return launch_pdl(k_quantize_int8<T, VEC, 4, true>, dim3(static_cast<unsigned>((rows + 7) / 8)),
-                      dim3(256), 0, s, xt, rows, K, qt, scale);
+  if (n <= 32 * 4) {
+    const int64_t blocks = (rows + 7) / 8, most = static_cast<int64_t>(sms) * 4;
+    return launch_pdl(k_quantize_int8<T, VEC, 4, true>,
+                      dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, s,
+                      xt, rows, K, qt, scale);
+  }
   int64_t threads = (n + 127) / 128 * 32;
   if (threads > 256) threads = 256;
-  return launch_pdl(k_quantize_int8<T, VEC, 4, false>, dim3(static_cast<unsigned>(rows)),
+  const int64_t most = static_cast<int64_t>(sms) * (1024 / threads);
+  return launch_pdl(k_quantize_int8<T, VEC, 4, false>,
+                    dim3(static_cast<unsigned>(rows < most ? rows : most)),
                     dim3(static_cast<unsigned>(threads)), 0, s, xt, rows, K, qt, scale);
 }
 
@@ -1162,14 +1180,14 @@ cudaError_t configure(int dev) {
 }  // namespace
 
 cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, void* q,
-                                 float* scale, cudaStream_t s) {
+                                 float* scale, int sms, cudaStream_t s) {
   const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0 &&
                    (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
   if (dtype == FMOE_DTYPE_BF16)
-    return vec ? quantize_rows<__nv_bfloat16, true>(x, rows, K, q, scale, s)
-               : quantize_rows<__nv_bfloat16, false>(x, rows, K, q, scale, s);
-  return vec ? quantize_rows<__half, true>(x, rows, K, q, scale, s)
-             : quantize_rows<__half, false>(x, rows, K, q, scale, s);
+    return vec ? quantize_rows<__nv_bfloat16, true>(x, rows, K, q, scale, sms, s)
+               : quantize_rows<__nv_bfloat16, false>(x, rows, K, q, scale, sms, s);
+  return vec ? quantize_rows<__half, true>(x, rows, K, q, scale, sms, s)
+             : quantize_rows<__half, false>(x, rows, K, q, scale, sms, s);
 }
 
 cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {

@@ -251,7 +251,7 @@ struct Int8Product {
   int zero_tail;        // rows from expert_base[E] on are zeroed
 };
 cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, void* q,
-                                 float* scale, cudaStream_t s);
+                                 float* scale, int sms, cudaStream_t s);
 cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s);
 cudaError_t take_int8_status(int32_t* status, cudaStream_t s);
 

@@ -270,7 +270,7 @@ int fmoe_quantize_int8(const void* x, int32_t dtype, int64_t R, int64_t K, void*
   int sms = 0;
   const int rc = device_sms(&sms);
   if (rc) return rc;
-  return done(launch_quantize_int8(x, dtype, R, K, q, scale, as_stream(stream)));
+  return done(launch_quantize_int8(x, dtype, R, K, q, scale, sms, as_stream(stream)));
 }
 
 int fmoe_int8_matmul(const void* a, const void* b, const float* a_scale, const float* b_scale,
