@@ -292,7 +292,7 @@ __device__ __forceinline__ LanePick lane_pick(const RowsArgs& a, const float* w,
 // are in flight per thread; a pick without a row adds 0 * 0, so the sums have no branches. With
 // single conversions and a branch per pick the kernel issued 75 instructions per row and granule.
 template <typename T>
-__global__ void __launch_bounds__(256, 3)
+__global__ void __launch_bounds__(256, 4)
     k_unsort_granules(const T* rows, const float* w, T* y, const RowsArgs a) {
   pdl_begin_in_order();
   const int64_t t = static_cast<int64_t>(blockIdx.x / a.chunks) * blockDim.y + threadIdx.y;
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(256, 3)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         q[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (p.r[j] >= 0) q[j] = __ldcg(in + p.r[j] * a.nvec + v);
+        if (p.r[j] >= 0) q[j] = load_row16(in + p.r[j] * a.nvec + v);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc = fma(gran_of<T>(q[j]), p.f[j], acc);
