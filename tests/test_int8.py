@@ -62,7 +62,8 @@ def test_quantize_ties_extremes_and_non_finite():
 # M, N, K: one token to several tiles, odd sizes, a K tail inside a 128-byte block, short K
 SIZES = [(1, 1, 16), (1, 4096, 7168), (2, 128, 144), (15, 129, 128), (16, 257, 2048),
          (17, 100, 400), (64, 2047, 512), (65, 128, 1040), (130, 384, 4096), (255, 65, 272),
-         (300, 1000, 1024), (517, 2047, 7168), (1025, 130, 96), (2049, 256, 2064), (33, 7168, 16)]
+         (300, 1000, 1024), (517, 2047, 7168), (1025, 130, 96), (2049, 256, 2064), (33, 7168, 16),
+         (1, 3, 32), (2, 17, 7168), (3, 4097, 2064), (4, 1030, 7168), (4, 33, 11776), (4, 33, 11792)]
 
 
 @pytest.mark.gpu
