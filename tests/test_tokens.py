@@ -33,7 +33,10 @@ ORDERS = [
     (1237, 6, 20, 40, 0, 160, 16),
     (4099, 2, 1024, 0, 0, 1024, 3),
     (2500, 8, 3, 0, 0, 3, 1),          # every pick several times in a token
-    (9000, 8, 256, 0, 0, 256, 128),    # blocks of more than the least chunk
+    (513, 8, 257, 0, 0, 512, 1),       # too many experts for one cluster
+    (8191, 8, 200, 20, -1, 256, 7),    # the most picks of one cluster, nearly
+    (8193, 8, 256, 0, 0, 256, 1),      # one token more than a cluster takes
+    (20000, 8, 256, 0, 0, 256, 128),   # blocks of more than the least chunk
 ]
 
 
@@ -277,7 +280,9 @@ def test_refusals_on_the_host():
         return lib.fmoe_sort_size(*a, ctypes.byref(rows), ctypes.byref(scratch))
     assert size(4, 2, 4, 16) == 0 and rows.value == 8 + 4 * 15 and scratch.value == 0
     assert size(1, 2, 64, 16) == 0 and rows.value == 2 + 2 * 15
-    assert size(4096, 8, 256, 1) == 0 and rows.value == 32768 and scratch.value > 0
+    assert size(4096, 8, 256, 1) == 0 and rows.value == 32768 and scratch.value == 0
+    assert size(16384, 8, 256, 1) == 0 and rows.value == 131072 and scratch.value > 0
+    assert size(4096, 8, 257, 1) == 0 and scratch.value > 0
     for bad in ((-1, 2, 4, 1), (4, 0, 4, 1), (4, 2, 0, 1), (4, 2, 1025, 1), (4, 2, 4, 0),
                 (4, 2, 4, 1025), (2 ** 28, 8, 4, 1)):
         assert size(*bad) == -2, bad
@@ -289,7 +294,7 @@ def test_refusals_on_the_host():
     assert lib.fmoe_sort_by_expert(16, 0, 16, ref, None, 0, None) == -2      # 8 rows are too few
     assert lib.fmoe_sort_by_expert(18, 0, 1, ref, None, 0, None) == -3
     assert lib.fmoe_sort_by_expert(8192, 0, 1, ref, None, 0, None) == -2     # overlaps row_pick
-    big = _lib.FmoeTokenOrder(4096, 8, 4, 32768, 1 << 20, 2 << 20, 3 << 20)
+    big = _lib.FmoeTokenOrder(16384, 8, 4, 131072, 1 << 20, 2 << 20, 3 << 20)
     assert lib.fmoe_sort_by_expert(16, 0, 1, ctypes.byref(big), None, 0, None) == -5
     few = _lib.FmoeTokenOrder(4, 2, 4, 7, 4096, 8192, 12288)
     assert lib.fmoe_sort_rows(16, 8, ctypes.byref(few), 1 << 20, 1, None) == -2
