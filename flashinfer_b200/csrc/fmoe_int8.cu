@@ -187,6 +187,7 @@ struct alignas(16) I8Tail {
   uint64_t tfull[2];
   uint64_t tempty[2];
   uint64_t drain;
+  uint64_t never;
   uint32_t tmem_base;
   int abort_flag;
   int tiles;
@@ -207,6 +208,10 @@ struct I8Args {
   int N, E, nkb, S;
   int dtype;                  // output
   int zero_tail;
+  // every bounded wait gives up after wait_ns; inject: the MMA warp first waits on a barrier that
+  // nothing arrives on (tests of the failure path only)
+  unsigned long long wait_ns;
+  int inject;
 };
 
 template <int BN>
@@ -268,11 +273,11 @@ __device__ __forceinline__ I8Tile decode_tile(int tile, int NT, const I8Tail* t,
   return r;
 }
 
-// Waits for the phase with the given parity; gives up after FMOE_WAIT_NS, or when another role of
+// Waits for the phase with the given parity; gives up after limit_ns, or when another role of
 // this CTA has (both looked at every few hundred polls). park: each poll may suspend the thread for
 // a while.
 __device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                        bool park) {
+                                        uint64_t limit_ns, bool park) {
   uint64_t t0 = 0;
   const uint32_t often = park ? 15u : 511u;
   for (uint32_t polls = 1;; ++polls) {
@@ -281,7 +286,7 @@ __device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, volatile
       if (*abort_flag) return false;
       const uint64_t now = global_timer_ns();
       if (t0 == 0) t0 = now;
-      if (now - t0 > FMOE_WAIT_NS) return false;
+      if (now - t0 > limit_ns) return false;
     }
   }
 }
@@ -515,6 +520,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       mbar_init(&tail->tempty[b], kI8EpiWarps * 32);
     }
     mbar_init(&tail->drain, 1);
+    mbar_init(&tail->never, 1);
     tail->abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tm_a);
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           // This producer issued iteration it - kI8Producers after that stage's release, and the
           // MMA warp releases in order, so with NS > kI8Producers the barrier is at most one
           // phase behind and the parity wait is unambiguous.
-          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, true)) {
+          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns, true)) {
             i8_abort(tail);
             ok = false;
             break;
@@ -608,20 +614,20 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
       int it = 0, n = 0;
-      bool ok = true;
+      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns, false);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
         const I8Tile u = decode_tile<BN>(tile, NT, tail, E);
         const uint32_t idesc = idesc_i8(kWRows, u.cols);
         const int b = n & 1, rb = n >> 1;
         const uint32_t d = tmem + b * BN;
-        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, false)) {
+        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns, false)) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % NS, r = it / NS;
-          if (!i8_wait(&tail->full[s], r & 1, abort_flag, false)) {
+          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns, false)) {
             ok = false;
             break;
           }
@@ -665,7 +671,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
       // after a wait that ran out, the warp still takes part in the barriers of later tiles
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, false));
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, false));
       if (!ok) {
         if (lane == 0) i8_abort(tail);
         continue;
@@ -799,6 +805,7 @@ struct alignas(16) PairTail {
   uint64_t tfull[2];
   uint64_t tempty[2];           // the leader's: every epilogue warp of both CTAs
   uint64_t drain;
+  uint64_t never;
   uint32_t tmem_base;
   int abort_flag;
   int tiles;
@@ -904,6 +911,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       mbar_init(&tail->tempty[b], 2 * kI8EpiWarps);
     }
     mbar_init(&tail->drain, 1);
+    mbar_init(&tail->never, 1);
     tail->abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tm_a);
@@ -976,7 +984,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           if (it % kI8Producers != pw) continue;
           const int s = it % kPairStages, r = it / kPairStages;
-          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, true)) {
+          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns, true)) {
             pair_abort(tail);
             ok = false;
             break;
@@ -995,20 +1003,20 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     // ---------------------------------------------------------------- MMA issuer (the leader's)
     if (rank == 0 && lane == 0) {
       int it = 0, n = 0;
-      bool ok = true;
+      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns, false);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
         const I8Tile u = decode_pair(tile, NT, tail, E);
         const uint32_t idesc = idesc_i8(2 * kWRows, u.cols);
         const int b = n & 1, rb = n >> 1;
         const uint32_t d = tmem + b * kPairTokens;
-        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, false)) {
+        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns, false)) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % kPairStages, r = it / kPairStages;
-          if (!i8_wait(&tail->full[s], r & 1, abort_flag, false)) {
+          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns, false)) {
             ok = false;
             break;
           }
@@ -1053,7 +1061,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
       // after a wait that ran out, the warp still takes part in the barriers of later tiles
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, false));
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, false));
       if (!ok) {
         if (lane == 0) pair_abort(tail);
         continue;
@@ -1191,6 +1199,8 @@ I8Args i8_args(const Int8Product& p, int S) {
   a.S = S;
   a.dtype = p.out_dtype;
   a.zero_tail = p.zero_tail;
+  a.wait_ns = p.wait_ns != 0 ? p.wait_ns : FMOE_WAIT_NS;
+  a.inject = p.wait_ns != 0;
   return a;
 }
 
@@ -1276,7 +1286,7 @@ cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
   // The tensor cores take 11.7 us for 1 to 4 tokens x 4096 x 7168 and 24.7 for 16384 channels, which
   // are enough tiles for every SM; this way 1, 2 and 4 tokens take 8.0, 9.3 and 9.0 us, and with
   // 16384 channels one token takes 20.8 and four take 29.0.
-  if (!p.expert_base && p.M <= kGemvTokens && p.M * p.K <= kGemvSmem &&
+  if (p.wait_ns == 0 && !p.expert_base && p.M <= kGemvTokens && p.M * p.K <= kGemvSmem &&
       (p.M <= 2 || p.N <= 64 * sms)) {
     switch (p.M) {
       case 1:

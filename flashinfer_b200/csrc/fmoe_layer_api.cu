@@ -69,7 +69,13 @@ int check_order(const FmoeTokenOrder* o, TokenOrder* out) {
 // Blocks of 256 threads along every row must fit one grid dimension.
 bool grid_fits(int64_t rows, int64_t units) { return rows * (units / 256 + 1) < INT32_MAX - 4096; }
 
-int int8_product(const Int8Product& p, void* stream) {
+// One-shot failure-path injection of fmoe_debug_arm_int8_timeout for this host thread's next product.
+thread_local unsigned long long g_int8_wait_ns = 0;
+
+int int8_product(const Int8Product& call, void* stream) {
+  Int8Product p = call;
+  p.wait_ns = g_int8_wait_ns;
+  g_int8_wait_ns = 0;
   if (p.M < 0 || p.M > INT32_MAX - 1024 || p.N < 1 || p.K < 16 || p.K % 16 != 0 || p.K > 131056 ||
       p.E < 1 || p.E > kMaxLocalExperts ||
       static_cast<int64_t>(p.E) * p.N > INT32_MAX - 1024)
@@ -277,7 +283,7 @@ int fmoe_int8_matmul(const void* a, const void* b, const float* a_scale, const f
                      const float* bias, int64_t m, int32_t n, int32_t k, void* out,
                      int32_t out_dtype, void* stream) {
   return int8_product(
-      Int8Product{a, b, a_scale, b_scale, bias, nullptr, out, m, n, k, 1, out_dtype, 0}, stream);
+      Int8Product{a, b, a_scale, b_scale, bias, nullptr, out, m, n, k, 1, out_dtype, 0, 0}, stream);
 }
 
 int fmoe_int8_expert_matmul(const void* rows, const void* weights, const float* row_scale,
@@ -286,8 +292,14 @@ int fmoe_int8_expert_matmul(const void* rows, const void* weights, const float* 
                             int32_t zero_tail, void* stream) {
   if (R > 0 && !expert_base) return FMOE_ERR_NULL;
   return int8_product(Int8Product{rows, weights, row_scale, weight_scale, nullptr, expert_base, out,
-                                  R, n, k, E, out_dtype, zero_tail},
+                                  R, n, k, E, out_dtype, zero_tail, 0},
                       stream);
+}
+
+int fmoe_debug_arm_int8_timeout(uint64_t wait_ns) {
+  if (wait_ns < 100000ull || wait_ns > 2000000000ull) return FMOE_ERR_SHAPE;
+  g_int8_wait_ns = wait_ns;
+  return FMOE_OK;
 }
 
 int fmoe_int8_status(int32_t* status, void* stream) {

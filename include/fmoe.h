@@ -416,6 +416,11 @@ FMOE_API int fmoe_int8_expert_matmul(const void* rows, const void* weights, cons
  * last call (its output is not valid), else 0; synchronises the stream and clears the word. */
 FMOE_API int fmoe_int8_status(int32_t* status, void* cuda_stream);
 
+/* Failure-path test, as fmoe_debug_arm_timeout: the next int8 product of the calling host thread
+ * first waits on a barrier nothing arrives on, every wait of it limited to wait_ns (100 us .. 2 s).
+ * The kernel gives up, sets the status bit and returns; its output is not valid. One-shot. */
+FMOE_API int fmoe_debug_arm_int8_timeout(uint64_t wait_ns);
+
 /* The norms before and after a block, with its gate and the residual scale. Per token:
  *   n = post_weight ? branch * rsqrt(mean(branch^2) + eps) * post_weight : branch
  *   hidden = residual_scale * residual + gate * n

@@ -246,3 +246,30 @@ def test_refusals_on_the_host():
     assert lib.fmoe_quantize_int8(A, 1, 4, 8, A, S, None) == -2
     assert lib.fmoe_quantize_int8(A, 1, 0, 8, None, None, None) == 0
     assert lib.fmoe_int8_status(None, None) == -1
+    assert lib.fmoe_debug_arm_int8_timeout(10) == -2             # below 100 us
+    assert lib.fmoe_debug_arm_int8_timeout(3_000_000_000) == -2  # above 2 s
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(40, 1024, 4096), (200, 12800, 256), (600, 2048, 4096),
+                                   (2048, 4096, 256)])
+def test_a_wait_that_runs_out_ends_the_product(M, N, K):
+    """One CTA per tile, its K split, CTA pairs and theirs: a wait that nothing ends gives up after
+    its 5 ms, the status says so once, and the next product (which needs the same tensor memory) is
+    right."""
+    import time
+    g = _gen(M)
+    a, w = _int8(g, M, K), _int8(g, N, K)
+    a_s, w_s = torch.rand(M, generator=g, device="cuda"), torch.rand(N, generator=g, device="cuda")
+    fb.int8_matmul(a, w, a_s, w_s)
+    assert fb.int8_status() == 0
+    assert _lib.load().fmoe_debug_arm_int8_timeout(5_000_000) == 0
+    t0 = time.perf_counter()
+    fb.int8_matmul(a, w, a_s, w_s)
+    assert fb.int8_status() == _lib.STATUS_TIMEOUT_INT8
+    assert time.perf_counter() - t0 < 1.0
+    assert fb.int8_status() == 0
+    y = fb.int8_matmul(a, w, a_s, w_s)
+    ref, err = R.product(a, w, a_s, w_s)
+    R.check(y, ref, err, "after")
+    assert fb.int8_status() == 0
