@@ -464,18 +464,19 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// The eight sums of a block's threads, added in a fixed order (lane tree, warps ascending), to
+// N (4 or 8) sums of a block's threads, added in a fixed order (lane tree, warps ascending), to
 // dw[t, k0 ..]. One barrier: the next call uses another `part`.
-__device__ __forceinline__ void store_dots(float (&dot)[8], float* dw, int64_t t, int k0, int K,
+template <int N>
+__device__ __forceinline__ void store_dots(float (&dot)[N], float* dw, int64_t t, int k0, int K,
                                            float (*part)[8]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarp = blockDim.x >> 5;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < N; ++j) {
     const float s = warp_sum_f32(dot[j]);
     if (lane == 0) part[warp][j] = s;
   }
   __syncthreads();
-  if (threadIdx.x < 8 && k0 + static_cast<int>(threadIdx.x) < K) {
+  if (threadIdx.x < N && k0 + static_cast<int>(threadIdx.x) < K) {
     float s = 0.0f;
     for (int i = 0; i < nwarp; ++i) s += part[i][threadIdx.x];
     dw[t * K + k0 + threadIdx.x] = s;
@@ -512,7 +513,8 @@ __global__ void __launch_bounds__(256, 3)
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot2[j] = make_float2(0.0f, 0.0f);
       // whole warps keep going for the shuffles
-      for (int v0 = 0; v0 < nvec; v0 += blockDim.x) {
+      const bool any = (__ballot_sync(0xffffffffu, p.r >= 0) >> k & 0xffu) != 0;
+      for (int v0 = 0; any && v0 < nvec; v0 += blockDim.x) {
         const int v = v0 + threadIdx.x;
         uint4 gq = make_uint4(0u, 0u, 0u, 0u), q[8];
         if (v < nvec) gq = __ldcg(g_in + v);
@@ -610,20 +612,33 @@ __device__ __forceinline__ uint4 granule(const uint8_t* base, int64_t g, int64_t
   return q;
 }
 
-// Bytes [by, by + 16) of the 32 bytes lo, hi (0 <= by < 16).
+// The granule of a row's reader: rows before the tensor's last (`last` is uniform) have at least
+// 512 bytes behind them, so only the lane's place in its own row needs a look.
+__device__ __forceinline__ uint4 row_granule(const uint8_t* base, int64_t g, int64_t total, bool last,
+                                             bool near) {
+  if (last || g < 0) return granule(base, g, total);
+  uint4 q = make_uint4(0u, 0u, 0u, 0u);
+  if (near) q = __ldcg(reinterpret_cast<const uint4*>(base) + g);
+  return q;
+}
+
+// Bytes [by, by + 16) of the 32 bytes lo, hi (0 <= by < 16, the same in the whole warp).
 __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int by) {
-  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  if (by & 8) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-  }
-  if (by & 4) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  }
   const int bits = (by & 3) * 8;
-  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
-                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+  switch (by >> 2) {
+    case 0:
+      return make_uint4(__funnelshift_r(lo.x, lo.y, bits), __funnelshift_r(lo.y, lo.z, bits),
+                        __funnelshift_r(lo.z, lo.w, bits), __funnelshift_r(lo.w, hi.x, bits));
+    case 1:
+      return make_uint4(__funnelshift_r(lo.y, lo.z, bits), __funnelshift_r(lo.z, lo.w, bits),
+                        __funnelshift_r(lo.w, hi.x, bits), __funnelshift_r(hi.x, hi.y, bits));
+    case 2:
+      return make_uint4(__funnelshift_r(lo.z, lo.w, bits), __funnelshift_r(lo.w, hi.x, bits),
+                        __funnelshift_r(hi.x, hi.y, bits), __funnelshift_r(hi.y, hi.z, bits));
+    default:
+      return make_uint4(__funnelshift_r(lo.w, hi.x, bits), __funnelshift_r(hi.x, hi.y, bits),
+                        __funnelshift_r(hi.y, hi.z, bits), __funnelshift_r(hi.z, hi.w, bits));
+  }
 }
 
 // Stores the bytes [lo, hi) of q to the granule at p (element size E).
@@ -657,14 +672,15 @@ struct Granules3 {
   uint4 before, at, after;
 };
 
-__device__ __forceinline__ Granules3 load3(const uint8_t* base, int64_t g, int64_t total) {
+__device__ __forceinline__ Granules3 load3(const uint8_t* base, int64_t g, int64_t total, bool last,
+                                           bool near) {
   const int lane = threadIdx.x & 31;
   Granules3 t;
-  t.at = granule(base, g, total);
+  t.at = row_granule(base, g, total, last, near);
   t.before = shfl_granule(t.at, lane - 1 < 0 ? 0 : lane - 1);
   t.after = shfl_granule(t.at, lane + 1 > 31 ? 31 : lane + 1);
-  if (lane == 0) t.before = granule(base, g - 1, total);
-  if (lane == 31) t.after = granule(base, g + 1, total);
+  if (lane == 0) t.before = row_granule(base, g - 1, total, last, near);
+  if (lane == 31) t.after = row_granule(base, g + 1, total, last, near);
   return t;
 }
 
@@ -690,7 +706,8 @@ __global__ void __launch_bounds__(256)
   const int64_t v = static_cast<int64_t>(blockIdx.x % a.chunks) * blockDim.x + threadIdx.x;
   const int64_t start = t * a.bytes;
   const int from = static_cast<int>(start & 15);
-  const Granules3 g = load3(x, start / 16 + v, a.T * a.bytes);
+  const bool near = v * 16 < a.bytes + 32;
+  const Granules3 g = load3(x, start / 16 + v, a.T * a.bytes, t == a.T - 1, near);
   const int32_t* pr = a.pick_row + t * a.K;
   for (int k0 = 0; k0 < a.K; k0 += 8) {
     int picks[8];
@@ -710,44 +727,44 @@ __global__ void __launch_bounds__(256)
 }
 
 // As k_unsort_granules. Each of the eight rows is read at this token's offset: a granule and its
-// neighbour, which the next lane has.
+// neighbour, which the next lane has; the last lane of a warp only lends its granule, so a warp
+// finishes 31.
 template <typename T>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, 3)
     k_unsort_shifted(const T* rows, const float* w, T* y, const RowsArgs a) {
   pdl_begin_in_order();
   const int64_t t = blockIdx.x / a.chunks;
-  const int64_t v = static_cast<int64_t>(blockIdx.x % a.chunks) * blockDim.x + threadIdx.x;
   const int lane = threadIdx.x & 31;
+  const int warp = (blockIdx.x % a.chunks) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int64_t v = static_cast<int64_t>(warp) * 31 + lane;
   const uint8_t* in = reinterpret_cast<const uint8_t*>(rows);
   const int64_t start = t * a.bytes, total = a.R * a.bytes;
   const int to = static_cast<int>(start & 15);
+  const bool near = v * 16 < a.bytes + 32;
   Gran<T> acc;
   zero(acc);
   for (int k0 = 0; k0 < a.K; k0 += 8) {
     const Picks p = load_picks(a, w, t, k0);
-    uint4 q[8], last[8];
+    uint4 q[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      q[j] = last[j] = make_uint4(0u, 0u, 0u, 0u);
+      q[j] = make_uint4(0u, 0u, 0u, 0u);
       if (p.r[j] >= 0) {
         // this granule's bytes lie at row start + v * 16 - to
         const int64_t at = p.r[j] * a.bytes + v * 16 - to;
-        const int64_t g = at >= 0 ? at / 16 : -1;  // at > -16
-        q[j] = granule(in, g, total);
-        if (lane == 31) last[j] = granule(in, g + 1, total);
+        q[j] = row_granule(in, at >= 0 ? at / 16 : -1, total, p.r[j] == a.R - 1, near);  // at > -16
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      uint4 next = shfl_granule(q[j], lane + 1 > 31 ? 31 : lane + 1);
-      if (lane == 31) next = last[j];
-      if (p.r[j] < 0) continue;
+      if (p.r[j] < 0) continue;  // the same in the whole warp
+      const uint4 next = shfl_granule(q[j], lane < 31 ? lane + 1 : 31);
       const int by = static_cast<int>((p.r[j] * a.bytes + 16 - to) & 15);
       acc = fma(gran_of<T>(shifted(q[j], next, by)), p.f[j], acc);
     }
   }
   const int64_t lo = to - v * 16, hi = to + a.bytes - v * 16;
-  if (hi > 0)
+  if (hi > 0 && lane < 31)
     store_part<sizeof(T)>(reinterpret_cast<uint8_t*>(y) + (start - to) + v * 16, words_of(acc),
                           static_cast<int>(lo < 0 ? 0 : lo), static_cast<int>(hi > 16 ? 16 : hi));
 }
@@ -755,7 +772,7 @@ __global__ void __launch_bounds__(256, 2)
 // As k_unsort_back_granules: dy is shifted to each row's offset; bytes of neighbouring rows count
 // as zero in the sums.
 template <typename T>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, 3)
     k_unsort_back_shifted(const T* dy, const T* rows, const float* w, T* drows, float* dw,
                           const RowsArgs a) {
   pdl_begin_in_order();
@@ -769,24 +786,28 @@ __global__ void __launch_bounds__(256, 2)
   const int64_t start = t * a.bytes, total = a.R * a.bytes;
   const int from = static_cast<int>(start & 15);
   const uint8_t* in = reinterpret_cast<const uint8_t*>(rows);
-  for (int k0 = 0; k0 < a.K; k0 += 8) {
+  // four picks at a time: eight take 120 registers (4096 x 2047: 115 us with eight, 106 with four)
+  for (int k0 = 0; k0 < a.K; k0 += 4) {
     const Picks p = load_picks(a, w, t, k0);
-    float2 dot2[8];
+    float2 dot2[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dot2[j] = make_float2(0.0f, 0.0f);
-    for (int64_t v0 = 0; v0 < a.nvec; v0 += blockDim.x) {
+    for (int j = 0; j < 4; ++j) dot2[j] = make_float2(0.0f, 0.0f);
+    const bool any = p.r[0] >= 0 || p.r[1] >= 0 || p.r[2] >= 0 || p.r[3] >= 0;
+    for (int64_t v0 = 0; any && v0 < a.nvec; v0 += blockDim.x) {
       const int64_t v = v0 + threadIdx.x;
-      uint4 q[8];
+      uint4 q[4];
       if (dw) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j) {
           q[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (p.r[j] >= 0 && v < a.nvec) q[j] = granule(in, p.r[j] * a.bytes / 16 + v, total);
+          if (p.r[j] >= 0 && v < a.nvec)
+            q[j] = row_granule(in, p.r[j] * a.bytes / 16 + v, total, p.r[j] == a.R - 1, true);
         }
       }
-      const Granules3 g3 = load3(reinterpret_cast<const uint8_t*>(dy), start / 16 + v, a.T * a.bytes);
+      const Granules3 g3 = load3(reinterpret_cast<const uint8_t*>(dy), start / 16 + v, a.T * a.bytes,
+                                 t == a.T - 1, v < a.nvec);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
         if (p.r[j] < 0) continue;
         const int to = static_cast<int>((p.r[j] * a.bytes) & 15);
         const int64_t lo64 = to - v * 16, hi64 = to + a.bytes - v * 16;
@@ -812,10 +833,10 @@ __global__ void __launch_bounds__(256, 2)
       }
     }
     if (dw) {
-      float dot[8];
+      float dot[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot[j] = p.r[j] >= 0 ? dot2[j].x + dot2[j].y : 0.0f;
-      store_dots(dot, dw, t, k0, a.K, part[(k0 >> 3) & 1]);
+      for (int j = 0; j < 4; ++j) dot[j] = p.r[j] >= 0 ? dot2[j].x + dot2[j].y : 0.0f;
+      store_dots(dot, dw, t, k0, a.K, part[(k0 >> 2) & 1]);
     }
   }
 }
@@ -889,12 +910,13 @@ RowPath row_path(int64_t bytes, std::initializer_list<const void*> tensors) {
   return bytes % 16 == 0 ? kGranules : bytes >= 512 ? kShifted : kElements;
 }
 
-// Blocks along the granules of a shifted row (at most two more than its size gives).
-RowGrid shifted_grid(int64_t T, int64_t bytes) {
-  const int64_t n = bytes / 16 + 2;
+// Blocks along the granules of a shifted row (at most two more than its size gives), of which a warp
+// finishes per_warp.
+RowGrid shifted_grid(int64_t T, int64_t bytes, int per_warp) {
+  const int64_t warps = (bytes / 16 + 2 + per_warp - 1) / per_warp;
   RowGrid g{};
-  g.chunks = static_cast<int>((n + 255) / 256);
-  g.block = dim3(static_cast<unsigned>(((n + g.chunks - 1) / g.chunks + 31) / 32 * 32), 1);
+  g.chunks = static_cast<int>((warps + 7) / 8);
+  g.block = dim3(static_cast<unsigned>((warps + g.chunks - 1) / g.chunks * 32), 1);
   g.blocks = T * g.chunks;
   return g;
 }
@@ -903,7 +925,7 @@ template <int E>
 cudaError_t sort_shifted(const void* x, void* rows, const TokenOrder& o, int64_t row_bytes,
                          int zero_tail, int num_sms, cudaStream_t s) {
   RowsArgs a = rows_args(o, 0, row_bytes);
-  const RowGrid g = shifted_grid(o.T, row_bytes);
+  const RowGrid g = shifted_grid(o.T, row_bytes, 32);
   a.chunks = g.chunks;
   a.copy_blocks = static_cast<int>(g.blocks);
   a.zero_tail = zero_tail;
@@ -917,7 +939,7 @@ cudaError_t unsort_rows(const void* rows, const float* w, void* y, const TokenOr
   const int64_t bytes = H * static_cast<int64_t>(sizeof(T));
   const RowPath path = row_path(bytes, {rows, y});
   RowsArgs a = rows_args(o, path == kGranules ? H / kV<T> : H, bytes);
-  const RowGrid g = path == kShifted ? shifted_grid(o.T, bytes)
+  const RowGrid g = path == kShifted ? shifted_grid(o.T, bytes, 31)
                                      : row_grid(o.T, a.nvec, path == kGranules ? 1 : 4);
   a.chunks = g.chunks;
   return launch_pdl(path == kGranules  ? k_unsort_granules<T>
