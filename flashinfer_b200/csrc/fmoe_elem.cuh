@@ -193,6 +193,26 @@ __device__ __forceinline__ uint4 words_of(const Gran<T>& g) {
   }
 }
 
+// Stores the bytes [lo, hi) of q to the granule at p (element size E).
+template <int E>
+__device__ __forceinline__ void store_part(uint8_t* p, const uint4& q, int lo, int hi) {
+  if (lo <= 0 && hi >= 16) {
+    *reinterpret_cast<uint4*>(p) = q;
+    return;
+  }
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 16; i += E) {
+    if (i < lo || i >= hi) continue;
+    if constexpr (E == 4)
+      *reinterpret_cast<uint32_t*>(p + i) = w[i / 4];
+    else if constexpr (E == 2)
+      *reinterpret_cast<uint16_t*>(p + i) = static_cast<uint16_t>(w[i / 4] >> (8 * (i % 4)));
+    else
+      p[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
 __device__ __forceinline__ float warp_sum_f32(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

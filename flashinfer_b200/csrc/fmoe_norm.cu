@@ -538,21 +538,15 @@ __device__ __forceinline__ Gran<T> get_own(const float4* p, int stride) {
   return r;
 }
 
-// V columns from column col0 on, whose place is p; columns outside the row stay. A granule across
-// the row's edge goes element by element, by way of the thread's `edge` slot.
+// V columns from column col0 on, whose place is p; columns outside the row stay.
 template <typename T, bool ODD>
-__device__ __forceinline__ void store_granule(T* p, int col0, int H, const Gran<T>& g,
-                                              uint4* edge) {
+__device__ __forceinline__ void store_granule(T* p, int col0, int H, const Gran<T>& g) {
+  constexpr int S = sizeof(T);
   const uint4 w = words_of(g);
-  if (!ODD || (col0 >= 0 && col0 + kV<T> <= H)) {
+  if constexpr (ODD)
+    store_part<S>(reinterpret_cast<uint8_t*>(p), w, -col0 * S, (H - col0) * S);
+  else
     *reinterpret_cast<uint4*>(p) = w;
-  } else {
-    *edge = w;
-    const int hi = H - col0 < kV<T> ? H - col0 : kV<T>;
-#pragma unroll 1
-    for (int j = col0 < 0 ? -col0 : 0; j < hi; ++j)
-      p[j] = reinterpret_cast<const T*>(edge)[j];
-  }
 }
 
 // Where a thread stands: its group, its columns (granule i starts at col0 + i * step, of which the
@@ -602,7 +596,6 @@ __global__ void __launch_bounds__(kRingThreads, 2)
   constexpr int V = kV<T>;
   extern __shared__ uint4 ring[];   // [stages][gpb][narr][slots], then wg and wq per thread
   __shared__ float4 sums[4][kRingThreads / 64][4];  // [row parity and call site][group]
-  __shared__ uint4 edge[ODD ? kRingThreads : 1];
   const RowWalk<T, VPT, ODD> w(a, r);
   const int H = a.H, G = r.G;
   const bool has_f = COMMON || in.f != nullptr, has_wq = COMMON || in.wq != nullptr;
@@ -610,7 +603,6 @@ __global__ void __launch_bounds__(kRingThreads, 2)
   float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * r.narr * r.slots) +
                 threadIdx.x;
   const int own_step = blockDim.x * (V / 4);
-  uint4* my_edge = &edge[ODD ? threadIdx.x : 0];
   for (int i = threadIdx.x; i < static_cast<int>(sizeof(sums) / 16); i += blockDim.x)
     (&sums[0][0][0])[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   __syncthreads();
@@ -684,7 +676,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
         }
         if (has_h)
           store_granule<T, ODD>(static_cast<T*>(out.h) + off + i * w.step, w.col0 + i * w.step, H,
-                                h[i], my_edge);
+                                h[i]);
         dot(sq, h[i], h[i]);
       }
     }
@@ -732,7 +724,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
         }
       }
       if (live)
-        store_granule<T, ODD>(static_cast<T*>(out.y) + off + i * w.step, col, H, h[i], my_edge);
+        store_granule<T, ODD>(static_cast<T*>(out.y) + off + i * w.step, col, H, h[i]);
     }
   }
   cp_async_wait(0);
@@ -746,7 +738,6 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   constexpr int V = kV<T>;
   extern __shared__ uint4 ring[];   // [stages][gpb][narr][slots], then wg and wq per thread
   __shared__ float4 sums[2][kRingThreads / 64][3 * 4];  // [row parity][group][sum]
-  __shared__ uint4 edge[ODD ? kRingThreads : 1];
   const RowWalk<T, VPT, ODD> w(a, r);
   const int H = a.H, G = r.G;
   const bool has_f = COMMON || in.f != nullptr;
@@ -756,7 +747,6 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   float4* own = reinterpret_cast<float4*>(ring + static_cast<size_t>(r.stages) * r.gpb * r.narr * r.slots) +
                 threadIdx.x;
   const int own_step = blockDim.x * (V / 4);
-  uint4* my_edge = &edge[ODD ? threadIdx.x : 0];
   for (int i = threadIdx.x; i < static_cast<int>(sizeof(sums) / 16); i += blockDim.x)
     (&sums[0][0][0])[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   __syncthreads();
@@ -868,7 +858,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         const Gran<T> dh = fma(h[i], -c, tt[i]);
         if (d.dx)
           store_granule<T, ODD>(static_cast<T*>(d.dx) + at, col, H,
-                                a.s == 1.0f ? dh : mul(dh, a.s), my_edge);
+                                a.s == 1.0f ? dh : mul(dh, a.s));
         if (has_f) {
           const Gran<T> f = read_granule<T>(row + fa + i * G, w.skip(i));
           const Gran<T> wg = get_own<T>(own + i * own_step, blockDim.x);
@@ -876,13 +866,12 @@ __global__ void __launch_bounds__(kRingThreads, 1)
           if (full) {
             if (d.dg_row)
               store_granule<T, ODD>(static_cast<T*>(d.dg_row) + at, col, H,
-                                    mul(mul(f, wg), mul(dh, r1)), my_edge);
+                                    mul(mul(f, wg), mul(dh, r1)));
             gd = mul(gd, read_granule<T>(row + ga + i * G, w.skip(i)));
           }
           C[i] = fma(gd, f, C[i]);
           if (d.df)
-            store_granule<T, ODD>(static_cast<T*>(d.df) + at, col, H, fma(f, -k1, mul(gd, wg)),
-                                  my_edge);
+            store_granule<T, ODD>(static_cast<T*>(d.df) + at, col, H, fma(f, -k1, mul(gd, wg)));
         }
       }
     }
@@ -1043,7 +1032,7 @@ cudaError_t norm_direct(const BlockNorm& p, int sms, cudaStream_t s) {
 
 // Dynamic shared memory of a block: two blocks per SM in the forward pass, whose barriers each
 // other's work hides, and one in the backward pass, which holds its sums over rows in registers.
-// Static shared memory (sums, edges) comes on top.
+// Static shared memory (sums) comes on top.
 constexpr int kNormSmem = 212 * 1024;
 
 // The ring's shape for rows of ng granules, or stages = 0 if not even one stage fits.

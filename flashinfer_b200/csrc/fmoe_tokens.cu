@@ -641,26 +641,6 @@ __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int b
   }
 }
 
-// Stores the bytes [lo, hi) of q to the granule at p (element size E).
-template <int E>
-__device__ __forceinline__ void store_part(uint8_t* p, const uint4& q, int lo, int hi) {
-  if (lo <= 0 && hi >= 16) {
-    *reinterpret_cast<uint4*>(p) = q;
-    return;
-  }
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 16; i += E) {
-    if (i < lo || i >= hi) continue;
-    if constexpr (E == 4)
-      *reinterpret_cast<uint32_t*>(p + i) = w[i / 4];
-    else if constexpr (E == 2)
-      *reinterpret_cast<uint16_t*>(p + i) = static_cast<uint16_t>(w[i / 4] >> (8 * (i % 4)));
-    else
-      p[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
-  }
-}
-
 __device__ __forceinline__ uint4 shfl_granule(const uint4& q, int from) {
   return make_uint4(__shfl_sync(0xffffffffu, q.x, from), __shfl_sync(0xffffffffu, q.y, from),
                     __shfl_sync(0xffffffffu, q.z, from), __shfl_sync(0xffffffffu, q.w, from));
