@@ -87,6 +87,54 @@ def test_forward_and_gradients(T, H, dtype, post, gate, s, pre, f32):
             R.check(v, w, err[n], n)
 
 
+def _shifted(v):
+    """The same values in a tensor that starts one element off a 16-byte boundary."""
+    if v is None:
+        return None
+    out = torch.empty(v.numel() + 1, dtype=v.dtype, device="cuda")[1:].view(v.shape)
+    return out.copy_(v)
+
+
+# T, H, dtype, off the boundary: rows that take the kernels without a ring, and beside them rows
+# that take the ring
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,dtype,off", [(5, 200, "bf16", True), (3, 1000, "fp16", True),
+                                           (2, 2500, "fp32", True), (2, 16384, "fp32", False),
+                                           (6, 512, "bf16", False), (6, 513, "bf16", False)])
+@pytest.mark.parametrize("branch,post,gate,pre", [(False, False, "none", True),
+                                                  (True, False, "none", True),
+                                                  (True, True, "none", False),
+                                                  (True, True, "token", True),
+                                                  (True, False, "channel", True),
+                                                  (True, True, "full", True),
+                                                  (True, False, "full", False)])
+def test_every_form_on_every_path(T, H, dtype, off, branch, post, gate, pre):
+    dt, s = DT[dtype], 0.75
+    t = _inputs(T, H, dt, post, gate, pre, branch=branch)
+    leaves = R.norm_leaves(*t)
+    rh, ry = R.block_norm(*leaves, s, EPS)
+    eh, ey, *_ = R.block_norm_bounds(*[None if v is None else v.detach() for v in leaves], s, EPS)
+    if off:
+        t = [_shifted(v) for v in t]
+    t = [None if v is None else v.requires_grad_() for v in t]
+    hidden, normed = _call(t, s)
+    R.check(hidden, rh.detach(), eh, "hidden")
+    if pre:
+        R.check(normed, ry.detach(), ey, "normed")
+    g = torch.Generator().manual_seed(5)
+    da = torch.randn(T, H, generator=g).to(dt).cuda()
+    dy = torch.randn(T, H, generator=g).to(dt).cuda() if pre else None
+    names = [n for n, v in zip(("branch", "residual", "post_w", "gate", "pre_w"), t)
+             if v is not None]
+    live = [v for v in t if v is not None]
+    got = torch.autograd.grad((hidden, normed) if pre else (hidden,), live, (da, dy) if pre else (da,))
+    ref = torch.autograd.grad((rh, ry) if pre else (rh,), [v for v in leaves if v is not None],
+                              (da.double(), dy.double()) if pre else (da.double(),))
+    err = R.block_norm_grad_bounds(leaves, s, EPS, da, dy)
+    for n, v, w in zip(names, got, ref):
+        R.check(v, w, err[n], n)
+
+
 @pytest.mark.gpu
 def test_gradients_against_differences():
     """<gradient, v> against central differences of the 64-bit form along random v."""
