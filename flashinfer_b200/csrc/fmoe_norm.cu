@@ -9,12 +9,14 @@
 // fused expert layer's input (scale = max(amax, 1e-30) / 448, [H / 128, T]). h is kept in fp32
 // between the two norms and rounded once, on its way out.
 //
-// Gradients, from da (of h), dy (of y) and the saved r1, r2: with u = dy * wq, t = da + r2 * u,
-// m = f * wp (or f) and c = r2^3 / H * sum(u * h),
+// Gradients, from da (of h), dy (of y) and the saved r1, r2: with u = dy * wq, t = da + r2 * u
+// and c = r2^3 / H * sum(u * h),
 //   dh = t - c * h,  dx = s * dh,  dwq = sum over rows of dy * h * r2
-//   df = r1 * (g * wp * dh) - f * r1^3 / H * S1,  S1 = sum(g * m * dh) = sum(g m t) - c * sum(g m h)
+//   df = r1 * (g * wp * dh) - f * r1^2 / H * S1,  S1 = sum(g n dh) = sum(g n t) - c * sum(g n h)
 //   dwp = sum over rows of dh * g * f * r1,  dg = dh * n (summed over what the gate broadcasts to)
-// so one pass over the row collects all three sums before anything is written.
+// so one pass over the row collects all three sums before anything is written. r1 enters the sums,
+// and the cube of r2 is multiplied up from the sum's side, because without eps r1, r2 and f are of
+// opposite size: f * wp * h and r^3 alone leave fp32 for rows of 1e-13.
 // All sums and statistics are fp32; the sums over rows run in a fixed order (rows of a block
 // ascending, then blocks ascending).
 #include <atomic>
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(MAXT)
         for (int j = 0; j < V; ++j) tt[j] = fmaf(r2 * dy[j], wq[j], tt[j]);
       }
     };
-    float sum[3] = {0.0f, 0.0f, 0.0f};  // u h; (g) m t; (g) m h
+    float sum[3] = {0.0f, 0.0f, 0.0f};  // u h; (g) n t; (g) n h
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
@@ -332,22 +334,22 @@ __global__ void __launch_bounds__(MAXT)
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float m = tok ? f[j] * w[j] : g[j] * f[j] * w[j];
+          const float m = f[j] * r1 * (tok ? w[j] : g[j] * w[j]);
           sum[1] = fmaf(m, tt[j], sum[1]);
           sum[2] = fmaf(m, h[j], sum[2]);
         }
       }
     }
     block_sum<3>(sum, buf[flip]);
-    const float c = r2 * r2 * r2 * (sum[0] / a.H);
+    const float c = r2 * (r2 * (r2 * (sum[0] / a.H)));
     const float gm = sum[1] - c * sum[2];
     if (tok && d.dg_row && threadIdx.x == 0) {
       if (a.g_f32)
-        static_cast<float*>(d.dg_row)[t] = r1 * gm;
+        static_cast<float*>(d.dg_row)[t] = gm;
       else
-        from_f32(r1 * gm, static_cast<T*>(d.dg_row) + t);
+        from_f32(gm, static_cast<T*>(d.dg_row) + t);
     }
-    const float k1 = in.wp ? r1 * r1 * r1 * ((tok ? g_tok * gm : gm) / a.H) : 0.0f;
+    const float k1 = in.wp ? r1 * (r1 * ((tok ? g_tok * gm : gm) / a.H)) : 0.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
@@ -836,7 +838,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     cp_async_wait(r.stages - 1);
     const uint4* row = mine + s * stage;
     Gran<T> h[VPT], tt[VPT];
-    float2 s0 = make_float2(0.0f, 0.0f), s1 = s0, s2 = s0;  // u h; m t; m h (no token gate in m)
+    float2 s0 = make_float2(0.0f, 0.0f), s1 = s0, s2 = s0;  // u h; n t; n h (a token's gate apart)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       if (i < w.live) {
@@ -844,10 +846,10 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         Gran<T> m;
         zero(m);
         if (has_f) {
-          m = mul(read_granule<T>(row + fa + i * G, w.skip(i)),
+          m = mul(mul(read_granule<T>(row + fa + i * G, w.skip(i)), r1),
                   get_own<T>(own + i * own_step, blockDim.x));
           if (full) m = mul(m, read_granule<T>(row + ga + i * G, w.skip(i)));
-          h[i] = fma(m, rg, h[i]);
+          h[i] = fma(m, g_tok, h[i]);
         }
         zero(tt[i]);
         if (has_da) tt[i] = read_granule<T>(row + da + i * G, w.skip(i));
@@ -866,15 +868,15 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     fetch_first(s, ahead, off_ahead);  // x, da and dy are in registers now, as h and t
     float sum[3] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y};
     group_sum<3>(sum, &sums[flip][gr][0].x, w.group, G);
-    const float c = r2 * r2 * r2 * (sum[0] * inv_h);
+    const float c = r2 * (r2 * (r2 * (sum[0] * inv_h)));
     const float gm = sum[1] - c * sum[2];
     if (tok && d.dg_row && w.g == 0) {
       if (a.g_f32)
-        static_cast<float*>(d.dg_row)[t] = r1 * gm;
+        static_cast<float*>(d.dg_row)[t] = gm;
       else
-        from_f32(r1 * gm, static_cast<T*>(d.dg_row) + t);
+        from_f32(gm, static_cast<T*>(d.dg_row) + t);
     }
-    const float k1 = in.wp ? r1 * r1 * r1 * (g_tok * gm * inv_h) : 0.0f;
+    const float k1 = in.wp ? r1 * (r1 * (g_tok * gm * inv_h)) : 0.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       if (i < w.live) {

@@ -136,6 +136,30 @@ def test_every_form_on_every_path(T, H, dtype, off, branch, post, gate, pre):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("off", [False, True])
+def test_gradients_of_tiny_rows_without_eps(off):
+    """Rows of 1e-15 with eps 0: their norms' cubes leave fp32, the gradients do not."""
+    T, H, eps = 3, 264, 0.0
+    g = torch.Generator().manual_seed(4)
+    t = [(1e-15 * torch.randn(T, H, generator=g)).cuda(), (1e-15 * torch.randn(T, H, generator=g)).cuda(),
+         (1 + torch.rand(H, generator=g)).cuda(), None, (1 + torch.rand(H, generator=g)).cuda()]
+    t[2] = t[2] * 1e-15                      # the normed branch is of the residual's size
+    da = (1e15 * torch.randn(T, H, generator=g)).cuda()
+    dy = torch.randn(T, H, generator=g).cuda()
+    leaves = R.norm_leaves(*t)
+    rh, ry = R.block_norm(*leaves, 1.0, eps)
+    names = ("branch", "residual", "post_w", "pre_w")
+    ref = torch.autograd.grad((rh, ry), [v for v in leaves if v is not None],
+                              (da.double(), dy.double()))
+    err = R.block_norm_grad_bounds(leaves, 1.0, eps, da, dy)
+    t = [None if v is None else (_shifted(v) if off else v).requires_grad_() for v in t]
+    h, y = fb.block_norm(t[0], t[1], post_weight=t[2], pre_weight=t[4], eps=eps)
+    got = torch.autograd.grad((h, y), [v for v in t if v is not None], (da, dy))
+    for n, v, w in zip(names, got, ref):
+        R.check(v, w, err[n], n)
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences():
     """<gradient, v> against central differences of the 64-bit form along random v."""
     s, T, H = 0.7, 6, 72
