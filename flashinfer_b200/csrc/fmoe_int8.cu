@@ -46,7 +46,7 @@ __device__ __forceinline__ uint32_t abs_max2(__half*, uint32_t a, uint32_t b) {
 // exact, so the corrected v is the rounded quotient: a quotient halfway between integers comes out
 // as that, and any other is 2^-18 (relative) or more away from halfway, x and amax having at most
 // 11 bits. Adding 1.5 * 2^23 then rounds to the even integer. Against one IEEE division per
-// element, quantising 8192 x 7168 took 84.9 us with it.
+// element, quantising 8192 x 7168 took 84.9 us with it (58.1 without division but with a tie test).
 __device__ __forceinline__ uint2 quant2(float2 x, float den, float inv) {
   const float2 c = make_float2(127.0f / 256.0f, 127.0f / 256.0f);
   const float2 i2 = make_float2(inv, inv), d2 = make_float2(-den, -den);
@@ -61,7 +61,7 @@ __device__ __forceinline__ uint2 quant2(float2 x, float den, float inv) {
 // .... Up to VPT 16-byte granules (VEC; else single elements) of a row per thread stay in registers
 // between the maximum and the rounding, and the next row's are on their way meanwhile; what a longer
 // row has beyond them is read a second time. One row per block, without the next row's loads:
-// 8192 x 7168 took 44.7 us.
+// 8192 x 7168 took 44.7 us; it takes 31.5 (86% of the copy bandwidth over its 176 MB).
 template <typename T, bool VEC, int VPT, bool WARP>
 __global__ void __launch_bounds__(256, 4)
     k_quantize_int8(const T* x, int64_t rows, int64_t K, int8_t* q, float* scale) {
@@ -308,11 +308,23 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float
     static_cast<float*>(out)[i] = v;
 }
 
-__device__ __forceinline__ void zero_out(void* out, int dtype, int64_t i) {
-  if (dtype == FMOE_DTYPE_F32)
-    static_cast<float*>(out)[i] = 0.0f;
-  else
-    static_cast<uint16_t*>(out)[i] = 0;
+// Zeroes output rows [from, to) by 16-byte stores, single 16-bit words at the ends; thread `tid` of
+// `threads`. Rows of experts that live elsewhere can be most of the output: with 4096 of 32768 rows
+// live, a product of depth 1024 to 4096 bf16 channels takes 73 us, with element stores it took 78.
+__device__ __forceinline__ void zero_rows_out(const I8Args& a, int64_t from, int64_t to, int64_t tid,
+                                              int64_t threads) {
+  const int64_t row = static_cast<int64_t>(a.N) * (a.dtype == FMOE_DTYPE_F32 ? 4 : 2);
+  const int64_t bytes = (to - from) * row;
+  if (bytes <= 0) return;
+  uint8_t* p = static_cast<uint8_t*>(a.out) + from * row;
+  int64_t head = (16 - static_cast<int64_t>(reinterpret_cast<uintptr_t>(p) & 15u)) & 15;
+  if (head > bytes) head = bytes;
+  const int64_t wide = (bytes - head) / 16;
+  for (int64_t i = tid; i < wide; i += threads)
+    reinterpret_cast<uint4*>(p + head)[i] = make_uint4(0u, 0u, 0u, 0u);
+  const int64_t rest = bytes - head - wide * 16;  // like head an even number below 16
+  if (tid < head / 2) reinterpret_cast<uint16_t*>(p)[tid] = 0;
+  if (tid < rest / 2) reinterpret_cast<uint16_t*>(p + head + wide * 16)[tid] = 0;
 }
 
 // The epilogue of one warp: its 32 channels (one per lane) of the tile's columns c0, c0 + 16, ... in
@@ -651,12 +663,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     const int q = warp & 3;              // TMEM lane quarter of this warp
     const int g = (warp - kI8Epi0) >> 2; // which 16 of kI8EpiCols columns
     const int etid = threadIdx.x - kI8Epi0 * 32;
-    if (args.zero_tail) {
-      const int64_t total = (args.M - tail->live) * static_cast<int64_t>(args.N);
-      const int64_t i0 = tail->live * static_cast<int64_t>(args.N);
-      for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kI8EpiWarps * 32) + etid; i < total;
-           i += static_cast<int64_t>(gridDim.x) * (kI8EpiWarps * 32))
-        zero_out(args.out, args.dtype, i0 + i);
+    if (args.zero_tail) {  // rows of no expert
+      const int64_t tid = static_cast<int64_t>(blockIdx.x) * (kI8EpiWarps * 32) + etid;
+      const int64_t threads = static_cast<int64_t>(gridDim.x) * (kI8EpiWarps * 32);
+      zero_rows_out(args, 0, tail->ebase[0], tid, threads);
+      zero_rows_out(args, tail->live, args.M, tid, threads);
     }
     int n = 0;
     bool ok = true;
@@ -790,7 +801,9 @@ __global__ void __launch_bounds__(kGemvThreads)
 // (cta_group::2, M = 256) reads both CTAs' shared memory: each holds its own 128 weight rows and
 // half of the tokens, so a K block costs an SM 32 KB of shared-memory fill instead of 48 for the same
 // 128 x 256 outputs. One CTA per tile was bound by that fill: about 53 bytes a cycle per SM, 192 us
-// for 8192 x 4096 x 7168.
+// for 8192 x 4096 x 7168; pairs take 171 to 179 (2.7 to 2.8 POP/s, by the card's power). With the
+// loads taken out the same MMAs took 141 on the same data, and on constant data 105: the clock under
+// the power limit, then the fill, bound it.
 //
 // Both CTAs load into their own stages and count on the leader's (rank 0's) barrier; the leader
 // issues the MMAs and commits to the barriers of both. Each CTA stores its own weight rows' outputs.
@@ -1041,12 +1054,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     const int g = (warp - kI8Epi0) >> 2;
     const int etid = threadIdx.x - kI8Epi0 * 32;
     const uint32_t tempty[2] = {at_rank(&tail->tempty[0], lead), at_rank(&tail->tempty[1], lead)};
-    if (args.zero_tail) {
-      const int64_t total = (args.M - tail->live) * static_cast<int64_t>(args.N);
-      const int64_t i0 = tail->live * static_cast<int64_t>(args.N);
-      for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kI8EpiWarps * 32) + etid; i < total;
-           i += static_cast<int64_t>(gridDim.x) * (kI8EpiWarps * 32))
-        zero_out(args.out, args.dtype, i0 + i);
+    if (args.zero_tail) {  // rows of no expert
+      const int64_t tid = static_cast<int64_t>(blockIdx.x) * (kI8EpiWarps * 32) + etid;
+      const int64_t threads = static_cast<int64_t>(gridDim.x) * (kI8EpiWarps * 32);
+      zero_rows_out(args, 0, tail->ebase[0], tid, threads);
+      zero_rows_out(args, tail->live, args.M, tid, threads);
     }
     int n = 0;
     bool ok = true;

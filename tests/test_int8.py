@@ -138,6 +138,33 @@ def test_expert_matmul(Rn, E, N, K, counts):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Rn,N,lo,hi", [(9, 33, 4, 6), (40, 64, 40, 40), (700, 2047, 300, 311),
+                                        (2000, 130, 1, 1999), (3, 1, 1, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_no_expert(Rn, N, lo, hi, dtype):
+    """A part of an order's experts: rows before the first and behind the last are zero in a new
+    tensor and stay in a given one, at every alignment of their ends."""
+    g = _gen(Rn)
+    base = torch.tensor([lo, (lo + hi) // 2, hi], dtype=torch.int32, device="cuda")
+    rows, w = _int8(g, Rn, 48), _int8(g, 2, N, 48)
+    one, ws = torch.ones(Rn, device="cuda"), torch.ones(2, N, device="cuda")
+    mid = (lo + hi) // 2
+    ref = torch.zeros(Rn, N, dtype=torch.float64, device="cuda")
+    ref[lo:mid] = rows[lo:mid].double() @ w[0].double().t()
+    ref[mid:hi] = rows[mid:hi].double() @ w[1].double().t()
+    # dirty blocks of the allocator's, so that a row that is not written shows
+    dirt = [torch.full((Rn, N), 5.0, dtype=dtype, device="cuda") for _ in range(3)]
+    del dirt
+    y = fb.int8_expert_matmul(rows, w, one, ws, base, out_dtype=dtype)
+    assert torch.equal(y, ref.to(dtype))
+    flat = torch.full((Rn * N + 1,), 3.0, dtype=dtype, device="cuda")
+    out = flat[1:].view(Rn, N)
+    fb.int8_expert_matmul(rows, w, one, ws, base, output=out)
+    ref[:lo], ref[hi:] = 3.0, 3.0
+    assert torch.equal(out, ref.to(dtype)) and float(flat[0]) == 3.0
+
+
+@pytest.mark.gpu
 def test_expert_bases_out_of_range_are_clamped():
     """Bases below 0, above R or stepping back stay inside the tensors."""
     g = _gen(9)
