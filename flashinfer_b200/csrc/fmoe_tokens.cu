@@ -58,7 +58,7 @@ __device__ __forceinline__ int pick_key(const int32_t* ids, int64_t p, int64_t e
 }
 
 // The lanes of the warp whose key equals this lane's, by a vote per bit. match_any gives the same;
-// with it the cluster kernel took 11.8 us for 32768 picks, not 9.6.
+// with it the cluster kernel took 11.8 us for 32768 picks, not 9.2.
 __device__ __forceinline__ unsigned same_key(int key, int bits) {
   unsigned same = 0xffffffffu;
   for (int b = 0; b < bits; ++b) {
@@ -195,8 +195,8 @@ __global__ void __launch_bounds__(1024)
 
 // The same as a count and a place kernel in one launch: a cluster of eight CTAs takes up to 65536
 // picks, the counts of the others come through distributed shared memory, and each pick's expert
-// stays in a register between counting and placing. 32768 picks of 256 experts take 9.6 us, in two
-// launches 11.0; 7422 picks of 20 experts 5.4 against 7.0.
+// stays in a register between counting and placing. 32768 picks of 256 experts take 9.2 us, in two
+// launches 11.0; 7422 picks of 20 experts 5.2 against 7.0.
 constexpr int kClusterCtas = 8;
 constexpr int kClusterRounds = 8;                          // of 32 picks per warp
 constexpr int kClusterPicks = kClusterCtas * 1024 * kClusterRounds;
@@ -343,7 +343,8 @@ __device__ __forceinline__ int64_t zero_limit(const RowsArgs& a) {
   return live < a.R ? live : a.R;
 }
 
-// Copies token rows to their picks' rows: each token is read once and stored K times.
+// Copies token rows to their picks' rows: each token is read once and stored K times. Bound by the
+// stores: 4096 x 7168 (bf16, top 8) takes 87 us, 93% of the copy bandwidth over its 529 MB.
 template <typename U>
 __global__ void __launch_bounds__(256) k_sort_rows(const U* x, U* rows, const RowsArgs a) {
   pdl_begin_in_order();
@@ -412,7 +413,9 @@ __device__ __forceinline__ LanePick lane_pick(const RowsArgs& a, const float* w,
 
 // y[t] = sum_k w[t, k] * rows[pick_row[t, k]] (w null: 1), k ascending, in fp32. Eight rows' loads
 // are in flight per thread; a pick without a row adds 0 * 0, so the sums have no branches. With
-// single conversions and a branch per pick the kernel issued 75 instructions per row and granule.
+// single conversions and a branch per pick the kernel issued 75 instructions per row and granule and
+// took 135 us for 4096 x 7168 (bf16, top 8); it takes 100, 81% of the copy bandwidth, and waits for
+// its rows, which lie all over the input. A grid that stays resident was no faster.
 template <typename T>
 __global__ void __launch_bounds__(256, 4)
     k_unsort_granules(const T* rows, const float* w, T* y, const RowsArgs a) {
@@ -484,7 +487,9 @@ __device__ __forceinline__ void store_dots(float (&dot)[N], float* dw, int64_t t
 }
 
 // One block per token at a time: drows[pick_row[t, k]] = w[t, k] * dy[t]; dw[t, k] =
-// <dy[t], rows[..]> (dw null: rows are not read; drows null: not written). Eight picks at a time.
+// <dy[t], rows[..]> (dw null: rows are not read; drows null: not written). Eight picks at a time:
+// their rows are loaded before dy is used. 4096 x 7168 (bf16, top 8) takes 164 us, 93% of the copy
+// bandwidth.
 template <typename T>
 __global__ void __launch_bounds__(256, 3)
     k_unsort_back_granules(const T* dy, const T* rows, const float* w, T* drows, float* dw,
@@ -594,7 +599,8 @@ __global__ void __launch_bounds__(256)
 // still go by aligned 16-byte granules. A row's granules are those that hold a byte of it; the
 // first and last may hold bytes of its neighbours. Moving a row to one with another offset in its
 // granules shifts two neighbouring granules against each other. Single-element accesses took 70 us
-// to sort 4096 x 2047 (bf16, top 8), granules take 25 us for 2048.
+// to sort 4096 x 2047 (bf16, top 8); it takes 30 this way (2048: 27), unsort 50 (26) and its gradients
+// 106 (51): there the shifts and the edges of eight rows are most of the instructions.
 
 // Granule g of a tensor of `total` bytes; bytes outside the tensor read as zero.
 __device__ __forceinline__ uint4 granule(const uint8_t* base, int64_t g, int64_t total) {
