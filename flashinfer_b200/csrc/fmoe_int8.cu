@@ -169,16 +169,21 @@ constexpr int kI8Epi0 = 4;
 constexpr int kI8EpiWarps = 16;   // with 8 the stores of 8192 x 7168 outputs took 70 us at any K
 constexpr int kI8EpiCols = kI8EpiWarps / 4 * 16;  // columns that the warps take at a time
 constexpr int kWRows = 128;       // weight rows per tile (MMA M)
-constexpr int kKB = 128;          // K bytes per stage (one 128-byte swizzled row)
-constexpr int kI8MaxStages = 12;
+constexpr int kKB = 128;          // K bytes of a block (one 128-byte swizzled row)
+// K blocks per stage. After each stage the issued MMAs are committed to the stage's barrier, which
+// costs the tensor pipe about 250 cycles, a block's four MMAs 516: with one block per stage
+// 8192 x 4096 x 7168 took 176 us, with two it takes 167. Three would leave two stages in flight.
+constexpr int kSub = 2;
+constexpr int kI8MaxStages = 6;
 
 template <int BN>
 struct I8Cfg {
-  static constexpr int STAGE = (kWRows + BN) * kKB;
-  static constexpr int NS = BN == 16 ? 12 : BN == 64 ? 9 : 6;
+  static constexpr int BLOCK = (kWRows + BN) * kKB;
+  static constexpr int STAGE = kSub * BLOCK;
+  static constexpr int NS = BN == 16 ? 6 : BN == 64 ? 4 : 3;
   static constexpr int BOX = BN == 16 ? 16 : 64;   // token rows per TMA box
   static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;
-  static_assert(NS > kI8Producers && NS <= kI8MaxStages, "producer parity and barrier arrays");
+  static_assert(NS >= kI8Producers && NS <= kI8MaxStages, "producer parity and barrier arrays");
 };
 
 struct alignas(16) I8Tail {
@@ -596,16 +601,16 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       for (int tile = first; tile < tiles && ok; tile += step) {
         const I8Tile u = decode_tile<BN>(tile, NT, tail, E);
         const int boxes = (u.cols + C::BOX - 1) / C::BOX;
-        const uint32_t bytes = kWRows * kKB + boxes * C::BOX * kKB;
+        const uint32_t block_bytes = (kWRows + boxes * C::BOX) * kKB;
         // a weight tile that several token tiles read stays in L2; one that is read once goes first
         const uint64_t pol_w =
             tail->etile[u.e + 1] - tail->etile[u.e] > 1 ? pol_last : pol_first;
         const int wrow = u.e * args.N + u.n0;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           if (it % kI8Producers != pw) continue;
           const int s = it % NS, r = it / NS;
           // This producer issued iteration it - kI8Producers after that stage's release, and the
-          // MMA warp releases in order, so with NS > kI8Producers the barrier is at most one
+          // MMA warp releases in order, so with NS >= kI8Producers the barrier is at most one
           // phase behind and the parity wait is unambiguous.
           if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns, true)) {
             i8_abort(tail);
@@ -613,11 +618,15 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             break;
           }
           uint8_t* st = smem + s * C::STAGE;
-          mbar_arrive_expect_tx(&tail->full[s], bytes);
-          tma_load_2d(st, &tm_w, &tail->full[s], kb * kKB, wrow, pol_w);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(st + (kWRows + b * C::BOX) * kKB, &tm_a, &tail->full[s], kb * kKB,
-                        static_cast<int>(u.row0) + b * C::BOX, pol_last);
+          const int blocks = min(kSub, kb1 - kb);
+          mbar_arrive_expect_tx(&tail->full[s], blocks * block_bytes);
+          for (int j = 0; j < blocks; ++j, st += C::BLOCK) {
+            const int k = (kb + j) * kKB;
+            tma_load_2d(st, &tm_w, &tail->full[s], k, wrow, pol_w);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(st + (kWRows + b * C::BOX) * kKB, &tm_a, &tail->full[s], k,
+                          static_cast<int>(u.row0) + b * C::BOX, pol_last);
+          }
           tail->last_issue[pw][s] = r;
         }
       }
@@ -637,19 +646,24 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           break;
         }
         tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        uint32_t more = 0;  // the tile's first MMA overwrites
+        for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           const int s = it % NS, r = it / NS;
           if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns, false)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * C::STAGE);
-          const uint64_t w_desc = smem_desc_k128(st);
-          const uint64_t a_desc = smem_desc_k128(st + kWRows * kKB);
+          uint32_t st = smem_u32(smem + s * C::STAGE);
+          for (int left = min(kSub, kb1 - kb); left > 0; --left, st += C::BLOCK) {
+            const uint64_t w_desc = smem_desc_k128(st);
+            const uint64_t a_desc = smem_desc_k128(st + kWRows * kKB);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_i8(d, w_desc + 2 * j, a_desc + 2 * j, idesc, kb > kb0 || j > 0 ? 1u : 0u);
+            for (int j = 0; j < 4; ++j) {
+              mma_i8(d, w_desc + 2 * j, a_desc + 2 * j, idesc, more);
+              more = 1u;
+            }
+          }
           mma_commit(&tail->empty[s]);
         }
         if (ok) mma_commit(&tail->tfull[b]);
@@ -800,16 +814,16 @@ __global__ void __launch_bounds__(kGemvThreads)
 // For many tokens: two CTAs share a tile of 256 weight rows x up to 256 tokens. One MMA
 // (cta_group::2, M = 256) reads both CTAs' shared memory: each holds its own 128 weight rows and
 // half of the tokens, so a K block costs an SM 32 KB of shared-memory fill instead of 48 for the same
-// 128 x 256 outputs. One CTA per tile was bound by that fill: about 53 bytes a cycle per SM, 192 us
-// for 8192 x 4096 x 7168; pairs take 171 to 179 (2.7 to 2.8 POP/s, by the card's power). With the
-// loads taken out the same MMAs took 141 on the same data, and on constant data 105: the clock under
-// the power limit, then the fill, bound it.
+// 128 x 256 outputs. 8192 x 4096 x 7168 takes 167 us (2.9 POP/s), with one CTA per tile 192. Without
+// the loads and stores its MMAs take 111 us on what shared memory happens to hold; real operands
+// draw more power and lower the clock.
 //
 // Both CTAs load into their own stages and count on the leader's (rank 0's) barrier; the leader
 // issues the MMAs and commits to the barriers of both. Each CTA stores its own weight rows' outputs.
 constexpr int kPairTokens = 256;
-constexpr int kPairStage = (kWRows + kPairTokens / 2) * kKB;  // 32 KB
-constexpr int kPairStages = 6;
+constexpr int kPairBlock = (kWRows + kPairTokens / 2) * kKB;  // 32 KB
+constexpr int kPairStage = kSub * kPairBlock;
+constexpr int kPairStages = 3;
 constexpr int kPairBox = 32;                                  // token rows per TMA box
 
 struct alignas(16) PairTail {
@@ -830,7 +844,7 @@ struct alignas(16) PairTail {
 constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStage + sizeof(PairTail) + 1024;
 static_assert((kPairTokens + 4 * 15) * kWRows * 4 <= kPairStages * kPairStage,
               "four shares of a tile's partial sums fit the stages");
-static_assert(kPairSmem <= 227 * 1024 && kPairStages > kI8Producers, "pair shared memory, parity");
+static_assert(kPairSmem <= 227 * 1024 && kPairStages >= kI8Producers, "pair shared memory, parity");
 
 // Loads a box into this CTA's shared memory, its bytes counted on a barrier of the pair.
 __device__ __forceinline__ void tma_load_pair(void* dst, const void* tmap, uint32_t bar, int32_t c0,
@@ -989,12 +1003,12 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         const I8Tile u = decode_pair(tile, NT, tail, E);
         const int half = u.cols / 2;
         const int boxes = (half + kPairBox - 1) / kPairBox;
-        const uint32_t bytes = 2 * (kWRows + boxes * kPairBox) * kKB;
+        const uint32_t block_bytes = 2 * (kWRows + boxes * kPairBox) * kKB;
         const uint64_t pol_w =
             tail->etile[u.e + 1] - tail->etile[u.e] > 1 ? pol_last : pol_first;
         const int wrow = u.e * args.N + u.n0 + rank * kWRows;
         const int arow = static_cast<int>(u.row0) + rank * half;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           if (it % kI8Producers != pw) continue;
           const int s = it % kPairStages, r = it / kPairStages;
           if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns, true)) {
@@ -1003,12 +1017,16 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             break;
           }
           uint8_t* st = smem + s * kPairStage;
-          if (rank == 0) mbar_arrive_expect_tx(&tail->full[s], bytes);
+          const int blocks = min(kSub, kb1 - kb);
+          if (rank == 0) mbar_arrive_expect_tx(&tail->full[s], blocks * block_bytes);
           const uint32_t bar = at_rank(&tail->full[s], lead);
-          tma_load_pair(st, &tm_w, bar, kb * kKB, wrow, pol_w);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_pair(st + (kWRows + b * kPairBox) * kKB, &tm_a, bar, kb * kKB,
-                          arow + b * kPairBox, pol_last);
+          for (int j = 0; j < blocks; ++j, st += kPairBlock) {
+            const int k = (kb + j) * kKB;
+            tma_load_pair(st, &tm_w, bar, k, wrow, pol_w);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_pair(st + (kWRows + b * kPairBox) * kKB, &tm_a, bar, k, arow + b * kPairBox,
+                            pol_last);
+          }
         }
       }
     }
@@ -1027,19 +1045,24 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           break;
         }
         tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        uint32_t more = 0;
+        for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           const int s = it % kPairStages, r = it / kPairStages;
           if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns, false)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * kPairStage);
-          const uint64_t w_desc = smem_desc_k128(st);
-          const uint64_t a_desc = smem_desc_k128(st + kWRows * kKB);
+          uint32_t st = smem_u32(smem + s * kPairStage);
+          for (int left = min(kSub, kb1 - kb); left > 0; --left, st += kPairBlock) {
+            const uint64_t w_desc = smem_desc_k128(st);
+            const uint64_t a_desc = smem_desc_k128(st + kWRows * kKB);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_i8_pair(d, w_desc + 2 * j, a_desc + 2 * j, idesc, kb > kb0 || j > 0 ? 1u : 0u);
+            for (int j = 0; j < 4; ++j) {
+              mma_i8_pair(d, w_desc + 2 * j, a_desc + 2 * j, idesc, more);
+              more = 1u;
+            }
+          }
           commit_pair(&tail->empty[s], lead);
         }
         if (ok) commit_pair(&tail->tfull[b], lead);
@@ -1165,13 +1188,17 @@ struct I8Plan {
 };
 
 // The tile width and K split with the shortest estimated time in cycles: rounds of tiles over the
-// SMs times the K blocks of a tile, a K block costing the slower of its MMAs (2.7 cycles per token
-// column, for 128 weight rows per SM) and its fill of shared memory (about 53 bytes a cycle). A
-// split adds the exchange of partial tiles (20 cycles a column, measured about 2 us for 192) and
-// the cluster's barriers.
+// SMs times the K blocks of a tile, a K block costing the slower of its MMAs (four of 129 cycles
+// however few the tokens, and its share of the commit) and its fill of shared memory (about 75 bytes
+// a cycle); then the last tile's stores, the exchange of partial tiles and the cluster's barriers
+// where K is split, and a pair's own set-up. The last four are fitted to the times of every width and
+// split for 119 products of 5 to 3000 tokens and 24 of 8 to 8192 rows of experts: the choice is 0.4%
+// from the fastest on average and 9% at worst. An expert is taken to have up to twice its even
+// share: with the even share alone the worst choice was 30% off.
 I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms, int dev) {
   const int64_t used = M < E ? M : E;
-  const int64_t per = (M + used - 1) / used;  // tokens of an expert, evenly spread
+  int64_t per = (M + used - 1) / used;
+  if (grouped) per = 2 * per < M ? 2 * per : M;
   I8Plan best{256, 1};
   double best_cost = 1e30;
   for (const int bn : {16, 64, 128, 256}) {
@@ -1181,13 +1208,14 @@ I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms, int dev)
     const int64_t tiles = mt * used * NT;
     const int64_t most = (grouped ? M / bn + used : mt) * NT;  // no spread has more tiles
     const int64_t cols = ((per + mt - 1) / mt + 15) / 16 * 16;
-    const double fill = (kWRows + cols / ctas) * kKB / 53.0;
-    const double kb = cols * 2.7 > fill ? cols * 2.7 : fill;
+    const double fill = (kWRows + cols / ctas) * kKB / 75.0;
+    const double mma = 4 * 129.0 + 250.0 / kSub;
+    const double kb = mma > fill ? mma : fill;
     for (int S = 1; S <= 4; ++S) {
       if (S > 1 && (nkb < 2 * S || most > max_clusters(S * ctas, dev))) break;
       const int64_t waves = S > 1 ? 1 : (tiles + sms / ctas - 1) / (sms / ctas);
-      const double cost = waves * ((nkb + S - 1) / S) * kb + cols * 20.0 +
-                          (S > 1 ? cols * 20.0 + 1500.0 : 0.0);
+      const double cost = waves * ((nkb + S - 1) / S) * kb + cols * 50.0 +
+                          (ctas > 1 ? 2300.0 : 0.0) + (S > 1 ? cols * 50.0 + 5400.0 : 0.0);
       if (cost < best_cost) {
         best_cost = cost;
         best = I8Plan{bn, S};
