@@ -126,7 +126,8 @@ def block_norm(branch: Optional[torch.Tensor], residual: torch.Tensor, *,
     ``normed = norm(hidden) * pre_weight``, with ``norm(v) = v / sqrt(mean(v^2) + eps)`` per token.
 
     branch, residual [T, H] of one type (bf16, fp16, fp32), H up to 16384; branch None where no
-    block came before (``hidden`` is then the scaled residual). post_weight [H]: None for no norm
+    block came before (``hidden`` is then the scaled residual; with scale 1 and no gradient
+    recorded it is ``residual`` itself). post_weight [H]: None for no norm
     after the block. gate: one factor per token [T, 1], per channel [H] or per element [T, H], or
     None. pre_weight [H]: None for no norm before the next block (``normed`` is then None). Weights
     and gate are of the activations' type or fp32. hidden stays in fp32 between the two norms.

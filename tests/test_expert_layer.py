@@ -3,6 +3,7 @@ step, in a captured graph, on tensors beyond 2^31 elements; and the C structs th
 import ctypes
 import os
 import subprocess
+import threading
 
 import numpy as np
 import pytest
@@ -146,6 +147,33 @@ def test_layer_captured_and_replayed():
             for k in ("hidden", "up", "down", "y", "out"):
                 assert torch.equal(got[k], want[k]), k
             assert torch.equal(got["q8"][0].view(torch.uint8), want["q8"][0].view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_layer_from_several_threads_at_once():
+    """Four host threads, each on its own stream: the bits of one call after the other."""
+    args = [_layer_inputs(T, 512, 256, 32, 30 + T) for T in (3, 40, 200, 64)]
+    want = [_layer(*a, 0) for a in args]
+    torch.cuda.synchronize()
+    got = [None] * len(args)
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                r = _layer(*args[i], 0)
+            s.synchronize()
+        got[i] = r
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(args))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        for k in ("hidden", "up", "down", "y", "out"):
+            assert torch.equal(g[k], w[k]), k
+    assert fb.int8_status() == 0
 
 
 @pytest.mark.gpu
