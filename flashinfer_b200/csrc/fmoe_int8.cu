@@ -695,8 +695,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       named_bar_sync(1, kI8EpiWarps * 32);  // the previous tile's a_scale is no longer read
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
-      // after a wait that ran out, the warp still takes part in the barriers of later tiles
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, false));
+      // after a wait that ran out, the warp still takes part in the barriers of later tiles. Parked:
+      // sixteen warps polling without a pause slow the MMA warp down (517 x 2047 x 7168: 20.3 us)
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, true));
       if (!ok) {
         if (lane == 0) i8_abort(tail);
         continue;
@@ -1096,7 +1097,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
       // after a wait that ran out, the warp still takes part in the barriers of later tiles
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, false));
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, true));
       if (!ok) {
         if (lane == 0) pair_abort(tail);
         continue;
