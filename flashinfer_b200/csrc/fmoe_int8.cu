@@ -170,9 +170,9 @@ constexpr int kI8EpiWarps = 16;   // with 8 the stores of 8192 x 7168 outputs to
 constexpr int kI8EpiCols = kI8EpiWarps / 4 * 16;  // columns that the warps take at a time
 constexpr int kWRows = 128;       // weight rows per tile (MMA M)
 constexpr int kKB = 128;          // K bytes of a block (one 128-byte swizzled row)
-// K blocks per stage. After each stage the issued MMAs are committed to the stage's barrier, which
-// costs the tensor pipe about 250 cycles, a block's four MMAs 516: with one block per stage
-// 8192 x 4096 x 7168 took 176 us, with two it takes 167. Three would leave two stages in flight.
+// K blocks per stage. A stage costs the MMA warp's loop about 0.3 us beside its MMAs (which take
+// 0.15 us a block to issue and 0.27 to run at 256 tokens): with one block per stage
+// 8192 x 4096 x 7168 took 176 us, with two 167. Three would leave two stages in flight.
 constexpr int kSub = 2;
 constexpr int kI8MaxStages = 6;
 
@@ -279,15 +279,15 @@ __device__ __forceinline__ I8Tile decode_tile(int tile, int NT, const I8Tail* t,
 }
 
 // Waits for the phase with the given parity; gives up after limit_ns, or when another role of
-// this CTA has (both looked at every few hundred polls). park: each poll may suspend the thread for
-// a while.
+// this CTA has (both looked at every few polls). Each poll may suspend the thread for a while:
+// warps that poll without a pause slow the MMA warp down (517 x 2047 x 7168 took 20.3 us with the
+// epilogue's polling, 18.5 with the MMA warp's own, 17.5 with none).
 __device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                        uint64_t limit_ns, bool park) {
+                                        uint64_t limit_ns) {
   uint64_t t0 = 0;
-  const uint32_t often = park ? 15u : 511u;
   for (uint32_t polls = 1;; ++polls) {
-    if (park ? mbar_try_wait_sleep(bar, parity, 2000u) : mbar_test_wait(bar, parity)) return true;
-    if ((polls & often) == 0) {
+    if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
+    if ((polls & 15u) == 0) {
       if (*abort_flag) return false;
       const uint64_t now = global_timer_ns();
       if (t0 == 0) t0 = now;
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           // This producer issued iteration it - kI8Producers after that stage's release, and the
           // MMA warp releases in order, so with NS >= kI8Producers the barrier is at most one
           // phase behind and the parity wait is unambiguous.
-          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns, true)) {
+          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns)) {
             i8_abort(tail);
             ok = false;
             break;
@@ -635,13 +635,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
       int it = 0, n = 0;
-      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns, false);
+      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
         const I8Tile u = decode_tile<BN>(tile, NT, tail, E);
         const uint32_t idesc = idesc_i8(kWRows, u.cols);
         const int b = n & 1, rb = n >> 1;
         const uint32_t d = tmem + b * BN;
-        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns, false)) {
+        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns)) {
           ok = false;
           break;
         }
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         uint32_t more = 0;  // the tile's first MMA overwrites
         for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           const int s = it % NS, r = it / NS;
-          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns, false)) {
+          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns)) {
             ok = false;
             break;
           }
@@ -695,9 +695,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       named_bar_sync(1, kI8EpiWarps * 32);  // the previous tile's a_scale is no longer read
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
-      // after a wait that ran out, the warp still takes part in the barriers of later tiles. Parked:
-      // sixteen warps polling without a pause slow the MMA warp down (517 x 2047 x 7168: 20.3 us)
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, true));
+      // after a wait that ran out, the warp still takes part in the barriers of later tiles
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns));
       if (!ok) {
         if (lane == 0) i8_abort(tail);
         continue;
@@ -815,7 +814,7 @@ __global__ void __launch_bounds__(kGemvThreads)
 // For many tokens: two CTAs share a tile of 256 weight rows x up to 256 tokens. One MMA
 // (cta_group::2, M = 256) reads both CTAs' shared memory: each holds its own 128 weight rows and
 // half of the tokens, so a K block costs an SM 32 KB of shared-memory fill instead of 48 for the same
-// 128 x 256 outputs. 8192 x 4096 x 7168 takes 167 us (2.9 POP/s), with one CTA per tile 192. Without
+// 128 x 256 outputs. 8192 x 4096 x 7168 takes 164 us (2.9 POP/s), with one CTA per tile 192. Without
 // the loads and stores its MMAs take 111 us on what shared memory happens to hold; real operands
 // draw more power and lower the clock.
 //
@@ -1012,7 +1011,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           if (it % kI8Producers != pw) continue;
           const int s = it % kPairStages, r = it / kPairStages;
-          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns, true)) {
+          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns)) {
             pair_abort(tail);
             ok = false;
             break;
@@ -1035,13 +1034,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     // ---------------------------------------------------------------- MMA issuer (the leader's)
     if (rank == 0 && lane == 0) {
       int it = 0, n = 0;
-      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns, false);
+      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
         const I8Tile u = decode_pair(tile, NT, tail, E);
         const uint32_t idesc = idesc_i8(2 * kWRows, u.cols);
         const int b = n & 1, rb = n >> 1;
         const uint32_t d = tmem + b * kPairTokens;
-        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns, false)) {
+        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns)) {
           ok = false;
           break;
         }
@@ -1049,7 +1048,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         uint32_t more = 0;
         for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           const int s = it % kPairStages, r = it / kPairStages;
-          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns, false)) {
+          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns)) {
             ok = false;
             break;
           }
@@ -1097,7 +1096,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
       // after a wait that ran out, the warp still takes part in the barriers of later tiles
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns, true));
+      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns));
       if (!ok) {
         if (lane == 0) pair_abort(tail);
         continue;
@@ -1189,9 +1188,8 @@ struct I8Plan {
 };
 
 // The tile width and K split with the shortest estimated time in cycles: rounds of tiles over the
-// SMs times the K blocks of a tile, a K block costing the slower of its MMAs (four of 129 cycles
-// however few the tokens, and its share of the commit) and its fill of shared memory (about 75 bytes
-// a cycle); then the last tile's stores, the exchange of partial tiles and the cluster's barriers
+// SMs times the K blocks of a tile, a K block costing the slower of its round in the MMA warp (about
+// 640 cycles, however few the tokens) and its fill of shared memory (about 75 bytes a cycle); then the last tile's stores, the exchange of partial tiles and the cluster's barriers
 // where K is split, and a pair's own set-up. The last four are fitted to the times of every width and
 // split for 119 products of 5 to 3000 tokens and 24 of 8 to 8192 rows of experts: the choice is 0.4%
 // from the fastest on average and 9% at worst. An expert is taken to have up to twice its even
@@ -1210,8 +1208,7 @@ I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms, int dev)
     const int64_t most = (grouped ? M / bn + used : mt) * NT;  // no spread has more tiles
     const int64_t cols = ((per + mt - 1) / mt + 15) / 16 * 16;
     const double fill = (kWRows + cols / ctas) * kKB / 75.0;
-    const double mma = 4 * 129.0 + 250.0 / kSub;
-    const double kb = mma > fill ? mma : fill;
+    const double kb = fill > 640.0 ? fill : 640.0;
     for (int S = 1; S <= 4; ++S) {
       if (S > 1 && (nkb < 2 * S || most > max_clusters(S * ctas, dev))) break;
       const int64_t waves = S > 1 ? 1 : (tiles + sms / ctas - 1) / (sms / ctas);
