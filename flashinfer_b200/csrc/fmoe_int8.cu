@@ -170,8 +170,7 @@ constexpr int kI8EpiWarps = 16;   // with 8 the stores of 8192 x 7168 outputs to
 constexpr int kI8EpiCols = kI8EpiWarps / 4 * 16;  // columns that the warps take at a time
 constexpr int kWRows = 128;       // weight rows per tile (MMA M)
 constexpr int kKB = 128;          // K bytes of a block (one 128-byte swizzled row)
-// K blocks per stage. A stage costs the MMA warp's loop about 0.3 us beside its MMAs (which take
-// 0.15 us a block to issue and 0.27 to run at 256 tokens): with one block per stage
+// K blocks per stage. A stage costs the MMA warp's loop time beside its MMAs: with one block per stage
 // 8192 x 4096 x 7168 took 176 us, with two 167. Three would leave two stages in flight.
 constexpr int kSub = 2;
 constexpr int kI8MaxStages = 6;
@@ -276,6 +275,16 @@ __device__ __forceinline__ I8Tile decode_tile(int tile, int NT, const I8Tail* t,
   r.rows = max(0, min(per, count - m * per));
   r.cols = max(16, (r.rows + 15) / 16 * 16);
   return r;
+}
+
+// True in one lane of a whole warp. The MMAs of a branch on it issue faster than those of a branch on
+// the lane's number: 517 x 2047 x 7168 takes 13.8 us, 17.6 with the other.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 // Waits for the phase with the given parity; gives up after limit_ns, or when another role of
@@ -633,7 +642,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       int it = 0, n = 0;
       bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
@@ -814,7 +823,7 @@ __global__ void __launch_bounds__(kGemvThreads)
 // For many tokens: two CTAs share a tile of 256 weight rows x up to 256 tokens. One MMA
 // (cta_group::2, M = 256) reads both CTAs' shared memory: each holds its own 128 weight rows and
 // half of the tokens, so a K block costs an SM 32 KB of shared-memory fill instead of 48 for the same
-// 128 x 256 outputs. 8192 x 4096 x 7168 takes 164 us (2.9 POP/s), with one CTA per tile 192. Without
+// 128 x 256 outputs. 8192 x 4096 x 7168 takes 162 us (3.0 POP/s), with one CTA per tile 192. Without
 // the loads and stores its MMAs take 111 us on what shared memory happens to hold; real operands
 // draw more power and lower the clock.
 //
@@ -1032,7 +1041,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer (the leader's)
-    if (rank == 0 && lane == 0) {
+    if (rank == 0 && elect_one()) {
       int it = 0, n = 0;
       bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
