@@ -1200,8 +1200,8 @@ struct I8Plan {
 // SMs times the K blocks of a tile, a K block costing the slower of its round in the MMA warp (about
 // 640 cycles, however few the tokens) and its fill of shared memory (about 75 bytes a cycle); then the last tile's stores, the exchange of partial tiles and the cluster's barriers
 // where K is split, and a pair's own set-up. The last four are fitted to the times of every width and
-// split for 119 products of 5 to 3000 tokens and 24 of 8 to 8192 rows of experts: the choice is 0.4%
-// from the fastest on average and 9% at worst. An expert is taken to have up to twice its even
+// split for 119 products of 5 to 3000 tokens and 24 of 8 to 8192 rows of experts: the choice was 0.4%
+// from the fastest on average and 9% at worst (with MMAs issued for lane 0, not under elect.sync). An expert is taken to have up to twice its even
 // share: with the even share alone the worst choice was 30% off.
 I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms, int dev) {
   const int64_t used = M < E ? M : E;
