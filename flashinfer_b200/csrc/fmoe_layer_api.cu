@@ -58,7 +58,7 @@ int check_order(const FmoeTokenOrder* o, TokenOrder* out) {
   const int rc = order_size(o->num_tokens, o->top_k, o->num_local_experts, 1, &least, &scratch);
   if (rc) return rc;
   if (o->num_rows < least || o->num_rows > INT32_MAX - 1024) return FMOE_ERR_SHAPE;
-  if (!o->expert_base || (o->num_tokens > 0 && (!o->row_pick || !o->pick_row)))
+  if (!o->expert_base || (o->num_rows > 0 && !o->row_pick) || (o->num_tokens > 0 && !o->pick_row))
     return FMOE_ERR_NULL;
   if (!at(o->expert_base, 4) || !at(o->row_pick, 4) || !at(o->pick_row, 4)) return FMOE_ERR_ALIGN;
   *out = TokenOrder{o->expert_base, o->row_pick, o->pick_row, o->num_tokens,

@@ -1,0 +1,45 @@
+"""Calls at the edges of what the operators around the experts allow: empty batches in tables of a fixed
+size, autograd modes, given outputs, hand-made orders, sizes beyond 32 bits."""
+import ctypes
+
+import pytest
+import torch
+
+import flashinfer_b200 as fb
+from flashinfer_b200 import _lib
+
+
+def _order_struct(T, K, E, R, base=4096, row_pick=8192, pick_row=12288):
+    return ctypes.byref(_lib.FmoeTokenOrder(T, K, E, R, base, row_pick, pick_row))
+
+
+def test_rows_without_tokens_need_their_table():
+    """No tokens but rows: the kernels write and read row_pick, so it must be there."""
+    lib = _lib.load()
+    o = _order_struct(0, 2, 4, 8, row_pick=None, pick_row=None)
+    assert lib.fmoe_sort_by_expert(None, 0, 1, o, None, 0, None) == -1
+    assert lib.fmoe_sort_rows(None, 8, o, 1 << 20, 1, None) == -1
+    assert lib.fmoe_unsort_rows(1 << 20, 0, 8, o, None, None, None) == -1
+    assert lib.fmoe_unsort_rows_backward(None, None, 0, 8, o, None, 1 << 20, None, None) == -1
+    # neither tokens nor rows: nothing to read
+    none = _order_struct(0, 2, 4, 0, row_pick=None, pick_row=None)
+    assert lib.fmoe_sort_rows(None, 8, none, None, 1, None) == 0
+    assert lib.fmoe_unsort_rows(None, 0, 8, none, None, None, None) == 0
+
+
+@pytest.mark.gpu
+def test_no_tokens_in_tables_of_a_fixed_size():
+    """Zero tokens and eight rows: the order says that no row holds a pick, sorted rows are zero with
+    zero_tail and left alone without."""
+    lib = _lib.load()
+    stream = torch.cuda.current_stream().cuda_stream
+    base = torch.full((5,), 7, dtype=torch.int32, device="cuda")
+    row_pick = torch.full((8,), 7, dtype=torch.int32, device="cuda")
+    o = _order_struct(0, 2, 4, 8, base.data_ptr(), row_pick.data_ptr(), None)
+    assert lib.fmoe_sort_by_expert(None, 0, 1, o, None, 0, stream) == 0
+    assert base.tolist() == [0] * 5 and row_pick.tolist() == [-1] * 8
+    rows = torch.full((8, 6), 3.0, device="cuda")
+    assert lib.fmoe_sort_rows(None, 24, o, rows.data_ptr(), 0, stream) == 0
+    assert bool((rows == 3.0).all())
+    assert lib.fmoe_sort_rows(None, 24, o, rows.data_ptr(), 1, stream) == 0
+    assert not bool(rows.any())
