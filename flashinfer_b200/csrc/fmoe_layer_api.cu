@@ -245,9 +245,16 @@ int fmoe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtyp
   if (rc) return rc;
   if (!float_type(dtype)) return FMOE_ERR_DTYPE;
   if (H < 1 || H > (INT32_MAX >> 2) || !grid_fits(o.T, H)) return FMOE_ERR_SHAPE;
-  if (o.T == 0 || (!grad_rows && !grad_weights)) return FMOE_OK;
-  if (!grad_y || (grad_weights && !rows)) return FMOE_ERR_NULL;
   const size_t e = elem(dtype);
+  if (o.T == 0) {
+    // no tokens: no row has a pick
+    const size_t bytes = static_cast<size_t>(o.R) * H * e;
+    if (!grad_rows || bytes == 0) return FMOE_OK;
+    if (!at(grad_rows, e)) return FMOE_ERR_ALIGN;
+    return done(cudaMemsetAsync(grad_rows, 0, bytes, as_stream(stream)));
+  }
+  if (!grad_rows && !grad_weights) return FMOE_OK;
+  if (!grad_y || (grad_weights && !rows)) return FMOE_ERR_NULL;
   if (!at(grad_y, e) || !at(rows, e) || !at(grad_rows, e) || !at(weights, 4) ||
       !at(grad_weights, 4))
     return FMOE_ERR_ALIGN;

@@ -43,3 +43,21 @@ def test_no_tokens_in_tables_of_a_fixed_size():
     assert bool((rows == 3.0).all())
     assert lib.fmoe_sort_rows(None, 24, o, rows.data_ptr(), 1, stream) == 0
     assert not bool(rows.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tag,dtype", [(0, torch.float32), (1, torch.bfloat16)])
+def test_gradient_of_rows_without_tokens_is_zero(tag, dtype):
+    """Every row's gradient is written, also where a batch of no tokens meets a table of a fixed size."""
+    lib = _lib.load()
+    stream = torch.cuda.current_stream().cuda_stream
+    base = torch.zeros(5, dtype=torch.int32, device="cuda")
+    row_pick = torch.full((8,), -1, dtype=torch.int32, device="cuda")
+    o = _order_struct(0, 2, 4, 8, base.data_ptr(), row_pick.data_ptr(), None)
+    flat = torch.full((8 * 33 + 2,), 3.0, dtype=dtype, device="cuda")
+    grad = flat[1:-1]
+    assert lib.fmoe_unsort_rows_backward(None, None, tag, 33, o, None, grad.data_ptr(), None,
+                                         stream) == 0
+    assert not bool(grad.any()) and float(flat[0]) == 3.0 and float(flat[-1]) == 3.0
+    assert lib.fmoe_unsort_rows_backward(None, None, tag, 33, o, None, grad.data_ptr() + 1, None,
+                                         stream) == -3
