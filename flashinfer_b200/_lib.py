@@ -61,7 +61,7 @@ EXPORTS = ("fmoe_workspace_size", "fmoe_workspace_layout", "fmoe_run", "fmoe_rou
            "fmoe_debug_arm_timeout", "fmoe_sort_size", "fmoe_sort_by_expert", "fmoe_sort_rows",
            "fmoe_unsort_rows", "fmoe_unsort_rows_backward", "fmoe_quantize_int8",
            "fmoe_int8_matmul", "fmoe_int8_expert_matmul", "fmoe_int8_status",
-           "fmoe_debug_arm_int8_timeout",
+           "fmoe_debug_arm_int8_timeout", "fmoe_debug_arm_int8_plan",
            "fmoe_block_norm_workspace_size", "fmoe_block_norm", "fmoe_block_norm_backward")
 
 
@@ -198,6 +198,7 @@ def load() -> ctypes.CDLL:
                                             c_int64, c_int32, c_int32, c_int32, c_void_p, c_int32,
                                             c_int32, c_void_p]
     lib.fmoe_debug_arm_int8_timeout.argtypes = [ctypes.c_uint64]
+    lib.fmoe_debug_arm_int8_plan.argtypes = [c_int32, c_int32]
     lib.fmoe_int8_status.argtypes = [POINTER(c_int32), c_void_p]
     lib.fmoe_block_norm_workspace_size.argtypes = [c_int64, c_int32, POINTER(c_size_t)]
     lib.fmoe_block_norm.argtypes = [POINTER(FmoeBlockNormArgs), c_void_p]

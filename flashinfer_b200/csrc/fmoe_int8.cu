@@ -454,7 +454,9 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void send_partials(uint32_t taddr, int g, const I8Tile& u, int per,
                                               uint8_t* part, int mine, int rank0, int rank_step,
                                               int channel) {
-  for (int c = g * 16; c < u.cols; c += kI8EpiCols) {
+  // to the last token, not the last column: the columns, which pairs round up to 32, can hold a group
+  // beyond the S shares, of a receiver that does not exist
+  for (int c = g * 16; c < u.rows; c += kI8EpiCols) {
     float v[16];
     tmem_ld_32x32b_x16(taddr + c, v);
     tmem_ld_wait16(v);
@@ -1333,7 +1335,7 @@ cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
   // The tensor cores take 11.7 us for 1 to 4 tokens x 4096 x 7168 and 24.7 for 16384 channels, which
   // are enough tiles for every SM; this way 1, 2 and 4 tokens take 8.0, 9.3 and 9.0 us, and with
   // 16384 channels one token takes 20.8 and four take 29.0.
-  if (p.wait_ns == 0 && !p.expert_base && p.M <= kGemvTokens && p.M * p.K <= kGemvSmem &&
+  if (p.wait_ns == 0 && p.tile_tokens == 0 && !p.expert_base && p.M <= kGemvTokens && p.M * p.K <= kGemvSmem &&
       (p.M <= 2 || p.N <= 64 * sms)) {
     switch (p.M) {
       case 1:
@@ -1350,8 +1352,10 @@ cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   const cudaError_t e = configure(dev);
   if (e != cudaSuccess) return e;
-  const I8Plan plan =
-      i8_plan(p.M, p.N, p.E, (p.K + kKB - 1) / kKB, p.expert_base != nullptr, sms, dev);
+  const I8Plan plan = p.tile_tokens != 0
+                          ? I8Plan{p.tile_tokens, p.split}
+                          : i8_plan(p.M, p.N, p.E, (p.K + kKB - 1) / kKB, p.expert_base != nullptr,
+                                    sms, dev);
   switch (plan.bn) {
     case 16:
       return run_mm<16>(p, plan.S, sms, s);

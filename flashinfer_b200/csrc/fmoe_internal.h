@@ -250,6 +250,7 @@ struct Int8Product {
   int out_dtype;
   int zero_tail;        // rows from expert_base[E] on are zeroed
   unsigned long long wait_ns;  // failure-path test: the limit of an injected wait, else 0
+  int tile_tokens, split;      // kernel test: the tile width and K split to use, else 0
 };
 cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, void* q,
                                  float* scale, int sms, cudaStream_t s);

@@ -71,17 +71,27 @@ bool grid_fits(int64_t rows, int64_t units) { return rows * (units / 256 + 1) < 
 
 // One-shot failure-path injection of fmoe_debug_arm_int8_timeout for this host thread's next product.
 thread_local unsigned long long g_int8_wait_ns = 0;
+// One-shot choice of fmoe_debug_arm_int8_plan for this host thread's next product.
+thread_local int g_int8_tile_tokens = 0, g_int8_split = 0;
 
 int int8_product(const Int8Product& call, void* stream) {
   Int8Product p = call;
   p.wait_ns = g_int8_wait_ns;
+  p.tile_tokens = g_int8_tile_tokens;
+  p.split = g_int8_split;
   g_int8_wait_ns = 0;
+  g_int8_tile_tokens = g_int8_split = 0;
   if (p.M < 0 || p.M > INT32_MAX - 1024 || p.N < 1 || p.K < 16 || p.K % 16 != 0 || p.K > 131056 ||
       p.E < 1 || p.E > kMaxLocalExperts ||
       static_cast<int64_t>(p.E) * p.N > INT32_MAX - 1024)
     return FMOE_ERR_SHAPE;
   if (!float_type(p.out_dtype)) return FMOE_ERR_DTYPE;
   if (p.M == 0) return FMOE_OK;
+  // every part of a split needs a K block, every tile a block of the grid
+  if (p.tile_tokens != 0 &&
+      ((p.K + 127) / 128 < p.split ||
+       (p.M / p.tile_tokens + p.E) * ((p.N + 127) / 128) * 8 > INT32_MAX))
+    return FMOE_ERR_SHAPE;
   for (const void* q : {p.a, p.w, static_cast<const void*>(p.a_scale),
                         static_cast<const void*>(p.w_scale), static_cast<const void*>(p.out)})
     if (!q) return FMOE_ERR_NULL;
@@ -290,7 +300,8 @@ int fmoe_int8_matmul(const void* a, const void* b, const float* a_scale, const f
                      const float* bias, int64_t m, int32_t n, int32_t k, void* out,
                      int32_t out_dtype, void* stream) {
   return int8_product(
-      Int8Product{a, b, a_scale, b_scale, bias, nullptr, out, m, n, k, 1, out_dtype, 0, 0}, stream);
+      Int8Product{a, b, a_scale, b_scale, bias, nullptr, out, m, n, k, 1, out_dtype, 0, 0, 0, 0},
+      stream);
 }
 
 int fmoe_int8_expert_matmul(const void* rows, const void* weights, const float* row_scale,
@@ -299,13 +310,22 @@ int fmoe_int8_expert_matmul(const void* rows, const void* weights, const float* 
                             int32_t zero_tail, void* stream) {
   if (R > 0 && !expert_base) return FMOE_ERR_NULL;
   return int8_product(Int8Product{rows, weights, row_scale, weight_scale, nullptr, expert_base, out,
-                                  R, n, k, E, out_dtype, zero_tail, 0},
+                                  R, n, k, E, out_dtype, zero_tail, 0, 0, 0},
                       stream);
 }
 
 int fmoe_debug_arm_int8_timeout(uint64_t wait_ns) {
   if (wait_ns < 100000ull || wait_ns > 2000000000ull) return FMOE_ERR_SHAPE;
   g_int8_wait_ns = wait_ns;
+  return FMOE_OK;
+}
+
+int fmoe_debug_arm_int8_plan(int32_t tile_tokens, int32_t split) {
+  if ((tile_tokens != 16 && tile_tokens != 64 && tile_tokens != 128 && tile_tokens != 256) ||
+      split < 1 || split > 4)
+    return FMOE_ERR_SHAPE;
+  g_int8_tile_tokens = tile_tokens;
+  g_int8_split = split;
   return FMOE_OK;
 }
 

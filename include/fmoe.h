@@ -422,6 +422,12 @@ FMOE_API int fmoe_int8_status(int32_t* status, void* cuda_stream);
  * The kernel gives up, sets the status bit and returns; its output is not valid. One-shot. */
 FMOE_API int fmoe_debug_arm_int8_timeout(uint64_t wait_ns);
 
+/* Kernel test: the next int8 product of the calling host thread runs on the tensor cores with tiles
+ * of tile_tokens (16, 64 or 128: one CTA per tile; 256: CTA pairs) and K split in `split` (1 .. 4)
+ * instead of what the size would choose. FMOE_ERR_SHAPE from that call if K has fewer blocks of 128
+ * than parts. One-shot; the result is the same. */
+FMOE_API int fmoe_debug_arm_int8_plan(int32_t tile_tokens, int32_t split);
+
 /* The norms before and after a block, with its gate and the residual scale. Per token:
  *   n = post_weight ? branch * rsqrt(mean(branch^2) + eps) * post_weight : branch
  *   hidden = residual_scale * residual + gate * n

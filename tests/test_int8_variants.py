@@ -1,0 +1,62 @@
+"""Every tensor-core variant of the int8 products -- tiles of 16, 64 and 128 tokens, CTA pairs, each with
+K whole and split in 2 to 4 -- on the same sizes, whatever the size would choose."""
+import time
+
+import pytest
+import torch
+
+import flashinfer_b200 as fb
+from flashinfer_b200 import _lib
+from tests import layer_refs as R
+
+VARIANTS = [(bn, s) for bn in (16, 64, 128, 256) for s in (1, 2, 3, 4)]
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _int8(g, *shape):
+    return torch.randint(-128, 128, shape, generator=g, device="cuda", dtype=torch.int8)
+
+
+def _arm(bn, split):
+    assert _lib.load().fmoe_debug_arm_int8_plan(bn, split) == 0
+
+
+def test_no_group_of_a_tile_lies_beyond_its_shares():
+    """The arithmetic of a split tile: its tokens in groups of 16 up to the last token, its shares of
+    whole groups. Every group belongs to one of the S shares."""
+    for rows in range(1, 257):
+        for S in (2, 3, 4):
+            per = -(-(-(-rows // S)) // 16) * 16
+            assert all(c // per < S for c in range(0, rows, 16)), (rows, S)
+    # while the MMA's columns, which pairs round up to 32, do have groups beyond: 144 of 160
+    assert 144 // 48 == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [33, 129, 130, 144, 300, 517])
+def test_pairs_whose_columns_exceed_their_shares(M):
+    N, K = 257, 1040
+    g = _gen(M)
+    a, w = _int8(g, M, K), _int8(g, N, K)
+    a_s = torch.rand(M, generator=g, device="cuda") + 0.01
+    w_s = torch.rand(N, generator=g, device="cuda")
+    ref, err = R.product(a, w, a_s, w_s)
+    _arm(256, 3)
+    R.check(fb.int8_matmul(a, w, a_s, w_s, out_dtype=torch.float32), ref, err, "split in 3")
+    assert fb.int8_status() == 0
+
+
+def test_refusals_of_a_variant():
+    lib = _lib.load()
+    for bad in ((0, 1), (32, 1), (256, 0), (256, 5), (-16, 1)):
+        assert lib.fmoe_debug_arm_int8_plan(*bad) == -2
+    A, B, S, W, O = 1 << 20, 2 << 20, 3 << 20, 4 << 20, 5 << 20
+    assert lib.fmoe_debug_arm_int8_plan(64, 4) == 0
+    # three K blocks for four parts; refused once, the next call is back to its own choice
+    assert lib.fmoe_int8_matmul(A, B, S, W, None, 4, 8, 384, O, 1, None) == -2
+    assert lib.fmoe_debug_arm_int8_plan(16, 2) == 0
+    assert lib.fmoe_int8_matmul(A, B, S, W, None, 0, 8, 32, O, 1, None) == 0     # used up
+    assert lib.fmoe_int8_matmul(A, B, S, W, None, 4, 8, 32, A + 64, 1, None) == -2
