@@ -356,6 +356,7 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int c0, int c_step
   O* mine = out + (PAIRS ? lane & ~1 : lane);
   const bool writes = lane < live;  // N is even with PAIRS, so both channels of a pair exist
   for (int c = c0; c < cols; c += c_step) {
+    __syncwarp();  // the tensor memory is read by the whole warp, which the stores below divide
     float v[16];
     tmem_ld_32x32b_x16(taddr + c, v);
     tmem_ld_wait16(v);
@@ -376,19 +377,19 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int c0, int c_step
         w[i] = odd ? pack2(static_cast<O*>(nullptr), other, v[i + 8])
                    : pack2(static_cast<O*>(nullptr), v[i], other);
       }
-      if (!writes) continue;
-      O* p = mine + static_cast<int64_t>(c + (odd ? 8 : 0)) * N;
-      const int left = rows - c - (odd ? 8 : 0);
-      if (left >= 8) {
+      if (writes) {
+        O* p = mine + static_cast<int64_t>(c + (odd ? 8 : 0)) * N;
+        const int left = rows - c - (odd ? 8 : 0);
+        if (left >= 8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i, p += N) *reinterpret_cast<uint32_t*>(p) = w[i];
-      } else {
+          for (int i = 0; i < 8; ++i, p += N) *reinterpret_cast<uint32_t*>(p) = w[i];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i, p += N)
-          if (i < left) *reinterpret_cast<uint32_t*>(p) = w[i];
+          for (int i = 0; i < 8; ++i, p += N)
+            if (i < left) *reinterpret_cast<uint32_t*>(p) = w[i];
+        }
       }
-    } else {
-      if (!writes) continue;
+    } else if (writes) {
       O* p = mine + static_cast<int64_t>(c) * N;
       const int left = rows - c;
       if (left >= 16) {
@@ -401,6 +402,7 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int c0, int c_step
       }
     }
   }
+  __syncwarp();
 }
 
 // The same for the call's output type.
@@ -457,6 +459,7 @@ __device__ __forceinline__ void send_partials(uint32_t taddr, int g, const I8Til
   // to the last token, not the last column: the columns, which pairs round up to 32, can hold a group
   // beyond the S shares, of a receiver that does not exist
   for (int c = g * 16; c < u.rows; c += kI8EpiCols) {
+    __syncwarp();
     float v[16];
     tmem_ld_32x32b_x16(taddr + c, v);
     tmem_ld_wait16(v);

@@ -262,12 +262,15 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
 }
 
 // Every thread of every CTA of the cluster: arrive (release: this thread's earlier shared-memory
-// writes become visible cluster-wide) / wait for all arrivals (acquire).
+// writes become visible cluster-wide) / wait for all arrivals (acquire). Both are warp-wide
+// instructions, so a warp that branches have divided comes together first.
 __device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 

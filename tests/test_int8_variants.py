@@ -24,6 +24,35 @@ def _arm(bn, split):
     assert _lib.load().fmoe_debug_arm_int8_plan(bn, split) == 0
 
 
+# M, N, K: a few tokens, one past a tile, odd N, K that ends inside a block, many K blocks (the ring
+# wraps several times), more tiles than run at a time (a CTA takes several, over both accumulators)
+SIZES = [(5, 33, 528), (33, 257, 2064), (130, 384, 4096), (255, 65, 1040), (300, 1000, 7168),
+         (517, 2047, 1616), (1100, 7200, 2064)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("bn,split", VARIANTS)
+def test_matmul(bn, split, M, N, K):
+    g = _gen(M + N + K)
+    a, w = _int8(g, M, K), _int8(g, N, K)
+    a_s = torch.rand(M, generator=g, device="cuda") + 0.01
+    w_s = torch.rand(N, generator=g, device="cuda") * 1e-6     # inside fp16's range
+    bias = torch.randn(N, generator=g, device="cuda")
+    for dtype, b in ((torch.bfloat16, None), (torch.float32, bias), (torch.float16, bias)):
+        ref, err = R.product(a, w, a_s, w_s, b)
+        _arm(bn, split)
+        R.check(fb.int8_matmul(a, w, a_s, w_s, b, out_dtype=dtype), ref, err, str(dtype))
+    # an output between other values: nothing beyond it is written
+    flat = torch.full((M * N + 2,), 3.0, device="cuda", dtype=torch.bfloat16)
+    _arm(bn, split)
+    fb.int8_matmul(a, w, a_s, w_s, output=flat[1:-1].view(M, N))
+    ref, err = R.product(a, w, a_s, w_s)
+    R.check(flat[1:-1].view(M, N), ref, err, "view")
+    assert float(flat[0]) == 3.0 and float(flat[-1]) == 3.0
+    assert fb.int8_status() == 0
+
+
 def test_no_group_of_a_tile_lies_beyond_its_shares():
     """The arithmetic of a split tile: its tokens in groups of 16 up to the last token, its shares of
     whole groups. Every group belongs to one of the S shares."""
