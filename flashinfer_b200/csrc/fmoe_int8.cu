@@ -851,6 +851,9 @@ struct alignas(16) PairTail {
   int abort_flag;
   int tiles;
   int live;
+  int gave_up;                  // set in every CTA of the cluster after a leader's abort
+  int last_round[kPairStages];  // the latest round of copies that this CTA issued into the stage,
+  int last_bytes[kPairStages];  // -1 for none, and its bytes
   alignas(16) float a_scale[kPairTokens];
   int ebase[kMaxLocalExperts + 1];
   int etile[kMaxLocalExperts + 1];
@@ -858,7 +861,8 @@ struct alignas(16) PairTail {
 constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStage + sizeof(PairTail) + 1024;
 static_assert((kPairTokens + 4 * 15) * kWRows * 4 <= kPairStages * kPairStage,
               "four shares of a tile's partial sums fit the stages");
-static_assert(kPairSmem <= 227 * 1024 && kPairStages >= kI8Producers, "pair shared memory, parity");
+static_assert(kPairSmem <= 227 * 1024, "pair shared memory");
+static_assert(kPairStages == kI8Producers, "a stage has one producer: parity, last_round");
 
 // Loads a box into this CTA's shared memory, its bytes counted on a barrier of the pair.
 __device__ __forceinline__ void tma_load_pair(void* dst, const void* tmap, uint32_t bar, int32_t c0,
@@ -926,6 +930,27 @@ __device__ __forceinline__ void pair_abort(PairTail* t) {
   atomicOr(&g_int8_status, FMOE_STATUS_TIMEOUT_INT8);
 }
 
+// After an abort, by the leader once no role of either CTA issues any more: waits (bounded) until the
+// copies issued into every stage have landed, in both CTAs. A round needs both CTAs' copies and the
+// next needs both CTAs' stages, so a CTA is at most one round ahead of the other; the half of a
+// round that was never issued is taken off what the barrier expects.
+__device__ __forceinline__ void pair_drain(PairTail* t, int peer) {
+  for (int s = 0; s < kPairStages; ++s) {
+    const int mine = t->last_round[s], other = ld_dsmem_s32(&t->last_round[s], peer);
+    const int r = max(mine, other);
+    if (r < 0) continue;
+    if (mine < r) {
+      mbar_arrive_expect_tx(&t->full[s], ld_dsmem_s32(&t->last_bytes[s], peer));
+    } else if (other < r) {
+      asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(
+                       smem_u32(&t->full[s])),
+                   "r"(t->last_bytes[s])
+                   : "memory");
+    }
+    (void)mbar_wait(&t->full[s], r & 1);
+  }
+}
+
 // SPLIT: the S pairs of a cluster share one tile, each with a range of K.
 template <bool SPLIT>
 __global__ void __launch_bounds__(kI8Threads, 1)
@@ -954,6 +979,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     mbar_init(&tail->drain, 1);
     mbar_init(&tail->never, 1);
     tail->abort_flag = 0;
+    tail->gave_up = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tm_a);
     tma_prefetch_desc(&tm_w);
@@ -1011,8 +1037,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     if (lane == 0) {
       const uint64_t pol_first = policy_evict_first();
       const uint64_t pol_last = policy_evict_last();
+      tail->last_round[pw] = -1;
       int it = 0;
-      bool ok = true;
+      // the injected failure also leaves rounds that one CTA of the pair alone has issued
+      bool ok = args.inject == 0 || pw != 2 - rank;
       for (int tile = first; tile < tiles && ok; tile += step) {
         const I8Tile u = decode_pair(tile, NT, tail, E);
         const int half = u.cols / 2;
@@ -1041,6 +1069,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
               tma_load_pair(st + (kWRows + b * kPairBox) * kKB, &tm_a, bar, k, arow + b * kPairBox,
                             pol_last);
           }
+          tail->last_round[s] = r;
+          tail->last_bytes[s] = blocks * (block_bytes / 2);
         }
       }
     }
@@ -1129,19 +1159,22 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   tc_fence_before();
   __syncthreads();
   // Never leave a bulk copy in flight into shared memory that is about to be released. Without an
-  // abort the leader's MMAs have waited for all of them; after one, two milliseconds pass, far
-  // beyond any copy's time.
-  if (threadIdx.x == 0 && *abort_flag) {
-    const uint64_t t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 2000000ull) {
-    }
+  // abort of the leader its MMAs have waited for all of them.
+  if (threadIdx.x == 0 && rank == 0 && *abort_flag)
+    for (int c = 0; c < 2 * S; ++c)
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at_rank(&tail->gave_up, c)), "r"(1)
+                   : "memory");
+  cluster_arrive();  // every pair's MMAs are done, their stages free
+  cluster_wait();
+  tc_fence_after();
+  if (*reinterpret_cast<volatile int*>(&tail->gave_up)) {
+    if (threadIdx.x == 0 && rank == 0) pair_drain(tail, cta + 1);
+    cluster_arrive();
+    cluster_wait();
   }
   if constexpr (SPLIT) {
     const I8Tile u = first < tiles ? decode_pair(first, NT, tail, E) : I8Tile{};
     const int per = split_share(u.rows, S);
-    cluster_arrive();  // every pair's MMAs are done, their stages free
-    cluster_wait();
-    tc_fence_after();
     if (warp >= kI8Epi0 && u.rows > 0)
       send_partials(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), (warp - kI8Epi0) >> 2, u,
                     per, smem, cta >> 1, rank, 2, (warp & 3) * 32 + lane);
@@ -1149,10 +1182,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     cluster_arrive();
     cluster_wait();
     if (u.rows > 0) finish_split(args, u, u.n0 + rank * kWRows, per, smem, S, cta >> 1);
+    // the pair gives its tensor memory back together
+    cluster_arrive();
+    cluster_wait();
   }
-  // no CTA's memory or barriers go away while another may still use them
-  cluster_arrive();
-  cluster_wait();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)

@@ -78,6 +78,34 @@ def test_pairs_whose_columns_exceed_their_shares(M):
     assert fb.int8_status() == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bn,split", VARIANTS)
+def test_a_wait_that_runs_out_ends_the_product(bn, split):
+    """A wait that nothing ends gives up after its 5 ms in every variant, the status says so once, and
+    the next product of the same variant (which needs the same tensor memory) is right. In a CTA pair
+    the injected failure also leaves one stage that only the leader has filled and one that only the
+    other CTA has: waiting for copies that were never issued would take 2 s."""
+    M, N, K = 300, 1000, 4096
+    g = _gen(bn + split)
+    a, w = _int8(g, M, K), _int8(g, N, K)
+    a_s, w_s = torch.rand(M, generator=g, device="cuda"), torch.rand(N, generator=g, device="cuda")
+    _arm(bn, split)
+    fb.int8_matmul(a, w, a_s, w_s)
+    assert fb.int8_status() == 0
+    assert _lib.load().fmoe_debug_arm_int8_timeout(5_000_000) == 0
+    _arm(bn, split)
+    t0 = time.perf_counter()
+    fb.int8_matmul(a, w, a_s, w_s)
+    assert fb.int8_status() == _lib.STATUS_TIMEOUT_INT8
+    assert time.perf_counter() - t0 < 1.0
+    assert fb.int8_status() == 0
+    _arm(bn, split)
+    y = fb.int8_matmul(a, w, a_s, w_s)
+    ref, err = R.product(a, w, a_s, w_s)
+    R.check(y, ref, err, "after")
+    assert fb.int8_status() == 0
+
+
 def test_refusals_of_a_variant():
     lib = _lib.load()
     for bad in ((0, 1), (32, 1), (256, 0), (256, 5), (-16, 1)):
