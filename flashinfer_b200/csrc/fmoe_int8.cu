@@ -16,6 +16,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <mutex>
 #include <type_traits>
 
 #include "fmoe_elem.cuh"
@@ -305,8 +306,12 @@ __device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, volatile
   }
 }
 
-// Set by a product whose bounded wait ran out, until take_int8_status reads it.
+// Set by a product whose bounded wait ran out, until take_int8_status takes it to g_int8_taken.
 __device__ int32_t g_int8_status;
+__device__ int32_t g_int8_taken;
+
+// Reads and clears in one step: a product on another stream may set the word at any time.
+__global__ void k_take_int8_status() { g_int8_taken = atomicExch(&g_int8_status, 0); }
 
 __device__ __forceinline__ void i8_abort(I8Tail* t) {
   *reinterpret_cast<volatile int*>(&t->abort_flag) = 1;
@@ -1406,11 +1411,14 @@ cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
 }
 
 cudaError_t take_int8_status(int32_t* status, cudaStream_t s) {
+  static std::mutex one_at_a_time;  // g_int8_taken is one call's until it has been copied out
+  const std::lock_guard<std::mutex> hold(one_at_a_time);
   void* p = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&p, g_int8_status);
+  cudaError_t e = cudaGetSymbolAddress(&p, g_int8_taken);
   if (e != cudaSuccess) return e;
-  e = cudaMemcpyAsync(status, p, sizeof(int32_t), cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int32_t), s);
+  k_take_int8_status<<<1, 1, 0, s>>>();
+  e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, sizeof(int32_t), cudaMemcpyDeviceToHost, s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   return e;
 }

@@ -110,7 +110,8 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
 
 def int8_status(device: Optional[torch.device] = None) -> int:
     """``_lib.STATUS_TIMEOUT_INT8`` if a wait inside an int8 product on the device ran out since the
-    last call (its output is not valid), else 0. Synchronises the current stream."""
+    last call (its output is not valid), else 0. Synchronises the current stream: products on other
+    streams are covered as far as they had finished, and by the next call otherwise."""
     index = None if device is None else torch.device(device).index
     if index is None:
         index = torch.cuda.current_device()

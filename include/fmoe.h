@@ -414,7 +414,9 @@ FMOE_API int fmoe_int8_expert_matmul(const void* rows, const void* weights, cons
                                      void* cuda_stream);
 
 /* FMOE_STATUS_TIMEOUT_INT8 if a wait of an int8 product on the current device ran out since the
- * last call (its output is not valid), else 0; synchronises the stream and clears the word. */
+ * last call (its output is not valid), else 0; synchronises the stream and clears the word. Covers
+ * the products that had finished by then: those of this stream, and of others as far as they were;
+ * what fails later is told to the next call. */
 FMOE_API int fmoe_int8_status(int32_t* status, void* cuda_stream);
 
 /* Failure-path test, as fmoe_debug_arm_timeout: the next int8 product of the calling host thread

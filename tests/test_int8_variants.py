@@ -1,5 +1,6 @@
 """Every tensor-core variant of the int8 products -- tiles of 16, 64 and 128 tokens, CTA pairs, each with
 K whole and split in 2 to 4 -- on the same sizes, whatever the size would choose."""
+import threading
 import time
 
 import pytest
@@ -103,6 +104,47 @@ def test_a_wait_that_runs_out_ends_the_product(bn, split):
     y = fb.int8_matmul(a, w, a_s, w_s)
     ref, err = R.product(a, w, a_s, w_s)
     R.check(y, ref, err, "after")
+    assert fb.int8_status() == 0
+
+
+@pytest.mark.gpu
+def test_no_failure_is_lost_to_a_concurrent_status_call():
+    """A thread asks for the status without pause while products fail on another stream: each failure is
+    seen by a call that ends after it."""
+    M, N, K = 16, 128, 256
+    g = _gen(0)
+    a, w = _int8(g, M, K), _int8(g, N, K)
+    a_s, w_s = torch.ones(M, device="cuda"), torch.ones(N, device="cuda")
+    fb.int8_matmul(a, w, a_s, w_s)
+    assert fb.int8_status() == 0
+    torch.cuda.synchronize()
+    state = {"polls": 0, "seen": 0, "stop": False}
+
+    def poll():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            while not state["stop"]:
+                if fb.int8_status():
+                    state["seen"] += 1
+                state["polls"] += 1
+
+    t = threading.Thread(target=poll)
+    t.start()
+    lost = 0
+    try:
+        for _ in range(400):
+            before = state["seen"]
+            assert _lib.load().fmoe_debug_arm_int8_timeout(100_000) == 0
+            fb.int8_matmul(a, w, a_s, w_s)
+            torch.cuda.current_stream().synchronize()
+            polls = state["polls"]
+            end = time.perf_counter() + 5
+            while state["polls"] < polls + 2 and time.perf_counter() < end:
+                time.sleep(0)
+            lost += state["seen"] == before
+    finally:
+        state["stop"] = True
+        t.join()
+    assert lost == 0
     assert fb.int8_status() == 0
 
 
