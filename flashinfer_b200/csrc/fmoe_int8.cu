@@ -278,6 +278,27 @@ __device__ __forceinline__ I8Tile decode_tile(int tile, int NT, const I8Tail* t,
   return r;
 }
 
+// The bases as a running maximum (by one warp): where one steps back, the rows before the largest so
+// far stay with the experts that have them. So no row is written twice, and no spread of the rows has
+// more tiles than the host's bound, which is the grid of a split.
+__device__ __forceinline__ void ascending_bases(int* base, int E, bool grouped) {
+  const int lane = threadIdx.x & 31;
+  if (!grouped) return;
+  int carry = 0;
+  for (int e0 = 0; e0 <= E; e0 += 32) {
+    const int e = e0 + lane;
+    int most = max(carry, e <= E ? base[e] : 0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, most, o);
+      if (lane >= o) most = max(most, up);
+    }
+    if (e <= E) base[e] = most;
+    carry = __shfl_sync(0xffffffffu, most, 31);
+  }
+  __syncwarp();
+}
+
 // True in one lane of a whole warp. The MMAs of a branch on it issue faster than those of a branch on
 // the lane's number: 517 x 2047 x 7168 takes 13.8 us, 17.6 with the other.
 __device__ __forceinline__ bool elect_one() {
@@ -574,7 +595,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   }
   __syncthreads();
   if (warp == 0) {
-    // token tiles per expert and their running sum; a base that steps back counts as empty
+    ascending_bases(tail->ebase, E, args.expert_base != nullptr);
+    // token tiles per expert and their running sum
     int carry = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + lane;
@@ -1003,6 +1025,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   }
   __syncthreads();
   if (warp == 0) {
+    ascending_bases(tail->ebase, E, args.expert_base != nullptr);
     int carry = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + lane;

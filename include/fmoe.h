@@ -404,8 +404,9 @@ FMOE_API int fmoe_int8_matmul(const void* a, const void* b, const float* a_scale
 
 /* The same with one matrix per expert: rows expert_base[e] .. expert_base[e + 1] of `rows`
  * int8 [R, K] are multiplied with weights[e] (int8 [E, N, K], scales [E, N]); expert_base int32
- * [E + 1] stays on the device. Bases outside [0, R] are clamped, an expert whose rows end before
- * they start has none. Rows before expert_base[0] and from expert_base[E] on are zeroed if zero_tail
+ * [E + 1] stays on the device. Bases outside [0, R] are clamped, and one that is smaller than an
+ * earlier one counts as that one: the expert before it has no rows, and every row has at most one
+ * expert. Rows before expert_base[0] and from expert_base[E] on are zeroed if zero_tail
  * is set and left as they were otherwise. num_local_experts: 1..256. */
 FMOE_API int fmoe_int8_expert_matmul(const void* rows, const void* weights, const float* row_scale,
                                      const float* weight_scale, const int32_t* expert_base,

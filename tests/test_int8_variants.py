@@ -79,6 +79,39 @@ def test_pairs_whose_columns_exceed_their_shares(M):
     assert fb.int8_status() == 0
 
 
+# bases that step back, over 700 rows: every expert names all rows (five times the tiles that 700 rows
+# have), and steps in the middle, at the end and out of range
+STEPS = [[0, 700, 0, 700, 0, 700], [5, 300, 20, 450, 450, 440], [-3, 90, 9000, -1, 650, 600],
+         [700, 600, 500, 400, 300, 0]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("base", STEPS)
+@pytest.mark.parametrize("bn,split", VARIANTS)
+def test_bases_that_step_back_give_every_row_one_expert(bn, split, base):
+    Rn, E, N, K = 700, 5, 257, 528
+    g = _gen(base[1])
+    rows, w = _int8(g, Rn, K), _int8(g, E, N, K)
+    r_s = torch.rand(Rn, generator=g, device="cuda") + 0.01
+    w_s = torch.rand(E, N, generator=g, device="cuda")
+    up, most = [], 0
+    for b in base:
+        most = max(most, min(max(b, 0), Rn))
+        up.append(most)
+    ref = torch.zeros(Rn, N, dtype=torch.float64, device="cuda")
+    err = torch.zeros_like(ref)
+    for e in range(E):
+        a, b = up[e], up[e + 1]
+        ref[a:b], err[a:b] = R.product(rows[a:b], w[e], r_s[a:b], w_s[e])
+    bases = torch.tensor(base, dtype=torch.int32, device="cuda")
+    _arm(bn, split)
+    y = fb.int8_expert_matmul(rows, w, r_s, w_s, bases, out_dtype=torch.float32)
+    R.check(y, ref, err, "rows")
+    _arm(bn, split)
+    assert torch.equal(y, fb.int8_expert_matmul(rows, w, r_s, w_s, bases, out_dtype=torch.float32))
+    assert fb.int8_status() == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("bn,split", VARIANTS)
 def test_a_wait_that_runs_out_ends_the_product(bn, split):
