@@ -79,6 +79,43 @@ def test_pairs_whose_columns_exceed_their_shares(M):
     assert fb.int8_status() == 0
 
 
+# E, N, K, first row, counts per expert, rows behind the last expert
+GROUPS = [(4, 130, 528, 0, [0, 3, 0, 2], 0),
+          (8, 96, 2064, 5, [0, 0, 50, 1, 0, 17, 0, 0], 32),
+          (5, 301, 1040, 0, [257, 0, 600, 16, 127], 9),
+          (2, 2100, 4112, 3, [2999, 1], 0),
+          (3, 200, 528, 40, [0, 0, 0], 0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,N,K,lo,counts,tail", GROUPS)
+@pytest.mark.parametrize("bn,split", VARIANTS)
+def test_expert_matmul(bn, split, E, N, K, lo, counts, tail):
+    g = _gen(E + N)
+    base = [lo]
+    for c in counts:
+        base.append(base[-1] + c)
+    Rn = base[-1] + tail
+    rows, w = _int8(g, Rn, K), _int8(g, E, N, K)
+    r_s = torch.rand(Rn, generator=g, device="cuda") + 0.01
+    w_s = torch.rand(E, N, generator=g, device="cuda") * 1e-3
+    ref = torch.zeros(Rn, N, dtype=torch.float64, device="cuda")
+    err = torch.zeros_like(ref)
+    for e in range(E):
+        a, b = base[e], base[e + 1]
+        ref[a:b], err[a:b] = R.product(rows[a:b], w[e], r_s[a:b], w_s[e])
+    bases = torch.tensor(base, dtype=torch.int32, device="cuda")
+    _arm(bn, split)
+    R.check(fb.int8_expert_matmul(rows, w, r_s, w_s, bases), ref, err, "rows")
+    out = torch.full((Rn, N), 3.0, device="cuda")
+    _arm(bn, split)
+    fb.int8_expert_matmul(rows, w, r_s, w_s, bases, output=out)
+    ref[:lo] = 3.0
+    ref[base[-1]:] = 3.0
+    R.check(out, ref, err, "given output")
+    assert fb.int8_status() == 0
+
+
 # bases that step back, over 700 rows: every expert names all rows (five times the tiles that 700 rows
 # have), and steps in the middle, at the end and out of range
 STEPS = [[0, 700, 0, 700, 0, 700], [5, 300, 20, 450, 450, 440], [-3, 90, 9000, -1, 650, 600],
