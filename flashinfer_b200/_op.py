@@ -81,6 +81,13 @@ def first_order_only() -> None:
         raise RuntimeError("this operator has no second derivative (create_graph=True)")
 
 
+def no_gradient(what: str, *tensors) -> None:
+    """Refuses a call that autograd would have to record: its result would be cut off from them."""
+    if recording(*tensors):
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached "
+                         "tensors")
+
+
 def recording(*tensors) -> bool:
     """Whether autograd records a call on these tensors (None among them allowed)."""
     if torch.is_grad_enabled():

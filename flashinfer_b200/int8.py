@@ -2,7 +2,9 @@
 
 ``quantize_int8`` turns activations (or, once, weights) into int8 rows and their scales;
 ``int8_matmul`` multiplies them with one weight matrix and ``int8_expert_matmul`` with one matrix
-per expert, over rows in the expert order of ``sort_by_expert``. Sums are exact in int32.
+per expert, over rows in the expert order of ``sort_by_expert``. Sums are exact in int32. None of them
+has a gradient: a call that autograd would record (a tensor that requires a gradient, outside
+``torch.no_grad()``) is refused.
 """
 from __future__ import annotations
 
@@ -12,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, call, first, need, ptr
+from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, call, first, need, no_gradient, ptr
 
 _HALVES = (torch.bfloat16, torch.float16)
 
@@ -29,6 +31,7 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     R, K = x.shape
     if K < 1:
         raise ValueError("x needs at least one column")
+    no_gradient("quantize_int8", x)
     q = x.new_empty((R, K), dtype=torch.int8)
     scale = x.new_empty(R, dtype=torch.float32)
     call("fmoe_quantize_int8", index, x.data_ptr(), DTYPE_TAG[x.dtype], R, K, q.data_ptr(),
@@ -70,6 +73,7 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
     need(b_scale, "b_scale", index, (N,), F32)
     if bias is not None:
         need(bias, "bias", index, (N,), F32)
+    no_gradient("int8_matmul", a_scale, b_scale, bias, output)
     output = _output(output, out_dtype, a, index, (M, N))
     call("fmoe_int8_matmul", index, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(),
          b_scale.data_ptr(), ptr(bias), M, N, K, output.data_ptr(), DTYPE_TAG[output.dtype])
@@ -100,6 +104,7 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
     need(row_scale, "row_scale", index, (R,), F32)
     need(weight_scale, "weight_scale", index, (E, N), F32)
     need(expert_base, "expert_base", index, (E + 1,), I32)
+    no_gradient("int8_expert_matmul", row_scale, weight_scale, output)
     zero_tail = output is None
     output = _output(output, out_dtype, rows, index, (R, N))
     call("fmoe_int8_expert_matmul", index, rows.data_ptr(), weights.data_ptr(),

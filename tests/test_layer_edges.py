@@ -61,3 +61,34 @@ def test_gradient_of_rows_without_tokens_is_zero(tag, dtype):
     assert not bool(grad.any()) and float(flat[0]) == 3.0 and float(flat[-1]) == 3.0
     assert lib.fmoe_unsort_rows_backward(None, None, tag, 33, o, None, grad.data_ptr() + 1, None,
                                          stream) == -3
+
+
+def _int8_calls():
+    """The int8 operators' calls and, for each, the float tensors that it takes."""
+    x = torch.randn(4, 32, device="cuda").to(torch.bfloat16)
+    a = torch.ones((4, 32), dtype=torch.int8, device="cuda")
+    w = torch.ones((6, 32), dtype=torch.int8, device="cuda")
+    s4, s6, bias = (torch.ones(n, device="cuda") for n in (4, 6, 6))
+    out = torch.zeros((4, 6), device="cuda")
+    base = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    return [(lambda: fb.quantize_int8(x), (x,)),
+            (lambda: fb.int8_matmul(a, w, s4, s6, bias, output=out), (s4, s6, bias, out)),
+            (lambda: fb.int8_expert_matmul(a, w[None], s4, s6[None], base, output=out),
+             (s4, s6, out))]
+
+
+@pytest.mark.gpu
+def test_int8_operators_are_not_recorded():
+    """A float tensor that requires a gradient is refused, unless nothing is recorded."""
+    for call, tensors in _int8_calls():
+        call()
+        for t in tensors:
+            t.requires_grad_()
+            with pytest.raises(ValueError, match="no gradient"):
+                call()
+            with torch.no_grad():
+                call()
+            with torch.inference_mode():
+                call()
+            t.requires_grad_(False)
+        call()
