@@ -9,6 +9,7 @@ from typing import Optional
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -89,7 +90,13 @@ def no_gradient(what: str, *tensors) -> None:
 
 
 def recording(*tensors) -> bool:
-    """Whether autograd records a call on these tensors (None among them allowed)."""
+    """Whether autograd records a call on these tensors (None among them allowed). Refuses dual
+    tensors: the library would drop their tangents, which need neither ``requires_grad`` nor grad
+    mode."""
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("this operator has no forward-mode derivative")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

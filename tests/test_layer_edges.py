@@ -4,9 +4,10 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flashinfer_b200 as fb
-from flashinfer_b200 import _lib
+from flashinfer_b200 import _lib, _op
 
 
 def _order_struct(T, K, E, R, base=4096, row_pick=8192, pick_row=12288):
@@ -92,3 +93,38 @@ def test_int8_operators_are_not_recorded():
                 call()
             t.requires_grad_(False)
         call()
+
+
+def test_dual_tensors_are_refused():
+    """A dual tensor does not require a gradient, but a result without a tangent would be wrong."""
+    t = torch.ones(3)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(t, t)
+        assert not _op.recording(t, None)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                _op.recording(t, None, d)
+    assert not _op.recording(t, None)
+
+
+@pytest.mark.gpu
+def test_dual_tensors_are_refused_by_every_operator():
+    order = fb.sort_by_expert(torch.zeros((4, 1), dtype=torch.int32, device="cuda"), 1)
+    x, y, w = (torch.randn(*s, device="cuda") for s in ((4, 32), (4, 32), (32,)))
+    weights = torch.rand(4, 1, device="cuda")
+    calls = [(lambda x: fb.block_norm(x, y, post_weight=w, pre_weight=w), x),
+             (lambda x: fb.block_norm(y, x, pre_weight=w), x),
+             (lambda p: fb.block_norm(x, y, post_weight=p), w),
+             (lambda p: fb.block_norm(x, y, gate=p), w),
+             (lambda p: fb.block_norm(x, y, pre_weight=p), w),
+             (lambda x: fb.sort_tokens(x, order), x),
+             (lambda x: fb.unsort_tokens(x, order, weights), x),
+             (lambda p: fb.unsort_tokens(x, order, p), weights),
+             (lambda x: fb.quantize_int8(x.to(torch.bfloat16)), x)]
+    for call, t in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            call(t)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
