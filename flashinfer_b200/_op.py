@@ -9,6 +9,8 @@ from typing import Optional
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
+from torch._C import _get_tracing_state as _tracing_state
+from torch._C import _len_torch_dispatch_stack as _dispatch_modes
 from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
@@ -40,6 +42,7 @@ def _refuse(t, name: str, index: Optional[int], shape, dtypes) -> None:
 
 def first(t, name: str, dtypes, dim: int) -> int:
     """The device index of a call's first tensor: CUDA, contiguous, ``dim`` axes, of ``dtypes``."""
+    not_traced()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dim() != dim:
@@ -55,6 +58,18 @@ def need(t, name: str, index: int, shape, dtypes) -> None:
             and (shape is None or t.shape == shape) and (dtypes is None or t.dtype in dtypes)
             and t.is_contiguous()):
         _refuse(t, name, index, shape, dtypes)
+
+
+def not_traced() -> None:
+    """Refuses ``torch.jit.trace`` and ``make_fx``: what they record would hold the outputs' allocation
+    and not the call that writes them."""
+    if _tracing_state() is not None or (_dispatch_modes() and _fx_tracing()):
+        raise RuntimeError("this operator cannot be traced (torch.jit.trace, make_fx)")
+
+
+def _fx_tracing() -> bool:
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
 
 
 def ptr(t: Optional[torch.Tensor]):

@@ -16,7 +16,8 @@ import torch
 
 from . import _lib
 from ._lib import FmoeTokenOrder
-from ._op import DTYPE_TAG, F32, I32, call, first, first_order_only, need, ptr, recording
+from ._op import (DTYPE_TAG, F32, I32, call, first, first_order_only, need, not_traced, ptr,
+                  recording)
 
 
 class ExpertOrder:
@@ -144,6 +145,7 @@ class _UnsortTokens(torch.autograd.Function):
 
 
 def _check(t, name: str, order, n: int) -> None:
+    not_traced()
     if not isinstance(order, ExpertOrder):
         raise TypeError("order must be an ExpertOrder (sort_by_expert)")
     need(t, name, order._index, None, None)

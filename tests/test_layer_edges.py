@@ -5,6 +5,7 @@ import ctypes
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import flashinfer_b200 as fb
 from flashinfer_b200 import _lib, _op
@@ -128,3 +129,29 @@ def test_dual_tensors_are_refused_by_every_operator():
             call(t)
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (t,), (torch.ones_like(t),))
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("call", [
+    lambda x: fb.block_norm(None, x, pre_weight=x[0]), lambda x: fb.quantize_int8(x),
+    lambda x: fb.sort_by_expert(x, 4).expert_base, lambda x: fb.sort_tokens(x, None),
+    lambda x: fb.unsort_tokens(x, None), lambda x: fb.int8_matmul(x, x, x, x),
+    lambda x: fb.int8_expert_matmul(x, x, x, x, x)])
+def test_tracing_is_refused(call):
+    """Before anything else is looked at: a trace would return memory that nothing wrote."""
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, torch.ones(4, 8))
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(torch.ones(4, 8))
+
+
+@pytest.mark.gpu
+def test_other_dispatch_modes_are_left_alone():
+    class Pass(torch.utils._python_dispatch.TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x = torch.randn(4, 32, device="cuda")
+    want = fb.block_norm(None, x, pre_weight=x[0])[1]
+    with Pass():
+        assert torch.equal(fb.block_norm(None, x, pre_weight=x[0])[1], want)
