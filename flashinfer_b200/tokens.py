@@ -27,22 +27,39 @@ class ExpertOrder:
     last entry is where the rows end. ``row_pick`` int32 [num_rows]: the flat pick ``t * top_k + k``
     of each row, -1 for a row without one (padding, and every row from ``expert_base[E]`` on).
     ``pick_row`` int32 [T, top_k]: the row of each pick, -1 if its expert is not local. Rows are
-    ordered by expert, within an expert by pick.
+    ordered by expert, within an expert by pick. The attributes cannot be set: the library is given the
+    tables' addresses once.
     """
 
-    __slots__ = ("expert_base", "row_pick", "pick_row", "num_tokens", "top_k", "num_rows",
-                 "device", "_index", "_c", "_ref")
+    __slots__ = ("_tables", "_sizes", "_index", "_c", "_ref")
 
-    def __init__(self, expert_base, row_pick, pick_row):
-        self.expert_base, self.row_pick, self.pick_row = expert_base, row_pick, pick_row
-        self.num_tokens, self.top_k = pick_row.shape
-        self.num_rows = row_pick.shape[0]
-        self.device = pick_row.device
-        self._index = pick_row.get_device()
-        self._c = FmoeTokenOrder(self.num_tokens, self.top_k, expert_base.shape[0] - 1,
-                                 self.num_rows, expert_base.data_ptr(), row_pick.data_ptr(),
-                                 pick_row.data_ptr())
+    def __init__(self, expert_base: torch.Tensor, row_pick: torch.Tensor, pick_row: torch.Tensor):
+        index = first(pick_row, "pick_row", I32, 2)
+        need(expert_base, "expert_base", index, None, I32)
+        need(row_pick, "row_pick", index, None, I32)
+        T, K = pick_row.shape
+        if expert_base.dim() != 1 or not 2 <= expert_base.shape[0] <= 1025:
+            raise ValueError(f"expert_base must hold 2..1025 rows, got {tuple(expert_base.shape)}")
+        if K < 1 or row_pick.dim() != 1 or row_pick.shape[0] < T * K:
+            raise ValueError(f"row_pick {tuple(row_pick.shape)} must hold a row for every pick of "
+                             f"pick_row {(T, K)}")
+        self._set(index, expert_base, row_pick, pick_row)
+
+    def _set(self, index: int, expert_base, row_pick, pick_row) -> None:
+        T, K = pick_row.shape
+        rows = row_pick.shape[0]
+        self._tables, self._sizes, self._index = (expert_base, row_pick, pick_row), (T, K, rows), index
+        self._c = FmoeTokenOrder(T, K, expert_base.shape[0] - 1, rows, expert_base.data_ptr(),
+                                 row_pick.data_ptr(), pick_row.data_ptr())
         self._ref = ctypes.byref(self._c)
+
+    expert_base = property(lambda self: self._tables[0])
+    row_pick = property(lambda self: self._tables[1])
+    pick_row = property(lambda self: self._tables[2])
+    num_tokens = property(lambda self: self._sizes[0])
+    top_k = property(lambda self: self._sizes[1])
+    num_rows = property(lambda self: self._sizes[2])
+    device = property(lambda self: self._tables[2].device)
 
 
 @lru_cache(maxsize=1024)
@@ -74,8 +91,9 @@ def sort_by_expert(topk_ids: torch.Tensor, num_local_experts: int, local_expert_
     if not 1 <= align <= 1024:
         raise ValueError(f"align must be 1..1024, got {align}")
     rows, scratch_bytes = _sizes(T, K, num_local_experts, align)
-    order = ExpertOrder(topk_ids.new_empty(num_local_experts + 1), topk_ids.new_empty(rows),
-                        topk_ids.new_empty((T, K)))
+    order = ExpertOrder.__new__(ExpertOrder)  # of tables that need no checks
+    order._set(index, topk_ids.new_empty(num_local_experts + 1), topk_ids.new_empty(rows),
+               topk_ids.new_empty((T, K)))
     scratch = topk_ids.new_empty(scratch_bytes // 4) if scratch_bytes else None
     call("fmoe_sort_by_expert", index, topk_ids.data_ptr(), local_expert_offset, align, order._ref,
          ptr(scratch), scratch_bytes)

@@ -155,3 +155,38 @@ def test_other_dispatch_modes_are_left_alone():
     want = fb.block_norm(None, x, pre_weight=x[0])[1]
     with Pass():
         assert torch.equal(fb.block_norm(None, x, pre_weight=x[0])[1], want)
+
+
+def test_an_order_of_host_tables_is_refused():
+    base, rows = torch.zeros(5, dtype=torch.int32), torch.zeros(8, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        fb.ExpertOrder(base, rows, torch.zeros((4, 2), dtype=torch.int32))
+    with pytest.raises(ValueError, match="axes"):
+        fb.ExpertOrder(base, rows, rows)
+    with pytest.raises(TypeError, match="Tensor"):
+        fb.ExpertOrder(base, rows, None)
+
+
+@pytest.mark.gpu
+def test_the_tables_of_an_order_are_checked_and_stay():
+    """A hand-made order is checked as every argument is; its attributes cannot be set, since the library
+    would keep the old table's address."""
+    ids = torch.tensor([[0, 3], [1, 0], [2, 2], [3, 1]], dtype=torch.int32, device="cuda")
+    made = fb.sort_by_expert(ids, 4)
+    base, rows, picks = made.expert_base, made.row_pick, made.pick_row
+    order = fb.ExpertOrder(base, rows, picks)
+    x = torch.randn(4, 8, device="cuda")
+    assert torch.equal(fb.sort_tokens(x, order), fb.sort_tokens(x, made))
+    assert (order.num_tokens, order.top_k, order.num_rows) == (4, 2, 8)
+    assert order.device == x.device
+    for name in ("expert_base", "row_pick", "pick_row", "num_tokens", "top_k", "num_rows", "device"):
+        with pytest.raises(AttributeError):
+            setattr(order, name, getattr(order, name))
+    for bad in ((base.long(), rows, picks), (base, rows.long(), picks), (base, rows, picks.long())):
+        with pytest.raises(TypeError, match="int32"):
+            fb.ExpertOrder(*bad)
+    for bad in ((base.cpu(), rows, picks), (base, rows.cpu(), picks),
+                (base, rows.repeat(2)[::2], picks), (base, rows, picks.t()), (base, rows[:7], picks),
+                (base[:1], rows, picks), (base[None], rows, picks), (base, rows[None], picks)):
+        with pytest.raises(ValueError):
+            fb.ExpertOrder(*bad)
