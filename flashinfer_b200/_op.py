@@ -12,6 +12,7 @@ from torch._C import _cuda_getCurrentRawStream as _raw_stream
 from torch._C import _get_tracing_state as _tracing_state
 from torch._C import _len_torch_dispatch_stack as _dispatch_modes
 from torch.autograd import forward_ad as _forward_ad
+from torch.autograd.graph import increment_version as _increment_version
 
 from . import _lib
 
@@ -70,6 +71,13 @@ def not_traced() -> None:
 def _fx_tracing() -> bool:
     from torch.fx.experimental.proxy_tensor import get_proxy_mode
     return get_proxy_mode() is not None
+
+
+def written(output: torch.Tensor) -> torch.Tensor:
+    """A given output after the call: autograd learns that its values changed, so that a backward pass
+    which saved them raises instead of using the new ones."""
+    _increment_version(output)
+    return output
 
 
 def ptr(t: Optional[torch.Tensor]):

@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, call, first, need, no_gradient, ptr
+from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, call, first, need, no_gradient, ptr, written
 
 _HALVES = (torch.bfloat16, torch.float16)
 
@@ -74,10 +74,11 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
     if bias is not None:
         need(bias, "bias", index, (N,), F32)
     no_gradient("int8_matmul", a_scale, b_scale, bias, output)
+    given = output is not None
     output = _output(output, out_dtype, a, index, (M, N))
     call("fmoe_int8_matmul", index, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(),
          b_scale.data_ptr(), ptr(bias), M, N, K, output.data_ptr(), DTYPE_TAG[output.dtype])
-    return output
+    return written(output) if given else output
 
 
 def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: torch.Tensor,
@@ -105,12 +106,12 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
     need(weight_scale, "weight_scale", index, (E, N), F32)
     need(expert_base, "expert_base", index, (E + 1,), I32)
     no_gradient("int8_expert_matmul", row_scale, weight_scale, output)
-    zero_tail = output is None
+    given = output is not None
     output = _output(output, out_dtype, rows, index, (R, N))
     call("fmoe_int8_expert_matmul", index, rows.data_ptr(), weights.data_ptr(),
          row_scale.data_ptr(), weight_scale.data_ptr(), expert_base.data_ptr(), R, E, N, K,
-         output.data_ptr(), DTYPE_TAG[output.dtype], int(zero_tail))
-    return output
+         output.data_ptr(), DTYPE_TAG[output.dtype], int(not given))
+    return written(output) if given else output
 
 
 def int8_status(device: Optional[torch.device] = None) -> int:

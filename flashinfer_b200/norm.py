@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import FmoeBlockNormArgs
-from ._op import DTYPE_TAG, FLOATS, call, first, first_order_only, need, ptr, recording
+from ._op import DTYPE_TAG, FLOATS, call, first, first_order_only, need, ptr, recording, written
 
 BLOCK = 128
 
@@ -38,7 +38,8 @@ def _forward(branch, residual, post_weight, gate, pre_weight, kind, residual_sca
              hidden, want_stats):
     a = _args(branch, residual, post_weight, gate, pre_weight, kind, residual_scale, eps)
     T, H = residual.shape
-    if hidden is not None:
+    given = hidden is not None
+    if given:
         a.hidden = hidden.data_ptr()
     elif branch is None and residual_scale == 1.0 and not want_stats:
         hidden = residual  # without a block output and with scale 1 it is what it was
@@ -58,6 +59,8 @@ def _forward(branch, residual, post_weight, gate, pre_weight, kind, residual_sca
         stats = residual.new_empty((T, 2), dtype=torch.float32)
         a.stats = stats.data_ptr()
     call("fmoe_block_norm", residual.get_device(), ctypes.byref(a))
+    if given:
+        written(hidden)
     return hidden, normed, stats
 
 

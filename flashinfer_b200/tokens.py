@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import FmoeTokenOrder
 from ._op import (DTYPE_TAG, F32, I32, call, first, first_order_only, need, not_traced, ptr,
-                  recording)
+                  recording, written)
 
 
 class ExpertOrder:
@@ -105,22 +105,23 @@ def _rows_shape(x: torch.Tensor, n: int):
 
 
 def _sort(x: torch.Tensor, order: ExpertOrder, output: Optional[torch.Tensor]) -> torch.Tensor:
-    zero_tail = output is None
-    if output is None:
+    given = output is not None
+    if not given:
         output = x.new_empty(_rows_shape(x, order.num_rows))
     row_bytes = x.element_size() * (1 if x.dim() == 1 else x.shape[1])
     call("fmoe_sort_rows", order._index, x.data_ptr(), row_bytes, order._ref, output.data_ptr(),
-         int(zero_tail))
-    return output
+         int(not given))
+    return written(output) if given else output
 
 
 def _unsort(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor],
             output: Optional[torch.Tensor]) -> torch.Tensor:
-    if output is None:
+    given = output is not None
+    if not given:
         output = rows.new_empty(_rows_shape(rows, order.num_tokens))
     call("fmoe_unsort_rows", order._index, rows.data_ptr(), DTYPE_TAG[rows.dtype],
          1 if rows.dim() == 1 else rows.shape[1], order._ref, ptr(weights), output.data_ptr())
-    return output
+    return written(output) if given else output
 
 
 class _SortTokens(torch.autograd.Function):

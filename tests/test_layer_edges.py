@@ -190,3 +190,33 @@ def test_the_tables_of_an_order_are_checked_and_stay():
                 (base[:1], rows, picks), (base[None], rows, picks), (base, rows[None], picks)):
         with pytest.raises(ValueError):
             fb.ExpertOrder(*bad)
+
+
+@pytest.mark.gpu
+def test_a_given_output_counts_as_changed():
+    """A tensor that a recorded operation saved and a later call writes to: the backward pass raises, as
+    it does for torch's own operations in place."""
+    order = fb.sort_by_expert(torch.zeros((4, 1), dtype=torch.int32, device="cuda"), 1)
+    x, y, w = (torch.randn(*s, device="cuda") for s in ((4, 32), (4, 32), (32,)))
+    a = torch.ones((4, 32), dtype=torch.int8, device="cuda")
+    b = torch.ones((32, 32), dtype=torch.int8, device="cuda")
+    s4, s32 = torch.ones(4, device="cuda"), torch.ones(32, device="cuda")
+    base = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    calls = [lambda o: fb.block_norm(x, o, pre_weight=w, output=o)[0],       # in place
+             lambda o: fb.block_norm(x, y, output=o)[0],
+             lambda o: fb.sort_tokens(x, order, output=o),
+             lambda o: fb.unsort_tokens(x, order, output=o),
+             lambda o: fb.int8_matmul(a, b, s4, s32, output=o),
+             lambda o: fb.int8_expert_matmul(a, b[None], s4, s32[None], base, output=o)]
+    for call in calls:
+        out = torch.randn(4, 32, device="cuda")
+        p = torch.ones(4, 32, device="cuda", requires_grad=True)
+        loss = (p * out).sum()
+        before = out._version
+        with torch.no_grad():
+            assert call(out) is out
+        assert out._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.inference_mode():
+            call(torch.zeros(4, 32, device="cuda"))
