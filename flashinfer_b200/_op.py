@@ -22,6 +22,7 @@ I8 = (torch.int8,)
 I32 = (torch.int32,)
 F32 = (torch.float32,)
 FLOATS = tuple(DTYPE_TAG)
+INT_MAX = 2 ** 31 - 1  # what is passed as a C int; ctypes drops the bits above without a word
 
 
 _FUNCTIONS = {}  # the library's entry points by name

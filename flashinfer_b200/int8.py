@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, call, first, need, no_gradient, ptr, written
+from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, INT_MAX, call, first, need, no_gradient, ptr, written
 
 _HALVES = (torch.bfloat16, torch.float16)
 
@@ -39,7 +39,9 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return q, scale
 
 
-def _check_depth(K: int) -> None:
+def _check_sizes(channels: int, K: int) -> None:
+    if channels > INT_MAX:
+        raise ValueError(f"at most 2^31 - 1 output channels are possible, got {channels}")
     if K < 16 or K % 16 or K > 131056:
         raise ValueError(f"the depth K must be a multiple of 16 from 16 to 131056, got {K}")
 
@@ -68,7 +70,7 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
         raise ValueError(f"a [M, K] and b [N, K] do not fit: {tuple(a.shape)}, {tuple(b.shape)}")
     M, K = a.shape
     N = b.shape[0]
-    _check_depth(K)
+    _check_sizes(N, K)
     need(a_scale, "a_scale", index, (M,), F32)
     need(b_scale, "b_scale", index, (N,), F32)
     if bias is not None:
@@ -101,7 +103,7 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
     E, N, _ = weights.shape
     if not 1 <= E <= 256:
         raise ValueError(f"weights must hold 1..256 experts, got {E}")
-    _check_depth(K)
+    _check_sizes(N, K)
     need(row_scale, "row_scale", index, (R,), F32)
     need(weight_scale, "weight_scale", index, (E, N), F32)
     need(expert_base, "expert_base", index, (E + 1,), I32)

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import FmoeTokenOrder
-from ._op import (DTYPE_TAG, F32, I32, call, first, first_order_only, need, not_traced, ptr,
+from ._op import (DTYPE_TAG, F32, I32, INT_MAX, call, first, first_order_only, need, not_traced, ptr,
                   recording, written)
 
 
@@ -86,10 +86,13 @@ def sort_by_expert(topk_ids: torch.Tensor, num_local_experts: int, local_expert_
         raise ValueError("topk_ids needs at least one pick per token")
     if not 1 <= num_local_experts <= 1024:
         raise ValueError(f"num_local_experts must be 1..1024, got {num_local_experts}")
-    if local_expert_offset < 0:
-        raise ValueError(f"local_expert_offset must not be negative, got {local_expert_offset}")
+    if not 0 <= local_expert_offset <= INT_MAX:
+        raise ValueError("local_expert_offset must not be negative, nor beyond int32, got "
+                         f"{local_expert_offset}")
     if not 1 <= align <= 1024:
         raise ValueError(f"align must be 1..1024, got {align}")
+    if T * K > INT_MAX:
+        raise ValueError(f"topk_ids holds {T * K} picks: fewer than 2^31 rows are possible")
     rows, scratch_bytes = _sizes(T, K, num_local_experts, align)
     order = ExpertOrder.__new__(ExpertOrder)  # of tables that need no checks
     order._set(index, topk_ids.new_empty(num_local_experts + 1), topk_ids.new_empty(rows),

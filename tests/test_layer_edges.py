@@ -220,3 +220,30 @@ def test_a_given_output_counts_as_changed():
             loss.backward()
         with torch.inference_mode():
             call(torch.zeros(4, 32, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_an_offset_beyond_32_bits_is_refused():
+    """As a C int it would be another offset: 2^32 would name expert 0."""
+    ids = torch.zeros((4, 2), dtype=torch.int32, device="cuda")
+    last = fb.sort_by_expert(ids, 4, 2 ** 31 - 1)
+    assert last.expert_base.tolist() == [0] * 5 and bool((last.pick_row == -1).all())
+    for offset in (2 ** 31, 2 ** 32, 2 ** 32 + 3, -1):
+        with pytest.raises(ValueError, match="local_expert_offset"):
+            fb.sort_by_expert(ids, 4, offset)
+
+
+def test_channels_beyond_32_bits_are_refused():
+    from flashinfer_b200.int8 import _check_sizes
+    _check_sizes(2 ** 31 - 1, 16)
+    for channels in (2 ** 31, 2 ** 32 + 8):
+        with pytest.raises(ValueError, match="channels"):
+            _check_sizes(channels, 16)
+
+
+@pytest.mark.gpu
+def test_picks_beyond_32_bits_are_refused():
+    """2^32 + 4 tokens: as a C int four. The tensor is only allocated (17 GB), and read by nothing."""
+    ids = torch.empty((2 ** 32 + 4, 1), dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="picks"):
+        fb.sort_by_expert(ids, 4)
