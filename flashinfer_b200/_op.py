@@ -9,7 +9,7 @@ from typing import Optional
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
-from torch._C import _get_tracing_state as _tracing_state
+from torch._C import _is_tracing
 from torch._C import _len_torch_dispatch_stack as _dispatch_modes
 from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.graph import increment_version as _increment_version
@@ -44,7 +44,8 @@ def _refuse(t, name: str, index: Optional[int], shape, dtypes) -> None:
 
 def first(t, name: str, dtypes, dim: int) -> int:
     """The device index of a call's first tensor: CUDA, contiguous, ``dim`` axes, of ``dtypes``."""
-    not_traced()
+    if _is_tracing() or _dispatch_modes():
+        not_traced()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dim() != dim:
@@ -65,7 +66,7 @@ def need(t, name: str, index: int, shape, dtypes) -> None:
 def not_traced() -> None:
     """Refuses ``torch.jit.trace`` and ``make_fx``: what they record would hold the outputs' allocation
     and not the call that writes them."""
-    if _tracing_state() is not None or (_dispatch_modes() and _fx_tracing()):
+    if _is_tracing() or (_dispatch_modes() and _fx_tracing()):
         raise RuntimeError("this operator cannot be traced (torch.jit.trace, make_fx)")
 
 
@@ -106,11 +107,9 @@ def first_order_only() -> None:
         raise RuntimeError("this operator has no second derivative (create_graph=True)")
 
 
-def no_gradient(what: str, *tensors) -> None:
-    """Refuses a call that autograd would have to record: its result would be cut off from them."""
-    if recording(*tensors):
-        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached "
-                         "tensors")
+def no_gradient(what: str) -> None:
+    """Refuses a call that autograd would have to record: its result would be cut off."""
+    raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def recording(*tensors) -> bool:

@@ -14,7 +14,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._op import DTYPE_TAG, F32, FLOATS, I32, I8, INT_MAX, call, first, need, no_gradient, ptr, written
+from ._op import (DTYPE_TAG, F32, FLOATS, I32, I8, INT_MAX, call, first, need, no_gradient, ptr,
+                  recording, written)
 
 _HALVES = (torch.bfloat16, torch.float16)
 
@@ -31,7 +32,8 @@ def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     R, K = x.shape
     if K < 1:
         raise ValueError("x needs at least one column")
-    no_gradient("quantize_int8", x)
+    if recording(x):
+        no_gradient("quantize_int8")
     q = x.new_empty((R, K), dtype=torch.int8)
     scale = x.new_empty(R, dtype=torch.float32)
     call("fmoe_quantize_int8", index, x.data_ptr(), DTYPE_TAG[x.dtype], R, K, q.data_ptr(),
@@ -75,7 +77,8 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
     need(b_scale, "b_scale", index, (N,), F32)
     if bias is not None:
         need(bias, "bias", index, (N,), F32)
-    no_gradient("int8_matmul", a_scale, b_scale, bias, output)
+    if recording(a_scale, b_scale, bias, output):
+        no_gradient("int8_matmul")
     given = output is not None
     output = _output(output, out_dtype, a, index, (M, N))
     call("fmoe_int8_matmul", index, a.data_ptr(), b.data_ptr(), a_scale.data_ptr(),
@@ -107,7 +110,8 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
     need(row_scale, "row_scale", index, (R,), F32)
     need(weight_scale, "weight_scale", index, (E, N), F32)
     need(expert_base, "expert_base", index, (E + 1,), I32)
-    no_gradient("int8_expert_matmul", row_scale, weight_scale, output)
+    if recording(row_scale, weight_scale, output):
+        no_gradient("int8_expert_matmul")
     given = output is not None
     output = _output(output, out_dtype, rows, index, (R, N))
     call("fmoe_int8_expert_matmul", index, rows.data_ptr(), weights.data_ptr(),
