@@ -1263,12 +1263,16 @@ struct I8Plan {
 };
 
 // The tile width and K split with the shortest estimated time in cycles: rounds of tiles over the
-// SMs times the K blocks of a tile, a K block costing the slower of its round in the MMA warp (about
-// 640 cycles, however few the tokens) and its fill of shared memory (about 75 bytes a cycle); then the last tile's stores, the exchange of partial tiles and the cluster's barriers
-// where K is split, and a pair's own set-up. The last four are fitted to the times of every width and
-// split for 119 products of 5 to 3000 tokens and 24 of 8 to 8192 rows of experts: the choice was 0.4%
-// from the fastest on average and 9% at worst (with MMAs issued for lane 0, not under elect.sync). An expert is taken to have up to twice its even
-// share: with the even share alone the worst choice was 30% off.
+// SMs times the K blocks of a tile, a K block costing the slower of its round in the MMA warp (640
+// cycles, however few the tokens) and its fill of shared memory (about 75 bytes a cycle); then the last
+// tile's stores, the exchange of partial tiles and the cluster's barriers where K is split, and a
+// pair's own set-up. An expert is taken to have up to twice its even share: with the even share alone
+// the worst choice was 30% off.
+// The constants are of a loop that issued its MMAs for lane 0. Under elect.sync a round takes about a
+// third less, so 640 is too long: it hides the widths' differences, and splits look better than they
+// are. Against every width and split on the present kernels: 113 products of 5 to 8192 tokens 3.6%
+// from the fastest on average, 30% at worst (2048 x 512 x 7168: 16.4 us, with 64-token tiles 12.6; 256 x
+// 4096 x 7168: 17.1, 14.5), 30 of experts (8 to 8192 rows) 1.1% and 10%; within 1% for two in three.
 I8Plan i8_plan(int64_t M, int N, int E, int nkb, bool grouped, int sms, int dev) {
   const int64_t used = M < E ? M : E;
   int64_t per = (M + used - 1) / used;
@@ -1396,9 +1400,10 @@ cudaError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t
 }
 
 cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
-  // The tensor cores take 11.7 us for 1 to 4 tokens x 4096 x 7168 and 24.7 for 16384 channels, which
-  // are enough tiles for every SM; this way 1, 2 and 4 tokens take 8.0, 9.3 and 9.0 us, and with
-  // 16384 channels one token takes 20.8 and four take 29.0.
+  // The tensor cores take 10.4 us for 1 to 4 tokens x 4096 x 7168, this way 1, 2 and 4 tokens take 8.0,
+  // 9.2 and 9.0 (2048 x 2048: 5.6 against 2.8, 3.3 and 3.2). More channels are enough tiles for every
+  // SM: 9472 x 7168 takes 14.6 and 14.2, 17.3 and 15.3, 16384 x 7168 takes 20.9, and 20.6 and 22.3 for one
+  // token and two. With short rows the set-up counts again: 9472 x 1024 takes 5.0 against 2.8, 2.9 and 4.0.
   if (p.wait_ns == 0 && p.tile_tokens == 0 && !p.expert_base && p.M <= kGemvTokens && p.M * p.K <= kGemvSmem &&
       (p.M <= 2 || p.N <= 64 * sms)) {
     switch (p.M) {
