@@ -187,6 +187,10 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder, *,
     _check(x, "x", order, order.num_tokens if isinstance(order, ExpertOrder) else 0)
     if output is not None:
         need(output, "output", order._index, _rows_shape(x, order.num_rows), (x.dtype,))
+        if output.is_conj():
+            raise ValueError("output must not be a conjugate view")
+    if x.is_conj():  # its bytes are those before the conjugation
+        x = x.resolve_conj()
     if recording(x, output):
         if output is not None:
             raise ValueError("output cannot be given where gradients are recorded")

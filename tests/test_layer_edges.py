@@ -247,3 +247,18 @@ def test_picks_beyond_32_bits_are_refused():
     ids = torch.empty((2 ** 32 + 4, 1), dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="picks"):
         fb.sort_by_expert(ids, 4)
+
+
+@pytest.mark.gpu
+def test_rows_of_conjugate_views():
+    """Rows of any type, complex ones among them: a conjugate view shares the bytes of its base."""
+    ids = torch.tensor([[0, 3], [1, 0], [2, 2], [3, 1]], dtype=torch.int32, device="cuda")
+    order = fb.sort_by_expert(ids, 4)
+    x = torch.randn(4, 5, dtype=torch.complex64, device="cuda")
+    want = fb.sort_tokens(x.conj().resolve_conj(), order)
+    assert torch.equal(want[:, 0], x.conj()[order.row_pick.long() // 2][:, 0])
+    assert torch.equal(fb.sort_tokens(x.conj(), order), want)
+    out = torch.empty_like(want)
+    assert torch.equal(fb.sort_tokens(x.conj(), order, output=out), want)
+    with pytest.raises(ValueError, match="conjugate"):
+        fb.sort_tokens(x, order, output=out.conj())
