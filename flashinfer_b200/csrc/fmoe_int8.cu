@@ -1404,8 +1404,8 @@ cudaError_t launch_int8_product(const Int8Product& p, int sms, cudaStream_t s) {
   // 9.2 and 9.0 (2048 x 2048: 5.6 against 2.8, 3.3 and 3.2). More channels are enough tiles for every
   // SM: 9472 x 7168 takes 14.6 and 14.2, 17.3 and 15.3, 16384 x 7168 takes 20.9, and 20.6 and 22.3 for one
   // token and two. With short rows the set-up counts again: 9472 x 1024 takes 5.0 against 2.8, 2.9 and 4.0.
-  if (p.wait_ns == 0 && p.tile_tokens == 0 && !p.expert_base && p.M <= kGemvTokens && p.M * p.K <= kGemvSmem &&
-      (p.M <= 2 || p.N <= 64 * sms)) {
+  if (p.wait_ns == 0 && p.tile_tokens == 0 && !p.expert_base && p.M <= kGemvTokens &&
+      p.M * p.K <= kGemvSmem && (p.M <= 2 || p.N <= 64 * sms)) {
     switch (p.M) {
       case 1:
         return launch_gemv<1>(p, sms, s);

@@ -94,7 +94,8 @@ def int8_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, row_scale: tor
 
     rows int8 [R, K] in expert order, weights int8 [E, N, K] (E up to 256), row_scale fp32 [R],
     weight_scale fp32 [E, N], expert_base int32 [E+1] (``ExpertOrder.expert_base``), read on the
-    device. Returns [R, N]; rows before ``expert_base[0]`` and from ``expert_base[E]`` on are zero
+    device: a base smaller than an earlier one counts as that one, so a row has one expert at most.
+    Returns [R, N]; rows before ``expert_base[0]`` and from ``expert_base[E]`` on are zero
     in a new tensor and left as they were in a given ``output``.
     """
     index = first(rows, "rows", I8, 2)
