@@ -52,6 +52,7 @@ STATUS_TIMEOUT_GEMM1 = 0x1
 STATUS_TIMEOUT_GEMM2 = 0x2
 STATUS_TIMEOUT_INT8 = 0x4
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = 0, 1, 2, 3
+SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
 
 EXPORTS = ("fmoe_workspace_size", "fmoe_workspace_layout", "fmoe_run", "fmoe_route",
            "fmoe_read_status", "fmoe_device_sm_count", "fmoe_version",
@@ -62,7 +63,9 @@ EXPORTS = ("fmoe_workspace_size", "fmoe_workspace_layout", "fmoe_run", "fmoe_rou
            "fmoe_unsort_rows", "fmoe_unsort_rows_backward", "fmoe_quantize_int8",
            "fmoe_int8_matmul", "fmoe_int8_expert_matmul", "fmoe_int8_status",
            "fmoe_debug_arm_int8_timeout", "fmoe_debug_arm_int8_plan",
-           "fmoe_block_norm_workspace_size", "fmoe_block_norm", "fmoe_block_norm_backward")
+           "fmoe_block_norm_workspace_size", "fmoe_block_norm", "fmoe_block_norm_backward",
+           "fmoe_layer_norm_workspace_size", "fmoe_layer_norm", "fmoe_layer_norm_backward",
+           "fmoe_balance_workspace_size", "fmoe_balance_loss", "fmoe_balance_loss_backward")
 
 
 class FmoeArgs(Structure):
@@ -139,6 +142,24 @@ class FmoeBlockNormArgs(Structure):
         [("workspace_bytes", c_size_t)]
 
 
+class FmoeLayerNormArgs(Structure):
+    _fields_ = [("num_tokens", c_int64), ("hidden_size", c_int32), ("dtype", c_int32)] + \
+        [(n, c_void_p) for n in ("branch", "residual", "weight", "bias")] + \
+        [("weight_dtype", c_int32), ("bias_dtype", c_int32), ("eps", c_float)] + \
+        [(n, c_void_p) for n in ("hidden", "normed", "normed_q", "normed_scale", "stats",
+                                 "grad_hidden", "grad_normed", "grad_input", "grad_weight",
+                                 "grad_bias", "workspace")] + \
+        [("workspace_bytes", c_size_t)]
+
+
+class FmoeBalanceArgs(Structure):
+    _fields_ = [("num_tokens", c_int64)] + \
+        [(n, c_int32) for n in ("num_experts", "top_k", "num_sequences", "dtype", "scoring")] + \
+        [(n, c_void_p) for n in ("logits", "topk_ids", "sequence_base", "loss", "counts", "factor",
+                                 "grad_loss", "grad_logits", "workspace")] + \
+        [("workspace_bytes", c_size_t)]
+
+
 _lib = None
 
 
@@ -203,6 +224,12 @@ def load() -> ctypes.CDLL:
     lib.fmoe_block_norm_workspace_size.argtypes = [c_int64, c_int32, POINTER(c_size_t)]
     lib.fmoe_block_norm.argtypes = [POINTER(FmoeBlockNormArgs), c_void_p]
     lib.fmoe_block_norm_backward.argtypes = [POINTER(FmoeBlockNormArgs), c_void_p]
+    lib.fmoe_layer_norm_workspace_size.argtypes = [c_int64, c_int32, POINTER(c_size_t)]
+    lib.fmoe_layer_norm.argtypes = [POINTER(FmoeLayerNormArgs), c_void_p]
+    lib.fmoe_layer_norm_backward.argtypes = [POINTER(FmoeLayerNormArgs), c_void_p]
+    lib.fmoe_balance_workspace_size.argtypes = [c_int64, c_int32, c_int32, POINTER(c_size_t)]
+    lib.fmoe_balance_loss.argtypes = [POINTER(FmoeBalanceArgs), c_void_p]
+    lib.fmoe_balance_loss_backward.argtypes = [POINTER(FmoeBalanceArgs), c_void_p]
     lib.fmoe_version.restype = c_char_p
     for name in EXPORTS:
         if name != "fmoe_version":

@@ -1,0 +1,447 @@
+// fmoe_balance.cu -- the router's balance loss, the counts per expert it needs, and its gradient.
+//
+//   p[t, e]  = exp(u[t, e]) / sum_e' exp(u[t, e']),  u = logits, or log sigmoid(logits)
+//   n[s, e]  = picks of expert e by the T_s tokens of sequence s
+//   L_s      = sum_e  E n[s, e] / (K T_s) * (1 / T_s) sum_{t in s} p[t, e]
+//   loss     = mean of L_s over the sequences that have tokens
+// and with c[s, e] = E n[s, e] / (K T_s^2 S), S those sequences' number, g the gradient of the loss:
+//   d logits = g p (c - sum_e p c) * (1, or sigmoid(-logits))
+//
+// Forward: every block takes a range of tokens and adds up p (in registers, a lane's columns) and the
+// picks (in shared memory) of each sequence in it; one cluster then adds the blocks' shares in order.
+// The picks are counted beside the scores and need no pass of their own, and nothing has to be
+// zeroed first. Backward: one pass, a token per warp, the scores computed again. Logits are read once
+// per pass: bound by HBM, at small sizes by the two launches.
+#include <atomic>
+
+#include "fmoe_elem.cuh"
+#include "fmoe_internal.h"
+#include "fmoe_ptx.cuh"
+
+namespace fmoe {
+namespace {
+
+constexpr int kBalWarps = 8;
+constexpr int kBalThreads = kBalWarps * 32;
+constexpr int kBalCluster = 8;   // CTAs of the cluster that joins the shares
+constexpr int kBalMaxSmem = kBalWarps * kMaxBalanceExperts * 4 + kMaxBalanceExperts * 4 +
+                            (kMaxBalanceSequences + 1) * 4;
+
+struct BalArgs {
+  const void* logits;      // [T, E], or null: counts only (loss null), or no tokens
+  const int32_t* ids;      // [T, K]
+  const int32_t* base;     // [S + 1], or null: one sequence of all rows
+  int64_t T;
+  int E, K, S, sigmoid;
+  int rows;                // per block
+  int blocks;
+  float* part_p;           // [blocks + S][E]
+  int32_t* part_n;         // [blocks + S][E]
+  float* loss;
+  int32_t* counts;         // [S, E]
+  float* factor;           // [S]: E / (K T_s^2 S'), 0 for a sequence without tokens
+  // backward
+  const float* g;
+  void* d_logits;
+};
+
+// The sequences' first rows, and the end of the last, to shared memory: clamped to [0, T], and as a running
+// maximum, so that with a base that steps back no row belongs to two sequences. By the whole block, with a
+// barrier at the end.
+__device__ __forceinline__ void load_bases(const BalArgs& a, int* sbase) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int carry = 0;
+    for (int s0 = 0; s0 <= a.S; s0 += 32) {
+      const int s = s0 + lane;
+      int64_t b = 0;
+      if (s <= a.S) b = a.base ? __ldcg(a.base + s) : s == 0 ? 0 : a.T;
+      int most = max(carry, static_cast<int>(b < 0 ? 0 : b > a.T ? a.T : b));
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, most, o);
+        if (lane >= o) most = max(most, up);
+      }
+      if (s <= a.S) sbase[s] = most;
+      carry = __shfl_sync(0xffffffffu, most, 31);
+    }
+  }
+  __syncthreads();
+}
+
+// The first sequence that ends behind the row (S: none).
+__device__ __forceinline__ int sequence_of(const int* sbase, int S, int64_t row) {
+  int lo = 0, hi = S;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (sbase[mid + 1] > row)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+// A lane's values of one row: NV values in units of V, unit u of lane l being number u * 32 + l.
+template <typename T, int V, int NV>
+__device__ __forceinline__ void load_logits(const BalArgs& a, int64_t row, float (&v)[NV]) {
+  const int lane = threadIdx.x & 31, n = a.E / V;
+  const T* p = static_cast<const T*>(a.logits) + row * a.E;
+#pragma unroll
+  for (int u = 0; u < NV / V; ++u) {
+    const int i = u * 32 + lane;
+    float w[V];
+    if (i < n) {
+      unpack(load_pack<T, V>(p + i * V), w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[u * V + j] = w[j];
+  }
+}
+
+// v: logits in, exp(u - m) out, with m such that the largest are of ordinary size; slope:
+// d u / d logits (SLOPE). Returns 1 / sum, or 0 for a row whose logits are all -infinity (or whose
+// sigmoids all are 0): it has no scores. A NaN among the logits makes the sum NaN.
+//
+// sigmoid(l) itself is taken as the exponential (m = 0) unless every logit is below -60, where they
+// would run out of range: then sigmoid(l) exp(-m) = exp(l - m) / (1 + exp(l)) with m the largest logit.
+template <int NV, bool SLOPE>
+__device__ __forceinline__ float scores(float (&v)[NV], float (&slope)[SLOPE ? NV : 1], bool sigmoid) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) m = fmaxf(m, v[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float sum = 0.0f;
+  if (!sigmoid || m < -60.0f) {
+    const float shift = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      // below -60 the factor 1 / (1 + exp(l)) is 1 to fp32, as is d u / d logits
+      v[i] = expf(v[i] - shift);
+      if constexpr (SLOPE) slope[i] = 1.0f;
+      sum += v[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float t = expf(-fabsf(v[i]));
+      const float r = __fdividef(1.0f, 1.0f + t);
+      const bool neg = v[i] <= 0.0f;
+      const float e = (neg ? t : 1.0f) * r;
+      if constexpr (SLOPE) slope[i] = (neg ? 1.0f : t) * r;
+      v[i] = e;
+      sum += e;
+    }
+  }
+  sum = warp_sum_f32(sum);
+  return sum == 0.0f ? 0.0f : 1.0f / sum;
+}
+
+// The shares of a block of rows: one for each sequence that has rows in it. The share of (block b,
+// sequence s) is number b + s: along the rows either b or s goes up from one share to the next, so no
+// two have the same number.
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(kBalThreads) k_balance(const BalArgs a) {
+  extern __shared__ float bal_smem[];
+  float* sp = bal_smem;                                          // [kBalWarps][E]
+  int* sn = reinterpret_cast<int*>(sp + (a.logits ? kBalWarps * a.E : 0));  // [E]
+  int* sbase = sn + a.E;                                                   // [S + 1]
+  pdl_begin_in_order();
+  load_bases(a, sbase);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.rows;
+  const int64_t r1 = min(r0 + a.rows, a.T);
+  for (int s = sequence_of(sbase, a.S, r0); s < a.S && sbase[s] < r1; ++s) {
+    const int64_t b0 = max(static_cast<int64_t>(sbase[s]), r0);
+    const int64_t b1 = min(static_cast<int64_t>(sbase[s + 1]), r1);
+    if (b0 >= b1) continue;
+    for (int e = threadIdx.x; e < a.E; e += kBalThreads) sn[e] = 0;
+    __syncthreads();
+    const int64_t p1 = b1 * a.K;
+    for (int64_t p = b0 * a.K + threadIdx.x; p < p1; p += kBalThreads) {
+      const int id = __ldcg(a.ids + p);
+      if (id >= 0 && id < a.E) atomicAdd(sn + id, 1);
+    }
+    if (a.logits) {
+      float acc[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
+      for (int64_t row = b0 + warp; row < b1; row += kBalWarps) {
+        float v[NV], none[1];
+        load_logits<T, V, NV>(a, row, v);
+        const float inv = scores<NV, false>(v, none, a.sigmoid);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[i] = fmaf(v[i], inv, acc[i]);
+      }
+#pragma unroll
+      for (int u = 0; u < NV / V; ++u) {
+        const int i = u * 32 + lane;
+        if (i < a.E / V) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) sp[warp * a.E + i * V + j] = acc[u * V + j];
+        }
+      }
+    }
+    __syncthreads();
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) + s) * a.E;
+    for (int e = threadIdx.x; e < a.E; e += kBalThreads) {
+      a.part_n[at + e] = sn[e];
+      if (a.logits) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kBalWarps; ++w) sum += sp[w * a.E + e];
+        a.part_p[at + e] = sum;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Adds the blocks' shares. The cluster's CTAs take the sequences' (sequence, 32 experts) pieces in turn,
+// 32 threads by 8 parts of the shares each; the pieces' terms of the loss are added in double, in an
+// order that is the same in every run.
+constexpr int kJoinThreads = 1024;
+
+__global__ void __launch_bounds__(kJoinThreads) k_balance_join(const BalArgs a) {
+  extern __shared__ float bal_smem[];
+  int* sbase = reinterpret_cast<int*>(bal_smem);  // [S + 1]
+  __shared__ float bp[32][33];
+  __shared__ int bn[32][33];
+  __shared__ double part[32];
+  __shared__ double share;
+  __shared__ int live_seqs;
+  pdl_begin_in_order();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = static_cast<int>(cluster_ctarank());
+  if (threadIdx.x == 0) live_seqs = 0;
+  load_bases(a, sbase);
+  int mine = 0;
+  for (int s = threadIdx.x; s < a.S; s += kJoinThreads) mine += sbase[s + 1] > sbase[s];
+  if (mine) atomicAdd(&live_seqs, mine);
+  __syncthreads();
+  const double live = live_seqs;
+  const int chunks = (a.E + 31) / 32;
+  const int64_t pieces = static_cast<int64_t>(a.S) * chunks;
+  double sum = 0.0;  // of warp 0's lanes
+  for (int64_t piece = rank; piece < pieces; piece += kBalCluster) {
+    const int s = static_cast<int>(piece / chunks);
+    const int e = static_cast<int>(piece - static_cast<int64_t>(s) * chunks) * 32 + lane;
+    const int64_t b0 = sbase[s], b1 = sbase[s + 1];
+    float p = 0.0f;
+    int n = 0;
+    if (b0 < b1 && e < a.E) {
+      const int first = static_cast<int>(b0 / a.rows), last = static_cast<int>((b1 - 1) / a.rows);
+      const float* pp = a.part_p + static_cast<int64_t>(s) * a.E + e;
+      const int32_t* pn = a.part_n + static_cast<int64_t>(s) * a.E + e;
+      for (int b = first + warp; b <= last; b += 32 * 4) {
+        float tp[4];
+        int tn[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = b + 32 * i <= last;
+          const int64_t at = static_cast<int64_t>(b + 32 * i) * a.E;
+          tn[i] = in ? __ldcg(pn + at) : 0;
+          tp[i] = in && a.loss ? __ldcg(pp + at) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p += tp[i];
+          n += tn[i];
+        }
+      }
+    }
+    bp[warp][lane] = p;
+    bn[warp][lane] = n;
+    __syncthreads();
+    if (warp == 0) {
+      for (int i = 1; i < 32; ++i) {
+        p += bp[i][lane];
+        n += bn[i][lane];
+      }
+      if (e < a.E) a.counts[static_cast<int64_t>(s) * a.E + e] = n;
+      if (a.loss && b0 < b1) {
+        const double len = static_cast<double>(b1 - b0);
+        const double factor = a.E / (a.K * len * len * live);
+        sum += factor * n * p;
+        if (lane == 0 && e == 0) a.factor[s] = static_cast<float>(factor);
+      } else if (a.loss && lane == 0 && e == 0) {
+        a.factor[s] = 0.0f;
+      }
+    }
+    __syncthreads();
+  }
+  if (!a.loss) return;
+  if (warp == 0) {
+    part[lane] = sum;
+    __syncwarp();
+    if (lane == 0) {
+      double t = 0.0;
+      for (int i = 0; i < 32; ++i) t += part[i];
+      share = t;
+    }
+  }
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0 && threadIdx.x == 0) {
+    double t = 0.0;
+    for (int r = 0; r < kBalCluster; ++r) {
+      uint32_t at;
+      double v;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&share)), "r"(r));
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+      t += v;
+    }
+    *a.loss = static_cast<float>(t);
+  }
+  cluster_arrive();  // the others' shared memory stays until it has been read
+  cluster_wait();
+}
+
+// A token per warp, neighbouring tokens one after the other; c = counts * factor of its sequence stays in
+// registers while the sequence does. Rows of no sequence get zeros.
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(kBalThreads) k_balance_back(const BalArgs a) {
+  extern __shared__ float bal_smem[];
+  int* sbase = reinterpret_cast<int*>(bal_smem);  // [S + 1]
+  pdl_begin_in_order();
+  load_bases(a, sbase);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = a.E / V;
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kBalWarps + warp) * a.rows;
+  const int64_t r1 = min(r0 + a.rows, a.T);
+  if (r0 >= r1) return;
+  const float g = __ldcg(a.g);
+  int s = sequence_of(sbase, a.S, r0);
+  float c[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) c[i] = 0.0f;
+  int64_t b0 = 0, b1 = r0;  // of sequence s; in the rows behind the last sequence, none
+  for (int64_t row = r0; row < r1; ++row) {
+    if (row >= b1) {
+      while (s < a.S && sbase[s + 1] <= row) ++s;
+      b0 = s < a.S ? sbase[s] : a.T;
+      b1 = s < a.S ? sbase[s + 1] : a.T;
+      if (s < a.S) {
+        const float f = __ldcg(a.factor + s) * g;
+        const int32_t* cn = a.counts + static_cast<int64_t>(s) * a.E;
+#pragma unroll
+        for (int u = 0; u < NV / V; ++u) {
+          const int i = u * 32 + lane;
+          if (i < n) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[u * V + j] = static_cast<float>(__ldcg(cn + i * V + j)) * f;
+          }
+        }
+      }
+    }
+    float v[NV];
+    if (row < b0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = 0.0f;
+    } else {
+      float slope[NV];
+      load_logits<T, V, NV>(a, row, v);
+      const float inv = scores<NV, true>(v, slope, a.sigmoid);
+      float dot = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        v[i] *= inv;
+        dot = fmaf(v[i], c[i], dot);
+      }
+      dot = warp_sum_f32(dot);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = v[i] * (c[i] - dot) * slope[i];
+    }
+    T* out = static_cast<T*>(a.d_logits) + row * a.E;
+#pragma unroll
+    for (int u = 0; u < NV / V; ++u) {
+      const int i = u * 32 + lane;
+      float w[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = v[u * V + j];
+      if (i < n) store_pack(out + i * V, w);
+    }
+  }
+}
+
+template <typename T, int V, int NV>
+cudaError_t run(const BalArgs& given, bool back, int sms, cudaStream_t s) {
+  static std::atomic<bool> done[64];
+  BalArgs a = given;
+  const size_t bases = static_cast<size_t>(a.S + 1) * 4;
+  if (back) {
+    // rows per warp: two blocks of eight warps per SM share the rows evenly
+    a.rows = static_cast<int>((a.T + 16 * sms - 1) / (16 * sms));
+    const int64_t warps = (a.T + a.rows - 1) / a.rows;
+    return launch_pdl(k_balance_back<T, V, NV>,
+                      dim3(static_cast<unsigned>((warps + kBalWarps - 1) / kBalWarps)),
+                      dim3(kBalThreads), bases, s, a);
+  }
+  const size_t smem = ((a.logits ? kBalWarps * a.E : 0) + a.E) * 4 + bases;
+  if (smem > 48 * 1024) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev].load(std::memory_order_acquire)) {
+      const cudaError_t e = cudaFuncSetAttribute(
+          k_balance<T, V, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBalMaxSmem);
+      if (e != cudaSuccess) return e;
+      done[dev].store(true, std::memory_order_release);
+    }
+  }
+  if (a.blocks > 0) {
+    const cudaError_t e = launch_pdl(k_balance<T, V, NV>, dim3(a.blocks), dim3(kBalThreads), smem, s, a);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_pdl_cluster(k_balance_join, dim3(kBalCluster), dim3(kJoinThreads), bases, s,
+                            kBalCluster, a);
+}
+
+template <typename T>
+cudaError_t typed(const BalArgs& a, bool back, int sms, cudaStream_t s) {
+  const bool wide = a.E % kV<T> == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0 &&
+                    (reinterpret_cast<uintptr_t>(a.d_logits) & 15u) == 0;
+  if (a.E <= 256)
+    return wide ? run<T, kV<T>, 8>(a, back, sms, s) : run<T, 1, 8>(a, back, sms, s);
+  return wide ? run<T, kV<T>, 32>(a, back, sms, s) : run<T, 1, 32>(a, back, sms, s);
+}
+
+}  // namespace
+
+cudaError_t launch_balance(const Balance& p, int sms, cudaStream_t s) {
+  BalArgs a{};
+  a.logits = p.back || p.loss ? p.logits : nullptr;
+  a.ids = p.ids;
+  a.base = p.base;
+  a.T = p.T;
+  a.E = p.E;
+  a.K = p.K;
+  a.S = p.S;
+  a.sigmoid = p.sigmoid;
+  // two blocks per SM, of eight rows or more
+  const int64_t most = 2 * sms < kMaxBalanceBlocks ? 2 * sms : kMaxBalanceBlocks;
+  const int64_t even = ((p.T > 0 ? p.T : 1) + most - 1) / most;
+  a.rows = static_cast<int>((even + kBalWarps - 1) / kBalWarps * kBalWarps);
+  a.blocks = static_cast<int>((p.T + a.rows - 1) / a.rows);
+  a.part_n = static_cast<int32_t*>(p.workspace);
+  a.part_p = reinterpret_cast<float*>(a.part_n + (static_cast<int64_t>(a.blocks) + p.S) * p.E);
+  a.loss = p.loss;
+  a.counts = p.counts;
+  a.factor = p.factor;
+  a.g = p.grad_loss;
+  a.d_logits = p.grad_logits;
+  switch (p.dtype) {
+    case FMOE_DTYPE_F32:
+      return typed<float>(a, p.back, sms, s);
+    case FMOE_DTYPE_BF16:
+      return typed<__nv_bfloat16>(a, p.back, sms, s);
+    default:
+      return typed<__half>(a, p.back, sms, s);
+  }
+}
+
+}  // namespace fmoe

@@ -274,6 +274,43 @@ struct BlockNorm {
 };
 cudaError_t launch_block_norm(const BlockNorm& p, int sms, cudaStream_t s);
 
+constexpr int kMaxBalanceExperts = 1024;
+constexpr int kMaxBalanceSequences = 4096;
+constexpr int kMaxBalanceBlocks = 512;  // of the forward pass, two per SM
+struct Balance {
+  const void* logits;    // [T, E]
+  int dtype;
+  const int32_t* ids;    // [T, K]
+  const int32_t* base;   // [S + 1] or null
+  int64_t T;
+  int E, K, S, sigmoid;
+  float* loss;
+  int32_t* counts;       // [S, E]
+  float* factor;         // [S]
+  void* workspace;
+  bool back;
+  const float* grad_loss;
+  void* grad_logits;
+};
+cudaError_t launch_balance(const Balance& p, int sms, cudaStream_t s);
+
+constexpr int kMaxLnBlocks = 640;  // blocks of the layer norm's backward pass
+struct LayerNorm {
+  int dtype;
+  int64_t T;
+  int H;
+  const void *f, *x, *w, *b;
+  int w_dtype, b_dtype;
+  float eps;
+  void *h, *y, *q;
+  float *q_scale, *stats;
+  bool back;
+  const void *dh, *dy;
+  void *dx, *dw, *db;
+  float* part;
+};
+cudaError_t launch_layer_norm(const LayerNorm& p, int sms, cudaStream_t s);
+
 // ---------------------------------------------------------------- output stores
 // Eight fp32 values of an output row as bf16 (round to nearest even) or fp32; v counts groups of
 // eight columns.

@@ -1,5 +1,5 @@
 // fmoe_layer_api.cu -- argument checks and launches of the operators around the experts
-// (include/fmoe.h): tokens sorted by expert and back, int8 products, block norms.
+// (include/fmoe.h): tokens sorted by expert and back, int8 products, norms, balance loss.
 #include <initializer_list>
 
 #include "fmoe_internal.h"
@@ -164,6 +164,78 @@ uint64_t gate_count(const FmoeBlockNormArgs* a) {
   const uint64_t T = a->num_tokens, H = a->hidden_size;
   return a->gate_kind == FMOE_GATE_TOKEN ? T : a->gate_kind == FMOE_GATE_CHANNEL ? H
          : a->gate_kind == FMOE_GATE_FULL ? T * H : 0;
+}
+
+size_t layer_norm_workspace(int64_t T, int H) {
+  return static_cast<size_t>(2) * (T < kMaxLnBlocks ? T : kMaxLnBlocks) * H * 4;
+}
+
+// What the layer norm's forward and backward pass have in common.
+int check_layer_norm(const FmoeLayerNormArgs* a, LayerNorm* p) {
+  if (!a) return FMOE_ERR_NULL;
+  if (a->num_tokens < 0 || a->num_tokens > INT32_MAX - 1024 || a->hidden_size < 1 ||
+      a->hidden_size > 16384)
+    return FMOE_ERR_SHAPE;
+  if (!float_type(a->dtype)) return FMOE_ERR_DTYPE;
+  const auto param = [&](const void* q, int dtype) {
+    return !q || dtype == a->dtype || dtype == FMOE_DTYPE_F32;
+  };
+  if (!param(a->weight, a->weight_dtype) || !param(a->bias, a->bias_dtype)) return FMOE_ERR_DTYPE;
+  if (a->num_tokens > 0 && !a->residual) return FMOE_ERR_NULL;
+  const size_t e = elem(a->dtype);
+  if (!at(a->branch, e) || !at(a->residual, e) || !at(a->stats, 8) ||
+      (a->weight && !at(a->weight, elem(a->weight_dtype))) ||
+      (a->bias && !at(a->bias, elem(a->bias_dtype))))
+    return FMOE_ERR_ALIGN;
+  *p = LayerNorm{};
+  p->dtype = a->dtype;
+  p->T = a->num_tokens;
+  p->H = a->hidden_size;
+  p->f = a->branch;
+  p->x = a->residual;
+  p->w = a->weight;
+  p->b = a->bias;
+  p->w_dtype = a->weight_dtype;
+  p->b_dtype = a->bias_dtype;
+  p->eps = a->eps;
+  p->stats = a->stats;
+  return FMOE_OK;
+}
+
+size_t balance_workspace(int64_t T, int E, int S) {
+  const int64_t most = (T + 7) / 8;
+  return static_cast<size_t>((most < kMaxBalanceBlocks ? most : kMaxBalanceBlocks) + S) * E * 8;
+}
+
+int check_balance(const FmoeBalanceArgs* a, Balance* p) {
+  if (!a) return FMOE_ERR_NULL;
+  if (a->num_tokens < 0 || a->num_tokens > INT32_MAX - 1024 || a->num_experts < 1 ||
+      a->num_experts > kMaxBalanceExperts || a->top_k < 1 || a->num_sequences < 1 ||
+      a->num_sequences > kMaxBalanceSequences || (!a->sequence_base && a->num_sequences != 1) ||
+      (a->scoring != FMOE_SCORING_SOFTMAX && a->scoring != FMOE_SCORING_SIGMOID))
+    return FMOE_ERR_SHAPE;
+  if (!float_type(a->dtype)) return FMOE_ERR_DTYPE;
+  if (!at(a->logits, elem(a->dtype)) || !at(a->topk_ids, 4) || !at(a->sequence_base, 4) ||
+      !at(a->loss, 4) || !at(a->counts, 4) || !at(a->factor, 4) || !at(a->grad_loss, 4) ||
+      !at(a->grad_logits, elem(a->dtype)) || !at(a->workspace, 4))
+    return FMOE_ERR_ALIGN;
+  *p = Balance{};
+  p->logits = a->logits;
+  p->dtype = a->dtype;
+  p->ids = a->topk_ids;
+  p->base = a->sequence_base;
+  p->T = a->num_tokens;
+  p->E = a->num_experts;
+  p->K = a->top_k;
+  p->S = a->num_sequences;
+  p->sigmoid = a->scoring == FMOE_SCORING_SIGMOID;
+  p->loss = a->loss;
+  p->counts = a->counts;
+  p->factor = a->factor;
+  p->workspace = a->workspace;
+  p->grad_loss = a->grad_loss;
+  p->grad_logits = a->grad_logits;
+  return FMOE_OK;
 }
 
 }  // namespace
@@ -438,6 +510,137 @@ int fmoe_block_norm_backward(const FmoeBlockNormArgs* a, void* stream) {
   rc = device_sms(&sms);
   if (rc) return rc;
   return done(launch_block_norm(p, sms, s));
+}
+
+int fmoe_layer_norm_workspace_size(int64_t T, int32_t H, size_t* bytes) {
+  if (!bytes) return FMOE_ERR_NULL;
+  if (T < 0 || T > INT32_MAX - 1024 || H < 1 || H > 16384) return FMOE_ERR_SHAPE;
+  *bytes = layer_norm_workspace(T, H);
+  return FMOE_OK;
+}
+
+int fmoe_layer_norm(const FmoeLayerNormArgs* a, void* stream) {
+  LayerNorm p;
+  int rc = check_layer_norm(a, &p);
+  if (rc) return rc;
+  if ((a->normed && a->normed_q) || (a->normed_q && a->hidden_size % kBlock != 0))
+    return FMOE_ERR_SHAPE;
+  if (p.T == 0) return FMOE_OK;
+  if ((a->normed_q != nullptr) != (a->normed_scale != nullptr)) return FMOE_ERR_NULL;
+  const size_t e = elem(a->dtype);
+  if (!at(a->hidden, e) || !at(a->normed, e) || !at(a->normed_scale, 4)) return FMOE_ERR_ALIGN;
+  if (a->normed_q) {
+    for (const void* q : {a->branch, a->residual, a->weight, a->bias,
+                          static_cast<const void*>(a->hidden), static_cast<const void*>(a->normed_q)})
+      if (!at(q, 16)) return FMOE_ERR_ALIGN;
+  }
+  const uint64_t n = static_cast<uint64_t>(p.T) * p.H, row = n * e;
+  // hidden may be the residual itself: every element is read by the thread that writes it
+  const Span residual{a->hidden == a->residual ? nullptr : a->residual, row};
+  if (overlap({{a->hidden, row}, {a->normed, row}, {a->normed_q, n}, {a->normed_scale, n / kBlock * 4},
+               {a->stats, static_cast<uint64_t>(p.T) * 8}},
+              {{a->branch, row}, residual,
+               {a->weight, a->weight ? p.H * elem(a->weight_dtype) : 0},
+               {a->bias, a->bias ? p.H * elem(a->bias_dtype) : 0}}))
+    return FMOE_ERR_SHAPE;
+  if (!a->hidden && !a->normed && !a->normed_q && !a->stats) return FMOE_OK;
+  p.h = a->hidden;
+  p.y = a->normed;
+  p.q = a->normed_q;
+  p.q_scale = a->normed_scale;
+  int sms = 0;
+  rc = device_sms(&sms);
+  if (rc) return rc;
+  return done(launch_layer_norm(p, sms, as_stream(stream)));
+}
+
+int fmoe_layer_norm_backward(const FmoeLayerNormArgs* a, void* stream) {
+  LayerNorm p;
+  int rc = check_layer_norm(a, &p);
+  if (rc) return rc;
+  const size_t e = elem(a->dtype);
+  const size_t we = elem(a->weight_dtype), be = elem(a->bias_dtype);
+  const bool sums = a->grad_weight || a->grad_bias;
+  if ((a->grad_weight && !a->weight) || (a->grad_bias && !a->bias)) return FMOE_ERR_NULL;
+  if (!at(a->grad_hidden, e) || !at(a->grad_normed, e) || !at(a->grad_input, e) ||
+      !at(a->workspace, 4) || (a->grad_weight && !at(a->grad_weight, we)) ||
+      (a->grad_bias && !at(a->grad_bias, be)))
+    return FMOE_ERR_ALIGN;
+  cudaStream_t s = as_stream(stream);
+  if (p.T == 0) {  // no tokens: the sums over tokens are zero
+    if ((a->grad_weight && cudaMemsetAsync(a->grad_weight, 0, p.H * we, s) != cudaSuccess) ||
+        (a->grad_bias && cudaMemsetAsync(a->grad_bias, 0, p.H * be, s) != cudaSuccess))
+      return FMOE_ERR_CUDA;
+    return FMOE_OK;
+  }
+  if (!a->grad_input && !sums) return FMOE_OK;
+  if (!a->stats) return FMOE_ERR_NULL;
+  const size_t need = layer_norm_workspace(p.T, p.H);
+  if (sums && (!a->workspace || a->workspace_bytes < need)) return FMOE_ERR_WORKSPACE;
+  const uint64_t row = static_cast<uint64_t>(p.T) * p.H * e;
+  if (overlap({{a->grad_input, row},
+               {a->grad_weight, p.H * we},
+               {a->grad_bias, p.H * be},
+               {a->workspace, sums ? need : 0}},
+              {{a->branch, row}, {a->residual, row}, {a->weight, a->weight ? p.H * we : 0},
+               {a->grad_hidden, row}, {a->grad_normed, row},
+               {a->stats, static_cast<uint64_t>(p.T) * 8}}))
+    return FMOE_ERR_SHAPE;
+  p.back = true;
+  p.dh = a->grad_hidden;
+  p.dy = a->grad_normed;
+  p.dx = a->grad_input;
+  p.dw = a->grad_weight;
+  p.db = a->grad_bias;
+  p.part = static_cast<float*>(a->workspace);
+  int sms = 0;
+  rc = device_sms(&sms);
+  if (rc) return rc;
+  return done(launch_layer_norm(p, sms, s));
+}
+
+int fmoe_balance_workspace_size(int64_t T, int32_t E, int32_t S, size_t* bytes) {
+  if (!bytes) return FMOE_ERR_NULL;
+  if (T < 0 || T > INT32_MAX - 1024 || E < 1 || E > kMaxBalanceExperts || S < 1 ||
+      S > kMaxBalanceSequences)
+    return FMOE_ERR_SHAPE;
+  *bytes = balance_workspace(T, E, S);
+  return FMOE_OK;
+}
+
+int fmoe_balance_loss(const FmoeBalanceArgs* a, void* stream) {
+  Balance p;
+  int rc = check_balance(a, &p);
+  if (rc) return rc;
+  if (!p.counts || (p.loss && !p.factor) || (p.T > 0 && (!p.ids || (p.loss && !p.logits))))
+    return FMOE_ERR_NULL;
+  const size_t need = balance_workspace(p.T, p.E, p.S);
+  if (!p.workspace || a->workspace_bytes < need) return FMOE_ERR_WORKSPACE;
+  const uint64_t T = p.T, S = p.S;
+  if (overlap({{p.loss, 4}, {p.counts, S * p.E * 4}, {p.factor, S * 4}, {p.workspace, need}},
+              {{p.logits, T * p.E * elem(p.dtype)}, {p.ids, T * p.K * 4}, {p.base, (S + 1) * 4}}))
+    return FMOE_ERR_SHAPE;
+  int sms = 0;
+  rc = device_sms(&sms);
+  if (rc) return rc;
+  return done(launch_balance(p, sms, as_stream(stream)));
+}
+
+int fmoe_balance_loss_backward(const FmoeBalanceArgs* a, void* stream) {
+  Balance p;
+  int rc = check_balance(a, &p);
+  if (rc) return rc;
+  if (p.T == 0) return FMOE_OK;
+  if (!p.logits || !p.counts || !p.factor || !p.grad_loss || !p.grad_logits) return FMOE_ERR_NULL;
+  const uint64_t S = p.S, rows = static_cast<uint64_t>(p.T) * p.E * elem(p.dtype);
+  if (overlap({{p.grad_logits, rows}}, {{p.logits, rows}, {p.base, (S + 1) * 4},
+                                        {p.counts, S * p.E * 4}, {p.factor, S * 4}, {p.grad_loss, 4}}))
+    return FMOE_ERR_SHAPE;
+  p.back = true;
+  int sms = 0;
+  rc = device_sms(&sms);
+  if (rc) return rc;
+  return done(launch_balance(p, sms, as_stream(stream)));
 }
 
 }  // extern "C"

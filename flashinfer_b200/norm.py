@@ -1,8 +1,10 @@
-"""The RMS norms before and after a block, fused with the block's gate and the residual scale.
+"""The RMS norms before and after a block, fused with the block's gate and the residual scale, and
+the layer norm in front of a block, fused with the residual sum.
 
-One call sits between two blocks of a model: it normalises what the block returned, gates it, adds
-it to the scaled residual stream and normalises the sum for the next block; for an FP8 expert layer
-the result leaves as ``run``'s e4m3 input with its scales. Forward and backward are one pass each.
+One call sits between two blocks of a model: ``block_norm`` normalises what the block returned, gates it,
+adds it to the scaled residual stream and normalises the sum for the next block; ``layer_norm`` adds it
+and takes the mean away as well. For an FP8 expert layer the result leaves as ``run``'s e4m3 input with
+its scales. Forward and backward are one pass each.
 """
 from __future__ import annotations
 
@@ -13,7 +15,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from ._lib import FmoeBlockNormArgs
+from ._lib import FmoeBlockNormArgs, FmoeLayerNormArgs
 from ._op import DTYPE_TAG, FLOATS, call, first, first_order_only, need, ptr, recording, written
 
 BLOCK = 128
@@ -183,4 +185,136 @@ def block_norm(branch: Optional[torch.Tensor], residual: torch.Tensor, *,
                                 residual_scale, eps)
     hidden, normed, _ = _forward(branch, residual, post_weight, gate, pre_weight, kind,
                                  residual_scale, eps, quantize, output, False)
+    return hidden, normed
+
+
+# ------------------------------------------------------------------ layer norm
+def _layer_args(branch, residual, weight, bias, eps):
+    T, H = residual.shape
+    return FmoeLayerNormArgs(T, H, DTYPE_TAG[residual.dtype], ptr(branch), residual.data_ptr(),
+                             ptr(weight), ptr(bias), _tag(weight), _tag(bias), eps)
+
+
+def _layer_forward(branch, residual, weight, bias, eps, quantize, hidden, want_stats):
+    a = _layer_args(branch, residual, weight, bias, eps)
+    T, H = residual.shape
+    given = hidden is not None
+    if given:
+        a.hidden = hidden.data_ptr()
+    elif branch is None:
+        hidden = residual
+    else:
+        hidden = torch.empty_like(residual)
+        a.hidden = hidden.data_ptr()
+    stats = None
+    if quantize:
+        q = residual.new_empty((T, H), dtype=torch.float8_e4m3fn)
+        scale = residual.new_empty((H // BLOCK, T), dtype=torch.float32)
+        a.normed_q, a.normed_scale = q.data_ptr(), scale.data_ptr()
+        normed = (q, scale)
+    else:
+        normed = torch.empty_like(residual)
+        a.normed = normed.data_ptr()
+    if want_stats:
+        stats = residual.new_empty((T, 2), dtype=torch.float32)
+        a.stats = stats.data_ptr()
+    call("fmoe_layer_norm", residual.get_device(), ctypes.byref(a))
+    if given:
+        written(hidden)
+    return hidden, normed, stats
+
+
+@lru_cache(maxsize=1024)
+def _layer_workspace_bytes(T: int, H: int) -> int:
+    size = ctypes.c_size_t()
+    _lib.check(_lib.load().fmoe_layer_norm_workspace_size(T, H, ctypes.byref(size)),
+               "fmoe_layer_norm_workspace_size")
+    return size.value
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, branch, residual, weight, bias, eps):
+        hidden, normed, stats = _layer_forward(branch, residual, weight, bias, eps, False, None, True)
+        ctx.save_for_backward(branch, residual, weight, bias, stats)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return hidden, normed
+
+    @staticmethod
+    def backward(ctx, grad_hidden, grad_normed):
+        first_order_only()
+        branch, residual, weight, bias, stats = ctx.saved_tensors
+        a = _layer_args(branch, residual, weight, bias, ctx.eps)
+        if grad_hidden is not None:
+            grad_hidden = grad_hidden.contiguous()
+            a.grad_hidden = grad_hidden.data_ptr()
+        if grad_normed is not None:
+            grad_normed = grad_normed.contiguous()
+            a.grad_normed = grad_normed.data_ptr()
+        a.stats = stats.data_ptr()
+        need_f, need_x, need_w, need_b = ctx.needs_input_grad[:4]
+        d_x = d_w = d_b = workspace = None
+        if need_f or need_x:
+            d_x = torch.empty_like(residual)
+            a.grad_input = d_x.data_ptr()
+        if need_w:
+            d_w = torch.empty_like(weight)
+            a.grad_weight = d_w.data_ptr()
+        if need_b:
+            d_b = torch.empty_like(bias)
+            a.grad_bias = d_b.data_ptr()
+        if need_w or need_b:
+            size = _layer_workspace_bytes(*residual.shape)
+            workspace = stats.new_empty(size // 4)
+            a.workspace, a.workspace_bytes = ptr(workspace), size
+        call("fmoe_layer_norm_backward", residual.get_device(), ctypes.byref(a))
+        # one tensor for both: the sum's gradient is that of each of its terms
+        return d_x if need_f else None, d_x if need_x else None, d_w, d_b, None
+
+
+def layer_norm(branch: Optional[torch.Tensor], residual: torch.Tensor, *,
+               weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, quantize: bool = False, output: Optional[torch.Tensor] = None,
+               ) -> Tuple[torch.Tensor, Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]]:
+    """``hidden = residual + branch`` and
+    ``normed = (hidden - mean) / sqrt(var + eps) * weight + bias`` per token.
+
+    branch, residual [T, H] of one type (bf16, fp16, fp32), H up to 16384; branch None where no block
+    came before: ``hidden`` is then ``residual`` itself (a view of it where gradients are recorded).
+    weight and bias [H], of the activations' type or fp32, or None for one and zero. The variance is that
+    of the H values (not corrected), of their deviations from the mean; hidden stays in fp32 up to the norm.
+
+    Returns ``(hidden, normed)``. With ``quantize`` (H a multiple of 128, 16-byte aligned tensors)
+    normed is the pair ``(e4m3 [T, H], fp32 scales [H/128, T])`` that ``run`` takes as
+    ``hidden_states`` and ``hidden_states_scale``; that form has no gradient. ``output`` receives
+    hidden and may be ``residual`` itself (no gradient either). Otherwise differentiable in every
+    tensor; weight and bias gradients are summed over tokens in a fixed order. Squares are fp32: with
+    eps 0, rows whose deviations are all below 2^-63 are divided by too little.
+    """
+    index = first(residual, "residual", FLOATS, 2)
+    T, H = shape = residual.shape
+    if not 1 <= H <= 16384:
+        raise ValueError(f"the hidden size must be 1..16384, got {H}")
+    same, params = _ONE[residual.dtype], _PARAMS[residual.dtype]
+    if branch is not None:
+        need(branch, "branch", index, shape, same)
+    if weight is not None:
+        need(weight, "weight", index, (H,), params)
+    if bias is not None:
+        need(bias, "bias", index, (H,), params)
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if quantize and H % BLOCK:
+        raise ValueError(f"quantize needs a hidden size that is a multiple of {BLOCK}, got {H}")
+    if output is not None:
+        need(output, "output", index, shape, same)
+    if recording(branch, residual, weight, bias, output):
+        if quantize:
+            raise ValueError("the quantised form has no gradient: call it under torch.no_grad()")
+        if output is not None:
+            raise ValueError("output cannot be given where gradients are recorded")
+        return _LayerNorm.apply(branch, residual, weight, bias, eps)
+    hidden, normed, _ = _layer_forward(branch, residual, weight, bias, eps, quantize, output, False)
     return hidden, normed

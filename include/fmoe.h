@@ -488,6 +488,91 @@ FMOE_API int fmoe_block_norm_workspace_size(int64_t num_tokens, int32_t hidden_s
 FMOE_API int fmoe_block_norm(const FmoeBlockNormArgs* args, void* cuda_stream);
 FMOE_API int fmoe_block_norm_backward(const FmoeBlockNormArgs* args, void* cuda_stream);
 
+/* The layer norm of the residual stream in front of a block. Per token:
+ *   hidden = residual + branch (branch NULL: the residual)
+ *   normed = (hidden - mean) / sqrt(var + eps) * weight + bias
+ * with mean and variance (of all hidden_size columns, not corrected) in fp32; weight and bias, each of
+ * `dtype` or fp32 and tagged, may be NULL (one, zero). hidden is kept in fp32 up to the norm and rounded
+ * once for output. normed leaves as `dtype`, or with normed_q set as e4m3 [T, H] with fp32 scales
+ * [H/128, T] (fmoe_block_norm's layout and scale); H is then a multiple of 128 and every pointer 16-byte
+ * aligned. hidden may be NULL, and may be residual itself. hidden_size: 1..16384. stats fp32 [T, 2]
+ * (mean, 1 / sqrt(var + eps)), or NULL: what the backward pass needs.
+ * Backward: the forward's inputs and stats, grad_hidden and grad_normed (either may be NULL: zero) and the
+ * wanted gradients (NULL: not wanted), each of its input's type. grad_input is the gradient of residual
+ * and of branch alike. Workspace of fmoe_layer_norm_workspace_size bytes where the weight's or the
+ * bias's gradient is wanted. Sums over tokens run in a fixed order. */
+typedef struct FmoeLayerNormArgs {
+  int64_t num_tokens;
+  int32_t hidden_size;
+  int32_t dtype;
+  const void* branch;
+  const void* residual;
+  const void* weight;
+  const void* bias;
+  int32_t weight_dtype;
+  int32_t bias_dtype;
+  float eps;
+  void* hidden;
+  void* normed;
+  void* normed_q;
+  float* normed_scale;
+  float* stats;
+  const void* grad_hidden;
+  const void* grad_normed;
+  void* grad_input;
+  void* grad_weight;
+  void* grad_bias;
+  void* workspace;
+  size_t workspace_bytes;
+} FmoeLayerNormArgs;
+
+FMOE_API int fmoe_layer_norm_workspace_size(int64_t num_tokens, int32_t hidden_size,
+                                            size_t* bytes);
+FMOE_API int fmoe_layer_norm(const FmoeLayerNormArgs* args, void* cuda_stream);
+FMOE_API int fmoe_layer_norm_backward(const FmoeLayerNormArgs* args, void* cuda_stream);
+
+/* The balance loss of a router, with the picks per expert. logits [T, E] of `dtype`, topk_ids int32
+ * [T, top_k] (ids outside [0, E) are no picks). sequence_base int32 [S + 1] on the device, or NULL for
+ * one sequence of all rows (S = 1): sequence s has the rows sequence_base[s] .. sequence_base[s + 1];
+ * rows in no sequence count for nothing. Bases outside [0, T] are clamped, and one that is smaller
+ * than an earlier one counts as that one.
+ *   p[t, e] = softmax of row t (FMOE_SCORING_SOFTMAX), or sigmoid(l[t, e]) / sum_e' sigmoid(l[t, e'])
+ *   loss = mean over the sequences with tokens of
+ *          sum_e (E counts[s, e] / (top_k T_s)) * (1 / T_s) sum_{t in s} p[t, e]
+ * counts int32 [S, E]. A row whose logits are all -infinity has no scores and no gradient. loss: one fp32
+ * (0 without tokens), or NULL: the counts alone, without logits and factor. factor fp32 [S]: what the
+ * backward pass needs.
+ * Backward: the forward's logits, sequence_base, counts and factor, grad_loss (one fp32) ->
+ * grad_logits [T, E] of `dtype`, zero in rows of no sequence.
+ * num_experts: 1..1024, num_sequences: 1..4096. Workspace of fmoe_balance_workspace_size bytes in the
+ * forward pass. Results do not depend on the order in which blocks run. */
+#define FMOE_SCORING_SOFTMAX 0
+#define FMOE_SCORING_SIGMOID 1
+
+typedef struct FmoeBalanceArgs {
+  int64_t num_tokens;
+  int32_t num_experts;
+  int32_t top_k;
+  int32_t num_sequences;
+  int32_t dtype;
+  int32_t scoring;
+  const void* logits;
+  const int32_t* topk_ids;
+  const int32_t* sequence_base;
+  float* loss;
+  int32_t* counts;
+  float* factor;
+  const float* grad_loss;
+  void* grad_logits;
+  void* workspace;
+  size_t workspace_bytes;
+} FmoeBalanceArgs;
+
+FMOE_API int fmoe_balance_workspace_size(int64_t num_tokens, int32_t num_experts,
+                                         int32_t num_sequences, size_t* bytes);
+FMOE_API int fmoe_balance_loss(const FmoeBalanceArgs* args, void* cuda_stream);
+FMOE_API int fmoe_balance_loss_backward(const FmoeBalanceArgs* args, void* cuda_stream);
+
 /* Number of SMs the persistent GEMM kernels size their grid for on the current device. */
 FMOE_API int fmoe_device_sm_count(int32_t* sms);
 
