@@ -65,6 +65,7 @@ EXPORTS = ("fmoe_workspace_size", "fmoe_workspace_layout", "fmoe_run", "fmoe_rou
            "fmoe_debug_arm_int8_timeout", "fmoe_debug_arm_int8_plan",
            "fmoe_block_norm_workspace_size", "fmoe_block_norm", "fmoe_block_norm_backward",
            "fmoe_layer_norm_workspace_size", "fmoe_layer_norm", "fmoe_layer_norm_backward",
+           "fmoe_quantize_int4", "fmoe_dequantize_int4", "fmoe_int4_workspace_size", "fmoe_int4_matmul",
            "fmoe_balance_workspace_size", "fmoe_balance_loss", "fmoe_balance_loss_backward")
 
 
@@ -160,6 +161,13 @@ class FmoeBalanceArgs(Structure):
         [("workspace_bytes", c_size_t)]
 
 
+class FmoeInt4Args(Structure):
+    _fields_ = [("num_rows", c_int64)] + \
+        [(n, c_int32) for n in ("n", "k", "num_experts", "group", "dtype", "scale_dtype")] + \
+        [(n, c_void_p) for n in ("x", "weight", "scale", "zero", "bias", "expert_base", "out")] + \
+        [("zero_tail", c_int32), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
 _lib = None
 
 
@@ -230,6 +238,12 @@ def load() -> ctypes.CDLL:
     lib.fmoe_balance_workspace_size.argtypes = [c_int64, c_int32, c_int32, POINTER(c_size_t)]
     lib.fmoe_balance_loss.argtypes = [POINTER(FmoeBalanceArgs), c_void_p]
     lib.fmoe_balance_loss_backward.argtypes = [POINTER(FmoeBalanceArgs), c_void_p]
+    lib.fmoe_quantize_int4.argtypes = [c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p, c_void_p,
+                                       c_void_p, c_void_p]
+    lib.fmoe_dequantize_int4.argtypes = [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32,
+                                         c_int32, c_void_p, c_int32, c_void_p]
+    lib.fmoe_int4_workspace_size.argtypes = [c_int64, c_int32, c_int32, c_int32, POINTER(c_size_t)]
+    lib.fmoe_int4_matmul.argtypes = [POINTER(FmoeInt4Args), c_void_p]
     lib.fmoe_version.restype = c_char_p
     for name in EXPORTS:
         if name != "fmoe_version":

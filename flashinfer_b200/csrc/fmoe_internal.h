@@ -274,6 +274,37 @@ struct BlockNorm {
 };
 cudaError_t launch_block_norm(const BlockNorm& p, int sms, cudaStream_t s);
 
+// Weights of 4 bits with a scale and a zero point per group of a row.
+struct Int4Weights {
+  void* w;               // [rows, K] of dtype: read (quantise) or written
+  int dtype;
+  int64_t rows;
+  int K, group, groups;
+  int symmetric;
+  uint8_t* packed;       // [rows, K / 2]
+  void* scale;           // [rows, groups] of scale_dtype (quantise: of dtype)
+  int scale_dtype;
+  uint8_t* zero;         // [rows, groups] or null: 8
+};
+cudaError_t launch_quantize_int4(const Int4Weights& p, cudaStream_t s);
+cudaError_t launch_dequantize_int4(const Int4Weights& p, cudaStream_t s);
+
+struct Int4Product {
+  const void* x;         // [M, K] of dtype (bf16, fp16)
+  int dtype;
+  const uint8_t* w;      // [E, N, K / 2]
+  const void* scale;     // [E, N, groups] of scale_dtype (dtype or fp32)
+  int scale_dtype;
+  const uint8_t* zero;   // [E, N, groups] or null
+  const float* bias;     // [N] or null
+  const int32_t* expert_base;  // [E + 1], or null for one matrix (E = 1)
+  void* out;             // [M, N] of dtype
+  int64_t M;
+  int N, K, E, group;
+  int zero_tail;
+};
+cudaError_t launch_int4_product(const Int4Product& p, int sms, cudaStream_t s);
+
 constexpr int kMaxBalanceExperts = 1024;
 constexpr int kMaxBalanceSequences = 4096;
 constexpr int kMaxBalanceBlocks = 512;  // of the forward pass, two per SM

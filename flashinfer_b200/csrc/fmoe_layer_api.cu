@@ -1,5 +1,5 @@
 // fmoe_layer_api.cu -- argument checks and launches of the operators around the experts
-// (include/fmoe.h): tokens sorted by expert and back, int8 products, norms, balance loss.
+// (include/fmoe.h): tokens sorted by expert and back, int8 and int4 products, norms, balance loss.
 #include <initializer_list>
 
 #include "fmoe_internal.h"
@@ -164,6 +164,22 @@ uint64_t gate_count(const FmoeBlockNormArgs* a) {
   const uint64_t T = a->num_tokens, H = a->hidden_size;
   return a->gate_kind == FMOE_GATE_TOKEN ? T : a->gate_kind == FMOE_GATE_CHANNEL ? H
          : a->gate_kind == FMOE_GATE_FULL ? T * H : 0;
+}
+
+bool int4_group(int k, int group) {
+  return k >= 32 && k % 32 == 0 && k <= 131072 && (group == 32 || group == 64 || (group > 0 && group % 128 == 0));
+}
+
+// Weights in 4 bits, given or wanted: the checks of both directions.
+int check_int4_weights(const Int4Weights& p) {
+  if (p.rows < 0 || p.rows > INT32_MAX - 1024 || !int4_group(p.K, p.group)) return FMOE_ERR_SHAPE;
+  // a warp per 256 values (or fewer, where a group is longer), eight to a block
+  if (p.rows * ((p.K + 31) / 32) / 256 >= INT32_MAX - 4096) return FMOE_ERR_SHAPE;
+  if (!float_type(p.dtype) || !float_type(p.scale_dtype)) return FMOE_ERR_DTYPE;
+  if (p.rows == 0) return FMOE_OK;
+  if (!p.w || !p.packed || !p.scale) return FMOE_ERR_NULL;
+  if (!at(p.w, 16) || !at(p.packed, 16) || !at(p.scale, elem(p.scale_dtype))) return FMOE_ERR_ALIGN;
+  return FMOE_OK;
 }
 
 size_t layer_norm_workspace(int64_t T, int H) {
@@ -510,6 +526,90 @@ int fmoe_block_norm_backward(const FmoeBlockNormArgs* a, void* stream) {
   rc = device_sms(&sms);
   if (rc) return rc;
   return done(launch_block_norm(p, sms, s));
+}
+
+int fmoe_quantize_int4(const void* w, int32_t dtype, int64_t rows, int32_t k, int32_t group,
+                       void* packed, void* scale, void* zero, void* stream) {
+  if (group < 1) return FMOE_ERR_SHAPE;
+  const Int4Weights p{const_cast<void*>(w), dtype, rows, k, group, (k + group - 1) / group,
+                      zero == nullptr, static_cast<uint8_t*>(packed), scale, dtype,
+                      static_cast<uint8_t*>(zero)};
+  int rc = check_int4_weights(p);
+  if (rc || p.rows == 0) return rc;
+  const uint64_t n = static_cast<uint64_t>(p.rows) * p.K, g = static_cast<uint64_t>(p.rows) * p.groups;
+  if (overlap({{p.packed, n / 2}, {p.scale, g * elem(dtype)}, {p.zero, g}}, {{w, n * elem(dtype)}}))
+    return FMOE_ERR_SHAPE;
+  int sms = 0;
+  rc = device_sms(&sms);
+  if (rc) return rc;
+  return done(launch_quantize_int4(p, as_stream(stream)));
+}
+
+int fmoe_dequantize_int4(const void* packed, const void* scale, int32_t scale_dtype,
+                         const void* zero, int64_t rows, int32_t k, int32_t group, void* w,
+                         int32_t dtype, void* stream) {
+  if (group < 1) return FMOE_ERR_SHAPE;
+  const Int4Weights p{w, dtype, rows, k, group, (k + group - 1) / group, zero == nullptr,
+                      static_cast<uint8_t*>(const_cast<void*>(packed)), const_cast<void*>(scale),
+                      scale_dtype, static_cast<uint8_t*>(const_cast<void*>(zero))};
+  int rc = check_int4_weights(p);
+  if (rc || p.rows == 0) return rc;
+  const uint64_t n = static_cast<uint64_t>(p.rows) * p.K, g = static_cast<uint64_t>(p.rows) * p.groups;
+  if (overlap({{w, n * elem(dtype)}}, {{packed, n / 2}, {scale, g * elem(scale_dtype)}, {zero, g}}))
+    return FMOE_ERR_SHAPE;
+  int sms = 0;
+  rc = device_sms(&sms);
+  if (rc) return rc;
+  return done(launch_dequantize_int4(p, as_stream(stream)));
+}
+
+int fmoe_int4_workspace_size(int64_t m, int32_t n, int32_t k, int32_t E, size_t* bytes) {
+  if (!bytes) return FMOE_ERR_NULL;
+  if (m < 0 || m > INT32_MAX - 1024 || n < 1 || k < 32 || k % 32 != 0 || k > 131072 || E < 1 ||
+      E > kMaxLocalExperts)
+    return FMOE_ERR_SHAPE;
+  *bytes = 0;
+  return FMOE_OK;
+}
+
+int fmoe_int4_matmul(const FmoeInt4Args* a, void* stream) {
+  if (!a) return FMOE_ERR_NULL;
+  if (a->num_rows < 0 || a->num_rows > INT32_MAX - 1024 || a->n < 1 || !int4_group(a->k, a->group) ||
+      a->num_experts < 1 || a->num_experts > kMaxLocalExperts ||
+      static_cast<int64_t>(a->num_experts) * a->n > INT32_MAX - 1024)
+    return FMOE_ERR_SHAPE;
+  if (!a->expert_base && a->num_experts != 1) return FMOE_ERR_NULL;
+  if (a->expert_base && a->bias) return FMOE_ERR_SHAPE;
+  if ((a->dtype != FMOE_DTYPE_BF16 && a->dtype != FMOE_DTYPE_F16) ||
+      (a->scale_dtype != a->dtype && a->scale_dtype != FMOE_DTYPE_F32))
+    return FMOE_ERR_DTYPE;
+  if (a->num_rows == 0) return FMOE_OK;
+  for (const void* q : {a->x, a->weight, a->scale, static_cast<const void*>(a->out)})
+    if (!q) return FMOE_ERR_NULL;
+  if (!at(a->x, 16) || !at(a->weight, 16) || !at(a->scale, elem(a->scale_dtype)) || !at(a->bias, 4) ||
+      !at(a->expert_base, 4) || !at(a->out, 2) || !at(a->workspace, 16))
+    return FMOE_ERR_ALIGN;
+  size_t need = 0;
+  int rc = fmoe_int4_workspace_size(a->num_rows, a->n, a->k, a->num_experts, &need);
+  if (rc) return rc;
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return FMOE_ERR_WORKSPACE;
+  const uint64_t M = a->num_rows, EN = static_cast<uint64_t>(a->num_experts) * a->n;
+  const uint64_t g = EN * ((a->k + a->group - 1) / a->group);
+  if (overlap({{a->out, M * a->n * 2}, {a->workspace, need}},
+              {{a->x, M * a->k * 2},
+               {a->weight, EN * a->k / 2},
+               {a->scale, g * elem(a->scale_dtype)},
+               {a->zero, g},
+               {a->bias, static_cast<uint64_t>(a->n) * 4},
+               {a->expert_base, static_cast<uint64_t>(a->num_experts + 1) * 4}}))
+    return FMOE_ERR_SHAPE;
+  int sms = 0;
+  rc = device_sms(&sms);
+  if (rc) return rc;
+  const Int4Product p{a->x, a->dtype, static_cast<const uint8_t*>(a->weight), a->scale, a->scale_dtype,
+                      static_cast<const uint8_t*>(a->zero), a->bias, a->expert_base, a->out,
+                      a->num_rows, a->n, a->k, a->num_experts, a->group, a->zero_tail};
+  return done(launch_int4_product(p, sms, as_stream(stream)));
 }
 
 int fmoe_layer_norm_workspace_size(int64_t T, int32_t H, size_t* bytes) {

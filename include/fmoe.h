@@ -431,6 +431,56 @@ FMOE_API int fmoe_debug_arm_int8_timeout(uint64_t wait_ns);
  * than parts. One-shot; the result is the same. */
 FMOE_API int fmoe_debug_arm_int8_plan(int32_t tile_tokens, int32_t split);
 
+/* Weights of 4 bits with a scale and a zero point per group of `group` values along K (32, 64 or a multiple
+ * of 128; the last group of a row may be shorter): w[r, k] = scale[r, k / group] * (q - zero[r, k / group]),
+ * q and zero in 0 .. 15. packed uint8 [R, K / 2] holds value 2i in the low half of byte i, value 2i + 1 in
+ * the high half; scale [R, groups], groups = ceil(K / group); zero uint8 [R, groups] (the low four bits
+ * count) or NULL for 8 everywhere. K: a multiple of 32; w and packed start on 16-byte boundaries.
+ * fmoe_quantize_int4: from w [R, K] of `dtype`, scales of the same type. zero NULL: symmetric,
+ * scale = max|w| / 7, q = round(w / scale) + 8 in 1 .. 15. Else with low = min(w, 0), high = max(w, 0):
+ * scale = (high - low) / 15, zero = round(-low / scale), q = round(w / scale) + zero in 0 .. 15. Ties to
+ * even; the scale is rounded to its type first, and at least 2^-100 (fp16: 2^-24). A group with a NaN or
+ * an infinity has a NaN or infinite scale.
+ * fmoe_dequantize_int4: back to w of `dtype`, computed in fp32 and rounded once. */
+FMOE_API int fmoe_quantize_int4(const void* w, int32_t dtype, int64_t num_rows, int32_t k,
+                                int32_t group, void* packed, void* scale, void* zero,
+                                void* cuda_stream);
+FMOE_API int fmoe_dequantize_int4(const void* packed, const void* scale, int32_t scale_dtype,
+                                  const void* zero, int64_t num_rows, int32_t k, int32_t group,
+                                  void* w, int32_t dtype, void* cuda_stream);
+
+/* out[m, n] = sum_k x[m, k] * w[n, k] (+ bias[n]) for weights in that format: x [M, K] of `dtype`
+ * (FMOE_DTYPE_BF16 or _F16), weight [N, K / 2], scale [N, groups] of `dtype` or fp32, zero [N, groups] or
+ * NULL, bias fp32 [N] or NULL, out [M, N] of `dtype`, sums in fp32. With expert_base (int32 [E + 1] on the
+ * device): one matrix per expert (weight [E, N, K / 2], scale and zero [E, N, groups], no bias), rows
+ * expert_base[e] .. expert_base[e + 1] of x times expert e's; bases as in fmoe_int8_expert_matmul, rows of
+ * no expert zeroed if zero_tail is set and left as they were otherwise. expert_base NULL: one matrix
+ * (num_experts 1). x and weight start on 16-byte boundaries. K up to 131072, num_experts 1..256.
+ * workspace of fmoe_int4_workspace_size bytes (may be 0). */
+typedef struct FmoeInt4Args {
+  int64_t num_rows;
+  int32_t n;
+  int32_t k;
+  int32_t num_experts;
+  int32_t group;
+  int32_t dtype;
+  int32_t scale_dtype;
+  const void* x;
+  const void* weight;
+  const void* scale;
+  const void* zero;
+  const float* bias;
+  const int32_t* expert_base;
+  void* out;
+  int32_t zero_tail;
+  void* workspace;
+  size_t workspace_bytes;
+} FmoeInt4Args;
+
+FMOE_API int fmoe_int4_workspace_size(int64_t num_rows, int32_t n, int32_t k, int32_t num_experts,
+                                      size_t* bytes);
+FMOE_API int fmoe_int4_matmul(const FmoeInt4Args* args, void* cuda_stream);
+
 /* The norms before and after a block, with its gate and the residual scale. Per token:
  *   n = post_weight ? branch * rsqrt(mean(branch^2) + eps) * post_weight : branch
  *   hidden = residual_scale * residual + gate * n
