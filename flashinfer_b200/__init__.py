@@ -11,7 +11,8 @@ loss -- are in ``tokens``, ``int8``, ``int4``, ``norm`` and ``balance``.
 from .moe import run, route, quantize_activations, read_status, workspace_for, WorkspaceView  # noqa: F401,E501
 
 from .balance import balance_loss, expert_counts
-from .int4 import dequantize_int4, int4_expert_matmul, int4_matmul, quantize_int4
+from .int4 import (dequantize_int4, int4_expert_matmul, int4_matmul, int4_status,
+                   quantize_int4)
 from .int8 import int8_expert_matmul, int8_matmul, int8_status, quantize_int8
 from .norm import block_norm, layer_norm
 from .tokens import ExpertOrder, sort_by_expert, sort_tokens, unsort_tokens
@@ -20,4 +21,5 @@ __all__ = ["run", "route", "read_status", "workspace_for", "WorkspaceView",
            "ExpertOrder", "sort_by_expert", "sort_tokens", "unsort_tokens",
            "quantize_int8", "int8_matmul", "int8_expert_matmul", "int8_status", "block_norm",
            "layer_norm", "balance_loss", "expert_counts",
-           "quantize_int4", "dequantize_int4", "int4_matmul", "int4_expert_matmul"]
+           "quantize_int4", "dequantize_int4", "int4_matmul", "int4_expert_matmul",
+           "int4_status"]

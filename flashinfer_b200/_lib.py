@@ -51,6 +51,7 @@ GEMV_MAX_T = 2  # calls of at most this many tokens take the matrix-vector path 
 STATUS_TIMEOUT_GEMM1 = 0x1
 STATUS_TIMEOUT_GEMM2 = 0x2
 STATUS_TIMEOUT_INT8 = 0x4
+STATUS_TIMEOUT_INT4 = 0x8
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = 0, 1, 2, 3
 SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
 
@@ -66,6 +67,7 @@ EXPORTS = ("fmoe_workspace_size", "fmoe_workspace_layout", "fmoe_run", "fmoe_rou
            "fmoe_block_norm_workspace_size", "fmoe_block_norm", "fmoe_block_norm_backward",
            "fmoe_layer_norm_workspace_size", "fmoe_layer_norm", "fmoe_layer_norm_backward",
            "fmoe_quantize_int4", "fmoe_dequantize_int4", "fmoe_int4_workspace_size", "fmoe_int4_matmul",
+           "fmoe_int4_status", "fmoe_debug_arm_int4_timeout", "fmoe_debug_arm_int4_plan",
            "fmoe_balance_workspace_size", "fmoe_balance_loss", "fmoe_balance_loss_backward")
 
 
@@ -244,6 +246,9 @@ def load() -> ctypes.CDLL:
                                          c_int32, c_void_p, c_int32, c_void_p]
     lib.fmoe_int4_workspace_size.argtypes = [c_int64, c_int32, c_int32, c_int32, POINTER(c_size_t)]
     lib.fmoe_int4_matmul.argtypes = [POINTER(FmoeInt4Args), c_void_p]
+    lib.fmoe_int4_status.argtypes = [POINTER(c_int32), c_void_p]
+    lib.fmoe_debug_arm_int4_timeout.argtypes = [ctypes.c_uint64]
+    lib.fmoe_debug_arm_int4_plan.argtypes = [c_int32, c_int32]
     lib.fmoe_version.restype = c_char_p
     for name in EXPORTS:
         if name != "fmoe_version":

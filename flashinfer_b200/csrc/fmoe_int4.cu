@@ -428,6 +428,20 @@ cudaError_t launch_dequantize_int4(const Int4Weights& p, cudaStream_t s) {
   }
 }
 
+// An expert is taken to have up to twice its even share of the rows, which the device alone knows.
+Int4Plan int4_plan(int64_t M, int N, int K, int E, bool grouped) {
+  const int64_t used = M < E ? M : E;
+  int64_t per = used > 0 ? (M + used - 1) / used : 0;
+  if (per <= (grouped ? 8 : 16)) return Int4Plan{0, 1};
+  if (grouped) per = 2 * per < M ? 2 * per : M;
+  Int4Plan p{per <= 64 ? 64 : per <= 128 ? 128 : 256, 1};
+  const int64_t tiles = (per + p.bn - 1) / p.bn * used * ((N + 127) / 128);
+  // K in parts while there are fewer tiles than SMs (148), each of four blocks of 64 or more
+  const int64_t most = (K + 63) / 64 / 4;
+  while (p.S < 8 && (p.S + 1) * tiles <= 148 && p.S < most) ++p.S;
+  return p;
+}
+
 cudaError_t launch_int4_product(const Int4Product& p, int sms, cudaStream_t s) {
   I4Args a{};
   a.x = p.x;
@@ -445,6 +459,11 @@ cudaError_t launch_int4_product(const Int4Product& p, int sms, cudaStream_t s) {
   a.groups = (p.K + p.group - 1) / p.group;
   a.scale_f32 = p.scale_dtype == FMOE_DTYPE_F32;
   a.zero_tail = p.zero_tail;
+  a.part = p.part;
+  Int4Plan plan = int4_plan(p.M, p.N, p.K, p.E, p.expert_base != nullptr);
+  if (p.tile_tokens != 0) plan = Int4Plan{p.tile_tokens, p.split};
+  if (p.wait_ns != 0 && plan.bn == 0) plan.bn = 64;  // the kernel for few has no waits
+  if (plan.bn != 0) return launch_int4_mm(p, a, plan, sms, s);
   const int64_t used = p.M < p.E ? p.M : p.E;
   const int64_t per = (p.M + used - 1) / used;
   return p.dtype == FMOE_DTYPE_BF16 ? few<__nv_bfloat16>(a, per, sms, s) : few<__half>(a, per, sms, s);

@@ -23,6 +23,10 @@ struct I4Args {
   int zero_tail;
 };
 
+// fmoe_int4_mm.cu: the product on the tensor cores (plan.bn > 0).
+cudaError_t launch_int4_mm(const Int4Product& p, const I4Args& a, const Int4Plan& plan, int sms,
+                           cudaStream_t s);
+
 // Rows of expert e of a product of M rows: bases clamped to [0, M], one that is smaller than an earlier
 // one counting as that one. By a whole warp. Without bases all rows are expert 0's.
 __device__ __forceinline__ void expert_rows(const int32_t* base, int e, int64_t M, int64_t* r0,

@@ -299,34 +299,6 @@ __device__ __forceinline__ void ascending_bases(int* base, int E, bool grouped) 
   __syncwarp();
 }
 
-// True in one lane of a whole warp. The MMAs of a branch on it issue faster than those of a branch on
-// the lane's number: 517 x 2047 x 7168 takes 13.8 us, 17.6 with the other.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
-
-// Waits for the phase with the given parity; gives up after limit_ns, or when another role of
-// this CTA has (both looked at every few polls). Each poll may suspend the thread for a while:
-// warps that poll without a pause slow the MMA warp down (517 x 2047 x 7168 took 20.3 us with the
-// epilogue's polling, 18.5 with the MMA warp's own, 17.5 with none).
-__device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                        uint64_t limit_ns) {
-  uint64_t t0 = 0;
-  for (uint32_t polls = 1;; ++polls) {
-    if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
-    if ((polls & 15u) == 0) {
-      if (*abort_flag) return false;
-      const uint64_t now = global_timer_ns();
-      if (t0 == 0) t0 = now;
-      if (now - t0 > limit_ns) return false;
-    }
-  }
-}
-
 // Set by a product whose bounded wait ran out, until take_int8_status takes it to g_int8_taken.
 __device__ int32_t g_int8_status;
 __device__ int32_t g_int8_taken;
@@ -653,7 +625,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           // This producer issued iteration it - kI8Producers after that stage's release, and the
           // MMA warp releases in order, so with NS >= kI8Producers the barrier is at most one
           // phase behind and the parity wait is unambiguous.
-          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns)) {
+          if (r > 0 && !parked_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns)) {
             i8_abort(tail);
             ok = false;
             break;
@@ -676,13 +648,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     // ---------------------------------------------------------------- MMA issuer
     if (elect_one()) {
       int it = 0, n = 0;
-      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns);
+      bool ok = args.inject == 0 || parked_wait(&tail->never, 0, abort_flag, args.wait_ns);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
         const I8Tile u = decode_tile<BN>(tile, NT, tail, E);
         const uint32_t idesc = idesc_i8(kWRows, u.cols);
         const int b = n & 1, rb = n >> 1;
         const uint32_t d = tmem + b * BN;
-        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns)) {
+        if (rb > 0 && !parked_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns)) {
           ok = false;
           break;
         }
@@ -690,7 +662,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         uint32_t more = 0;  // the tile's first MMA overwrites
         for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           const int s = it % NS, r = it / NS;
-          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns)) {
+          if (!parked_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns)) {
             ok = false;
             break;
           }
@@ -737,7 +709,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
       // after a wait that ran out, the warp still takes part in the barriers of later tiles
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns));
+      if (ok) ok = __all_sync(0xffffffffu, parked_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns));
       if (!ok) {
         if (lane == 0) i8_abort(tail);
         continue;
@@ -1081,7 +1053,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           if (it % kI8Producers != pw) continue;
           const int s = it % kPairStages, r = it / kPairStages;
-          if (r > 0 && !i8_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns)) {
+          if (r > 0 && !parked_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, args.wait_ns)) {
             pair_abort(tail);
             ok = false;
             break;
@@ -1106,13 +1078,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     // ---------------------------------------------------------------- MMA issuer (the leader's)
     if (rank == 0 && elect_one()) {
       int it = 0, n = 0;
-      bool ok = args.inject == 0 || i8_wait(&tail->never, 0, abort_flag, args.wait_ns);
+      bool ok = args.inject == 0 || parked_wait(&tail->never, 0, abort_flag, args.wait_ns);
       for (int tile = first; tile < tiles && ok; tile += step, ++n) {
         const I8Tile u = decode_pair(tile, NT, tail, E);
         const uint32_t idesc = idesc_i8(2 * kWRows, u.cols);
         const int b = n & 1, rb = n >> 1;
         const uint32_t d = tmem + b * kPairTokens;
-        if (rb > 0 && !i8_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns)) {
+        if (rb > 0 && !parked_wait(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, args.wait_ns)) {
           ok = false;
           break;
         }
@@ -1120,7 +1092,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         uint32_t more = 0;
         for (int kb = kb0; kb < kb1; kb += kSub, ++it) {
           const int s = it % kPairStages, r = it / kPairStages;
-          if (!i8_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns)) {
+          if (!parked_wait(&tail->full[s], r & 1, abort_flag, args.wait_ns)) {
             ok = false;
             break;
           }
@@ -1168,7 +1140,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (etid < u.rows) tail->a_scale[etid] = __ldcg(args.a_scale + u.row0 + etid);
       named_bar_sync(1, kI8EpiWarps * 32);
       // after a wait that ran out, the warp still takes part in the barriers of later tiles
-      if (ok) ok = __all_sync(0xffffffffu, i8_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns));
+      if (ok) ok = __all_sync(0xffffffffu, parked_wait(&tail->tfull[b], rb & 1, abort_flag, args.wait_ns));
       if (!ok) {
         if (lane == 0) pair_abort(tail);
         continue;

@@ -302,8 +302,17 @@ struct Int4Product {
   int64_t M;
   int N, K, E, group;
   int zero_tail;
+  float* part;           // workspace of a split product
+  unsigned long long wait_ns;  // failure-path test: the limit of an injected wait, else 0
+  int tile_tokens, split;      // kernel test: the variant to use, else 0
 };
+// The kernel for a product: tokens per tile (0: the kernel for few) and the parts that K is split into.
+struct Int4Plan {
+  int bn, S;
+};
+Int4Plan int4_plan(int64_t M, int N, int K, int E, bool grouped);
 cudaError_t launch_int4_product(const Int4Product& p, int sms, cudaStream_t s);
+cudaError_t take_int4_status(int32_t* status, cudaStream_t s);
 
 constexpr int kMaxBalanceExperts = 1024;
 constexpr int kMaxBalanceSequences = 4096;

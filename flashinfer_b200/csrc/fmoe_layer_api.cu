@@ -73,6 +73,9 @@ bool grid_fits(int64_t rows, int64_t units) { return rows * (units / 256 + 1) < 
 thread_local unsigned long long g_int8_wait_ns = 0;
 // One-shot choice of fmoe_debug_arm_int8_plan for this host thread's next product.
 thread_local int g_int8_tile_tokens = 0, g_int8_split = 0;
+// The same two for the products with 4-bit weights.
+thread_local unsigned long long g_int4_wait_ns = 0;
+thread_local int g_int4_tile_tokens = 0, g_int4_split = 0;
 
 int int8_product(const Int8Product& call, void* stream) {
   Int8Product p = call;
@@ -568,11 +571,23 @@ int fmoe_int4_workspace_size(int64_t m, int32_t n, int32_t k, int32_t E, size_t*
   if (m < 0 || m > INT32_MAX - 1024 || n < 1 || k < 32 || k % 32 != 0 || k > 131072 || E < 1 ||
       E > kMaxLocalExperts)
     return FMOE_ERR_SHAPE;
-  *bytes = 0;
+  // whether the rows have bases is not known here: the larger of the two plans
+  size_t most = 0;
+  for (const bool grouped : {false, true}) {
+    if (!grouped && E > 1) continue;
+    const Int4Plan p = int4_plan(m, n, k, E, grouped);
+    const size_t need = p.S > 1 ? static_cast<size_t>(p.S) * m * n * 4 : 0;
+    if (need > most) most = need;
+  }
+  *bytes = most;
   return FMOE_OK;
 }
 
 int fmoe_int4_matmul(const FmoeInt4Args* a, void* stream) {
+  const unsigned long long wait_ns = g_int4_wait_ns;
+  const int tile_tokens = g_int4_tile_tokens, split = g_int4_split;
+  g_int4_wait_ns = 0;
+  g_int4_tile_tokens = g_int4_split = 0;
   if (!a) return FMOE_ERR_NULL;
   if (a->num_rows < 0 || a->num_rows > INT32_MAX - 1024 || a->n < 1 || !int4_group(a->k, a->group) ||
       a->num_experts < 1 || a->num_experts > kMaxLocalExperts ||
@@ -589,9 +604,15 @@ int fmoe_int4_matmul(const FmoeInt4Args* a, void* stream) {
   if (!at(a->x, 16) || !at(a->weight, 16) || !at(a->scale, elem(a->scale_dtype)) || !at(a->bias, 4) ||
       !at(a->expert_base, 4) || !at(a->out, 2) || !at(a->workspace, 16))
     return FMOE_ERR_ALIGN;
+  // the tiles of every spread of the rows are counted in 32 bits
+  if ((a->num_rows / 64 + a->num_experts) * ((a->n + 127ll) / 128) * 8 > INT32_MAX) return FMOE_ERR_SHAPE;
   size_t need = 0;
   int rc = fmoe_int4_workspace_size(a->num_rows, a->n, a->k, a->num_experts, &need);
   if (rc) return rc;
+  if (tile_tokens != 0) {
+    if ((a->k + 63) / 64 < split) return FMOE_ERR_SHAPE;
+    need = split > 1 ? static_cast<size_t>(split) * a->num_rows * a->n * 4 : 0;
+  }
   if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return FMOE_ERR_WORKSPACE;
   const uint64_t M = a->num_rows, EN = static_cast<uint64_t>(a->num_experts) * a->n;
   const uint64_t g = EN * ((a->k + a->group - 1) / a->group);
@@ -608,8 +629,28 @@ int fmoe_int4_matmul(const FmoeInt4Args* a, void* stream) {
   if (rc) return rc;
   const Int4Product p{a->x, a->dtype, static_cast<const uint8_t*>(a->weight), a->scale, a->scale_dtype,
                       static_cast<const uint8_t*>(a->zero), a->bias, a->expert_base, a->out,
-                      a->num_rows, a->n, a->k, a->num_experts, a->group, a->zero_tail};
+                      a->num_rows, a->n, a->k, a->num_experts, a->group, a->zero_tail,
+                      static_cast<float*>(a->workspace), wait_ns, tile_tokens, split};
   return done(launch_int4_product(p, sms, as_stream(stream)));
+}
+
+int fmoe_int4_status(int32_t* status, void* stream) {
+  if (!status) return FMOE_ERR_NULL;
+  return done(take_int4_status(status, as_stream(stream)));
+}
+
+int fmoe_debug_arm_int4_timeout(uint64_t wait_ns) {
+  if (wait_ns < 100000ull || wait_ns > 2000000000ull) return FMOE_ERR_SHAPE;
+  g_int4_wait_ns = wait_ns;
+  return FMOE_OK;
+}
+
+int fmoe_debug_arm_int4_plan(int32_t tile_tokens, int32_t split) {
+  if ((tile_tokens != 64 && tile_tokens != 128 && tile_tokens != 256) || split < 1 || split > 8)
+    return FMOE_ERR_SHAPE;
+  g_int4_tile_tokens = tile_tokens;
+  g_int4_split = split;
+  return FMOE_OK;
 }
 
 int fmoe_layer_norm_workspace_size(int64_t T, int32_t H, size_t* bytes) {

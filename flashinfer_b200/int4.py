@@ -164,3 +164,15 @@ def int4_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, scale: torch.T
     need(expert_base, "expert_base", index, (E + 1,), I32)
     return _product("int4_expert_matmul", rows, weights, scale, zero, None, expert_base, group, output,
                     index, E, N)
+
+
+def int4_status(device: Optional[torch.device] = None) -> int:
+    """``_lib.STATUS_TIMEOUT_INT4`` if a wait inside a 4-bit product on the device ran out since the last
+    call (its output is not valid), else 0. Synchronises the current stream: products on other streams are
+    covered as far as they had finished, and by the next call otherwise."""
+    index = None if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
+    status = ctypes.c_int32(0)
+    call("fmoe_int4_status", index, ctypes.byref(status))
+    return status.value

@@ -49,6 +49,7 @@ extern "C" {
 #define FMOE_STATUS_TIMEOUT_GEMM1  0x1
 #define FMOE_STATUS_TIMEOUT_GEMM2  0x2
 #define FMOE_STATUS_TIMEOUT_INT8   0x4  /* fmoe_int8_status */
+#define FMOE_STATUS_TIMEOUT_INT4   0x8  /* fmoe_int4_status */
 
 /* output dtypes */
 #define FMOE_OUT_BF16    0
@@ -480,6 +481,14 @@ typedef struct FmoeInt4Args {
 FMOE_API int fmoe_int4_workspace_size(int64_t num_rows, int32_t n, int32_t k, int32_t num_experts,
                                       size_t* bytes);
 FMOE_API int fmoe_int4_matmul(const FmoeInt4Args* args, void* cuda_stream);
+
+/* As fmoe_int8_status, fmoe_debug_arm_int8_timeout and fmoe_debug_arm_int8_plan, for fmoe_int4_matmul:
+ * the status bit is FMOE_STATUS_TIMEOUT_INT4; tile_tokens is 64, 128 or 256, split 1 .. 8, and the call needs
+ * a workspace of split * num_rows * n * 4 bytes where split is above 1. An armed timeout takes the tensor
+ * core kernel whatever the size. */
+FMOE_API int fmoe_int4_status(int32_t* status, void* cuda_stream);
+FMOE_API int fmoe_debug_arm_int4_timeout(uint64_t wait_ns);
+FMOE_API int fmoe_debug_arm_int4_plan(int32_t tile_tokens, int32_t split);
 
 /* The norms before and after a block, with its gate and the residual scale. Per token:
  *   n = post_weight ? branch * rsqrt(mean(branch^2) + eps) * post_weight : branch
