@@ -435,10 +435,12 @@ Int4Plan int4_plan(int64_t M, int N, int K, int E, bool grouped) {
   if (per <= (grouped ? 8 : 16)) return Int4Plan{0, 1};
   if (grouped) per = 2 * per < M ? 2 * per : M;
   Int4Plan p{per <= 64 ? 64 : per <= 128 ? 128 : 256, 1};
-  const int64_t tiles = (per + p.bn - 1) / p.bn * used * ((N + 127) / 128);
-  // K in parts while there are fewer tiles than SMs (148), each of four blocks of 64 or more
+  // a tile of 256 tokens has 256 weight rows and takes two SMs
+  const int rows = p.bn == 256 ? 256 : 128, slots = p.bn == 256 ? 74 : 148;
+  const int64_t tiles = (per + p.bn - 1) / p.bn * used * ((N + rows - 1) / rows);
+  // K in parts while there are fewer tiles than run at a time (148 SMs), each of four blocks of 64 or more
   const int64_t most = (K + 63) / 64 / 4;
-  while (p.S < 8 && (p.S + 1) * tiles <= 148 && p.S < most) ++p.S;
+  while (p.S < 8 && (p.S + 1) * tiles <= slots && p.S < most) ++p.S;
   return p;
 }
 

@@ -26,30 +26,29 @@
 namespace fmoe {
 namespace {
 
-constexpr int kI4Threads = 640;   // warp 0 loads tokens, 1 issues MMAs, 4..11 widen, 12..19 store
-constexpr int kI4Widen0 = 4, kI4WidenWarps = 8;
-constexpr int kI4Epi0 = 12, kI4EpiWarps = 8;
+constexpr int kI4Threads = 640;   // warp 0 loads tokens, 1 issues MMAs, 4..15 widen, 16..19 store
+constexpr int kI4Widen0 = 4;
+constexpr int kI4Groups = 3;      // of four widening warps, one thread per weight row
+constexpr int kI4Epi0 = kI4Widen0 + 4 * kI4Groups, kI4EpiWarps = 4;
 constexpr int kI4Rows = 128;      // weight rows per tile
 constexpr int kI4KB = 64;         // values of a K block: one 128-byte row
 constexpr int kI4MaxStages = 8;
+constexpr int kI4Ahead = 2;       // blocks whose weights are on their way in a thread's registers
 constexpr int kI4Invs = 16;       // tiles that the widening may be ahead of the stores, rounded up
 
-// SUB: K blocks per stage. D: stages whose weights are on their way in registers.
 template <int BN>
 struct I4Cfg {
-  static constexpr int SUB = BN == 64 ? 2 : 1;
-  static constexpr int D = 4;
   static constexpr int BLOCK_A = kI4Rows * 128, BLOCK_B = BN * 128;
-  static constexpr int STAGE = SUB * (BLOCK_A + BLOCK_B);
+  static constexpr int STAGE = BLOCK_A + BLOCK_B;
   static constexpr int NS = 192 * 1024 / STAGE;
   static constexpr int BOX = BN == 64 ? 32 : 64;  // token rows per TMA box
   static constexpr int COLS = 2 * BN;
-  static_assert(NS <= kI4MaxStages && NS + 2 < kI4Invs, "barrier arrays, factors in flight");
+  static_assert(NS > kI4Groups && NS <= kI4MaxStages && NS + 2 < kI4Invs, "barrier arrays, factors in flight");
 };
 
 struct alignas(16) I4Tail {
   uint64_t bfull[kI4MaxStages];  // tokens: the TMA copies
-  uint64_t afull[kI4MaxStages];  // weights: one arrival per widening warp
+  uint64_t afull[kI4MaxStages];  // weights: one arrival per warp of a widening group
   uint64_t empty[kI4MaxStages];
   uint64_t tfull[2];
   uint64_t tempty[2];
@@ -59,7 +58,9 @@ struct alignas(16) I4Tail {
   int abort_flag;
   int tiles;
   int live;
-  int last_issue[kI4MaxStages];
+  int last_issue[kI4MaxStages];  // the latest round of copies that this CTA issued into the stage,
+  int last_bytes[kI4MaxStages];  // -1 for none, and (pairs) its bytes
+  int gave_up;                   // pairs: set in both CTAs after the leader's abort
   alignas(16) float inv[kI4Invs][kI4Rows];  // fp16: what an output is multiplied with
   int ebase[kMaxLocalExperts + 1];
   int etile[kMaxLocalExperts + 1];          // token tiles before expert e
@@ -69,8 +70,7 @@ template <int BN>
 constexpr size_t i4_smem_bytes() {
   return static_cast<size_t>(I4Cfg<BN>::NS) * I4Cfg<BN>::STAGE + sizeof(I4Tail) + 1024;
 }
-static_assert(i4_smem_bytes<64>() <= 227 * 1024 && i4_smem_bytes<128>() <= 227 * 1024 &&
-                  i4_smem_bytes<256>() <= 227 * 1024,
+static_assert(i4_smem_bytes<64>() <= 227 * 1024 && i4_smem_bytes<128>() <= 227 * 1024,
               "shared memory per CTA");
 
 struct I4Run {
@@ -99,6 +99,11 @@ __device__ __forceinline__ uint32_t idesc_16(int M, int N) {
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+__device__ __forceinline__ void st_shared_v4(uint32_t to, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -115,17 +120,54 @@ __device__ __forceinline__ void i4_abort(I4Tail* t) {
   atomicOr(&g_int4_status, FMOE_STATUS_TIMEOUT_INT4);
 }
 
+// The bases as a running maximum, the token tiles (of bn) per expert and their running sum. By one warp.
+__device__ __forceinline__ void plan_tiles(const I4Args& args, int bn, int NT, I4Tail* tail) {
+  const int lane = threadIdx.x & 31, E = args.E;
+  int most = 0, tiles = 0;
+  for (int e0 = 0; e0 <= E; e0 += 32) {
+    const int e = e0 + lane;
+    int64_t b = 0;
+    if (e <= E) b = args.expert_base ? __ldcg(args.expert_base + e) : e == 0 ? 0 : args.M;
+    int v = max(most, static_cast<int>(b < 0 ? 0 : b > args.M ? args.M : b));
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = max(v, up);
+    }
+    // tiles of the expert before base e
+    const int before = __shfl_up_sync(0xffffffffu, v, 1);
+    int mt = e == 0 || e > E ? 0 : (v - (lane == 0 ? most : before) + bn - 1) / bn;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, mt, o);
+      if (lane >= o) mt += up;
+    }
+    if (e <= E) {
+      tail->ebase[e] = v;
+      tail->etile[e] = tiles + mt;
+    }
+    most = __shfl_sync(0xffffffffu, v, 31);
+    tiles += __shfl_sync(0xffffffffu, mt, 31);
+  }
+  __syncwarp();
+  if (lane == 0) {
+    tail->tiles = tail->etile[E] * NT;
+    tail->live = tail->ebase[E];
+  }
+}
+
 // A unit of work: a part of K of a tile. Order: expert, weight tile, token tile, part of K (fastest), so
 // that CTAs that run side by side share weight tiles. An expert's tokens are cut into equal tiles of at
 // most BN.
 struct I4Unit {
   int e, n0;         // expert, first weight row (channel)
   int64_t row0;      // first token row
-  int rows, cols;    // tokens in the tile, and the MMA's N (a multiple of 16)
+  int rows, cols;    // tokens in the tile, and the MMA's N
   int part, kb0, kb1;
 };
 
-template <int BN>
+// STEP: what a tile's tokens are a multiple of. ROWS: its weight rows.
+template <int STEP, int ROWS>
 __device__ __forceinline__ I4Unit decode_unit(int unit, int NT, const I4Tail* t, int E, const I4Run& r) {
   I4Unit u;
   const int tile = unit / r.S;
@@ -143,13 +185,13 @@ __device__ __forceinline__ I4Unit decode_unit(int unit, int NT, const I4Tail* t,
   const int n = local / mt;
   const int m = local - n * mt;
   const int count = t->ebase[lo + 1] - t->ebase[lo];
-  // at most BN: count <= mt * BN, and BN is a multiple of 16
-  const int per = ((count + mt - 1) / mt + 15) / 16 * 16;
+  // at most BN: count <= mt * BN, and BN is a multiple of STEP
+  const int per = ((count + mt - 1) / mt + STEP - 1) / STEP * STEP;
   u.e = lo;
-  u.n0 = n * kI4Rows;
+  u.n0 = n * ROWS;
   u.row0 = t->ebase[lo] + static_cast<int64_t>(m) * per;
   u.rows = max(0, min(per, count - m * per));
-  u.cols = max(16, (u.rows + 15) / 16 * 16);
+  u.cols = max(STEP, (u.rows + STEP - 1) / STEP * STEP);
   u.kb0 = u.part * r.nkb / r.S;
   u.kb1 = (u.part + 1) * r.nkb / r.S;
   return u;
@@ -181,31 +223,227 @@ __device__ __forceinline__ uint32_t fma2(__half*, uint32_t a, uint32_t b, uint32
 template <typename T, bool F32S>
 __device__ __forceinline__ uint4 weights8(uint32_t q, uint32_t zp, uint32_t hi, uint32_t lo) {
   T* type = nullptr;
+  // byte i holds values 2i and 2i + 1: from q its low half to a word's low 16 bits, from q >> 4 its high
+  // half to the high 16 bits
+  const uint32_t q4 = q >> 4, base = nibble_base(type);
   uint32_t v[4];
-  widen8<T>(q, zp, v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    v[i] = sub2(type, (__byte_perm(q, q4, i | (i + 4) << 8) & 0x000f000fu) | base, zp);
     if constexpr (F32S)
       v[i] = fma2(type, hi, v[i], mul2(type, lo, v[i]));
     else
       v[i] = mul2(type, hi, v[i]);
   }
-  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
-                    __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// The epilogue of one warp: its 32 channels (one per lane) of the tile's columns c0, c0 + c_step, ...; out
-// is the element of the tile's first token at this warp's first channel. PAIRS (outputs at 4-byte
+// Three groups of four warps, a thread per weight row: a group takes every third block of 64 values, so
+// that one is loading and waiting while the others store. With all warps on every block, two threads per
+// row, a block took 1,100 cycles (its MMAs take 512), with two groups 1,000: instruction latency, one
+// after the other.
+// first, step, units: the CTA's units of work; decode: a unit with the first of this CTA's own 128 weight
+// rows; arrive: counts a warp on the barrier of a stage's weights.
+template <typename T, bool F32S, int NS, int STAGE, typename Decode, typename Arrive>
+__device__ __forceinline__ void widen_blocks(const I4Args& args, const I4Run& run, I4Tail* tail,
+                                             uint8_t* smem, int first, int step, int units,
+                                             const Decode& decode, const Arrive& arrive) {
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  volatile int* abort_flag = &tail->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  T* type = nullptr;
+  const int r = threadIdx.x & 127;
+  const int grp = (warp - kI4Widen0) >> 2;
+  const bool g32 = run.group_magic == 0;
+  const bool whole = (args.K & 63) == 0;  // no row ends inside a block
+  const bool wide = whole && (reinterpret_cast<uintptr_t>(args.w) & 31u) == 0;
+  const auto group_of = [&](int k) {
+    const uint32_t k32 = static_cast<uint32_t>(k >> 5);
+    return static_cast<int>(g32 ? k32 : __umulhi(k32, run.group_magic));
+  };
+  // The blocks of all of this CTA's units, one after the other; where the next to be loaded is.
+  int total = 0;
+  for (int unit = first; unit < units; unit += step) {
+    const int part = unit % run.S;
+    total += (part + 1) * run.nkb / run.S - part * run.nkb / run.S;
+  }
+  int unit = first, kb = 0, kb1 = 0;
+  // of the row of this thread: its values, scales and zero points
+  const uint8_t *wr = nullptr, *sr = nullptr, *zr = nullptr;
+  constexpr int SB = F32S ? 4 : 2;
+  const auto row_of = [&](const I4Unit& u) {
+    // rows behind the last are the last, and are not stored
+    return static_cast<int64_t>(u.e) * args.N + min(u.n0 + r, args.N - 1);
+  };
+  const auto open = [&]() {
+    const I4Unit u = decode(unit);
+    const int64_t row = row_of(u);
+    wr = args.w + row * (args.K / 2);
+    sr = static_cast<const uint8_t*>(args.scale) + row * args.groups * SB;
+    zr = args.zero ? args.zero + row * args.groups : nullptr;
+    return u;
+  };
+  // to the unit that a position behind a unit's end belongs to
+  const auto settle = [&]() {
+    while (kb >= kb1 && unit < units) {
+      const int over = kb - kb1;
+      unit += step;
+      if (unit >= units) break;
+      const I4Unit u = open();
+      kb = u.kb0 + over;
+      kb1 = u.kb1;
+    }
+  };
+  // z1 kSame: the second half's scale and zero point are the first half's (not copied: a copy of a value
+  // that is still being loaded would wait for it)
+  constexpr uint32_t kSame = 0x100u;
+  struct Ahead {
+    uint32_t w[8], s0, s1, z0, z1;
+  };
+  Ahead q[kI4Ahead];
+  const auto fetch = [&](Ahead& to) {
+    if (unit >= units) return;
+    const uint8_t* w = wr + kb * 32;
+    const int at = group_of(kb * kI4KB);
+    const auto scale = [&](int i) {
+      return F32S ? reinterpret_cast<const uint32_t*>(sr)[i]
+                  : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(sr)[i]);
+    };
+    to.s0 = scale(at);
+    to.z0 = zr ? zr[at] : 8u;
+    to.z1 = kSame;
+    if (wide) {
+      ld_global_v8(w, to.w);
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(w);
+      to.w[0] = a.x, to.w[1] = a.y, to.w[2] = a.z, to.w[3] = a.w;
+    }
+    if (g32 || !wide) {
+      if (whole || kb * kI4KB + 32 < args.K) {
+        if (!wide) {
+          const uint4 b = *reinterpret_cast<const uint4*>(w + 16);
+          to.w[4] = b.x, to.w[5] = b.y, to.w[6] = b.z, to.w[7] = b.w;
+        }
+        if (g32) {
+          to.s1 = scale(at + 1);
+          to.z1 = zr ? zr[at + 1] : 8u;
+        }
+      } else {
+        to.s1 = 0;  // behind the row's end: zeros, whatever the values
+        to.z1 = 8u;
+      }
+    }
+    kb += kI4Groups;
+    settle();
+  };
+  float factor = 1.0f;
+  const auto scales = [&](uint32_t raw, uint32_t& hi, uint32_t& lo) {
+    if constexpr (F32S || HALF) {
+      float f = F32S ? __uint_as_float(raw) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
+      f *= factor;
+      T a;
+      from_f32(f, &a);
+      hi = pack2(type, to_f32(a), to_f32(a));
+      if constexpr (F32S) {  // what the rounding left; nothing of an infinite scale
+        const float rest = fabsf(f) < INFINITY && fabsf(to_f32(a)) < INFINITY ? f - to_f32(a) : 0.0f;
+        lo = pack2(type, rest, rest);
+      }
+    } else {
+      hi = raw * 0x00010001u;
+    }
+  };
+  if (unit < units) {
+    const I4Unit u = open();
+    kb = u.kb0 + grp;
+    kb1 = u.kb1;
+    settle();
+  }
+#pragma unroll
+  for (int d = 0; d < kI4Ahead; ++d) fetch(q[d]);
+  // fp16: the unit of the block at hand, its blocks behind this one, its number, its factor
+  int mine = first - step, left = 0, n = -1;
+  int skip = grp + 1;
+  const uint32_t base = smem_u32(smem) + r * 128;
+  const uint32_t swz = static_cast<uint32_t>(r & 7) << 4;
+  int s = grp, round = 0;
+  bool ok = true;
+  for (int it = grp; it < total && ok;) {
+#pragma unroll
+    for (int d = 0; d < kI4Ahead; ++d) {
+      if (it >= total) break;
+      if constexpr (HALF) {
+        bool entered = false;
+        while (left < skip) {
+          skip -= left;
+          mine += step;
+          ++n;
+          const int part = mine % run.S;
+          left = (part + 1) * run.nkb / run.S - part * run.nkb / run.S;
+          entered = true;
+        }
+        left -= skip;
+        skip = kI4Groups;
+        if (entered) {
+          // the largest scale of the unit's groups to [2^9, 2^10)
+          const I4Unit u = decode(mine);
+          const int64_t at = row_of(u) * args.groups;
+          const int g0 = group_of(u.kb0 * kI4KB), g1 = group_of(min(u.kb1 * kI4KB, args.K) - 1);
+          float most = 0.0f;
+          for (int i = g0; i <= g1; ++i)
+            most = fmaxf(most, fabsf(scale_at(args.scale, F32S, type, at + i)));
+          int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127 - 9;
+          if (most == 0.0f || ex > 110) ex = 0;  // nothing, or infinite
+          if (ex < -120) ex = -120;
+          factor = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+          // every group writes the same
+          tail->inv[n % kI4Invs][r] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+        }
+      }
+      if (round > 0)
+        ok = __all_sync(0xffffffffu, parked_wait(&tail->empty[s], (round & 1) ^ 1, abort_flag,
+                                                 run.wait_ns));
+      if (!ok) {
+        if (lane == 0) i4_abort(tail);
+        break;
+      }
+      const uint32_t to = (base + s * STAGE) ^ swz;
+      uint32_t hi, lo = 0;
+      scales(q[d].s0, hi, lo);
+      uint32_t z = nibble_base(type) + (q[d].z0 & 15u) * 0x00010001u;
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) st_shared_v4(to ^ (c << 4), weights8<T, F32S>(q[d].w[c], z, hi, lo));
+      if (q[d].z1 != kSame) {
+        scales(q[d].s1, hi, lo);
+        z = nibble_base(type) + (q[d].z1 & 15u) * 0x00010001u;
+      }
+#pragma unroll
+      for (uint32_t c = 4; c < 8; ++c) st_shared_v4(to ^ (c << 4), weights8<T, F32S>(q[d].w[c], z, hi, lo));
+      fence_async_smem();  // the MMAs read through the asynchronous proxy
+      __syncwarp();
+      if (lane == 0) arrive(s);
+      fetch(q[d]);  // behind the fence, which would wait for the loads
+      it += kI4Groups;
+      s += kI4Groups;
+      if (s >= NS) {
+        s -= NS;
+        ++round;
+      }
+    }
+  }
+}
+
+// The epilogue of one warp: its 32 channels (one per lane) of the tile's columns; out is the element of the
+// tile's first token at this warp's first channel. PAIRS (outputs at 4-byte
 // boundaries): neighbouring lanes exchange halves of their tokens, so that a lane stores two channels at
 // once. O float: the partial sums of a split product.
 template <typename O, bool PAIRS>
-__device__ __forceinline__ void store_tile(uint32_t taddr, int c0, int c_step, int cols, int rows,
-                                           float factor, float bias, O* out, int N, int live) {
+__device__ __forceinline__ void store_tile(uint32_t taddr, int cols, int rows, float factor, float bias,
+                                           O* out, int N, int live) {
   const int lane = threadIdx.x & 31;
   const bool odd = lane & 1;
   O* mine = out + (PAIRS ? lane & ~1 : lane);
   const bool writes = lane < live;  // N is even with PAIRS, so both channels of a pair exist
-  for (int c = c0; c < cols; c += c_step) {
+  for (int c = 0; c < cols; c += 16) {
     __syncwarp();
     float v[16];
     tmem_ld_32x32b_x16(taddr + c, v);
@@ -238,11 +476,38 @@ __device__ __forceinline__ void store_tile(uint32_t taddr, int c0, int c_step, i
   __syncwarp();
 }
 
+// Zeroes the rows of no expert, by the epilogue warps of all CTAs.
+__device__ __forceinline__ void zero_rows_beside(const I4Args& args, const I4Tail* tail) {
+  if (!args.zero_tail) return;
+  const int64_t tid = static_cast<int64_t>(blockIdx.x) * (kI4EpiWarps * 32) + threadIdx.x - kI4Epi0 * 32;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * (kI4EpiWarps * 32);
+  zero_rows16(args.out, args.N, 0, tail->ebase[0], tid, threads);
+  zero_rows16(args.out, args.N, tail->live, args.M, tid, threads);
+}
+
+// One epilogue warp's share of a unit, the n-th of this CTA, from its lanes of the accumulator at taddr.
+template <typename T, bool HALF>
+__device__ __forceinline__ void store_unit(const I4Args& args, const I4Run& run, const I4Tail* tail,
+                                           const I4Unit& u, int n, uint32_t taddr, bool pairs) {
+  const int at_row = (threadIdx.x >> 5 & 3) * 32, lane = threadIdx.x & 31;
+  const int n0 = u.n0 + at_row, live = args.N - n0;
+  const float bias = run.S == 1 && args.bias && lane < live ? __ldcg(args.bias + n0 + lane) : 0.0f;
+  const float factor = HALF ? tail->inv[n % kI4Invs][at_row + lane] : 1.0f;
+  const int64_t at = u.row0 * args.N + n0;
+  if (run.S > 1)
+    store_tile<float, false>(taddr, u.cols, u.rows, factor, 0.0f,
+                             args.part + static_cast<int64_t>(u.part) * args.M * args.N + at, args.N, live);
+  else if (pairs)
+    store_tile<T, true>(taddr, u.cols, u.rows, factor, bias, static_cast<T*>(args.out) + at, args.N, live);
+  else
+    store_tile<T, false>(taddr, u.cols, u.rows, factor, bias, static_cast<T*>(args.out) + at, args.N, live);
+}
+
 template <typename T, int BN, bool F32S>
 __global__ void __launch_bounds__(kI4Threads, 1)
     k_int4_mm(const __grid_constant__ CUtensorMap tm_x, const I4Args args, const I4Run run) {
   using C = I4Cfg<BN>;
-  constexpr int NS = C::NS, SUB = C::SUB, D = C::D;
+  constexpr int NS = C::NS;
   constexpr bool HALF = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -255,7 +520,7 @@ __global__ void __launch_bounds__(kI4Threads, 1)
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&tail->bfull[s], 1);
-      mbar_init(&tail->afull[s], kI4WidenWarps);
+      mbar_init(&tail->afull[s], 4);
       mbar_init(&tail->empty[s], 1);
       tail->last_issue[s] = -1;
     }
@@ -275,40 +540,7 @@ __global__ void __launch_bounds__(kI4Threads, 1)
   }
   // everything this kernel reads may have been written by the previous grid
   pdl_begin_in_order();
-  if (warp == 0) {
-    // the bases as a running maximum, token tiles per expert and their running sum
-    int most = 0, tiles = 0;
-    for (int e0 = 0; e0 <= E; e0 += 32) {
-      const int e = e0 + lane;
-      int64_t b = 0;
-      if (e <= E) b = args.expert_base ? __ldcg(args.expert_base + e) : e == 0 ? 0 : args.M;
-      int v = max(most, static_cast<int>(b < 0 ? 0 : b > args.M ? args.M : b));
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v = max(v, up);
-      }
-      // tiles of the expert before base e
-      const int before = __shfl_up_sync(0xffffffffu, v, 1);
-      int mt = e == 0 || e > E ? 0 : (v - (lane == 0 ? most : before) + BN - 1) / BN;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, mt, o);
-        if (lane >= o) mt += up;
-      }
-      if (e <= E) {
-        tail->ebase[e] = v;
-        tail->etile[e] = tiles + mt;
-      }
-      most = __shfl_sync(0xffffffffu, v, 31);
-      tiles += __shfl_sync(0xffffffffu, mt, 31);
-    }
-    __syncwarp();
-    if (lane == 0) {
-      tail->tiles = tail->etile[E] * NT;
-      tail->live = tail->ebase[E];
-    }
-  }
+  if (warp == 0) plan_tiles(args, BN, NT, tail);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -322,22 +554,20 @@ __global__ void __launch_bounds__(kI4Threads, 1)
       int it = 0;
       bool ok = true;
       for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
-        const I4Unit u = decode_unit<BN>(unit, NT, tail, E, run);
+        const I4Unit u = decode_unit<16, kI4Rows>(unit, NT, tail, E, run);
         const int boxes = (u.cols + C::BOX - 1) / C::BOX;
-        for (int kb = u.kb0; kb < u.kb1; kb += SUB, ++it) {
+        for (int kb = u.kb0; kb < u.kb1; ++kb, ++it) {
           const int s = it % NS, r = it / NS;
           if (r > 0 && !parked_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, run.wait_ns)) {
             i4_abort(tail);
             ok = false;
             break;
           }
-          uint8_t* st = smem + s * C::STAGE + SUB * C::BLOCK_A;
-          const int blocks = min(SUB, u.kb1 - kb);
-          mbar_arrive_expect_tx(&tail->bfull[s], blocks * boxes * C::BOX * 128);
-          for (int j = 0; j < blocks; ++j, st += C::BLOCK_B)
-            for (int b = 0; b < boxes; ++b)
-              tma_load_2d(st + b * C::BOX * 128, &tm_x, &tail->bfull[s], (kb + j) * 128,
-                          static_cast<int>(u.row0) + b * C::BOX, pol);
+          uint8_t* st = smem + s * C::STAGE + C::BLOCK_A;
+          mbar_arrive_expect_tx(&tail->bfull[s], boxes * C::BOX * 128);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(st + b * C::BOX * 128, &tm_x, &tail->bfull[s], kb * 128,
+                        static_cast<int>(u.row0) + b * C::BOX, pol);
           tail->last_issue[s] = r;
         }
       }
@@ -348,7 +578,7 @@ __global__ void __launch_bounds__(kI4Threads, 1)
       int it = 0, n = 0;
       bool ok = run.inject == 0 || parked_wait(&tail->never, 0, abort_flag, run.wait_ns);
       for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x, ++n) {
-        const I4Unit u = decode_unit<BN>(unit, NT, tail, E, run);
+        const I4Unit u = decode_unit<16, kI4Rows>(unit, NT, tail, E, run);
         const uint32_t idesc = idesc_16<T>(kI4Rows, u.cols);
         const int b = n & 1, rb = n >> 1;
         const uint32_t d = tmem + b * BN;
@@ -358,7 +588,7 @@ __global__ void __launch_bounds__(kI4Threads, 1)
         }
         tc_fence_after();
         uint32_t more = 0;  // the unit's first MMA overwrites
-        for (int kb = u.kb0; kb < u.kb1; kb += SUB, ++it) {
+        for (int kb = u.kb0; kb < u.kb1; ++kb, ++it) {
           const int s = it % NS, r = it / NS;
           if (!parked_wait(&tail->afull[s], r & 1, abort_flag, run.wait_ns) ||
               !parked_wait(&tail->bfull[s], r & 1, abort_flag, run.wait_ns)) {
@@ -366,14 +596,12 @@ __global__ void __launch_bounds__(kI4Threads, 1)
             break;
           }
           tc_fence_after();
-          uint32_t sa = smem_u32(smem + s * C::STAGE), sb = sa + SUB * C::BLOCK_A;
-          for (int left = min(SUB, u.kb1 - kb); left > 0; --left, sa += C::BLOCK_A, sb += C::BLOCK_B) {
-            const uint64_t wd = smem_desc_k128(sa), xd = smem_desc_k128(sb);
+          const uint32_t sa = smem_u32(smem + s * C::STAGE);
+          const uint64_t wd = smem_desc_k128(sa), xd = smem_desc_k128(sa + C::BLOCK_A);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // 16 values of K each
-              mma_f16(d, wd + 2 * j, xd + 2 * j, idesc, more);
-              more = 1u;
-            }
+          for (int j = 0; j < 4; ++j) {  // 16 values of K each
+            mma_f16(d, wd + 2 * j, xd + 2 * j, idesc, more);
+            more = 1u;
           }
           mma_commit(&tail->empty[s]);
         }
@@ -383,163 +611,28 @@ __global__ void __launch_bounds__(kI4Threads, 1)
       mma_commit(&tail->drain);
       (void)mbar_wait(&tail->drain, 0);
     }
-  } else if (warp >= kI4Widen0 && warp < kI4Widen0 + kI4WidenWarps) {
+  } else if (warp >= kI4Widen0 && warp < kI4Epi0) {
     // ---------------------------------------------------------------- widening
-    // Two threads per weight row, each with 32 of a block's 64 values.
-    T* type = nullptr;
-    const int tid = threadIdx.x - kI4Widen0 * 32;
-    const int r = tid >> 1, h = tid & 1;
-    const uint32_t swz = static_cast<uint32_t>(r & 7);
-    const auto group_of = [&](int k) {
-      const uint32_t k32 = static_cast<uint32_t>(k >> 5);
-      return static_cast<int>(run.group_magic == 0 ? k32 : __umulhi(k32, run.group_magic));
-    };
-    struct Cursor {
-      int unit, kb, kb0, kb1;
-      int64_t wrow;
-    };
-    const auto open = [&](Cursor& c) {
-      if (c.unit >= units) return;
-      const I4Unit u = decode_unit<BN>(c.unit, NT, tail, E, run);
-      c.kb = c.kb0 = u.kb0;
-      c.kb1 = u.kb1;
-      // rows behind the last are the last, and are not stored
-      c.wrow = static_cast<int64_t>(u.e) * args.N + min(u.n0 + r, args.N - 1);
-    };
-    const auto advance = [&](Cursor& c) {
-      c.kb += SUB;
-      if (c.kb >= c.kb1) {
-        c.unit += gridDim.x;
-        open(c);
-      }
-    };
-    uint4 q[D][SUB];
-    uint32_t sc[D][SUB], zp[D][SUB];
-    const auto fetch = [&](Cursor& c, uint4 (&to)[SUB], uint32_t (&ts)[SUB], uint32_t (&tz)[SUB]) {
-      if (c.unit >= units) return;
-#pragma unroll
-      for (int j = 0; j < SUB; ++j) {
-        const int k = (c.kb + j) * kI4KB + 32 * h;
-        if (c.kb + j < c.kb1 && k < args.K) {
-          to[j] = __ldcg(reinterpret_cast<const uint4*>(args.w + c.wrow * (args.K / 2) + k / 2));
-          const int64_t at = c.wrow * args.groups + group_of(k);
-          ts[j] = F32S ? __ldcg(static_cast<const uint32_t*>(args.scale) + at)
-                       : static_cast<uint32_t>(__ldcg(static_cast<const uint16_t*>(args.scale) + at));
-          tz[j] = args.zero ? __ldcg(args.zero + at) : 8u;
-        }
-      }
-      advance(c);
-    };
-    Cursor ahead{static_cast<int>(blockIdx.x), 0, 0, 0, 0};
-    open(ahead);
-    Cursor now = ahead;
-#pragma unroll
-    for (int d = 0; d < D; ++d) fetch(ahead, q[d], sc[d], zp[d]);
-    int it = 0, n = 0;
-    bool ok = true;
-    float factor = 1.0f;
-    while (now.unit < units && ok) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        if (now.unit >= units || !ok) break;
-        if (HALF && now.kb == now.kb0) {
-          // the largest scale of the unit's groups to [2^9, 2^10); the row's two threads share the search
-          const int g0 = group_of(now.kb0 * kI4KB), g1 = group_of(min(now.kb1 * kI4KB, args.K) - 1);
-          float most = 0.0f;
-          for (int i = g0 + h; i <= g1; i += 2)
-            most = fmaxf(most, fabsf(scale_at(args.scale, F32S, type, now.wrow * args.groups + i)));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127 - 9;
-          if (most == 0.0f || ex > 110) ex = 0;  // nothing, or infinite
-          if (ex < -120) ex = -120;
-          factor = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-          if (h == 0) tail->inv[n % kI4Invs][r] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
-        }
-        const int s = it % NS, round = it / NS;
-        if (round > 0)
-          ok = __all_sync(0xffffffffu, parked_wait(&tail->empty[s], (round & 1) ^ 1, abort_flag,
-                                                   run.wait_ns));
-        if (!ok) {
-          if (lane == 0) i4_abort(tail);
-          break;
-        }
-        uint8_t* st = smem + s * C::STAGE + r * 128;
-#pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-          if (now.kb + j >= now.kb1) break;
-          uint4* row = reinterpret_cast<uint4*>(st + j * C::BLOCK_A);
-          if ((now.kb + j) * kI4KB + 32 * h < args.K) {
-            uint32_t hi, lo = 0;
-            if constexpr (F32S || HALF) {
-              float f = F32S ? __uint_as_float(sc[d][j])
-                             : __half2float(__ushort_as_half(static_cast<uint16_t>(sc[d][j])));
-              f *= factor;
-              T a;
-              from_f32(f, &a);
-              hi = pack2(type, to_f32(a), to_f32(a));
-              // what the rounding left; nothing of an infinite scale
-              const float rest = fabsf(f) < INFINITY && fabsf(to_f32(a)) < INFINITY ? f - to_f32(a) : 0.0f;
-              if (F32S) lo = pack2(type, rest, rest);
-            } else {
-              hi = sc[d][j] * 0x00010001u;
-            }
-            const uint32_t z = nibble_base(type) + (zp[d][j] & 15u) * 0x00010001u;
-            const uint32_t w[4] = {q[d][j].x, q[d][j].y, q[d][j].z, q[d][j].w};
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) row[(4 * h + c) ^ swz] = weights8<T, F32S>(w[c], z, hi, lo);
-          } else {
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) row[(4 * h + c) ^ swz] = make_uint4(0u, 0u, 0u, 0u);
-          }
-        }
-        fetch(ahead, q[d], sc[d], zp[d]);
-        fence_async_smem();  // the MMAs read through the asynchronous proxy
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tail->afull[s]);
-        ++it;
-        const int was = now.unit;
-        advance(now);
-        if (now.unit != was) ++n;
-      }
-    }
+    widen_blocks<T, F32S, NS, C::STAGE>(
+        args, run, tail, smem, blockIdx.x, gridDim.x, units,
+        [&](int unit) { return decode_unit<16, kI4Rows>(unit, NT, tail, E, run); },
+        [&](int s) { mbar_arrive(&tail->afull[s]); });
   } else if (warp >= kI4Epi0) {
     // ---------------------------------------------------------------- epilogue
     const int quarter = warp & 3;              // TMEM lanes of this warp
-    const int g = (warp - kI4Epi0) >> 2;       // which 16 of 32 columns
-    if (args.zero_tail) {                      // rows of no expert
-      const int64_t tid = static_cast<int64_t>(blockIdx.x) * (kI4EpiWarps * 32) + threadIdx.x - kI4Epi0 * 32;
-      const int64_t threads = static_cast<int64_t>(gridDim.x) * (kI4EpiWarps * 32);
-      zero_rows16(args.out, args.N, 0, tail->ebase[0], tid, threads);
-      zero_rows16(args.out, args.N, tail->live, args.M, tid, threads);
-    }
+    zero_rows_beside(args, tail);
     const bool pairs = (args.N & 1) == 0 && (reinterpret_cast<uintptr_t>(args.out) & 3u) == 0;
     int n = 0;
-    bool ok = true;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x, ++n) {
-      const I4Unit u = decode_unit<BN>(unit, NT, tail, E, run);
+      const I4Unit u = decode_unit<16, kI4Rows>(unit, NT, tail, E, run);
       const int b = n & 1, rb = n >> 1;
-      const int ch = u.n0 + quarter * 32 + lane;
-      const float bias = run.S == 1 && args.bias && ch < args.N ? __ldcg(args.bias + ch) : 0.0f;
-      if (ok) ok = __all_sync(0xffffffffu, parked_wait(&tail->tfull[b], rb & 1, abort_flag, run.wait_ns));
-      if (!ok) {
+      if (!__all_sync(0xffffffffu, parked_wait(&tail->tfull[b], rb & 1, abort_flag, run.wait_ns))) {
         if (lane == 0) i4_abort(tail);
         break;
       }
       tc_fence_after();
-      const float factor = HALF ? tail->inv[n % kI4Invs][quarter * 32 + lane] : 1.0f;
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * BN;
-      const int n0 = u.n0 + quarter * 32, live = args.N - n0;
-      const int64_t at = u.row0 * args.N + n0;
-      if (run.S > 1)
-        store_tile<float, false>(taddr, g * 16, 32, u.cols, u.rows, factor, 0.0f,
-                                 args.part + static_cast<int64_t>(u.part) * args.M * args.N + at, args.N,
-                                 live);
-      else if (pairs)
-        store_tile<T, true>(taddr, g * 16, 32, u.cols, u.rows, factor, bias,
-                            static_cast<T*>(args.out) + at, args.N, live);
-      else
-        store_tile<T, false>(taddr, g * 16, 32, u.cols, u.rows, factor, bias,
-                             static_cast<T*>(args.out) + at, args.N, live);
+      store_unit<T, HALF>(args, run, tail, u, n,
+                          tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * BN, pairs);
       tc_fence_before();
       mbar_arrive(&tail->tempty[b]);
     }
@@ -557,6 +650,300 @@ __global__ void __launch_bounds__(kI4Threads, 1)
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+// ------------------------------------------------------------------ CTA pairs
+// For many tokens: two CTAs share a tile of 256 weight rows x up to 256 tokens. One MMA (cta_group::2,
+// M = 256) reads both CTAs' shared memory: each widens its own 128 weight rows and loads half of the tokens,
+// so a K block fills 32 KB of an SM's shared memory instead of 48 for the same 128 x 256 outputs. That fill
+// bounds a single CTA: with 256 tokens per tile its blocks took 800 cycles (540 with the widening left
+// out), at 75 to 92 bytes a cycle that shared memory takes beside the MMAs' reads.
+//
+// Both CTAs count on the leader's (rank 0's) barriers; the leader issues the MMAs and commits to the barriers
+// of both. Each CTA stores its own weight rows' outputs.
+constexpr int kI4PairTokens = 256;
+constexpr int kI4PairBlock = kI4Rows * 128;               // weights, and as much again of tokens
+constexpr int kI4PairStage = 2 * kI4PairBlock;
+constexpr int kI4PairStages = 6;
+constexpr int kI4PairBox = 32;                            // token rows per TMA box
+constexpr size_t kI4PairSmem =
+    static_cast<size_t>(kI4PairStages) * kI4PairStage + sizeof(I4Tail) + 1024;
+static_assert(kI4PairSmem <= 227 * 1024, "pair shared memory");
+static_assert(kI4PairStages <= kI4MaxStages && kI4PairStages + 2 < kI4Invs, "arrays");
+
+__device__ __forceinline__ uint32_t at_cta(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+
+// Loads a box into this CTA's shared memory, its bytes counted on a barrier of the pair.
+__device__ __forceinline__ void load_box_pair(void* dst, const void* tmap, uint32_t bar, int32_t c0,
+                                              int32_t c1, uint64_t hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile"
+      ".mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "l"(hint)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrives on the barrier at `bar`'s place in both CTAs when the issued MMAs have finished.
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// The arrival of a warp's weights on the leader's barrier. They are in this CTA's own shared memory, and
+// fence.proxy.async, before this, has handed them to the asynchronous proxy, through which the pair's MMAs
+// read them: the arrival carries no data of its own and has to follow that fence only. With .release.cluster it
+// also waits for the loads that the warp has under way: 8192 x 4096 x 7168 took 559 us with it, 418 without,
+// and 609 with a warp of its own that passes the arrivals on.
+__device__ __forceinline__ void arrive_weights(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// parked_wait for a phase that threads of the other CTA arrive on as well: acquires at cluster scope.
+__device__ __forceinline__ bool parked_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                 uint64_t limit_ns) {
+  uint64_t t0 = 0;
+  for (uint32_t polls = 1;; ++polls) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+        : "memory");
+    if (ok) return true;
+    if ((polls & 15u) == 0) {
+      if (*abort_flag) return false;
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > limit_ns) return false;
+    }
+  }
+}
+
+// After an abort, by the leader once no role of either CTA issues any more: waits (bounded) until the copies
+// issued into every stage have landed, in both CTAs. A round needs both CTAs' copies and the next needs
+// both CTAs' stages, so a CTA is at most one round ahead of the other; the half of a round that was never
+// issued is taken off what the barrier expects.
+__device__ __forceinline__ void drain_pair(I4Tail* t) {
+  for (int s = 0; s < kI4PairStages; ++s) {
+    const int mine = t->last_issue[s], other = ld_dsmem_s32(&t->last_issue[s], 1);
+    const int r = max(mine, other);
+    if (r < 0) continue;
+    if (mine < r) {
+      mbar_arrive_expect_tx(&t->bfull[s], ld_dsmem_s32(&t->last_bytes[s], 1));
+    } else if (other < r) {
+      asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(
+                       smem_u32(&t->bfull[s])),
+                   "r"(t->last_bytes[s])
+                   : "memory");
+    }
+    (void)mbar_wait(&t->bfull[s], r & 1);
+  }
+}
+
+template <typename T, bool F32S>
+__global__ void __launch_bounds__(kI4Threads, 1)
+    k_int4_pair(const __grid_constant__ CUtensorMap tm_x, const I4Args args, const I4Run run) {
+  constexpr int NS = kI4PairStages;
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  I4Tail* tail = reinterpret_cast<I4Tail*>(smem + NS * kI4PairStage);
+  volatile int* abort_flag = &tail->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int E = args.E;
+  const int NT = (args.N + 2 * kI4Rows - 1) / (2 * kI4Rows);
+  const int rank = static_cast<int>(cluster_ctarank());
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&tail->bfull[s], 1);
+      mbar_init(&tail->afull[s], 2 * 4);
+      mbar_init(&tail->empty[s], 1);
+      tail->last_issue[s] = -1;
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tail->tfull[b], 1);
+      mbar_init(&tail->tempty[b], 2 * kI4EpiWarps);
+    }
+    mbar_init(&tail->drain, 1);
+    mbar_init(&tail->never, 1);
+    tail->abort_flag = 0;
+    tail->gave_up = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_x);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tail->tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  pdl_begin_in_order();
+  if (warp == 0) plan_tiles(args, kI4PairTokens, NT, tail);
+  tc_fence_before();
+  __syncthreads();
+  // both CTAs' barriers are initialised and both have their tensor memory
+  cluster_arrive();
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem = tail->tmem_base;
+  const int units = tail->tiles * run.S;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- tokens
+    if (elect_one()) {
+      const uint64_t pol = policy_evict_last();
+      int it = 0;
+      // the injected failure also leaves a stage that one CTA of the pair alone has filled
+      const int stop = run.inject != 0 ? 2 - rank : -1;
+      bool ok = true;
+      for (int unit = first; unit < units && ok; unit += step) {
+        const I4Unit u = decode_unit<32, 2 * kI4Rows>(unit, NT, tail, E, run);
+        const int half = u.cols / 2;
+        const int boxes = (half + kI4PairBox - 1) / kI4PairBox;
+        const int bytes = boxes * kI4PairBox * 128;
+        const int row = static_cast<int>(u.row0) + rank * half;
+        for (int kb = u.kb0; kb < u.kb1; ++kb, ++it) {
+          const int s = it % NS, r = it / NS;
+          if (it == stop) {
+            ok = false;
+            break;
+          }
+          if (r > 0 && !parked_wait(&tail->empty[s], (r & 1) ^ 1, abort_flag, run.wait_ns)) {
+            i4_abort(tail);
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * kI4PairStage + kI4PairBlock;
+          if (rank == 0) mbar_arrive_expect_tx(&tail->bfull[s], 2 * bytes);
+          const uint32_t bar = at_cta(&tail->bfull[s], 0);
+          for (int b = 0; b < boxes; ++b)
+            load_box_pair(st + b * kI4PairBox * 128, &tm_x, bar, kb * 128, row + b * kI4PairBox, pol);
+          tail->last_issue[s] = r;
+          tail->last_bytes[s] = bytes;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMAs (the leader's)
+    if (rank == 0 && elect_one()) {
+      int it = 0, n = 0;
+      bool ok = run.inject == 0 || parked_wait(&tail->never, 0, abort_flag, run.wait_ns);
+      for (int unit = first; unit < units && ok; unit += step, ++n) {
+        const I4Unit u = decode_unit<32, 2 * kI4Rows>(unit, NT, tail, E, run);
+        const uint32_t idesc = idesc_16<T>(2 * kI4Rows, u.cols);
+        const int b = n & 1, rb = n >> 1;
+        const uint32_t d = tmem + b * kI4PairTokens;
+        if (rb > 0 && !parked_wait_pair(&tail->tempty[b], (rb & 1) ^ 1, abort_flag, run.wait_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t more = 0;
+        for (int kb = u.kb0; kb < u.kb1; ++kb, ++it) {
+          const int s = it % NS, r = it / NS;
+          if (!parked_wait_pair(&tail->afull[s], r & 1, abort_flag, run.wait_ns) ||
+              !parked_wait(&tail->bfull[s], r & 1, abort_flag, run.wait_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * kI4PairStage);
+          const uint64_t wd = smem_desc_k128(sa), xd = smem_desc_k128(sa + kI4PairBlock);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma_f16_pair(d, wd + 2 * j, xd + 2 * j, idesc, more);
+            more = 1u;
+          }
+          commit_both(&tail->empty[s]);
+        }
+        if (ok) commit_both(&tail->tfull[b]);
+      }
+      if (!ok) i4_abort(tail);
+      commit_both(&tail->drain);
+    }
+    if (lane == 0) (void)mbar_wait(&tail->drain, 0);
+  } else if (warp >= kI4Widen0 && warp < kI4Epi0) {
+    // ---------------------------------------------------------------- widening
+    widen_blocks<T, F32S, NS, kI4PairStage>(
+        args, run, tail, smem, first, step, units,
+        [&](int unit) {
+          I4Unit u = decode_unit<32, 2 * kI4Rows>(unit, NT, tail, E, run);
+          u.n0 += rank * kI4Rows;
+          return u;
+        },
+        [&](int s) { arrive_weights(at_cta(&tail->afull[s], 0)); });
+  } else if (warp >= kI4Epi0) {
+    // ---------------------------------------------------------------- epilogue
+    const int quarter = warp & 3;
+    zero_rows_beside(args, tail);
+    const bool pairs = (args.N & 1) == 0 && (reinterpret_cast<uintptr_t>(args.out) & 3u) == 0;
+    int n = 0;
+    for (int unit = first; unit < units; unit += step, ++n) {
+      I4Unit u = decode_unit<32, 2 * kI4Rows>(unit, NT, tail, E, run);
+      u.n0 += rank * kI4Rows;
+      const int b = n & 1, rb = n >> 1;
+      if (!__all_sync(0xffffffffu, parked_wait(&tail->tfull[b], rb & 1, abort_flag, run.wait_ns))) {
+        if (lane == 0) i4_abort(tail);
+        break;
+      }
+      tc_fence_after();
+      store_unit<T, HALF>(args, run, tail, u, n,
+                          tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * kI4PairTokens, pairs);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(at_cta(&tail->tempty[b], 0));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // Never leave a bulk copy in flight into shared memory that is about to be released. Without an abort of
+  // the leader its MMAs have waited for all of them.
+  if (threadIdx.x == 0 && rank == 0 && *abort_flag)
+    for (int c = 0; c < 2; ++c)
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at_cta(&tail->gave_up, c)), "r"(1)
+                   : "memory");
+  cluster_arrive();  // the pair's MMAs are done
+  cluster_wait();
+  tc_fence_after();
+  if (*reinterpret_cast<volatile int*>(&tail->gave_up)) {
+    if (threadIdx.x == 0 && rank == 0) drain_pair(tail);
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
   }
 }
 
@@ -603,22 +990,45 @@ __global__ void __launch_bounds__(256) k_int4_finish(const I4Args a, int S) {
 }
 
 // ------------------------------------------------------------------ launches
-template <typename T, int BN, bool F32S>
-cudaError_t launch_mm(const Int4Product& p, const I4Args& a, const Int4Plan& plan, int sms,
-                      cudaStream_t s) {
-  static std::atomic<bool> done[64];
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<bool> (&done)[64]) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!done[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_int4_mm<T, BN, F32S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(i4_smem_bytes<BN>()));
-    if (e != cudaSuccess) return e;
-    done[dev].store(true, std::memory_order_release);
-  }
+  if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(bytes));
+  if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+  return e;
+}
+
+template <typename T, int BN, bool F32S>
+cudaError_t launch_single(const CUtensorMap& tm_x, const I4Args& a, const I4Run& r, int64_t units, int sms,
+                          cudaStream_t s) {
+  static std::atomic<bool> done[64];
+  const cudaError_t e = allow_smem(k_int4_mm<T, BN, F32S>, i4_smem_bytes<BN>(), done);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(k_int4_mm<T, BN, F32S>, dim3(static_cast<unsigned>(units < sms ? units : sms)),
+                    dim3(kI4Threads), i4_smem_bytes<BN>(), s, tm_x, a, r);
+}
+
+template <typename T, bool F32S>
+cudaError_t launch_pair(const CUtensorMap& tm_x, const I4Args& a, const I4Run& r, int64_t units, int sms,
+                        cudaStream_t s) {
+  static std::atomic<bool> done[64];
+  const cudaError_t e = allow_smem(k_int4_pair<T, F32S>, kI4PairSmem, done);
+  if (e != cudaSuccess) return e;
+  const int64_t clusters = units < sms / 2 ? units : sms / 2;
+  return launch_pdl_cluster(k_int4_pair<T, F32S>, dim3(static_cast<unsigned>(2 * clusters)),
+                            dim3(kI4Threads), kI4PairSmem, s, 2, tm_x, a, r);
+}
+
+template <typename T, bool F32S>
+cudaError_t launch_mm(const Int4Product& p, const I4Args& a, const Int4Plan& plan, int sms,
+                      cudaStream_t s) {
+  const int box = plan.bn == 64 ? I4Cfg<64>::BOX : plan.bn == 128 ? I4Cfg<128>::BOX : kI4PairBox;
   CUtensorMap tm_x;
   const uint64_t row = static_cast<uint64_t>(p.K) * 2;
-  if (!tensor_map_u8(&tm_x, p.x, row, p.M, row, 128, I4Cfg<BN>::BOX)) return cudaErrorInvalidValue;
+  if (!tensor_map_u8(&tm_x, p.x, row, p.M, row, 128, box)) return cudaErrorInvalidValue;
   I4Run r{};
   r.nkb = (p.K + kI4KB - 1) / kI4KB;
   r.S = plan.S;
@@ -629,30 +1039,22 @@ cudaError_t launch_mm(const Int4Product& p, const I4Args& a, const Int4Plan& pla
   r.wait_ns = p.wait_ns != 0 ? p.wait_ns : FMOE_WAIT_NS;
   r.inject = p.wait_ns != 0;
   const int64_t used = p.M < p.E ? p.M : p.E;
-  const int64_t most = (p.expert_base ? p.M / BN + used : (p.M + BN - 1) / BN) *
-                       ((p.N + kI4Rows - 1) / kI4Rows) * plan.S;
-  const int grid = static_cast<int>(most < sms ? most : sms);
-  cudaError_t e = launch_pdl(k_int4_mm<T, BN, F32S>, dim3(grid), dim3(kI4Threads), i4_smem_bytes<BN>(), s,
-                             tm_x, a, r);
+  const int rows = plan.bn == kI4PairTokens ? 2 * kI4Rows : kI4Rows;
+  const int64_t units = (p.expert_base ? p.M / plan.bn + used : (p.M + plan.bn - 1) / plan.bn) *
+                        ((p.N + rows - 1) / rows) * plan.S;
+  cudaError_t e;
+  if (plan.bn == 64)
+    e = launch_single<T, 64, F32S>(tm_x, a, r, units, sms, s);
+  else if (plan.bn == 128)
+    e = launch_single<T, 128, F32S>(tm_x, a, r, units, sms, s);
+  else
+    e = launch_pair<T, F32S>(tm_x, a, r, units, sms, s);
   if (e != cudaSuccess || plan.S == 1) return e;
   const bool four = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7u) == 0;
   const int64_t blocks = (p.M * p.N / (four ? 4 : 1) + 255) / 256;
   const dim3 fgrid(static_cast<unsigned>(blocks < 8 * sms ? blocks : 8 * sms));
   if (four) return launch_pdl(k_int4_finish<T, 4>, fgrid, dim3(256), 0, s, a, plan.S);
   return launch_pdl(k_int4_finish<T, 1>, fgrid, dim3(256), 0, s, a, plan.S);
-}
-
-template <typename T, bool F32S>
-cudaError_t launch_mm(const Int4Product& p, const I4Args& a, const Int4Plan& plan, int sms,
-                      cudaStream_t s) {
-  switch (plan.bn) {
-    case 64:
-      return launch_mm<T, 64, F32S>(p, a, plan, sms, s);
-    case 128:
-      return launch_mm<T, 128, F32S>(p, a, plan, sms, s);
-    default:
-      return launch_mm<T, 256, F32S>(p, a, plan, sms, s);
-  }
 }
 
 }  // namespace

@@ -381,6 +381,15 @@ __device__ __forceinline__ void ld_global_nc_v8(const void* p, uint32_t (&w)[8])
                : "l"(p));
 }
 
+// The same for data that an earlier grid may have written, after the wait for it.
+__device__ __forceinline__ void ld_global_v8(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                 "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+
 // ---------------------------------------------------------------- programmatic dependent launch
 // Every kernel of the path is launched with programmatic stream serialisation. A kernel first
 // lets the next kernel in the stream be scheduled (its CTAs are placed as resources free up and
