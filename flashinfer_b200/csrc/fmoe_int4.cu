@@ -73,8 +73,17 @@ __device__ __forceinline__ void transpose_quad(uint4& q) {
   }
 }
 
+// Eight values less the zero point (zp: the base plus it, twice) as pairs (0, 4), (1, 5), (2, 6), (3, 7).
+template <typename T>
+__device__ __forceinline__ void widen8(uint32_t q, uint32_t zp, uint32_t (&v)[4]) {
+  T* type = nullptr;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = sub2(type, and_or(q >> (4 * i), 0x000f000fu, nibble_base(type)), zp);
+}
+
 template <typename T, int RT, int NT, int D, bool SPREAD>
-__global__ void __launch_bounds__(kFewWarps * 32) k_int4_few(const I4Args a) {
+__global__ void __launch_bounds__(kFewWarps * 32, 2) k_int4_few(const I4Args a, const uint32_t group_magic) {
   constexpr int ROWS = 16 * RT, COLS = 8 * NT;
   __shared__ float red[kFewWarps][COLS][ROWS + 1];
   T* type = nullptr;
@@ -90,102 +99,145 @@ __global__ void __launch_bounds__(kFewWarps * 32) k_int4_few(const I4Args a) {
   if (r0 >= r1) return;
 
   const int blocks = (a.K + 127) / 128;
-  const int64_t kbytes = a.K / 2;
-  // rows behind the last are the last, and are not stored
-  int64_t wrow[2 * RT];
+  const int ssize = a.scale_f32 ? 4 : 2;
+  // of the block's first row, and how far this lane's rows are from it (rows behind the last are the last,
+  // and are not stored)
+  const int64_t row0 = static_cast<int64_t>(e) * a.N + n0;
+  const uint8_t* wp = a.w + row0 * (a.K / 2);
+  const uint8_t* sp = static_cast<const uint8_t*>(a.scale) + row0 * a.groups * ssize;
+  const uint8_t* zp = a.zero ? a.zero + row0 * a.groups : nullptr;
+  int away[2 * RT];
 #pragma unroll
-  for (int i = 0; i < 2 * RT; ++i)
-    wrow[i] = static_cast<int64_t>(e) * a.N + min(n0 + 8 * i + g, a.N - 1);
-  const T* x = static_cast<const T*>(a.x);
+  for (int i = 0; i < 2 * RT; ++i) away[i] = min(8 * i + g, a.N - 1 - n0);
+  const auto scale = [&](int i, int grp) {  // as its bits
+    const int at = away[i] * a.groups + grp;
+    return a.scale_f32 ? reinterpret_cast<const uint32_t*>(sp)[at]
+                       : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(sp)[at]);
+  };
+  const auto zero = [&](int i, int grp) -> uint32_t { return zp ? zp[away[i] * a.groups + grp] : 8u; };
+  const auto number = [&](uint32_t bits) {
+    if (a.scale_f32) return __uint_as_float(bits);
+    if constexpr (std::is_same<T, __half>::value)
+      return __half2float(__ushort_as_half(static_cast<uint16_t>(bits)));
+    else
+      return __uint_as_float(bits << 16);
+  };
 
   for (int64_t m0 = r0; m0 < r1; m0 += COLS) {
-    uint4 q[D][2 * RT];
-    const auto fetch = [&](int b, uint4 (&to)[2 * RT]) {
-      const int k = b * 128 + 32 * t;  // K is a multiple of 32: a lane's 16 bytes are in the row or not
+    // the tokens of this lane's column, from its first value in a block on (SPREAD: in a step)
+    const T* xp[NT];
+    bool has[NT];
 #pragma unroll
-      for (int i = 0; i < 2 * RT; ++i)
-        to[i] = b < blocks && k < a.K
-                    ? load_row16(reinterpret_cast<const uint4*>(a.w + wrow[i] * kbytes + k / 2))
-                    : make_uint4(0u, 0u, 0u, 0u);
+    for (int j = 0; j < NT; ++j) {
+      const int64_t row = m0 + 8 * j + g;
+      has[j] = row < r1;
+      xp[j] = static_cast<const T*>(a.x) + (has[j] ? row : r0) * a.K + (SPREAD ? 8 : 32) * t;
+    }
+    struct Ahead {
+      uint4 w[2 * RT];
+      uint32_t s[SPREAD ? 1 : 2 * RT], z[SPREAD ? 1 : 2 * RT];
+    };
+    Ahead q[D];
+    const auto fetch = [&](int b, Ahead& to) {
+      if (b >= blocks) return;
+      // K is a multiple of 32: a lane's 16 bytes are in the row, or the tokens there are zeros
+      if (b * 128 + 32 * t < a.K) {
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i)
+          to.w[i] = load_row16(
+              reinterpret_cast<const uint4*>(wp + (away[i] * (a.K / 2) + b * 64 + 16 * t)));
+      }
+      if constexpr (!SPREAD) {
+        const int grp = static_cast<int>((static_cast<uint32_t>(b) * group_magic) >> 20);
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i) {
+          to.s[i] = scale(i, grp);
+          to.z[i] = zero(i, grp);
+        }
+      }
     };
 #pragma unroll
-    for (int d = 0; d < D; ++d) fetch(warp + d * kFewWarps, q[d]);
+    for (int d = 0; d < D; ++d) {
+#pragma unroll
+      for (int i = 0; i < 2 * RT; ++i) q[d].w[i] = make_uint4(0u, 0u, 0u, 0u);
+      fetch(warp + d * kFewWarps, q[d]);
+    }
     float acc[RT][NT][4] = {};
     for (int b0 = warp; b0 < blocks; b0 += D * kFewWarps) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
         const int b = b0 + d * kFewWarps;
-        if (b < blocks) {
-          const int kb = b * 128;
-          uint4 w[2 * RT];
+        if (b >= blocks) break;
+        uint4 v[NT][4];
 #pragma unroll
-          for (int i = 0; i < 2 * RT; ++i) {
-            w[i] = q[d][i];
-            if (SPREAD) transpose_quad(w[i]);
-          }
-          fetch(b + D * kFewWarps, q[d]);
-          uint32_t zp[2 * RT];
-          float sc[2 * RT];
-          float part[RT][NT][4];
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            // the values of this step: 8 from k on
-            const int k = kb + (SPREAD ? 32 * c + 8 * t : 32 * t + 8 * c);
-            // SPREAD: a step is 32 values of one group; else the piece is
-            const bool opens = SPREAD ? c == 0 || a.group == 32 || (c == 2) : c == 0;
-            if (opens) {
-              const int grp = (SPREAD ? kb + 32 * c : kb) / a.group;
+            const int k = b * 128 + (SPREAD ? 32 * c : 32 * t);
+            v[j][c] = make_uint4(0u, 0u, 0u, 0u);
+            if (has[j] && k < a.K)
+              v[j][c] = *reinterpret_cast<const uint4*>(xp[j] + b * 128 + (SPREAD ? 32 : 8) * c);
+          }
+        if constexpr (SPREAD) {
 #pragma unroll
-              for (int i = 0; i < 2 * RT; ++i) {
-                const int64_t at = wrow[i] * a.groups + min(grp, a.groups - 1);
-                // a step behind the row's end adds nothing, whatever the last scale
-                sc[i] = grp < a.groups ? scale_at(a.scale, a.scale_f32, type, at) : 0.0f;
-                const uint32_t z = a.zero ? a.zero[at] & 15u : 8u;
-                zp[i] = nibble_base(type) + z * 0x00010001u;
-                // 128 + z and 1024 + z have z in their low mantissa bits
+          for (int i = 0; i < 2 * RT; ++i) transpose_quad(q[d].w[i]);
+        }
+        float part[RT][NT][4] = {};  // of the group at hand
+        float sc[2 * RT];
+        uint32_t zb[2 * RT];
+        const auto open = [&](int grp) {
+#pragma unroll
+          for (int i = 0; i < 2 * RT; ++i) {
+            // a step behind the row's end adds nothing, whatever the last scale
+            const bool in = !SPREAD || grp < a.groups;
+            sc[i] = in ? number(SPREAD ? scale(i, grp) : q[d].s[SPREAD ? 0 : i]) : 0.0f;
+            const uint32_t z = in ? SPREAD ? zero(i, grp) : q[d].z[SPREAD ? 0 : i] : 8u;
+            zb[i] = nibble_base(type) + (z & 15u) * 0x00010001u;  // the base has the low four bits free
+          }
+        };
+        const auto close = [&]() {
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                acc[r][j][i] = fmaf(sc[2 * r + (i >> 1)], part[r][j][i], acc[r][j][i]);
+                part[r][j][i] = 0.0f;
               }
+        };
+        if constexpr (!SPREAD) open(0);
 #pragma unroll
-              for (int r = 0; r < RT; ++r)
+        for (int c = 0; c < 4; ++c) {
+          if constexpr (SPREAD) {  // a step is 32 values of one group
+            if (a.group == 32)
+              open(4 * b + c);
+            else if ((c & 1) == 0)
+              open(2 * b + c / 2);
+          }
+          uint32_t bf[NT][4];
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+          for (int j = 0; j < NT; ++j) {
+            bf[j][0] = __byte_perm(v[j][c].x, v[j][c].z, 0x5410);
+            bf[j][1] = __byte_perm(v[j][c].x, v[j][c].z, 0x7632);
+            bf[j][2] = __byte_perm(v[j][c].y, v[j][c].w, 0x5410);
+            bf[j][3] = __byte_perm(v[j][c].y, v[j][c].w, 0x7632);
+          }
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) part[r][j][i] = 0.0f;
-            }
-            uint32_t bf[NT][4];
+          for (int r = 0; r < RT; ++r) {
+            const uint4 &wl = q[d].w[2 * r], &wh = q[d].w[2 * r + 1];
+            uint32_t lo[4], hi[4];
+            widen8<T>(c == 0 ? wl.x : c == 1 ? wl.y : c == 2 ? wl.z : wl.w, zb[2 * r], lo);
+            widen8<T>(c == 0 ? wh.x : c == 1 ? wh.y : c == 2 ? wh.z : wh.w, zb[2 * r + 1], hi);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const int64_t row = m0 + 8 * j + g;
-              uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              if (row < r1 && k < a.K) v = *reinterpret_cast<const uint4*>(x + row * a.K + k);
-              bf[j][0] = __byte_perm(v.x, v.z, 0x5410);
-              bf[j][1] = __byte_perm(v.x, v.z, 0x7632);
-              bf[j][2] = __byte_perm(v.y, v.w, 0x5410);
-              bf[j][3] = __byte_perm(v.y, v.w, 0x7632);
-            }
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              const uint4 &wl = w[2 * r], &wh = w[2 * r + 1];
-              uint32_t lo[4], hi[4];
-              widen8<T>(c == 0 ? wl.x : c == 1 ? wl.y : c == 2 ? wl.z : wl.w, zp[2 * r], lo);
-              widen8<T>(c == 0 ? wh.x : c == 1 ? wh.y : c == 2 ? wh.z : wh.w, zp[2 * r + 1], hi);
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                mma_16816(type, part[r][j], {lo[0], hi[0], lo[1], hi[1]}, bf[j][0], bf[j][1]);
-                mma_16816(type, part[r][j], {lo[2], hi[2], lo[3], hi[3]}, bf[j][2], bf[j][3]);
-              }
-            }
-            const bool closes = SPREAD ? c == 3 || a.group == 32 || c == 1 : c == 3;
-            if (closes) {
-#pragma unroll
-              for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    acc[r][j][i] = fmaf(sc[2 * r + (i >> 1)], part[r][j][i], acc[r][j][i]);
+              mma_16816(type, part[r][j], {lo[0], hi[0], lo[1], hi[1]}, bf[j][0], bf[j][1]);
+              mma_16816(type, part[r][j], {lo[2], hi[2], lo[3], hi[3]}, bf[j][2], bf[j][3]);
             }
           }
+          if (SPREAD ? a.group == 32 || (c & 1) == 1 : c == 3) close();
         }
+        fetch(b + D * kFewWarps, q[d]);
       }
     }
 #pragma unroll
@@ -391,8 +443,13 @@ cudaError_t dequantise(const Int4Weights& p, cudaStream_t s) {
 template <typename T, int RT, int NT, int D>
 cudaError_t few(const I4Args& a, cudaStream_t s) {
   const dim3 grid((a.N + 16 * RT - 1) / (16 * RT), a.E);
-  if (a.group < 128) return launch_pdl(k_int4_few<T, RT, NT, D, true>, grid, dim3(kFewWarps * 32), 0, s, a);
-  return launch_pdl(k_int4_few<T, RT, NT, D, false>, grid, dim3(kFewWarps * 32), 0, s, a);
+  // a block of 128 values b, at most 1023, is in group (b * magic) >> 20 = b / (group / 128): the error of the
+  // product is below 2^-10
+  const int per = a.group / 128;
+  const uint32_t magic = per == 0 || per > 1024 ? 0u : (1u << 20) / per + 1;
+  if (a.group < 128)
+    return launch_pdl(k_int4_few<T, RT, NT, D, true>, grid, dim3(kFewWarps * 32), 0, s, a, magic);
+  return launch_pdl(k_int4_few<T, RT, NT, D, false>, grid, dim3(kFewWarps * 32), 0, s, a, magic);
 }
 
 template <typename T>
@@ -401,7 +458,7 @@ cudaError_t few(const I4Args& a, int64_t per, int sms, cudaStream_t s) {
   const int64_t used = a.M < a.E ? a.M : a.E;
   const bool tall = (a.N + 31) / 32 * used >= 4 * sms;
   if (per <= 8) return tall ? few<T, 2, 1, 2>(a, s) : few<T, 1, 1, 4>(a, s);
-  return tall ? few<T, 2, 2, 2>(a, s) : few<T, 1, 2, 4>(a, s);
+  return few<T, 1, 2, 2>(a, s);
 }
 
 }  // namespace

@@ -229,7 +229,7 @@ __device__ __forceinline__ uint4 weights8(uint32_t q, uint32_t zp, uint32_t hi, 
   uint32_t v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[i] = sub2(type, (__byte_perm(q, q4, i | (i + 4) << 8) & 0x000f000fu) | base, zp);
+    v[i] = sub2(type, and_or(__byte_perm(q, q4, i | (i + 4) << 8), 0x000f000fu, base), zp);
     if constexpr (F32S)
       v[i] = fma2(type, hi, v[i], mul2(type, lo, v[i]));
     else
