@@ -7,11 +7,12 @@
 //   d branch = d residual = dh + r * (u - mean(u) - n * mean(u * n))
 //   d weight = sum over rows of dy * n,  d bias = sum over rows of dy
 //
-// A row is read once and stays in registers, 32 values per thread (16 in the backward pass), so the
-// variance is taken of the deviations from the mean and not from a difference of squares. Rows of up to
-// 1024 (512) columns are a warp's, longer ones a block's. Everything is fp32 between the load and the
-// one rounding on the way out. Bound by HBM; the figures stand at the kernels.
+// A row is read once and stays in registers, up to 32 values per thread, so the variance is taken of the
+// deviations from the mean and not from a difference of squares. Short rows are a warp's, longer ones a
+// block's. Everything is fp32 between the load and the one rounding on the way out. Bound by HBM; the
+// figures stand at the kernels.
 #include <atomic>
+#include <type_traits>
 
 #include "fmoe_elem.cuh"
 #include "fmoe_internal.h"
@@ -37,404 +38,456 @@ struct LnArgs {
   int want_w, want_b;
 };
 
+// A unit of a row: V elements (a 16-byte granule, or 1 where rows are not on 16-byte boundaries) as fp32, in
+// pairs for the packed instructions or singly.
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float mad(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 mad(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float total(float a) { return a; }
+__device__ __forceinline__ float total(float2 a) { return a.x + a.y; }
+__device__ __forceinline__ void set(float& a, float s) { a = s; }
+__device__ __forceinline__ void set(float2& a, float s) { a = make_float2(s, s); }
+
+template <typename T, int V>
+struct Unit {
+  using P = typename std::conditional<V == 1, float, float2>::type;
+  static constexpr int N = V > 1 ? V / 2 : 1;
+  P p[N];
+};
+template <typename P>
+__device__ __forceinline__ P all(float s) {
+  P a;
+  set(a, s);
+  return a;
+}
+template <typename T, int V>
+__device__ __forceinline__ Unit<T, V> unit_of(const Pack<T, V>& r) {
+  Unit<T, V> u;
+  float v[V];
+  unpack(r, v);
+  if constexpr (V == 1) {
+    u.p[0] = v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < Unit<T, V>::N; ++i) u.p[i] = make_float2(v[2 * i], v[2 * i + 1]);
+  }
+  return u;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_unit(T* p, const Unit<T, V>& u) {
+  if constexpr (V == 1) {
+    from_f32(u.p[0], p);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(u.p[0].x, u.p[0].y, u.p[1].x, u.p[1].y);
+  } else {
+    T* type = nullptr;
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(type, u.p[0].x, u.p[0].y), pack2(type, u.p[1].x, u.p[1].y),
+                                              pack2(type, u.p[2].x, u.p[2].y), pack2(type, u.p[3].x, u.p[3].y));
+  }
+}
+
 // V consecutive parameters as fp32.
 template <typename T, int V>
-__device__ __forceinline__ void param(const void* p, int f32, int i, float (&v)[V]) {
-  if (f32) {
-    const float* s = static_cast<const float*>(p) + i;
-    if constexpr (V >= 4) {
-#pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const float4 w = __ldcg(reinterpret_cast<const float4*>(s + j));
-        v[j] = w.x;
-        v[j + 1] = w.y;
-        v[j + 2] = w.z;
-        v[j + 3] = w.w;
-      }
-    } else {
-      v[0] = __ldcg(s);
-    }
+__device__ __forceinline__ Unit<T, V> param(const void* p, int f32, int i) {
+  if (!f32) return unit_of(load_pack<T, V>(static_cast<const T*>(p) + i));
+  const float* s = static_cast<const float*>(p) + i;
+  Unit<T, V> u;
+  if constexpr (V == 1) {
+    u.p[0] = __ldcg(s);
   } else {
-    unpack(load_pack<T, V>(static_cast<const T*>(p) + i), v);
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+      const float4 w = __ldcg(reinterpret_cast<const float4*>(s + 4 * j));
+      u.p[2 * j] = make_float2(w.x, w.y);
+      u.p[2 * j + 1] = make_float2(w.z, w.w);
+    }
   }
+  return u;
 }
 
 // Parameters in shared memory as fp32: unit i's values in V / 4 planes of float4, so that a warp's
 // 16-byte reads are next to each other (V = 1: plain).
-template <int V>
-__device__ __forceinline__ void put_param(float* s, int n, int i, const float (&v)[V]) {
+template <typename T, int V>
+__device__ __forceinline__ void put_param(float* s, int n, int i, const Unit<T, V>& u) {
   if constexpr (V == 1) {
-    s[i] = v[0];
+    s[i] = u.p[0];
   } else {
 #pragma unroll
     for (int p = 0; p < V / 4; ++p)
       reinterpret_cast<float4*>(s)[p * n + i] =
-          make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+          make_float4(u.p[2 * p].x, u.p[2 * p].y, u.p[2 * p + 1].x, u.p[2 * p + 1].y);
   }
 }
-template <int V>
-__device__ __forceinline__ void get_param(const float* s, int n, int i, float (&v)[V]) {
+template <typename T, int V>
+__device__ __forceinline__ Unit<T, V> get_param(const float* s, int n, int i) {
+  Unit<T, V> u;
   if constexpr (V == 1) {
-    v[0] = s[i];
+    u.p[0] = s[i];
   } else {
 #pragma unroll
     for (int p = 0; p < V / 4; ++p) {
       const float4 w = reinterpret_cast<const float4*>(s)[p * n + i];
-      v[4 * p] = w.x;
-      v[4 * p + 1] = w.y;
-      v[4 * p + 2] = w.z;
-      v[4 * p + 3] = w.w;
+      u.p[2 * p] = make_float2(w.x, w.y);
+      u.p[2 * p + 1] = make_float2(w.z, w.w);
     }
   }
+  return u;
+}
+
+// Blocks per SM that the forward kernel's registers are to leave room for: 128 per thread with 32 values, else
+// 80. Fewer threads with more values each are better than the reverse, since a warp's sums and barrier cost
+// as much as the arithmetic of 16 values: 3000 x 7168 took 49 us with 512 threads per row.
+constexpr int ln_blocks(int G, int values) {
+  const int threads = G == 32 ? 256 : G;
+  const int most = (values > 16 ? 512 : 768) / threads;
+  return most < 1 ? 1 : most;
 }
 
 // ------------------------------------------------------------------ forward
-// T: element type. V: elements per unit (a 16-byte granule, or 1 where rows are not on 16-byte
-// boundaries). A thread has U = 32 / V units, G threads apart. WARP: a row per warp (G = 32), eight
-// warps per block; else a row per block of G threads. SP: the parameters are kept in shared memory for
-// the block's rows, else read where they are used (few rows per block).
-template <typename T, int V, bool WARP, bool SP>
-__global__ void __launch_bounds__(WARP ? 256 : 512) k_layer_norm(const LnArgs a) {
-  constexpr int U = 32 / V;
-  // 16-bit rows: the next row's loads are under way while this one is worked on
-  constexpr bool AHEAD = V == 8;
+// G threads share a row, U units each, G apart: a warp per row (G = 32, eight warps per block), or a block.
+// Both are known to the compiler, so that a thread's units are at fixed distances: with the block size left
+// open the kernel took 29 instructions per element, most of them addresses, and 8192 x 7168 172 us. SP: the
+// parameters are kept in shared memory for the block's rows, else read where they are used (few rows per
+// block).
+template <typename T, int V, int U, int G, bool SP>
+__global__ void __launch_bounds__(G == 32 ? 256 : G, ln_blocks(G, U * V))
+    k_layer_norm(const LnArgs a) {
+  constexpr bool WARP = G == 32, AHEAD = V > 1;
+  constexpr int WARPS = WARP ? 1 : G / 32;  // that share a row
+  using Un = Unit<T, V>;
+  using P = typename Un::P;
   extern __shared__ float4 ln_smem[];
   float* sw = reinterpret_cast<float*>(ln_smem);
   float* sb = sw + a.H;
-  __shared__ float2 part[2][16];
-  __shared__ float count[16], inv_count[16];
+  __shared__ float2 part[2][32];
+  __shared__ float2 count[32];
   pdl_begin_in_order();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int G = WARP ? 32 : static_cast<int>(blockDim.x);
   const int g = WARP ? lane : static_cast<int>(threadIdx.x);
   const int n = a.H / V;
-  const T* x = static_cast<const T*>(a.x);
-  const T* f = static_cast<const T*>(a.f);
   const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? 8 : 1);
   int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
+  const int64_t at = row * a.H + g * V, by = step * a.H;
+  const T* x = static_cast<const T*>(a.x) + at;
+  const T* f = a.f ? static_cast<const T*>(a.f) + at : nullptr;
+  T* h = a.h ? static_cast<T*>(a.h) + at : nullptr;
+  T* yo = a.y ? static_cast<T*>(a.y) + at : nullptr;
 
-  Pack<T, V> nx[AHEAD ? U : 1], nf[AHEAD ? U : 1];
-  const auto fetch = [&](int64_t r, int u) {
-    const int i = u * G + g;
-    if (r < a.T && i < n) {
-      const int64_t at = r * a.H + static_cast<int64_t>(i) * V;
-      nx[AHEAD ? u : 0] = load_pack<T, V>(x + at);
-      if (f) nf[AHEAD ? u : 0] = load_pack<T, V>(f + at);
+  Pack<T, V> nx[U], nf[U];
+  const auto fetch = [&](int64_t r) {
+    if (r >= a.T) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u * G + g < n) nx[u] = load_pack<T, V>(x + u * G * V);
+    x += by;
+    if (f) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u * G + g < n) nf[u] = load_pack<T, V>(f + u * G * V);
+      f += by;
     }
   };
-  if constexpr (AHEAD) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) fetch(row, u);
-  }
+  if constexpr (AHEAD) fetch(row);
 
-  if (SP) {
+  if constexpr (SP) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      float v[V];
-      if (a.w) {
-        param<T, V>(a.w, a.w_f32, i * V, v);
-        put_param<V>(sw, n, i, v);
-      }
-      if (a.b) {
-        param<T, V>(a.b, a.b_f32, i * V, v);
-        put_param<V>(sb, n, i, v);
-      }
+      if (a.w) put_param(sw, n, i, param<T, V>(a.w, a.w_f32, i * V));
+      if (a.b) put_param(sb, n, i, param<T, V>(a.b, a.b_f32, i * V));
     }
   }
-  // elements of this row that this warp has
+  // elements of a row that this warp has
   int mine = 0;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int first = u * G + (WARP ? 0 : warp * 32);
-    mine += max(0, min(32, n - first)) * V;
-  }
+  for (int u = 0; u < U; ++u) mine += max(0, min(32, n - u * G - (WARP ? 0 : warp * 32))) * V;
   const float own = static_cast<float>(mine > 0 ? mine : 1), cols = static_cast<float>(a.H);
-  if (!WARP && lane == 0) {
-    count[warp] = static_cast<float>(mine);
-    inv_count[warp] = mine > 0 ? 1.0f / own : 0.0f;
-  }
+  const float own_inv = mine > 0 ? 1.0f / own : 0.0f;
+  if (!WARP && lane == 0) count[warp] = make_float2(static_cast<float>(mine), own_inv);
   if (SP || !WARP) __syncthreads();
-  const float inv_h = 1.0f / static_cast<float>(a.H);
+  const float inv_h = 1.0f / cols;
 
   for (int flip = 0; row < a.T; row += step, flip ^= 1) {
-    float v[U][V];
-    float sum = 0.0f;
-    T* hr = static_cast<T*>(a.h) + row * a.H;
+    if constexpr (!AHEAD) fetch(row);
+    Un v[U];
+    P two = all<P>(0.0f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = u * G + g;
-      if constexpr (!AHEAD) fetch(row, u);
-      if (i < n) {
-        unpack(nx[AHEAD ? u : 0], v[u]);
-        if (f) {
-          float w[V];
-          unpack(nf[AHEAD ? u : 0], w);
+      if (u * G + g < n) {
+        v[u] = unit_of(nx[u]);
+        if (a.f) {
+          const Un w = unit_of(nf[u]);
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[u][j] += w[j];
+          for (int j = 0; j < Un::N; ++j) v[u].p[j] = add(v[u].p[j], w.p[j]);
         }
-        if (a.h) store_pack(hr + static_cast<int64_t>(i) * V, v[u]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum += v[u][j];
       }
     }
-    if constexpr (AHEAD) {
+    if constexpr (AHEAD) fetch(row + step);
+    if (h) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) fetch(row + step, u);
+      for (int u = 0; u < U; ++u)
+        if (u * G + g < n) store_unit(h + u * G * V, v[u]);
+      h += by;
     }
-    // the warp's own mean and squared deviations first, then all warps' joined: one barrier a row
-    sum = warp_sum_f32(sum);
-    // divided, not multiplied with a rounded 1 / H: equal values whose sum is exact are their mean
-    float mean = __fdiv_rn(sum, own);
-    float dev = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u * G + g < n) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = v[u][j] - mean;
-          dev = fmaf(d, d, dev);
+        for (int j = 0; j < Un::N; ++j) two = add(two, v[u].p[j]);
+      }
+    }
+    // the warp's own mean and squared deviations first, then all warps' joined: one barrier a row
+    const float sum = warp_sum_f32(total(two));
+    // the mean is divided, not multiplied with a rounded 1 / H: equal values whose sum is exact are their mean
+    float mean = WARP ? __fdiv_rn(sum, own) : sum * own_inv;
+    two = all<P>(0.0f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u * G + g < n) {
+#pragma unroll
+        for (int j = 0; j < Un::N; ++j) {
+          const P d = add(v[u].p[j], all<P>(-mean));
+          two = mad(d, d, two);
         }
       }
     }
-    dev = warp_sum_f32(dev);
-    if (!WARP) {
+    float dev = warp_sum_f32(total(two));
+    if constexpr (!WARP) {
       if (lane == 0) part[flip][warp] = make_float2(sum, dev);
       __syncthreads();
-      const int warps = G >> 5;
-      float total = 0.0f;
-      for (int i = 0; i < warps; ++i) total += part[flip][i].x;
-      mean = __fdiv_rn(total, cols);
-      dev = 0.0f;
-      for (int i = 0; i < warps; ++i) {
-        const float2 p = part[flip][i];
-        const float d = p.x * inv_count[i] - mean;
-        dev += fmaf(d * d, count[i], p.y);
-      }
+      // a lane per warp (all of them unrolled took too many registers)
+      const float2 p = lane < WARPS ? part[flip][lane] : make_float2(0.0f, 0.0f);
+      mean = __fdiv_rn(warp_sum_f32(p.x), cols);
+      const float2 c = lane < WARPS ? count[lane] : make_float2(0.0f, 0.0f);
+      const float d = p.x * c.y - mean;
+      dev = warp_sum_f32(fmaf(d * d, c.x, p.y));
     }
     const float r = rsqrtf(fmaf(dev, inv_h, a.eps));
     if (a.stats && g == 0) reinterpret_cast<float2*>(a.stats)[row] = make_float2(mean, r);
-    if (!a.y && !a.q) continue;
-    T* yr = static_cast<T*>(a.y) + row * a.H;
+    if (!yo && !a.q) continue;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = u * G + g;
       const bool in = i < n;
-      float y[V];
+      Un y;
+      if (in) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = in ? (v[u][j] - mean) * r : 0.0f;
-      if (in && a.w) {
-        float w[V];
-        if constexpr (SP)
-          get_param<V>(sw, n, i, w);
-        else
-          param<T, V>(a.w, a.w_f32, i * V, w);
+        for (int j = 0; j < Un::N; ++j) y.p[j] = mul(add(v[u].p[j], all<P>(-mean)), all<P>(r));
+        if (a.w) {
+          const Un w = SP ? get_param<T, V>(sw, n, i) : param<T, V>(a.w, a.w_f32, i * V);
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[j] *= w[j];
+          for (int j = 0; j < Un::N; ++j) y.p[j] = mul(y.p[j], w.p[j]);
+        }
+        if (a.b) {
+          const Un b = SP ? get_param<T, V>(sb, n, i) : param<T, V>(a.b, a.b_f32, i * V);
+#pragma unroll
+          for (int j = 0; j < Un::N; ++j) y.p[j] = add(y.p[j], b.p[j]);
+        }
+        if (yo) store_unit(yo + u * G * V, y);
       }
-      if (in && a.b) {
-        float w[V];
-        if constexpr (SP)
-          get_param<V>(sb, n, i, w);
-        else
-          param<T, V>(a.b, a.b_f32, i * V, w);
+      if constexpr (V > 1) {
+        if (a.q) {
+          // 128 columns are the units of 128 / V neighbouring lanes, which are inside the row or
+          // outside together (H is a multiple of 128)
+          float m = 0.0f;
+          if (in) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[j] += w[j];
-      }
-      if (a.y) {
-        if (in) store_pack(yr + static_cast<int64_t>(i) * V, y);
-      } else if constexpr (V > 1) {
-        // 128 columns are the units of 128 / V neighbouring lanes, which are inside the row or
-        // outside together (H is a multiple of 128)
-        float m = 0.0f;
+            for (int j = 0; j < Un::N; ++j) m = fmaxf(m, fmaxf(fabsf(y.p[j].x), fabsf(y.p[j].y)));
+          }
 #pragma unroll
-        for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(y[j]));
+          for (int o = 64 / V; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (in) {
+            const float scale = __fdiv_rn(fmaxf(m, 1e-30f), 448.0f);
+            uint32_t w[V / 4];
 #pragma unroll
-        for (int o = 64 / V; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (in) {
-          const float scale = __fdiv_rn(fmaxf(m, 1e-30f), 448.0f);
-          uint32_t w[V / 4];
-#pragma unroll
-          for (int j = 0; j < V; j += 4)
-            w[j / 4] = static_cast<uint32_t>(pack_e4m3x2(__fdiv_rn(y[j], scale),
-                                                         __fdiv_rn(y[j + 1], scale))) |
-                       static_cast<uint32_t>(pack_e4m3x2(__fdiv_rn(y[j + 2], scale),
-                                                         __fdiv_rn(y[j + 3], scale)))
-                           << 16;
-          uint8_t* q = a.q + row * a.H + static_cast<int64_t>(i) * V;
-          if constexpr (V == 8)
-            *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
-          else
-            *reinterpret_cast<uint32_t*>(q) = w[0];
-          if (i % (128 / V) == 0) a.q_scale[static_cast<int64_t>(i / (128 / V)) * a.T + row] = scale;
+            for (int j = 0; j < V / 4; ++j) {
+              const float2 lo = y.p[2 * j], hi = y.p[2 * j + 1];
+              w[j] = static_cast<uint32_t>(pack_e4m3x2(__fdiv_rn(lo.x, scale), __fdiv_rn(lo.y, scale))) |
+                     static_cast<uint32_t>(pack_e4m3x2(__fdiv_rn(hi.x, scale), __fdiv_rn(hi.y, scale)))
+                         << 16;
+            }
+            uint8_t* q = a.q + row * a.H + i * V;
+            if constexpr (V == 8)
+              *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+            else
+              *reinterpret_cast<uint32_t*>(q) = w[0];
+            if (i % (128 / V) == 0) a.q_scale[static_cast<int64_t>(i / (128 / V)) * a.T + row] = scale;
+          }
         }
       }
     }
+    if (yo) yo += by;
   }
 }
 
 // ------------------------------------------------------------------ backward
-// NV values per thread. WIDE (rows of more than 8192 columns): 32 values per thread, and the sums over
-// rows, each thread's own, in shared memory since the registers do not hold them.
-template <typename T, int V, int NV, bool WARP, bool WIDE>
-__global__ void __launch_bounds__(WARP ? 256 : 512) k_layer_norm_back(const LnArgs a) {
-  constexpr int U = NV / V;
-  constexpr bool AHEAD = V == 8 && !WIDE;
+// As above, a row's inputs loaded one row ahead where a thread has no more than 16 values. The sums over rows are in registers, or (WIDE, more than 16 values per thread) in shared memory, each
+// thread's own.
+template <typename T, int V, int U, int G, bool WIDE>
+__global__ void __launch_bounds__(G == 32 ? 256 : G, 1) k_layer_norm_back(const LnArgs a) {
+  constexpr bool WARP = G == 32, AHEAD = V > 1 && !WIDE;
+  constexpr int WARPS = WARP ? 1 : G / 32;
+  using Un = Unit<T, V>;
+  using P = typename Un::P;
+  constexpr int N = Un::N;
   extern __shared__ float4 ln_smem[];
-  float* acc = reinterpret_cast<float*>(ln_smem);  // WIDE: [2][NV][G]; WARP, at the end: [8][2][H]
+  float* sw = reinterpret_cast<float*>(ln_smem);   // weight [H]
+  P* acc = reinterpret_cast<P*>(sw + (a.H + 3) / 4 * 4);  // WIDE: [2][U * N][G]
+  float* rows = sw;                                // WARP, at the end: [8][2][H]
   __shared__ float2 part[2][16];
   pdl_begin_in_order();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int G = WARP ? 32 : static_cast<int>(blockDim.x);
   const int g = WARP ? lane : static_cast<int>(threadIdx.x);
   const int n = a.H / V;
-  const T *x = static_cast<const T*>(a.x), *f = static_cast<const T*>(a.f);
-  const T *dh = static_cast<const T*>(a.dh), *dy = static_cast<const T*>(a.dy);
   const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? 8 : 1);
   int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
+  const int64_t at = row * a.H + g * V, by = step * a.H;
+  const bool dy_in = a.dy != nullptr, f_in = dy_in && a.f != nullptr;
+  const T* x = static_cast<const T*>(a.x) + at;
+  const T* f = f_in ? static_cast<const T*>(a.f) + at : nullptr;
+  const T* dy = dy_in ? static_cast<const T*>(a.dy) + at : nullptr;
+  const T* dh = a.dh ? static_cast<const T*>(a.dh) + at : nullptr;
+  T* dx = a.dx ? static_cast<T*>(a.dx) + at : nullptr;
   const float inv_h = 1.0f / static_cast<float>(a.H);
 
-  constexpr int R = AHEAD ? U : 1;
-  Pack<T, V> nx[R], nf[R], ny[R], nh[U];
-  float2 nstat = make_float2(0.0f, 0.0f);
-  const auto fetch_stat = [&](int64_t r) {
-    if (r < a.T) nstat = __ldcg(reinterpret_cast<const float2*>(a.stats) + r);
-  };
-  const auto fetch = [&](int64_t r, int u) {
-    const int i = u * G + g, b = AHEAD ? u : 0;
-    if (r < a.T && i < n) {
-      const int64_t at = r * a.H + static_cast<int64_t>(i) * V;
-      if (dy) {
-        nx[b] = load_pack<T, V>(x + at);
-        if (f) nf[b] = load_pack<T, V>(f + at);
-        ny[b] = load_pack<T, V>(dy + at);
-      }
-      if (dh) nh[u] = load_pack<T, V>(dh + at);
+  struct Row {
+    Pack<T, V> x[U], f[U], dy[U];
+    float2 stat;
+  } next;
+  const auto fetch = [&](int64_t r) {
+    if (r >= a.T) return;
+    next.stat = __ldcg(reinterpret_cast<const float2*>(a.stats) + r);
+    if (dy_in) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u * G + g < n) next.x[u] = load_pack<T, V>(x + u * G * V);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u * G + g < n) next.dy[u] = load_pack<T, V>(dy + u * G * V);
+      x += by;
+      dy += by;
+    }
+    if (f) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u * G + g < n) next.f[u] = load_pack<T, V>(f + u * G * V);
+      f += by;
     }
   };
-  if constexpr (AHEAD) {
-    fetch_stat(row);
-#pragma unroll
-    for (int u = 0; u < U; ++u) fetch(row, u);
-  }
+  if constexpr (AHEAD) fetch(row);
 
-  float w[WIDE ? 1 : U][V], aw[WIDE ? 1 : U][V], ab[WIDE ? 1 : U][V];
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    Un one;
+#pragma unroll
+    for (int j = 0; j < N; ++j) one.p[j] = all<P>(1.0f);
+    put_param(sw, n, i, a.w ? param<T, V>(a.w, a.w_f32, i * V) : one);
+  }
+  Un aw[WIDE ? 1 : U], ab[WIDE ? 1 : U];
   if constexpr (WIDE) {
-    for (int i = threadIdx.x; i < 2 * NV * G; i += G) acc[i] = 0.0f;
+    for (int i = threadIdx.x; i < 2 * U * N * G; i += G) acc[i] = all<P>(0.0f);
   } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        w[u][j] = 1.0f;
-        aw[u][j] = ab[u][j] = 0.0f;
-      }
-      if (a.w && u * G + g < n) param<T, V>(a.w, a.w_f32, (u * G + g) * V, w[u]);
-    }
+      for (int j = 0; j < N; ++j) aw[u].p[j] = ab[u].p[j] = all<P>(0.0f);
   }
+  __syncthreads();
 
   for (int flip = 0; row < a.T; row += step, flip ^= 1) {
-    if constexpr (!AHEAD) fetch_stat(row);
-    const float mean = nstat.x, r = nstat.y;
-    float v[U][V], d[U][V];  // n, and dy and then u
+    if constexpr (!AHEAD) fetch(row);
+    const float mean = next.stat.x, r = next.stat.y;
+    Un v[U], d[U];  // n, and dy and then u
     Pack<T, V> ph[U];
-    float s1 = 0.0f, s2 = 0.0f;
+    P t1 = all<P>(0.0f), t2 = t1;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = u * G + g, b = AHEAD ? u : 0;
-      if constexpr (!AHEAD) fetch(row, u);
+      if (dh && u * G + g < n) ph[u] = load_pack<T, V>(dh + u * G * V);
+      if (dy_in && u * G + g < n) {
+        v[u] = unit_of(next.x[u]);
+        if (f_in) {
+          const Un t = unit_of(next.f[u]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[u][j] = d[u][j] = 0.0f;
-      if (i < n) {
-        if (dy) {
-          unpack(nx[b], v[u]);
-          if (f) {
-            float t[V];
-            unpack(nf[b], t);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[u][j] += t[j];
-          }
-          unpack(ny[b], d[u]);
-          float wt[V];
-          if constexpr (WIDE) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) wt[j] = 1.0f;
-            if (a.w) param<T, V>(a.w, a.w_f32, i * V, wt);
-          }
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            v[u][j] = (v[u][j] - mean) * r;
-            if constexpr (WIDE) {
-              float* mine = acc + (u * V + j) * G + g;
-              *mine = fmaf(d[u][j], v[u][j], *mine);
-              mine[NV * G] += d[u][j];
-              d[u][j] *= wt[j];
-            } else {
-              aw[u][j] = fmaf(d[u][j], v[u][j], aw[u][j]);
-              ab[u][j] += d[u][j];
-              d[u][j] *= w[u][j];
-            }
-            s1 += d[u][j];
-            s2 = fmaf(d[u][j], v[u][j], s2);
-          }
+          for (int j = 0; j < N; ++j) v[u].p[j] = add(v[u].p[j], t.p[j]);
         }
-        if (dh) ph[u] = nh[u];
+        d[u] = unit_of(next.dy[u]);
       }
     }
-    if constexpr (AHEAD) {
-      fetch_stat(row + step);
+    if (dh) dh += by;
+    if constexpr (AHEAD) fetch(row + step);
 #pragma unroll
-      for (int u = 0; u < U; ++u) fetch(row + step, u);
+    for (int u = 0; u < U; ++u) {
+      if (dy_in && u * G + g < n) {
+        const Un w = get_param<T, V>(sw, n, u * G + g);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          v[u].p[j] = mul(add(v[u].p[j], all<P>(-mean)), all<P>(r));
+          if constexpr (WIDE) {
+            P* m = acc + (u * N + j) * G + g;
+            m[0] = mad(d[u].p[j], v[u].p[j], m[0]);
+            m[U * N * G] = add(d[u].p[j], m[U * N * G]);
+          } else {
+            aw[u].p[j] = mad(d[u].p[j], v[u].p[j], aw[u].p[j]);
+            ab[u].p[j] = add(d[u].p[j], ab[u].p[j]);
+          }
+          d[u].p[j] = mul(d[u].p[j], w.p[j]);
+          t1 = add(t1, d[u].p[j]);
+          t2 = mad(d[u].p[j], v[u].p[j], t2);
+        }
+      }
     }
-    if (!a.dx) continue;
-    s1 = warp_sum_f32(s1);
-    s2 = warp_sum_f32(s2);
-    if (!WARP) {
+    if (!dx) continue;
+    float s1 = warp_sum_f32(total(t1));
+    float s2 = warp_sum_f32(total(t2));
+    if constexpr (!WARP) {
       if (lane == 0) part[flip][warp] = make_float2(s1, s2);
       __syncthreads();
-      s1 = s2 = 0.0f;
-      for (int i = 0; i < (G >> 5); ++i) {
-        const float2 p = part[flip][i];
-        s1 += p.x;
-        s2 += p.y;
-      }
+      const float2 p = lane < WARPS ? part[flip][lane] : make_float2(0.0f, 0.0f);
+      s1 = warp_sum_f32(p.x);
+      s2 = warp_sum_f32(p.y);
     }
     s1 *= inv_h;
     s2 *= inv_h;
-    T* out = static_cast<T*>(a.dx) + row * a.H;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = u * G + g;
-      if (i < n) {
-        float o[V];
+      if (u * G + g < n) {
+        Un o;
+        if (dy_in) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = r * (d[u][j] - fmaf(v[u][j], s2, s1));
-        if (!dy) {  // r may be infinite
+          for (int j = 0; j < N; ++j) {
+            const P m = mad(v[u].p[j], all<P>(-s2), add(d[u].p[j], all<P>(-s1)));
+            o.p[j] = mul(m, all<P>(r));
+          }
+        } else {
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] = 0.0f;
+          for (int j = 0; j < N; ++j) o.p[j] = all<P>(0.0f);
         }
         if (dh) {
-          float t[V];
-          unpack(ph[u], t);
+          const Un t = unit_of(ph[u]);
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] += t[j];
+          for (int j = 0; j < N; ++j) o.p[j] = add(o.p[j], t.p[j]);
         }
-        store_pack(out + static_cast<int64_t>(i) * V, o);
+        store_unit(dx + u * G * V, o);
       }
     }
+    dx += by;
   }
 
   if (!a.want_w && !a.want_b) return;
   float* pw = a.part + static_cast<int64_t>(blockIdx.x) * a.H;
   float* pb = pw + static_cast<int64_t>(gridDim.x) * a.H;
+  const auto put = [&](float* to, const P& p, int j) { *reinterpret_cast<P*>(to + 2 * j) = p; };
   if constexpr (WARP) {
-    float* mine = acc + warp * 2 * a.H;
+    __syncthreads();  // the weights are no longer read
+    float* own = rows + warp * 2 * a.H;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = u * G + g;
       if (i < n) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          mine[i * V + j] = aw[u][j];
-          mine[a.H + i * V + j] = ab[u][j];
+        for (int j = 0; j < N; ++j) {
+          put(own + i * V, aw[u].p[j], j);
+          put(own + a.H + i * V, ab[u].p[j], j);
         }
       }
     }
@@ -442,7 +495,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) k_layer_norm_back(const LnAr
     for (int c = threadIdx.x; c < 2 * a.H; c += blockDim.x) {
       float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += acc[i * 2 * a.H + c];
+      for (int i = 0; i < 8; ++i) s += rows[i * 2 * a.H + c];
       if (c < a.H)
         pw[c] = s;
       else
@@ -454,61 +507,74 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) k_layer_norm_back(const LnAr
       const int i = u * G + g;
       if (i < n) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if constexpr (WIDE) {
-            pw[i * V + j] = acc[(u * V + j) * G + g];
-            pb[i * V + j] = acc[(NV + u * V + j) * G + g];
-          } else {
-            pw[i * V + j] = aw[u][j];
-            pb[i * V + j] = ab[u][j];
-          }
+        for (int j = 0; j < N; ++j) {
+          put(pw + i * V, WIDE ? acc[(u * N + j) * G + g] : aw[WIDE ? 0 : u].p[j], j);
+          put(pb + i * V, WIDE ? acc[(U * N + u * N + j) * G + g] : ab[WIDE ? 0 : u].p[j], j);
         }
       }
     }
   }
 }
 
-// The blocks' shares of d weight (blockIdx.y 0) and d bias (1), added in a fixed order: 32 columns per
-// block, eight threads per column.
-template <typename T>
+// The blocks' shares of d weight (blockIdx.y 0) and d bias (1), added in a fixed order: 32 columns per block,
+// V of them per thread, 8 V threads per column, so that with V = 4 the usual 148 shares are one batch of
+// loads per thread.
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
     k_layer_norm_sums(const float* part, int blocks, int H, void* dw, void* db, int w_f32, int b_f32) {
   pdl_begin_in_order();
-  __shared__ float buf[8][33];
+  constexpr int ROWS = 8 * V;  // threads per column
+  __shared__ float buf[ROWS][33];
   void* out = blockIdx.y ? db : dw;
   if (!out) return;
   const int f32 = blockIdx.y ? b_f32 : w_f32;
-  const int c = blockIdx.x * 32 + threadIdx.x;
+  const int x = threadIdx.x % (32 / V) * V, y = threadIdx.x / (32 / V);
+  const int c = blockIdx.x * 32 + x;
   const float* p = part + static_cast<int64_t>(blockIdx.y) * blocks * H;
-  float sum = 0.0f;
-  if (c < H) {
-    for (int b0 = threadIdx.y; b0 < blocks; b0 += 64) {
-      float v[8];
+  float sum[V] = {};
+  if (c < H) {  // H is a multiple of V
+    for (int b0 = y; b0 < blocks; b0 += ROWS * 5) {
+      float v[5][V];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = b0 + 8 * i < blocks ? __ldcg(p + static_cast<int64_t>(b0 + 8 * i) * H + c) : 0.0f;
+      for (int i = 0; i < 5; ++i) {
+        const float* s = p + static_cast<int64_t>(b0 + ROWS * i) * H + c;
+        const bool in = b0 + ROWS * i < blocks;
+        if constexpr (V == 4) {
+          const float4 w = in ? __ldcg(reinterpret_cast<const float4*>(s)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[i][0] = w.x;
+          v[i][1] = w.y;
+          v[i][2] = w.z;
+          v[i][3] = w.w;
+        } else {
+          v[i][0] = in ? __ldcg(s) : 0.0f;
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += v[i];
+      for (int i = 0; i < 5; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) sum[k] += v[i][k];
     }
   }
-  buf[threadIdx.y][threadIdx.x] = sum;
+#pragma unroll
+  for (int k = 0; k < V; ++k) buf[y][x + k] = sum[k];
   __syncthreads();
-  if (threadIdx.y == 0 && c < H) {
-    for (int i = 1; i < 8; ++i) sum += buf[i][threadIdx.x];
+  if (threadIdx.x < 32 && blockIdx.x * 32 + threadIdx.x < H) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) s += buf[i][threadIdx.x];
+    const int col = blockIdx.x * 32 + threadIdx.x;
     if (f32)
-      static_cast<float*>(out)[c] = sum;
+      static_cast<float*>(out)[col] = s;
     else
-      from_f32(sum, static_cast<T*>(out) + c);
+      from_f32(s, static_cast<T*>(out) + col);
   }
 }
 
 // ------------------------------------------------------------------ launches
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-constexpr int kLnMaxSmem = 2 * 16384 * 4;  // two fp32 parameters, or the sums, of the longest row
-
-// Threads of a block that hold a row of n units, `units` per thread.
-int threads_for(int n, int units) { return ((n + units - 1) / units + 31) / 32 * 32; }
+// two fp32 parameters of the longest row; the weight and two sums
+constexpr int kLnMaxSmem = 3 * 16384 * 4;
 
 template <typename K>
 cudaError_t allow_smem(K kernel, std::atomic<bool> (&done)[64]) {
@@ -546,65 +612,90 @@ LnArgs args_of(const LayerNorm& p) {
   return a;
 }
 
-template <typename T, int V, bool WARP, bool SP>
-cudaError_t run_forward(const LnArgs& a, int threads, int64_t blocks, cudaStream_t s) {
+template <typename T, int V, int U, int G, bool SP>
+cudaError_t run_forward(const LnArgs& a, int64_t blocks, cudaStream_t s) {
   static std::atomic<bool> done[64];
   const size_t smem = SP ? static_cast<size_t>(a.H) * 8 : 0;
   if (smem > 48 * 1024) {
-    const cudaError_t e = allow_smem(k_layer_norm<T, V, WARP, SP>, done);
+    const cudaError_t e = allow_smem(k_layer_norm<T, V, U, G, SP>, done);
     if (e != cudaSuccess) return e;
   }
-  return launch_pdl(k_layer_norm<T, V, WARP, SP>, dim3(static_cast<unsigned>(blocks)), dim3(threads),
-                    smem, s, a);
+  return launch_pdl(k_layer_norm<T, V, U, G, SP>, dim3(static_cast<unsigned>(blocks)),
+                    dim3(G == 32 ? 256 : G), smem, s, a);
 }
 
-template <typename T, int V>
+template <typename T, int V, int U, int G>
 cudaError_t forward(const LayerNorm& p, int sms, cudaStream_t s) {
-  if (V == 1 && p.q) return cudaErrorInvalidValue;  // the caller checks the alignment
   const LnArgs a = args_of(p);
-  const int n = p.H / V;
-  if (p.H <= 1024) {
-    const int64_t rows = (p.T + 7) / 8, most = static_cast<int64_t>(sms) * 3;
-    if (rows <= most) return run_forward<T, V, true, false>(a, 256, rows, s);
-    return run_forward<T, V, true, true>(a, 256, most, s);
-  }
-  const int threads = threads_for(n, 32 / V);
-  const int64_t most = static_cast<int64_t>(sms) * (threads <= 256 ? 3 : threads <= 320 ? 2 : 1);
-  if (p.T <= most) return run_forward<T, V, false, false>(a, threads, p.T, s);
-  return run_forward<T, V, false, true>(a, threads, most, s);
+  const int64_t blocks = G == 32 ? (p.T + 7) / 8 : p.T;
+  // what runs at a time; with shared parameters for more rows than that
+  const int64_t most = static_cast<int64_t>(sms) * ln_blocks(G, U * V);
+  if (blocks <= most) return run_forward<T, V, U, G, false>(a, blocks, s);
+  return run_forward<T, V, U, G, true>(a, most, s);
 }
 
-template <typename T, int V, int NV, bool WARP, bool WIDE>
-cudaError_t run_backward(const LayerNorm& p, int threads, int64_t most, cudaStream_t s) {
+template <typename T, int V, int U, int G, bool WIDE>
+cudaError_t backward(const LayerNorm& p, int sms, cudaStream_t s) {
   static std::atomic<bool> done[64];
   const LnArgs a = args_of(p);
-  const size_t smem = WIDE ? static_cast<size_t>(2) * NV * threads * 4
-                      : WARP ? static_cast<size_t>(8) * 2 * p.H * 4 : 0;
+  size_t smem = (static_cast<size_t>(p.H) + 3) / 4 * 16;
+  if (WIDE) smem += sizeof(typename Unit<T, V>::P) * 2 * U * Unit<T, V>::N * G;
+  if (G == 32) smem = static_cast<size_t>(8) * 2 * p.H * 4;
   if (smem > 48 * 1024) {
-    const cudaError_t e = allow_smem(k_layer_norm_back<T, V, NV, WARP, WIDE>, done);
+    const cudaError_t e = allow_smem(k_layer_norm_back<T, V, U, G, WIDE>, done);
     if (e != cudaSuccess) return e;
   }
-  int64_t blocks = WARP ? (p.T + 7) / 8 : p.T;
+  int64_t blocks = G == 32 ? (p.T + 7) / 8 : p.T;
+  const int64_t most = static_cast<int64_t>(sms) * (G == 512 ? 1 : 2);
   if (blocks > most) blocks = most;
   if (blocks > kMaxLnBlocks) blocks = kMaxLnBlocks;
-  cudaError_t e = launch_pdl(k_layer_norm_back<T, V, NV, WARP, WIDE>,
-                             dim3(static_cast<unsigned>(blocks)), dim3(threads), smem, s, a);
+  cudaError_t e = launch_pdl(k_layer_norm_back<T, V, U, G, WIDE>, dim3(static_cast<unsigned>(blocks)),
+                             dim3(G == 32 ? 256 : G), smem, s, a);
   if (e != cudaSuccess || (!p.dw && !p.db)) return e;
-  return launch_pdl(k_layer_norm_sums<T>, dim3((p.H + 31) / 32, 2), dim3(32, 8), 0, s,
-                    static_cast<const float*>(p.part), static_cast<int>(blocks), p.H, p.dw, p.db,
-                    a.w_f32, a.b_f32);
+  const auto sums = p.H % 4 == 0 && on16(p.part) ? k_layer_norm_sums<T, 4> : k_layer_norm_sums<T, 1>;
+  return launch_pdl(sums, dim3((p.H + 31) / 32, 2), dim3(256), 0, s, static_cast<const float*>(p.part),
+                    static_cast<int>(blocks), p.H, p.dw, p.db, a.w_f32, a.b_f32);
 }
 
+// The smallest variant that holds a row of n units.
 template <typename T, int V>
-cudaError_t backward(const LayerNorm& p, int sms, cudaStream_t s) {
+cudaError_t sized(const LayerNorm& p, int sms, cudaStream_t s) {
   const int n = p.H / V;
-  if (p.H <= 512) return run_backward<T, V, 16, true, false>(p, 256, 2 * sms, s);
-  if (p.H <= 8192) {
-    const int threads = threads_for(n, 16 / V);
-    return run_backward<T, V, 16, false, false>(p, threads, sms * (threads > 256 ? 1 : 512 / threads),
-                                                s);
+  constexpr int A = V == 8 ? 1 : 2;  // of fp32, twice the units are as many values per thread
+  if constexpr (V > 1) {
+    if (p.back) {
+      if (n <= 32 * A) return backward<T, V, A, 32, false>(p, sms, s);
+      if (n <= 64 * A) return backward<T, V, 2 * A, 32, false>(p, sms, s);
+      if (n <= 256 * A) return backward<T, V, A, 256, false>(p, sms, s);
+      if (n <= 512 * A) return backward<T, V, 2 * A, 256, false>(p, sms, s);
+      if (n <= 1024 * A) return backward<T, V, 2 * A, 512, false>(p, sms, s);
+      return backward<T, V, 4 * A, 512, true>(p, sms, s);
+    }
+    if (n <= 32 * A) return forward<T, V, A, 32>(p, sms, s);
+    if (n <= 64 * A) return forward<T, V, 2 * A, 32>(p, sms, s);
+    if (n <= 128 * A) return forward<T, V, 4 * A, 32>(p, sms, s);
+    if (n <= 256 * A) return forward<T, V, 2 * A, 128>(p, sms, s);
+    if (n <= 512 * A) return forward<T, V, 4 * A, 128>(p, sms, s);
+    if (n <= 768 * A) return forward<T, V, 3 * A, 256>(p, sms, s);
+    if (n <= 1024 * A) return forward<T, V, 4 * A, 256>(p, sms, s);
+    return forward<T, V, 4 * A, 512>(p, sms, s);
+  } else {
+    if (p.back) {
+      if (n <= 128) return backward<T, 1, 4, 32, false>(p, sms, s);
+      if (n <= 1024) return backward<T, 1, 4, 256, false>(p, sms, s);
+      if (n <= 2048) return backward<T, 1, 8, 256, false>(p, sms, s);
+      if (n <= 4096) return backward<T, 1, 8, 512, false>(p, sms, s);
+      if (n <= 8192) return backward<T, 1, 16, 512, false>(p, sms, s);
+      return backward<T, 1, 32, 512, true>(p, sms, s);
+    }
+    if (p.q) return cudaErrorInvalidValue;  // the caller checks the alignment
+    if (n <= 128) return forward<T, 1, 4, 32>(p, sms, s);
+    if (n <= 1024) return forward<T, 1, 8, 128>(p, sms, s);
+    if (n <= 2048) return forward<T, 1, 16, 128>(p, sms, s);
+    if (n <= 4096) return forward<T, 1, 16, 256>(p, sms, s);
+    if (n <= 8192) return forward<T, 1, 32, 256>(p, sms, s);
+    return forward<T, 1, 32, 512>(p, sms, s);
   }
-  return run_backward<T, V, 32, false, true>(p, threads_for(n, 32 / V), sms, s);
 }
 
 template <typename T>
@@ -613,8 +704,7 @@ cudaError_t typed(const LayerNorm& p, int sms, cudaStream_t s) {
   for (const void* q : {p.f, p.x, p.w, p.b, p.dh, p.dy, static_cast<const void*>(p.h),
                         static_cast<const void*>(p.y), static_cast<const void*>(p.dx)})
     wide = wide && on16(q);
-  if (p.back) return wide ? backward<T, kV<T>>(p, sms, s) : backward<T, 1>(p, sms, s);
-  return wide ? forward<T, kV<T>>(p, sms, s) : forward<T, 1>(p, sms, s);
+  return wide ? sized<T, kV<T>>(p, sms, s) : sized<T, 1>(p, sms, s);
 }
 
 }  // namespace
