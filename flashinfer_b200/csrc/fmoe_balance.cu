@@ -21,10 +21,12 @@
 namespace fmoe {
 namespace {
 
-constexpr int kBalWarps = 8;
-constexpr int kBalThreads = kBalWarps * 32;
+// Warps of a block: what the registers of NV logits per lane leave room for, all on one SM. Few blocks have few
+// shares to join.
+constexpr int bal_warps(int NV) { return NV > 8 ? 16 : 32; }
+constexpr int kBackWarps = 8;     // of the backward pass
 constexpr int kBalCluster = 8;   // CTAs of the cluster that joins the shares
-constexpr int kBalMaxSmem = kBalWarps * kMaxBalanceExperts * 4 + kMaxBalanceExperts * 4 +
+constexpr int kBalMaxSmem = 16 * kMaxBalanceExperts * 4 + kMaxBalanceExperts * 4 +
                             (kMaxBalanceSequences + 1) * 4;
 
 struct BalArgs {
@@ -145,10 +147,11 @@ __device__ __forceinline__ float scores(float (&v)[NV], float (&slope)[SLOPE ? N
 // sequence s) is number b + s: along the rows either b or s goes up from one share to the next, so no
 // two have the same number.
 template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kBalThreads) k_balance(const BalArgs a) {
+__global__ void __launch_bounds__(bal_warps(NV) * 32) k_balance(const BalArgs a) {
+  constexpr int WARPS = bal_warps(NV), THREADS = WARPS * 32;
   extern __shared__ float bal_smem[];
-  float* sp = bal_smem;                                          // [kBalWarps][E]
-  int* sn = reinterpret_cast<int*>(sp + (a.logits ? kBalWarps * a.E : 0));  // [E]
+  float* sp = bal_smem;                                          // [WARPS][E]
+  int* sn = reinterpret_cast<int*>(sp + (a.logits ? WARPS * a.E : 0));  // [E]
   int* sbase = sn + a.E;                                                   // [S + 1]
   pdl_begin_in_order();
   load_bases(a, sbase);
@@ -159,10 +162,13 @@ __global__ void __launch_bounds__(kBalThreads) k_balance(const BalArgs a) {
     const int64_t b0 = max(static_cast<int64_t>(sbase[s]), r0);
     const int64_t b1 = min(static_cast<int64_t>(sbase[s + 1]), r1);
     if (b0 >= b1) continue;
-    for (int e = threadIdx.x; e < a.E; e += kBalThreads) sn[e] = 0;
+    float next[NV];  // the logits of this warp's next row
+    int64_t row = b0 + warp;
+    if (a.logits && row < b1) load_logits<T, V, NV>(a, row, next);
+    for (int e = threadIdx.x; e < a.E; e += THREADS) sn[e] = 0;
     __syncthreads();
     const int64_t p1 = b1 * a.K;
-    for (int64_t p = b0 * a.K + threadIdx.x; p < p1; p += kBalThreads) {
+    for (int64_t p = b0 * a.K + threadIdx.x; p < p1; p += THREADS) {
       const int id = __ldcg(a.ids + p);
       if (id >= 0 && id < a.E) atomicAdd(sn + id, 1);
     }
@@ -170,9 +176,11 @@ __global__ void __launch_bounds__(kBalThreads) k_balance(const BalArgs a) {
       float acc[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
-      for (int64_t row = b0 + warp; row < b1; row += kBalWarps) {
+      for (; row < b1; row += WARPS) {
         float v[NV], none[1];
-        load_logits<T, V, NV>(a, row, v);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = next[i];
+        if (row + WARPS < b1) load_logits<T, V, NV>(a, row + WARPS, next);
         const float inv = scores<NV, false>(v, none, a.sigmoid);
 #pragma unroll
         for (int i = 0; i < NV; ++i) acc[i] = fmaf(v[i], inv, acc[i]);
@@ -188,12 +196,12 @@ __global__ void __launch_bounds__(kBalThreads) k_balance(const BalArgs a) {
     }
     __syncthreads();
     const int64_t at = (static_cast<int64_t>(blockIdx.x) + s) * a.E;
-    for (int e = threadIdx.x; e < a.E; e += kBalThreads) {
+    for (int e = threadIdx.x; e < a.E; e += THREADS) {
       a.part_n[at + e] = sn[e];
       if (a.logits) {
         float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kBalWarps; ++w) sum += sp[w * a.E + e];
+#pragma unroll 8
+        for (int w = 0; w < WARPS; ++w) sum += sp[w * a.E + e];
         a.part_p[at + e] = sum;
       }
     }
@@ -201,9 +209,8 @@ __global__ void __launch_bounds__(kBalThreads) k_balance(const BalArgs a) {
   }
 }
 
-// Adds the blocks' shares. The cluster's CTAs take the sequences' (sequence, 32 experts) pieces in turn,
-// 32 threads by 8 parts of the shares each; the pieces' terms of the loss are added in double, in an
-// order that is the same in every run.
+// Adds the blocks' shares. The cluster's CTAs take the (sequence, 32 experts) pieces in turn, a warp every 32nd
+// share of a piece; the terms of the loss are added in double, in an order that is the same in every run.
 constexpr int kJoinThreads = 1024;
 
 __global__ void __launch_bounds__(kJoinThreads) k_balance_join(const BalArgs a) {
@@ -212,8 +219,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_balance_join(const BalArgs a) 
   __shared__ float bp[32][33];
   __shared__ int bn[32][33];
   __shared__ double part[32];
-  __shared__ double share;
+  __shared__ double shares[kBalCluster];  // of every CTA, in the first one
   __shared__ int live_seqs;
+  cluster_arrive();  // once all have arrived their shared memory can be written to
   pdl_begin_in_order();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = static_cast<int>(cluster_ctarank());
@@ -223,10 +231,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_balance_join(const BalArgs a) 
   for (int s = threadIdx.x; s < a.S; s += kJoinThreads) mine += sbase[s + 1] > sbase[s];
   if (mine) atomicAdd(&live_seqs, mine);
   __syncthreads();
-  const double live = live_seqs;
+  const float live = static_cast<float>(live_seqs);
   const int chunks = (a.E + 31) / 32;
   const int64_t pieces = static_cast<int64_t>(a.S) * chunks;
-  double sum = 0.0;  // of warp 0's lanes
+  double sum = 0.0;  // of each warp's first lane
   for (int64_t piece = rank; piece < pieces; piece += kBalCluster) {
     const int s = static_cast<int>(piece / chunks);
     const int e = static_cast<int>(piece - static_cast<int64_t>(s) * chunks) * 32 + lane;
@@ -257,95 +265,99 @@ __global__ void __launch_bounds__(kJoinThreads) k_balance_join(const BalArgs a) 
     bp[warp][lane] = p;
     bn[warp][lane] = n;
     __syncthreads();
-    if (warp == 0) {
-      for (int i = 1; i < 32; ++i) {
-        p += bp[i][lane];
-        n += bn[i][lane];
-      }
-      if (e < a.E) a.counts[static_cast<int64_t>(s) * a.E + e] = n;
-      if (a.loss && b0 < b1) {
-        const double len = static_cast<double>(b1 - b0);
-        const double factor = a.E / (a.K * len * len * live);
-        sum += factor * n * p;
-        if (lane == 0 && e == 0) a.factor[s] = static_cast<float>(factor);
-      } else if (a.loss && lane == 0 && e == 0) {
-        a.factor[s] = 0.0f;
+    // a warp per expert adds its 32 parts
+    p = warp_sum_f32(bp[lane][warp]);
+    n = __reduce_add_sync(0xffffffffu, bn[lane][warp]);
+    const int mine = e - lane + warp;
+    if (lane == 0 && mine < a.E) {
+      a.counts[static_cast<int64_t>(s) * a.E + mine] = n;
+      if (a.loss) {
+        const float len = static_cast<float>(b1 - b0);
+        const float factor = b0 < b1 ? static_cast<float>(a.E) / (static_cast<float>(a.K) * live * len * len) : 0.0f;
+        if (b0 < b1) sum += static_cast<double>(factor * n) * p;
+        if (mine == 0) a.factor[s] = factor;
       }
     }
     __syncthreads();
   }
-  if (!a.loss) return;
-  if (warp == 0) {
-    part[lane] = sum;
-    __syncwarp();
-    if (lane == 0) {
-      double t = 0.0;
-      for (int i = 0; i < 32; ++i) t += part[i];
-      share = t;
-    }
-  }
+  if (lane == 0) part[warp] = sum;
   __syncthreads();
+  cluster_wait();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int i = 0; i < 32; ++i) t += part[i];
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&shares[rank])), "r"(0));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(t) : "memory");
+  }
   cluster_arrive();
   cluster_wait();
-  if (rank == 0 && threadIdx.x == 0) {
+  if (a.loss && rank == 0 && threadIdx.x == 0) {
     double t = 0.0;
-    for (int r = 0; r < kBalCluster; ++r) {
-      uint32_t at;
-      double v;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&share)), "r"(r));
-      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
-      t += v;
-    }
+    for (int r = 0; r < kBalCluster; ++r) t += shares[r];
     *a.loss = static_cast<float>(t);
   }
-  cluster_arrive();  // the others' shared memory stays until it has been read
-  cluster_wait();
 }
 
 // A token per warp, neighbouring tokens one after the other; c = counts * factor of its sequence stays in
 // registers while the sequence does. Rows of no sequence get zeros.
 template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kBalThreads) k_balance_back(const BalArgs a) {
+__global__ void __launch_bounds__(kBackWarps * 32) k_balance_back(const BalArgs a) {
   extern __shared__ float bal_smem[];
   int* sbase = reinterpret_cast<int*>(bal_smem);  // [S + 1]
   pdl_begin_in_order();
   load_bases(a, sbase);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = a.E / V;
-  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kBalWarps + warp) * a.rows;
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kBackWarps + warp) * a.rows;
   const int64_t r1 = min(r0 + a.rows, a.T);
   if (r0 >= r1) return;
-  const float g = __ldcg(a.g);
+  const float g = *a.g;
   int s = sequence_of(sbase, a.S, r0);
   float c[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) c[i] = 0.0f;
   int64_t b0 = 0, b1 = r0;  // of sequence s; in the rows behind the last sequence, none
+  float next[NV];           // the next row's logits
+  load_logits<T, V, NV>(a, r0, next);
   for (int64_t row = r0; row < r1; ++row) {
     if (row >= b1) {
       while (s < a.S && sbase[s + 1] <= row) ++s;
       b0 = s < a.S ? sbase[s] : a.T;
       b1 = s < a.S ? sbase[s + 1] : a.T;
       if (s < a.S) {
-        const float f = __ldcg(a.factor + s) * g;
+        const float f = a.factor[s] * g;
         const int32_t* cn = a.counts + static_cast<int64_t>(s) * a.E;
 #pragma unroll
         for (int u = 0; u < NV / V; ++u) {
           const int i = u * 32 + lane;
           if (i < n) {
+            // through L1: every warp of the grid reads the same few lines (past it, 16384 x 256 took 22 us)
+            if constexpr (V > 1) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) c[u * V + j] = static_cast<float>(__ldcg(cn + i * V + j)) * f;
+              for (int j = 0; j < V; j += 4) {
+                const int4 w = *reinterpret_cast<const int4*>(cn + i * V + j);
+                c[u * V + j] = static_cast<float>(w.x) * f;
+                c[u * V + j + 1] = static_cast<float>(w.y) * f;
+                c[u * V + j + 2] = static_cast<float>(w.z) * f;
+                c[u * V + j + 3] = static_cast<float>(w.w) * f;
+              }
+            } else {
+              c[u] = static_cast<float>(cn[i]) * f;
+            }
           }
         }
       }
     }
     float v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = next[i];
+    if (row + 1 < r1) load_logits<T, V, NV>(a, row + 1, next);
     if (row < b0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) v[i] = 0.0f;
     } else {
       float slope[NV];
-      load_logits<T, V, NV>(a, row, v);
       const float inv = scores<NV, true>(v, slope, a.sigmoid);
       float dot = 0.0f;
 #pragma unroll
@@ -370,19 +382,28 @@ __global__ void __launch_bounds__(kBalThreads) k_balance_back(const BalArgs a) {
 }
 
 template <typename T, int V, int NV>
-cudaError_t run(const BalArgs& given, bool back, int sms, cudaStream_t s) {
+cudaError_t run(const BalArgs& given, void* workspace, bool back, int sms, cudaStream_t s) {
   static std::atomic<bool> done[64];
   BalArgs a = given;
   const size_t bases = static_cast<size_t>(a.S + 1) * 4;
   if (back) {
-    // rows per warp: two blocks of eight warps per SM share the rows evenly
-    a.rows = static_cast<int>((a.T + 16 * sms - 1) / (16 * sms));
+    // the warps that run at a time share the rows evenly
+    const int64_t most = static_cast<int64_t>(sms) * (NV > 8 ? 16 : 32);
+    a.rows = static_cast<int>((a.T + most - 1) / most);
     const int64_t warps = (a.T + a.rows - 1) / a.rows;
     return launch_pdl(k_balance_back<T, V, NV>,
-                      dim3(static_cast<unsigned>((warps + kBalWarps - 1) / kBalWarps)),
-                      dim3(kBalThreads), bases, s, a);
+                      dim3(static_cast<unsigned>((warps + kBackWarps - 1) / kBackWarps)),
+                      dim3(kBackWarps * 32), bases, s, a);
   }
-  const size_t smem = ((a.logits ? kBalWarps * a.E : 0) + a.E) * 4 + bases;
+  // one block per SM, of a row per warp or more
+  constexpr int WARPS = bal_warps(NV);
+  const int64_t most = sms < kMaxBalanceBlocks ? sms : kMaxBalanceBlocks;
+  const int64_t even = ((a.T > 0 ? a.T : 1) + most - 1) / most;
+  a.rows = static_cast<int>((even + WARPS - 1) / WARPS * WARPS);
+  a.blocks = static_cast<int>((a.T + a.rows - 1) / a.rows);
+  a.part_n = static_cast<int32_t*>(workspace);
+  a.part_p = reinterpret_cast<float*>(a.part_n + (static_cast<int64_t>(a.blocks) + a.S) * a.E);
+  const size_t smem = ((a.logits ? WARPS * a.E : 0) + a.E) * 4 + bases;
   if (smem > 48 * 1024) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
@@ -394,7 +415,7 @@ cudaError_t run(const BalArgs& given, bool back, int sms, cudaStream_t s) {
     }
   }
   if (a.blocks > 0) {
-    const cudaError_t e = launch_pdl(k_balance<T, V, NV>, dim3(a.blocks), dim3(kBalThreads), smem, s, a);
+    const cudaError_t e = launch_pdl(k_balance<T, V, NV>, dim3(a.blocks), dim3(WARPS * 32), smem, s, a);
     if (e != cudaSuccess) return e;
   }
   return launch_pdl_cluster(k_balance_join, dim3(kBalCluster), dim3(kJoinThreads), bases, s,
@@ -402,12 +423,13 @@ cudaError_t run(const BalArgs& given, bool back, int sms, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t typed(const BalArgs& a, bool back, int sms, cudaStream_t s) {
+cudaError_t typed(const BalArgs& a, void* workspace, bool back, int sms, cudaStream_t s) {
   const bool wide = a.E % kV<T> == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0 &&
-                    (reinterpret_cast<uintptr_t>(a.d_logits) & 15u) == 0;
+                    (reinterpret_cast<uintptr_t>(a.d_logits) & 15u) == 0 &&
+                    (!back || (reinterpret_cast<uintptr_t>(a.counts) & 15u) == 0);
   if (a.E <= 256)
-    return wide ? run<T, kV<T>, 8>(a, back, sms, s) : run<T, 1, 8>(a, back, sms, s);
-  return wide ? run<T, kV<T>, 32>(a, back, sms, s) : run<T, 1, 32>(a, back, sms, s);
+    return wide ? run<T, kV<T>, 8>(a, workspace, back, sms, s) : run<T, 1, 8>(a, workspace, back, sms, s);
+  return wide ? run<T, kV<T>, 32>(a, workspace, back, sms, s) : run<T, 1, 32>(a, workspace, back, sms, s);
 }
 
 }  // namespace
@@ -422,13 +444,6 @@ cudaError_t launch_balance(const Balance& p, int sms, cudaStream_t s) {
   a.K = p.K;
   a.S = p.S;
   a.sigmoid = p.sigmoid;
-  // two blocks per SM, of eight rows or more
-  const int64_t most = 2 * sms < kMaxBalanceBlocks ? 2 * sms : kMaxBalanceBlocks;
-  const int64_t even = ((p.T > 0 ? p.T : 1) + most - 1) / most;
-  a.rows = static_cast<int>((even + kBalWarps - 1) / kBalWarps * kBalWarps);
-  a.blocks = static_cast<int>((p.T + a.rows - 1) / a.rows);
-  a.part_n = static_cast<int32_t*>(p.workspace);
-  a.part_p = reinterpret_cast<float*>(a.part_n + (static_cast<int64_t>(a.blocks) + p.S) * p.E);
   a.loss = p.loss;
   a.counts = p.counts;
   a.factor = p.factor;
@@ -436,11 +451,11 @@ cudaError_t launch_balance(const Balance& p, int sms, cudaStream_t s) {
   a.d_logits = p.grad_logits;
   switch (p.dtype) {
     case FMOE_DTYPE_F32:
-      return typed<float>(a, p.back, sms, s);
+      return typed<float>(a, p.workspace, p.back, sms, s);
     case FMOE_DTYPE_BF16:
-      return typed<__nv_bfloat16>(a, p.back, sms, s);
+      return typed<__nv_bfloat16>(a, p.workspace, p.back, sms, s);
     default:
-      return typed<__half>(a, p.back, sms, s);
+      return typed<__half>(a, p.workspace, p.back, sms, s);
   }
 }
 

@@ -316,7 +316,7 @@ cudaError_t take_int4_status(int32_t* status, cudaStream_t s);
 
 constexpr int kMaxBalanceExperts = 1024;
 constexpr int kMaxBalanceSequences = 4096;
-constexpr int kMaxBalanceBlocks = 512;  // of the forward pass, two per SM
+constexpr int kMaxBalanceBlocks = 512;  // of the forward pass
 struct Balance {
   const void* logits;    // [T, E]
   int dtype;

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, 1) k_layer_norm_back(const 
   float* sw = reinterpret_cast<float*>(ln_smem);   // weight [H]
   P* acc = reinterpret_cast<P*>(sw + (a.H + 3) / 4 * 4);  // WIDE: [2][U * N][G]
   float* rows = sw;                                // WARP, at the end: [8][2][H]
-  __shared__ float2 part[2][16];
+  __shared__ float2 part[2][32];
   pdl_begin_in_order();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = WARP ? lane : static_cast<int>(threadIdx.x);
@@ -646,7 +646,7 @@ cudaError_t backward(const LayerNorm& p, int sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
   }
   int64_t blocks = G == 32 ? (p.T + 7) / 8 : p.T;
-  const int64_t most = static_cast<int64_t>(sms) * (G == 512 ? 1 : 2);
+  const int64_t most = static_cast<int64_t>(sms) * (G >= 512 ? 1 : 2);
   if (blocks > most) blocks = most;
   if (blocks > kMaxLnBlocks) blocks = kMaxLnBlocks;
   cudaError_t e = launch_pdl(k_layer_norm_back<T, V, U, G, WIDE>, dim3(static_cast<unsigned>(blocks)),
@@ -669,7 +669,7 @@ cudaError_t sized(const LayerNorm& p, int sms, cudaStream_t s) {
       if (n <= 256 * A) return backward<T, V, A, 256, false>(p, sms, s);
       if (n <= 512 * A) return backward<T, V, 2 * A, 256, false>(p, sms, s);
       if (n <= 1024 * A) return backward<T, V, 2 * A, 512, false>(p, sms, s);
-      return backward<T, V, 4 * A, 512, true>(p, sms, s);
+      return backward<T, V, 2 * A, 1024, true>(p, sms, s);
     }
     if (n <= 32 * A) return forward<T, V, A, 32>(p, sms, s);
     if (n <= 64 * A) return forward<T, V, 2 * A, 32>(p, sms, s);
@@ -686,7 +686,7 @@ cudaError_t sized(const LayerNorm& p, int sms, cudaStream_t s) {
       if (n <= 2048) return backward<T, 1, 8, 256, false>(p, sms, s);
       if (n <= 4096) return backward<T, 1, 8, 512, false>(p, sms, s);
       if (n <= 8192) return backward<T, 1, 16, 512, false>(p, sms, s);
-      return backward<T, 1, 32, 512, true>(p, sms, s);
+      return backward<T, 1, 16, 1024, true>(p, sms, s);
     }
     if (p.q) return cudaErrorInvalidValue;  // the caller checks the alignment
     if (n <= 128) return forward<T, 1, 4, 32>(p, sms, s);
