@@ -263,35 +263,47 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) k_int4_few(const I4Args a, 
 
 // ------------------------------------------------------------------ quantisation
 // Eight consecutive values of a row per lane. A group of up to 256 values is in the registers of up to 32
-// neighbouring lanes between its maximum and the rounding; a longer one (WIDE) is a warp's and read twice.
+// neighbouring lanes between its maximum and the rounding.
 //   symmetric: scale = max|w| / 7,             q = round(w / scale) + 8 in 1 .. 15
 //   else:      scale = (high - low) / 15,      zero = round(-low / scale), q = round(w / scale) + zero,
 //              low = min(w, 0), high = max(w, 0)
 // rounded to the weights' type before the division by it, and no smaller than the type's least scale.
-// Rounding is to the nearest integer, ties to even; the divisions are IEEE's.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; i += kV<T>) {
-    float w[kV<T>];
-    unpack(load_pack<T, kV<T>>(p + i), w);
-#pragma unroll
-    for (int j = 0; j < kV<T>; ++j) v[i + j] = w[j];
-  }
-}
-
+// Rounding is of the IEEE quotients to the nearest integer, ties to even.
 struct GroupRange {
   uint32_t amax;  // bits of the largest absolute value: NaN above infinity above all
   float low, high;
 };
 
-__device__ __forceinline__ void widen(GroupRange& r, const float (&v)[8]) {
+__device__ __forceinline__ void widen(GroupRange& r, const float (&v)[8], int symmetric) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.amax = max(r.amax, __float_as_uint(v[i]) & 0x7fffffffu);
+  if (symmetric) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    r.amax = max(r.amax, __float_as_uint(v[i]) & 0x7fffffffu);
     r.low = fminf(r.low, v[i]);
     r.high = fmaxf(r.high, v[i]);
   }
+}
+
+// The two values of a word, 16-bit floats, by their larger and smaller; a NaN stays in the larger.
+__device__ __forceinline__ uint32_t max2(__nv_bfloat16*, uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max2(__half*, uint32_t a, uint32_t b) {
+  const __half2 m =
+      __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t min2(__nv_bfloat16*, uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t min2(__half*, uint32_t a, uint32_t b) {
+  const __half2 m = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
 }
 
 template <typename T>
@@ -306,137 +318,308 @@ __device__ __forceinline__ float group_scale(const GroupRange& r, bool symmetric
   return to_f32(s);
 }
 
+// Eight values as q. 16-bit weights are not divided: v = w * inv is within two units of the quotient and
+// w - v * scale is exact, so the corrected v is the quotient where that is halfway between integers, and any
+// other quotient of 11-bit numbers is 2^-20 (relative) or more away from halfway. Adding 1.5 * 2^23 rounds to
+// the even integer, which is then the low byte of the sum. The zero point is added to four such bytes at a
+// time; of the results, 0 .. 16 (see zero and low, which are rounded alike), only 16 has to be brought back. Not so
+// where the scale itself was rounded among fp16's subnormal numbers: those are done value by value, like
+// fp32 weights.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise8(const float (&v)[8], float scale, float zero, float least) {
+__device__ __forceinline__ uint32_t quantise8(const float (&v)[8], float scale, float inv, int zero, int least) {
   uint32_t w = 0;
+  if (sizeof(T) == 4 || (std::is_same<T, __half>::value && scale < 0x1p-14f)) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = fminf(fmaxf(rintf(__fdiv_rn(v[i], scale)) + zero, least), 15.0f);
-    w |= static_cast<uint32_t>(q) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      const float r = rintf(__fdiv_rn(v[i], scale));
+      w |= static_cast<uint32_t>(max(least, min(15, static_cast<int>(r) + zero))) << (4 * i);
+    }
+    return w;
   }
-  return w;
+  const float2 s2 = make_float2(-scale, -scale), i2 = make_float2(inv, inv);
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 p = make_float2(v[i], v[i + 1]);
+    float2 r = __fmul2_rn(p, i2);
+    r = __ffma2_rn(__ffma2_rn(r, s2, p), i2, r);
+    r = __fadd2_rn(r, make_float2(12582912.0f, 12582912.0f));
+    b[i] = __float_as_uint(r.x);
+    b[i + 1] = __float_as_uint(r.y);
+  }
+  const uint32_t z4 = static_cast<uint32_t>(zero) * 0x01010101u;
+  uint32_t h[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo = __byte_perm(b[4 * i], b[4 * i + 1], 0x0040);
+    const uint32_t x = __byte_perm(lo, __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+    uint32_t q = ((x & 0x7f7f7f7fu) + z4) ^ (x & 0x80808080u);  // no byte carries into the next
+    q = (q - ((q >> 4) & 0x01010101u)) & 0x0f0f0f0fu;
+    h[i] = q | q >> 4;  // bytes 0 and 2 have two values each
+  }
+  return __byte_perm(h[0], h[1], 0x6420);
 }
 
-template <typename T, bool WIDE>
+// Eight values as they are in memory.
+template <typename T>
+struct Raw8 {
+  Pack<T, kV<T>> p[8 / kV<T>];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < 8 / kV<T>; ++i) r.p[i] = load_pack<T, kV<T>>(p + i * kV<T>);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void values8(const Raw8<T>& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8 / kV<T>; ++i) {
+    float w[kV<T>];
+    unpack(r.p[i], w);
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) v[i * kV<T> + j] = w[j];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ GroupRange range8(const Raw8<T>& raw, int symmetric) {
+  GroupRange r{0u, 0.0f, 0.0f};
+  if constexpr (sizeof(T) == 4) {
+    float v[8];
+    values8(raw, v);
+    widen(r, v, symmetric);
+  } else {
+    T* type = nullptr;
+    const uint32_t* w = raw.p[0].w;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max2(type, m, w[i] & 0x7fff7fffu);
+    float2 f = unpack2(type, m);
+    r.amax = max(__float_as_uint(f.x), __float_as_uint(f.y)) & 0x7fffffffu;
+    if (!symmetric) {
+      uint32_t lo = w[0], hi = w[0];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        lo = min2(type, lo, w[i]);
+        hi = max2(type, hi, w[i]);
+      }
+      f = unpack2(type, lo);
+      r.low = fminf(0.0f, fminf(f.x, f.y));
+      f = unpack2(type, hi);
+      r.high = fmaxf(0.0f, fmaxf(f.x, f.y));
+    }
+  }
+  return r;
+}
+
+// Joins the ranges of `width` neighbouring lanes (a power of two, the same in every thread).
+__device__ __forceinline__ void join_lanes(GroupRange& r, int width, int symmetric) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (o >= width) continue;
+    r.amax = max(r.amax, __shfl_xor_sync(0xffffffffu, r.amax, o));
+    if (!symmetric) {
+      r.low = fminf(r.low, __shfl_xor_sync(0xffffffffu, r.low, o));
+      r.high = fmaxf(r.high, __shfl_xor_sync(0xffffffffu, r.high, o));
+    }
+  }
+}
+
+template <typename T>
+struct GroupCode {
+  float s, inv;
+  int z, least;
+  __device__ __forceinline__ GroupCode(const GroupRange& r, int symmetric) {
+    s = group_scale<T>(r, symmetric);
+    inv = 1.0f / s;
+    z = symmetric ? 8 : static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(-r.low, s)), 0.0f), 15.0f));
+    least = symmetric ? 1 : 0;
+  }
+};
+
+// Groups of up to 256 values: a warp takes 256 values at a time, two such pieces side by side and the next two
+// on their way; blockIdx.y and gridDim.y share out a row's pieces. A warp per piece, its row found by a 64-bit
+// division and each value divided, took 51 us for 4096 x 7168.
+template <typename T>
 __global__ void __launch_bounds__(256)
     k_quantize_int4(const T* w, int64_t rows, int K, int group, int groups, int symmetric,
                     uint8_t* packed, T* scale, uint8_t* zero) {
   pdl_begin_in_order();
   const int lane = threadIdx.x & 31;
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  // pieces of a row: 256 values, or a group
-  const int pieces = WIDE ? groups : (K + 255) / 256;
-  const int64_t row = warp / pieces;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int piece = static_cast<int>(warp - row * pieces);
-  const int k0 = piece * (WIDE ? group : 256);
-  const int k1 = min(K, k0 + (WIDE ? group : 256));
-  const T* wr = w + row * K;
-  uint8_t* out = packed + row * (K / 2);
-  GroupRange r{0u, 0.0f, 0.0f};
-  float v[8];
-  if (WIDE) {
-    for (int k = k0 + 8 * lane; k < k1; k += 256) {
-      load8(wr + k, v);
-      widen(r, v);
-    }
-  } else if (k0 + 8 * lane < k1) {
-    load8(wr + k0 + 8 * lane, v);
-    widen(r, v);
-  }
-  // a group's lanes: group / 8 of them, a power of two and aligned (WIDE: all)
-  const int width = WIDE || group > 256 ? 32 : group / 8;
+  const T* wr = w + row * K + 8 * lane;
+  uint32_t* out = reinterpret_cast<uint32_t*>(packed + row * (K / 2)) + lane;
+  const int width = group / 8;              // lanes of a group
+  const int per = 256 / group;              // groups of a piece
+  const int mine = lane / width;
+  const bool first = (lane & (width - 1)) == 0;
+  const int step = gridDim.y;
+  const auto in = [&](int piece) { return piece * 256 + 8 * lane < K; };
+  Raw8<T> next[2];
+  int piece = blockIdx.y;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint32_t m = __shfl_xor_sync(0xffffffffu, r.amax, o);
-    const float l = __shfl_xor_sync(0xffffffffu, r.low, o), h = __shfl_xor_sync(0xffffffffu, r.high, o);
-    if (o < width) {
-      r.amax = max(r.amax, m);
-      r.low = fminf(r.low, l);
-      r.high = fmaxf(r.high, h);
+  for (int i = 0; i < 2; ++i)
+    if (in(piece + i * step)) next[i] = load_raw8(wr + (piece + i * step) * 256);
+  for (; piece * 256 < K; piece += 2 * step) {
+    Raw8<T> now[2];
+    GroupRange r[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r[i] = GroupRange{0u, 0.0f, 0.0f};
+      now[i] = next[i];
+      if (in(piece + i * step)) r[i] = range8(now[i], symmetric);
+      if (in(piece + (2 + i) * step)) next[i] = load_raw8(wr + (piece + (2 + i) * step) * 256);
     }
-  }
-  const float s = group_scale<T>(r, symmetric);
-  const float z = symmetric ? 8.0f : fminf(fmaxf(rintf(__fdiv_rn(-r.low, s)), 0.0f), 15.0f);
-  const float least = symmetric ? 1.0f : 0.0f;
-  const int k = k0 + 8 * lane;
-  if (k < k1 && (WIDE ? lane == 0 : k % group == 0)) {
-    const int64_t at = row * groups + k / group;
-    from_f32(s, scale + at);
-    if (zero) zero[at] = static_cast<uint8_t>(z);
-  }
-  if (WIDE) {
-    for (int j = k; j < k1; j += 256) {
-      load8(wr + j, v);
-      *reinterpret_cast<uint32_t*>(out + j / 2) = quantise8<T>(v, s, z, least);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) join_lanes(r[i], width, symmetric);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = piece + i * step;
+      if (!in(at)) continue;
+      const GroupCode<T> c(r[i], symmetric);
+      float v[8];
+      values8(now[i], v);
+      out[at * 32] = quantise8<T>(v, c.s, c.inv, c.z, c.least);
+      if (first) {
+        const int64_t g = row * groups + at * per + mine;
+        from_f32(c.s, scale + g);
+        if (zero) zero[g] = static_cast<uint8_t>(c.z);
+      }
     }
-  } else if (k < k1) {
-    *reinterpret_cast<uint32_t*>(out + k / 2) = quantise8<T>(v, s, z, least);
   }
 }
 
-// 32 values per thread, all of one group: 16 bytes in, scale * (q - zero) in fp32, rounded once.
+// Longer groups: a warp's at a time, read twice.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_quantize_int4_wide(const T* w, int64_t rows, int K, int group, int groups, int symmetric,
+                         uint8_t* packed, T* scale, uint8_t* zero) {
+  pdl_begin_in_order();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const T* wr = w + row * K;
+  uint8_t* out = packed + row * (K / 2);
+  for (int g = blockIdx.y; g < groups; g += gridDim.y) {
+    const int k0 = g * group, k = k0 + 8 * lane, k1 = K - k0 < group ? K : k0 + group;
+    GroupRange r{0u, 0.0f, 0.0f};
+    float v[8];
+#pragma unroll 4
+    for (int j = k; j < k1; j += 256) {
+      values8(load_raw8(wr + j), v);
+      widen(r, v, symmetric);
+    }
+    join_lanes(r, 32, symmetric);
+    const GroupCode<T> c(r, symmetric);
+    if (lane == 0) {
+      from_f32(c.s, scale + row * groups + g);
+      if (zero) zero[row * groups + g] = static_cast<uint8_t>(c.z);
+    }
+#pragma unroll 4
+    for (int j = k; j < k1; j += 256) {
+      values8(load_raw8(wr + j), v);
+      *reinterpret_cast<uint32_t*>(out + j / 2) = quantise8<T>(v, c.s, c.inv, c.z, c.least);
+    }
+  }
+}
+
+// Eight values per lane at a time, four of them on their way: scale * (q - zero) in fp32, rounded once. A warp
+// takes every gridDim.y-th 1024 values of a row.
 template <typename T, typename S>
 __global__ void __launch_bounds__(256)
     k_dequantize_int4(const uint8_t* packed, const S* scale, const uint8_t* zero, int64_t rows, int K,
-                      int group, int groups, T* out) {
+                      int groups, uint32_t magic, T* out) {
   pdl_begin_in_order();
-  const int per = K / 32;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t row = i / per;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int k = static_cast<int>(i - row * per) * 32;
-  const uint4 q = load_row16(reinterpret_cast<const uint4*>(packed + row * (K / 2) + k / 2));
-  const int64_t at = row * groups + k / group;
-  const float s = to_f32(scale[at]);
-  const float z = zero ? static_cast<float>(zero[at] & 15u) : 8.0f;
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  T* o = out + row * K + k;
+  const uint32_t* p = reinterpret_cast<const uint32_t*>(packed + row * (K / 2));
+  const S* sr = scale + row * groups;
+  const uint8_t* zr = zero ? zero + row * groups : nullptr;
+  T* o = out + row * K;
+  const int n = K / 8;
+  for (int u0 = blockIdx.y * 128 + lane; u0 < n; u0 += gridDim.y * 128) {
+    uint32_t q[4], z[4];
+    S s[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < 4; ++i) {
+      const int u = u0 + 32 * i;
+      if (u < n) {
+        q[i] = __ldcg(p + u);
+        const uint32_t g = __umulhi(static_cast<uint32_t>(u), magic);
+        s[i] = sr[g];
+        z[i] = zr ? zr[g] & 15u : 8u;
+      }
+    }
 #pragma unroll
-    for (int h = 0; h < 8; h += kV<T>) {
-      float v[kV<T>];
+    for (int i = 0; i < 4; ++i) {
+      const int u = u0 + 32 * i;
+      if (u >= n) break;
+      if constexpr (std::is_same<T, S>::value && sizeof(T) == 2) {
+        // the product has at most 15 bits: rounded in 16 bits it is what fp32 would round to
+        T* type = nullptr;
+        const uint32_t hi = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&s[i])) * 0x00010001u;
+        *reinterpret_cast<uint4*>(o + 8 * u) =
+            weights8<T, false>(q[i], nibble_base(type) + z[i] * 0x00010001u, hi, 0u);
+        continue;
+      }
+      // 2^23 + q less 2^23 + zero: exact
+      const float base = 8388608.0f + static_cast<float>(z[i]), scale = to_f32(s[i]);
 #pragma unroll
-      for (int l = 0; l < kV<T>; ++l)
-        v[l] = (static_cast<float>((w[j] >> (4 * (h + l))) & 15u) - z) * s;
-      store_pack(o + 8 * j + h, v);
+      for (int h = 0; h < 8; h += kV<T>) {
+        float v[kV<T>];
+#pragma unroll
+        for (int l = 0; l < kV<T>; ++l)
+          v[l] = (__uint_as_float(((q[i] >> (4 * (h + l))) & 15u) | 0x4b000000u) - base) * scale;
+        store_pack(o + 8 * u + h, v);
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------ launches
+// Blocks of eight rows, and how many blocks share a row: until there are 32 warps per SM.
+dim3 row_grid(int64_t rows, int pieces, int sms) {
+  const int64_t blocks = (rows + 7) / 8;
+  int64_t share = (4 * sms + blocks - 1) / blocks;
+  if (share > pieces) share = pieces;
+  return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(share));
+}
+
 template <typename T>
-cudaError_t quantise(const Int4Weights& p, cudaStream_t s) {
-  const bool wide = p.group > 256;
-  const int64_t pieces = p.rows * (wide ? p.groups : (p.K + 255) / 256);
-  const dim3 grid(static_cast<unsigned>((pieces + 7) / 8));
+cudaError_t quantise(const Int4Weights& p, int sms, cudaStream_t s) {
   const T* w = static_cast<const T*>(p.w);
   T* scale = static_cast<T*>(p.scale);
-  if (wide)
-    return launch_pdl(k_quantize_int4<T, true>, grid, dim3(256), 0, s, w, p.rows, p.K, p.group, p.groups,
-                      p.symmetric, p.packed, scale, p.zero);
-  return launch_pdl(k_quantize_int4<T, false>, grid, dim3(256), 0, s, w, p.rows, p.K, p.group, p.groups,
-                    p.symmetric, p.packed, scale, p.zero);
+  if (p.group > 256)
+    return launch_pdl(k_quantize_int4_wide<T>, row_grid(p.rows, p.groups, sms), dim3(256), 0, s, w, p.rows,
+                      p.K, p.group, p.groups, p.symmetric, p.packed, scale, p.zero);
+  return launch_pdl(k_quantize_int4<T>, row_grid(p.rows, (p.K + 255) / 256, sms), dim3(256), 0, s, w,
+                    p.rows, p.K, p.group, p.groups, p.symmetric, p.packed, scale, p.zero);
 }
 
 template <typename T, typename S>
-cudaError_t dequantise(const Int4Weights& p, cudaStream_t s) {
-  const int64_t threads = p.rows * (p.K / 32);
-  return launch_pdl(k_dequantize_int4<T, S>, dim3(static_cast<unsigned>((threads + 255) / 256)),
-                    dim3(256), 0, s, p.packed, static_cast<const S*>(p.scale), p.zero, p.rows, p.K,
-                    p.group, p.groups, static_cast<T*>(p.w));
+cudaError_t dequantise(const Int4Weights& p, int sms, cudaStream_t s) {
+  // u * magic >> 32 is u / (group / 8): u is below 2^14, which makes the product's error less than 2^-18, and a
+  // longer group than that is all there is
+  const uint32_t g8 = static_cast<uint32_t>(p.group / 8);
+  const uint32_t magic = g8 > 16384 ? 0u : static_cast<uint32_t>((1ull << 32) / g8 + 1);
+  return launch_pdl(k_dequantize_int4<T, S>, row_grid(p.rows, (p.K + 1023) / 1024, sms), dim3(256), 0, s,
+                    static_cast<const uint8_t*>(p.packed), static_cast<const S*>(p.scale),
+                    static_cast<const uint8_t*>(p.zero), p.rows, p.K, p.groups, magic, static_cast<T*>(p.w));
 }
 
 template <typename T>
-cudaError_t dequantise(const Int4Weights& p, cudaStream_t s) {
+cudaError_t dequantise(const Int4Weights& p, int sms, cudaStream_t s) {
   switch (p.scale_dtype) {
     case FMOE_DTYPE_F32:
-      return dequantise<T, float>(p, s);
+      return dequantise<T, float>(p, sms, s);
     case FMOE_DTYPE_BF16:
-      return dequantise<T, __nv_bfloat16>(p, s);
+      return dequantise<T, __nv_bfloat16>(p, sms, s);
     default:
-      return dequantise<T, __half>(p, s);
+      return dequantise<T, __half>(p, sms, s);
   }
 }
 
@@ -463,25 +646,25 @@ cudaError_t few(const I4Args& a, int64_t per, int sms, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_quantize_int4(const Int4Weights& p, cudaStream_t s) {
+cudaError_t launch_quantize_int4(const Int4Weights& p, int sms, cudaStream_t s) {
   switch (p.dtype) {
     case FMOE_DTYPE_F32:
-      return quantise<float>(p, s);
+      return quantise<float>(p, sms, s);
     case FMOE_DTYPE_BF16:
-      return quantise<__nv_bfloat16>(p, s);
+      return quantise<__nv_bfloat16>(p, sms, s);
     default:
-      return quantise<__half>(p, s);
+      return quantise<__half>(p, sms, s);
   }
 }
 
-cudaError_t launch_dequantize_int4(const Int4Weights& p, cudaStream_t s) {
+cudaError_t launch_dequantize_int4(const Int4Weights& p, int sms, cudaStream_t s) {
   switch (p.dtype) {
     case FMOE_DTYPE_F32:
-      return dequantise<float>(p, s);
+      return dequantise<float>(p, sms, s);
     case FMOE_DTYPE_BF16:
-      return dequantise<__nv_bfloat16>(p, s);
+      return dequantise<__nv_bfloat16>(p, sms, s);
     default:
-      return dequantise<__half>(p, s);
+      return dequantise<__half>(p, sms, s);
   }
 }
 

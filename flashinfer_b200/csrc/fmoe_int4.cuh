@@ -98,6 +98,47 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t b
   return r;
 }
 
+__device__ __forceinline__ uint32_t mul2(__nv_bfloat16*, uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                      *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t mul2(__half*, uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2_rn(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t fma2(__nv_bfloat16*, uint32_t a, uint32_t b, uint32_t c) {
+  const __nv_bfloat162 r =
+      __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b),
+              *reinterpret_cast<const __nv_bfloat162*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t fma2(__half*, uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                            *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Eight values of one group as 16-bit weights, in order. hi, lo: the scale (twice) and, with F32S, what its
+// rounding left.
+template <typename T, bool F32S>
+__device__ __forceinline__ uint4 weights8(uint32_t q, uint32_t zp, uint32_t hi, uint32_t lo) {
+  T* type = nullptr;
+  // byte i holds values 2i and 2i + 1: from q its low half to a word's low 16 bits, from q >> 4 its high
+  // half to the high 16 bits
+  const uint32_t q4 = q >> 4, base = nibble_base(type);
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = sub2(type, and_or(__byte_perm(q, q4, i | (i + 4) << 8), 0x000f000fu, base), zp);
+    if constexpr (F32S)
+      v[i] = fma2(type, hi, v[i], mul2(type, lo, v[i]));
+    else
+      v[i] = mul2(type, hi, v[i]);
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 __device__ __forceinline__ float scale_at(const void* scale, int f32, __nv_bfloat16*, int64_t i) {
   return f32 ? static_cast<const float*>(scale)[i]
              : __bfloat162float(static_cast<const __nv_bfloat16*>(scale)[i]);

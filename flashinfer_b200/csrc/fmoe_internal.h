@@ -286,8 +286,8 @@ struct Int4Weights {
   int scale_dtype;
   uint8_t* zero;         // [rows, groups] or null: 8
 };
-cudaError_t launch_quantize_int4(const Int4Weights& p, cudaStream_t s);
-cudaError_t launch_dequantize_int4(const Int4Weights& p, cudaStream_t s);
+cudaError_t launch_quantize_int4(const Int4Weights& p, int sms, cudaStream_t s);
+cudaError_t launch_dequantize_int4(const Int4Weights& p, int sms, cudaStream_t s);
 
 struct Int4Product {
   const void* x;         // [M, K] of dtype (bf16, fp16)

@@ -176,8 +176,6 @@ bool int4_group(int k, int group) {
 // Weights in 4 bits, given or wanted: the checks of both directions.
 int check_int4_weights(const Int4Weights& p) {
   if (p.rows < 0 || p.rows > INT32_MAX - 1024 || !int4_group(p.K, p.group)) return FMOE_ERR_SHAPE;
-  // a warp per 256 values (or fewer, where a group is longer), eight to a block
-  if (p.rows * ((p.K + 31) / 32) / 256 >= INT32_MAX - 4096) return FMOE_ERR_SHAPE;
   if (!float_type(p.dtype) || !float_type(p.scale_dtype)) return FMOE_ERR_DTYPE;
   if (p.rows == 0) return FMOE_OK;
   if (!p.w || !p.packed || !p.scale) return FMOE_ERR_NULL;
@@ -545,7 +543,7 @@ int fmoe_quantize_int4(const void* w, int32_t dtype, int64_t rows, int32_t k, in
   int sms = 0;
   rc = device_sms(&sms);
   if (rc) return rc;
-  return done(launch_quantize_int4(p, as_stream(stream)));
+  return done(launch_quantize_int4(p, sms, as_stream(stream)));
 }
 
 int fmoe_dequantize_int4(const void* packed, const void* scale, int32_t scale_dtype,
@@ -563,7 +561,7 @@ int fmoe_dequantize_int4(const void* packed, const void* scale, int32_t scale_dt
   int sms = 0;
   rc = device_sms(&sms);
   if (rc) return rc;
-  return done(launch_dequantize_int4(p, as_stream(stream)));
+  return done(launch_dequantize_int4(p, sms, as_stream(stream)));
 }
 
 int fmoe_int4_workspace_size(int64_t m, int32_t n, int32_t k, int32_t E, size_t* bytes) {
