@@ -197,6 +197,36 @@ __device__ __forceinline__ I4Unit decode_unit(int unit, int NT, const I4Tail* t,
   return u;
 }
 
+// The largest absolute value of the scales `at` + g0 .. `at` + g1 of a row of fp16 weights, or of whole 16-byte
+// pieces around them where rows have such (a bound of other groups' scales too does as well): one load per
+// scale, every lane in a row of its own, took a third of 37 x 2047 x 7168 in groups of 32. NaN counts as
+// infinite.
+template <bool F32S>
+__device__ __forceinline__ float largest_scale(const I4Args& args, int64_t at, int g0, int g1) {
+  constexpr int SB = F32S ? 4 : 2, PER = 16 / SB;
+  const uint8_t* row = static_cast<const uint8_t*>(args.scale) + at * SB;
+  uint32_t m = 0;
+  if (args.groups % PER == 0 && (reinterpret_cast<uintptr_t>(args.scale) & 15u) == 0) {
+#pragma unroll 4
+    for (int c = g0 / PER; c <= g1 / PER; ++c) {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + c * 16);
+      if constexpr (F32S)
+        m = max(m, max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu)));
+      else
+        m = __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)),
+                     __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    }
+  } else {
+#pragma unroll 8
+    for (int g = g0; g <= g1; ++g)
+      m = max(m, F32S ? reinterpret_cast<const uint32_t*>(row)[g] & 0x7fffffffu
+                      : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[g]) & 0x7fffu);
+  }
+  if constexpr (F32S) return __uint_as_float(m);
+  m = max(m & 0xffffu, m >> 16);  // as integers non-negative floats keep their order
+  return __half2float(__ushort_as_half(static_cast<uint16_t>(m)));
+}
+
 // Three groups of four warps, a thread per weight row: a group takes every third block of 64 values, so
 // that one is loading and waiting while the others store. With all warps on every block, two threads per
 // row, a block took 1,100 cycles (its MMAs take 512), with two groups 1,000: instruction latency, one
@@ -345,11 +375,8 @@ __device__ __forceinline__ void widen_blocks(const I4Args& args, const I4Run& ru
         if (entered) {
           // the largest scale of the unit's groups to [2^9, 2^10)
           const I4Unit u = decode(mine);
-          const int64_t at = row_of(u) * args.groups;
           const int g0 = group_of(u.kb0 * kI4KB), g1 = group_of(min(u.kb1 * kI4KB, args.K) - 1);
-          float most = 0.0f;
-          for (int i = g0; i <= g1; ++i)
-            most = fmaxf(most, fabsf(scale_at(args.scale, F32S, type, at + i)));
+          const float most = largest_scale<F32S>(args, row_of(u) * args.groups, g0, g1);
           int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127 - 9;
           if (most == 0.0f || ex > 110) ex = 0;  // nothing, or infinite
           if (ex < -120) ex = -120;
