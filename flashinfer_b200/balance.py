@@ -42,6 +42,8 @@ def _sequences(base: Optional[torch.Tensor], index: int) -> int:
 
 def _forward(logits, topk_ids, E, S, scoring, base):
     T, K = topk_ids.shape
+    if T * K > INT_MAX:
+        raise ValueError(f"topk_ids holds {T * K} picks: counts are int32")
     a = FmoeBalanceArgs(T, E, K, S, 0 if logits is None else DTYPE_TAG[logits.dtype], scoring,
                         ptr(logits), topk_ids.data_ptr(), ptr(base))
     counts = topk_ids.new_empty((E,) if base is None else (S, E))
@@ -129,7 +131,5 @@ def expert_counts(topk_ids: torch.Tensor, num_experts: int, *,
         raise ValueError("topk_ids needs at least one pick per token")
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"num_experts must be 1..{MAX_EXPERTS}, got {num_experts}")
-    if topk_ids.numel() > INT_MAX:
-        raise ValueError(f"topk_ids holds {topk_ids.numel()} picks: counts are int32")
     S = _sequences(sequence_base, index)
     return _forward(None, topk_ids, num_experts, S, 0, sequence_base)[1]

@@ -20,8 +20,8 @@ SOURCES = ["fmoe_api.cu", "fmoe_kernels.cu", "fmoe_gemm.cu", "fmoe_gemv.cu", "fm
            "fmoe_quant.cu", "fmoe_ep.cu", "fmoe_peak.cu", "fmoe_tokens.cu", "fmoe_int8.cu",
            "fmoe_norm.cu", "fmoe_layernorm.cu", "fmoe_balance.cu", "fmoe_int4.cu",
            "fmoe_int4_mm.cu", "fmoe_layer_api.cu"]
-HEADERS = ["fmoe_internal.h", "fmoe_elem.cuh", "fmoe_ptx.cuh", "fmoe_int4.cuh", "fmoe_gemm_common.cuh", "fmoe_route.cuh",
-           os.path.join("..", "..", "include", "fmoe.h")]
+HEADERS = ["fmoe_internal.h", "fmoe_elem.cuh", "fmoe_ptx.cuh", "fmoe_int4.cuh", "fmoe_gemm_common.cuh",
+           "fmoe_route.cuh", os.path.join("..", "..", "include", "fmoe.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

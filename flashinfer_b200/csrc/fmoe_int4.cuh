@@ -139,12 +139,4 @@ __device__ __forceinline__ uint4 weights8(uint32_t q, uint32_t zp, uint32_t hi, 
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-__device__ __forceinline__ float scale_at(const void* scale, int f32, __nv_bfloat16*, int64_t i) {
-  return f32 ? static_cast<const float*>(scale)[i]
-             : __bfloat162float(static_cast<const __nv_bfloat16*>(scale)[i]);
-}
-__device__ __forceinline__ float scale_at(const void* scale, int f32, __half*, int64_t i) {
-  return f32 ? static_cast<const float*>(scale)[i] : __half2float(static_cast<const __half*>(scale)[i]);
-}
-
 }  // namespace fmoe

@@ -170,12 +170,13 @@ uint64_t gate_count(const FmoeBlockNormArgs* a) {
 }
 
 bool int4_group(int k, int group) {
-  return k >= 32 && k % 32 == 0 && k <= 131072 && (group == 32 || group == 64 || (group > 0 && group % 128 == 0));
+  if (k < 32 || k % 32 != 0 || k > 131072 || group > INT32_MAX - 131072) return false;
+  return group == 32 || group == 64 || (group > 0 && group % 128 == 0);
 }
 
 // Weights in 4 bits, given or wanted: the checks of both directions.
 int check_int4_weights(const Int4Weights& p) {
-  if (p.rows < 0 || p.rows > INT32_MAX - 1024 || !int4_group(p.K, p.group)) return FMOE_ERR_SHAPE;
+  if (p.rows < 0 || p.rows > INT32_MAX - 1024) return FMOE_ERR_SHAPE;
   if (!float_type(p.dtype) || !float_type(p.scale_dtype)) return FMOE_ERR_DTYPE;
   if (p.rows == 0) return FMOE_OK;
   if (!p.w || !p.packed || !p.scale) return FMOE_ERR_NULL;
@@ -531,7 +532,7 @@ int fmoe_block_norm_backward(const FmoeBlockNormArgs* a, void* stream) {
 
 int fmoe_quantize_int4(const void* w, int32_t dtype, int64_t rows, int32_t k, int32_t group,
                        void* packed, void* scale, void* zero, void* stream) {
-  if (group < 1) return FMOE_ERR_SHAPE;
+  if (!int4_group(k, group)) return FMOE_ERR_SHAPE;
   const Int4Weights p{const_cast<void*>(w), dtype, rows, k, group, (k + group - 1) / group,
                       zero == nullptr, static_cast<uint8_t*>(packed), scale, dtype,
                       static_cast<uint8_t*>(zero)};
@@ -549,7 +550,7 @@ int fmoe_quantize_int4(const void* w, int32_t dtype, int64_t rows, int32_t k, in
 int fmoe_dequantize_int4(const void* packed, const void* scale, int32_t scale_dtype,
                          const void* zero, int64_t rows, int32_t k, int32_t group, void* w,
                          int32_t dtype, void* stream) {
-  if (group < 1) return FMOE_ERR_SHAPE;
+  if (!int4_group(k, group)) return FMOE_ERR_SHAPE;
   const Int4Weights p{w, dtype, rows, k, group, (k + group - 1) / group, zero == nullptr,
                       static_cast<uint8_t*>(const_cast<void*>(packed)), const_cast<void*>(scale),
                       scale_dtype, static_cast<uint8_t*>(const_cast<void*>(zero))};
@@ -751,6 +752,7 @@ int fmoe_balance_loss(const FmoeBalanceArgs* a, void* stream) {
   Balance p;
   int rc = check_balance(a, &p);
   if (rc) return rc;
+  if (static_cast<int64_t>(p.T) * p.K > INT32_MAX) return FMOE_ERR_SHAPE;  // the counts are int32
   if (!p.counts || (p.loss && !p.factor) || (p.T > 0 && (!p.ids || (p.loss && !p.logits))))
     return FMOE_ERR_NULL;
   const size_t need = balance_workspace(p.T, p.E, p.S);

@@ -436,7 +436,8 @@ FMOE_API int fmoe_debug_arm_int8_plan(int32_t tile_tokens, int32_t split);
  * of 128; the last group of a row may be shorter): w[r, k] = scale[r, k / group] * (q - zero[r, k / group]),
  * q and zero in 0 .. 15. packed uint8 [R, K / 2] holds value 2i in the low half of byte i, value 2i + 1 in
  * the high half; scale [R, groups], groups = ceil(K / group); zero uint8 [R, groups] (the low four bits
- * count) or NULL for 8 everywhere. K: a multiple of 32; w and packed start on 16-byte boundaries.
+ * count) or NULL for 8 everywhere. K: a multiple of 32, at most 131072; group at most 2^31 - 1 - 131072;
+ * w and packed start on 16-byte boundaries.
  * fmoe_quantize_int4: from w [R, K] of `dtype`, scales of the same type. zero NULL: symmetric,
  * scale = max|w| / 7, q = round(w / scale) + 8 in 1 .. 15. Else with low = min(w, 0), high = max(w, 0):
  * scale = (high - low) / 15, zero = round(-low / scale), q = round(w / scale) + zero in 0 .. 15. Ties to

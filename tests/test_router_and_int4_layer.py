@@ -319,3 +319,20 @@ def test_a_changed_input_is_noticed_by_the_backward_pass():
         f.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         n.sum().backward()
+
+
+def test_counts_that_pass_int32_are_refused():
+    """2^31 picks and more: the counts are int32. Shapes alone, nothing is read."""
+    lib, P = _lib.load(), 1 << 20
+    for T, K, rc in ((2 ** 30, 2, -2), (2 ** 30 + 1, 4, -2), (5, 2 ** 31 - 1, -2), (2 ** 30 - 1, 2, -5)):
+        a = _lib.FmoeBalanceArgs(T, 4, K, 1, _lib.DTYPE_BF16, 0, P, P, None, P, P, P)
+        assert lib.fmoe_balance_loss(ctypes.byref(a), None) == rc        # -5: no workspace
+
+
+def test_groups_that_pass_int32_are_refused():
+    lib, P = _lib.load(), 1 << 20
+    for group in (2 ** 31 - 128, 2 ** 31 - 131072, 0, -128, 48, 96):
+        assert lib.fmoe_quantize_int4(P, 1, 4, 256, group, 2 * P, 3 * P, None, None) == -2
+        assert lib.fmoe_dequantize_int4(P, 2 * P, 1, None, 4, 256, group, 3 * P, 1, None) == -2
+        a = _lib.FmoeInt4Args(1, 8, 256, 1, group, 1, 1, P, 2 * P, 3 * P, None, None, None, 4 * P, 0)
+        assert lib.fmoe_int4_matmul(ctypes.byref(a), None) == -2
