@@ -28,8 +28,8 @@ CONFIG = os.path.join(HERE, "config.toml")
 
 # Python modules of the package the slot needs (the operator, its C-ABI binding, the build and
 # the TVM-FFI registration); every CUDA source and header of csrc; the public header.
-PY_MODULES = ["__init__.py", "_lib.py", "_op.py", "build.py", "int8.py", "moe.py", "norm.py",
-              "tokens.py", "tvm_binding.py"]
+PY_MODULES = ["__init__.py", "_lib.py", "_op.py", "balance.py", "build.py", "int4.py", "int8.py", "moe.py",
+              "norm.py", "tokens.py", "tvm_binding.py"]
 
 
 def load_config(path: str = CONFIG) -> dict:

@@ -4,6 +4,7 @@ elements; what they refuse; and the C structs they pass."""
 import ctypes
 import os
 import subprocess
+import sys
 import threading
 
 import pytest
@@ -336,3 +337,16 @@ def test_groups_that_pass_int32_are_refused():
         assert lib.fmoe_dequantize_int4(P, 2 * P, 1, None, 4, 256, group, 3 * P, 1, None) == -2
         a = _lib.FmoeInt4Args(1, 8, 256, 1, group, 1, 1, P, 2 * P, 3 * P, None, None, None, 4 * P, 0)
         assert lib.fmoe_int4_matmul(ctypes.byref(a), None) == -2
+
+
+def test_the_packed_solution_imports_on_its_own(tmp_path):
+    """The modules that the package imports are all among those that the solution packs."""
+    from flashinfer_b200 import solution
+    dest = tmp_path / "sol"
+    solution.unpack(solution.pack(), str(dest))
+    code = ("import flashinfer_b200 as f; print(f.__file__, f.balance_loss.__module__, "
+            "f.int4_matmul.__module__, f.layer_norm.__module__)")
+    r = subprocess.run([sys.executable, "-c", code], cwd=dest, capture_output=True, text=True,
+                       env={**os.environ, "PYTHONPATH": str(dest)})
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.startswith(str(dest))
