@@ -15,8 +15,8 @@ namespace fmoe {
 namespace {
 
 // ------------------------------------------------------------------ few tokens
-// A stream of the weights, 16 rows (times RT) per block: the block's eight warps take 128-value pieces of
-// K in turn, so that a step of the block reads 512 consecutive bytes of each row. Lane (g, t), g = lane / 4,
+// A stream of the weights, 16 rows (times RT) per block: the block's W warps take 128-value pieces of K in
+// turn, so that a step of the block reads 64 W consecutive bytes of each row. Lane (g, t), g = lane / 4,
 // t = lane % 4, loads the 16 bytes of values 32 t .. 32 t + 31 of rows g and g + 8, D pieces ahead, and
 // turns them into the fragments of mma.m16n8k16 in its own registers: which values of k a lane has is free
 // as long as the tokens' fragment has the same ones. No shared memory before the end, when the warps' sums
@@ -28,8 +28,6 @@ namespace {
 //
 // SPREAD (group 32 or 64): an MMA sums over all four lanes of a quad, which must then be in one group: the
 // quad's 4 x 4 words are transposed by shuffles, after which step c of lane t has values 32 c + 8 t ...
-constexpr int kFewWarps = 8;
-
 __device__ __forceinline__ void mma_16816(__nv_bfloat16*, float (&c)[4], const uint32_t (&a)[4],
                                           uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -82,10 +80,10 @@ __device__ __forceinline__ void widen8(uint32_t q, uint32_t zp, uint32_t (&v)[4]
     v[i] = sub2(type, and_or(q >> (4 * i), 0x000f000fu, nibble_base(type)), zp);
 }
 
-template <typename T, int RT, int NT, int D, bool SPREAD>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) k_int4_few(const I4Args a, const uint32_t group_magic) {
+template <typename T, int RT, int NT, int D, int W, bool SPREAD>
+__global__ void __launch_bounds__(W * 32, 16 / W) k_int4_few(const I4Args a, const uint32_t group_magic) {
   constexpr int ROWS = 16 * RT, COLS = 8 * NT;
-  __shared__ float red[kFewWarps][COLS][ROWS + 1];
+  __shared__ float red[W][COLS][ROWS + 1];
   T* type = nullptr;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -160,13 +158,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) k_int4_few(const I4Args a, 
     for (int d = 0; d < D; ++d) {
 #pragma unroll
       for (int i = 0; i < 2 * RT; ++i) q[d].w[i] = make_uint4(0u, 0u, 0u, 0u);
-      fetch(warp + d * kFewWarps, q[d]);
+      fetch(warp + d * W, q[d]);
     }
     float acc[RT][NT][4] = {};
-    for (int b0 = warp; b0 < blocks; b0 += D * kFewWarps) {
+    for (int b0 = warp; b0 < blocks; b0 += D * W) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        const int b = b0 + d * kFewWarps;
+        const int b = b0 + d * W;
         if (b >= blocks) break;
         uint4 v[NT][4];
 #pragma unroll
@@ -237,7 +235,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) k_int4_few(const I4Args a, 
           }
           if (SPREAD ? a.group == 32 || (c & 1) == 1 : c == 3) close();
         }
-        fetch(b + D * kFewWarps, q[d]);
+        fetch(b + D * W, q[d]);
       }
     }
 #pragma unroll
@@ -248,12 +246,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) k_int4_few(const I4Args a, 
         for (int i = 0; i < 4; ++i)
           red[warp][8 * j + 2 * t + (i & 1)][16 * r + 8 * (i >> 1) + g] = acc[r][j][i];
     __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * COLS; i += kFewWarps * 32) {
+    for (int i = threadIdx.x; i < ROWS * COLS; i += W * 32) {
       const int c = i / ROWS, r = i - c * ROWS;
       if (m0 + c < r1 && n0 + r < a.N) {
         float sum = a.bias ? a.bias[n0 + r] : 0.0f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) sum += red[w][c][r];
+        for (int w = 0; w < W; ++w) sum += red[w][c][r];
         from_f32(sum, static_cast<T*>(a.out) + (m0 + c) * a.N + n0 + r);
       }
     }
@@ -623,7 +621,7 @@ cudaError_t dequantise(const Int4Weights& p, int sms, cudaStream_t s) {
   }
 }
 
-template <typename T, int RT, int NT, int D>
+template <typename T, int RT, int NT, int D, int W>
 cudaError_t few(const I4Args& a, cudaStream_t s) {
   const dim3 grid((a.N + 16 * RT - 1) / (16 * RT), a.E);
   // a block of 128 values b, at most 1023, is in group (b * magic) >> 20 = b / (group / 128): the error of the
@@ -631,17 +629,28 @@ cudaError_t few(const I4Args& a, cudaStream_t s) {
   const int per = a.group / 128;
   const uint32_t magic = per == 0 || per > 1024 ? 0u : (1u << 20) / per + 1;
   if (a.group < 128)
-    return launch_pdl(k_int4_few<T, RT, NT, D, true>, grid, dim3(kFewWarps * 32), 0, s, a, magic);
-  return launch_pdl(k_int4_few<T, RT, NT, D, false>, grid, dim3(kFewWarps * 32), 0, s, a, magic);
+    return launch_pdl(k_int4_few<T, RT, NT, D, W, true>, grid, dim3(W * 32), 0, s, a, magic);
+  return launch_pdl(k_int4_few<T, RT, NT, D, W, false>, grid, dim3(W * 32), 0, s, a, magic);
+}
+
+template <typename T, int RT, int NT, int D>
+cudaError_t few(const I4Args& a, int64_t used, int sms, cudaStream_t s) {
+  // Short rows leave eight warps a step or two each, and the block's barrier at its end as long as its work.
+  // Four warps and twice the blocks per SM, where there are blocks enough: 128 rows over 32 experts of 7168 x
+  // 2048 take 95 us instead of 125, one of 7168 x 2048 5.2 instead of 6.2. But with 256 blocks four warps
+  // leave SMs idle (1 x 4096 x 4096: 8.2 instead of 5.7), and with long rows eight are as good or better (32
+  // rows over 16 experts of 4096 x 7168: 68 against 70, 128 rows: 130 against 150).
+  const int64_t blocks = (a.N + 16ll * RT - 1) / (16 * RT) * used;
+  if (a.K <= 4096 && blocks >= 2 * sms) return few<T, RT, NT, D, 4>(a, s);
+  return few<T, RT, NT, D, 8>(a, s);
 }
 
 template <typename T>
-cudaError_t few(const I4Args& a, int64_t per, int sms, cudaStream_t s) {
+cudaError_t few(const I4Args& a, int64_t used, int64_t per, int sms, cudaStream_t s) {
   // 32 rows per block share the tokens' loads, as long as there are blocks enough
-  const int64_t used = a.M < a.E ? a.M : a.E;
   const bool tall = (a.N + 31) / 32 * used >= 4 * sms;
-  if (per <= 8) return tall ? few<T, 2, 1, 2>(a, s) : few<T, 1, 1, 4>(a, s);
-  return few<T, 1, 2, 2>(a, s);
+  if (per <= 8) return tall ? few<T, 2, 1, 2>(a, used, sms, s) : few<T, 1, 1, 4>(a, used, sms, s);
+  return few<T, 1, 2, 2>(a, used, sms, s);
 }
 
 }  // namespace
@@ -708,7 +717,8 @@ cudaError_t launch_int4_product(const Int4Product& p, int sms, cudaStream_t s) {
   if (plan.bn != 0) return launch_int4_mm(p, a, plan, sms, s);
   const int64_t used = p.M < p.E ? p.M : p.E;
   const int64_t per = (p.M + used - 1) / used;
-  return p.dtype == FMOE_DTYPE_BF16 ? few<__nv_bfloat16>(a, per, sms, s) : few<__half>(a, per, sms, s);
+  return p.dtype == FMOE_DTYPE_BF16 ? few<__nv_bfloat16>(a, used, per, sms, s)
+                                    : few<__half>(a, used, per, sms, s);
 }
 
 }  // namespace fmoe

@@ -175,3 +175,35 @@ def test_refusals_of_a_variant():
     assert lib.fmoe_int4_matmul(ctypes.byref(a), None) == 0           # used up
     a.num_rows, a.out = 4, 1 << 20
     assert lib.fmoe_int4_matmul(ctypes.byref(a), None) == -2          # the output over x
+
+
+# M, N, K, group: blocks enough for four warps each, of 16 rows, 32 rows and two sets of eight tokens; depths
+# of one block of 128, of less than a warp each and of several steps; the next depth has eight warps again
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,N,K,group", [
+    (1, 4801, 4064, 128), (5, 4777, 96, 32), (8, 4730, 1120, 64), (2, 18977, 544, 128), (7, 18931, 2080, 32),
+    (12, 4801, 4096, 64), (16, 4720, 288, 384), (9, 9473, 4128, 128), (3, 18931, 4128, 64)])
+def test_few_tokens_of_short_rows(M, N, K, group, dtype):
+    g = _gen(M + N + K)
+    for zero in (False, True):
+        x, packed, scale, z = _case(g, M, N, K, group, dtype, zero, zero)
+        bias = torch.randn(N, generator=g, device="cuda") if zero else None
+        R.check(fb.int4_matmul(x, packed, scale, z, bias, group=group),
+                *_product(x, packed, scale, z, group, bias), zero)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("N,K,group", [(421, 1056, 128), (610, 224, 32), (100, 4096, 64), (421, 4128, 128)])
+def test_experts_of_short_rows(N, K, group, dtype):
+    """Experts without rows, with one, with more than a set of eight."""
+    g = _gen(N + K)
+    counts = [0, 1, 20, 3, 8, 9, 0, 7] * 6
+    E, M = len(counts), sum(counts) + 11
+    base = (torch.tensor([0] + counts, device="cuda").cumsum(0) + 4).to(torch.int32)
+    for zero in (False, True):
+        x, packed, scale, z = _case(g, M, N, K, group, dtype, zero, zero, E)
+        y = fb.int4_expert_matmul(x, packed, scale, base, z, group=group)
+        _expert_check(y, x, packed, scale, z, group, base)
+        assert not bool(y[:4].any()) and not bool(y[4 + sum(counts):].any())
