@@ -616,7 +616,7 @@ template <typename T, int V, int U, int G, bool SP>
 cudaError_t run_forward(const LnArgs& a, int64_t blocks, cudaStream_t s) {
   static std::atomic<bool> done[64];
   const size_t smem = SP ? static_cast<size_t>(a.H) * 8 : 0;
-  if (smem > 48 * 1024) {
+  if (smem > 44 * 1024) {  // of the 48 KB without opting in, some are static
     const cudaError_t e = allow_smem(k_layer_norm<T, V, U, G, SP>, done);
     if (e != cudaSuccess) return e;
   }
@@ -641,7 +641,7 @@ cudaError_t backward(const LayerNorm& p, int sms, cudaStream_t s) {
   size_t smem = (static_cast<size_t>(p.H) + 3) / 4 * 16;
   if (WIDE) smem += sizeof(typename Unit<T, V>::P) * 2 * U * Unit<T, V>::N * G;
   if (G == 32) smem = static_cast<size_t>(8) * 2 * p.H * 4;
-  if (smem > 48 * 1024) {
+  if (smem > 44 * 1024) {  // of the 48 KB without opting in, some are static
     const cudaError_t e = allow_smem(k_layer_norm_back<T, V, U, G, WIDE>, done);
     if (e != cudaSuccess) return e;
   }

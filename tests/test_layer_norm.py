@@ -382,3 +382,11 @@ def test_refusals_on_the_host():
     assert run(back, **ok, workspace_bytes=2 * 4 * 128 * 4 - 1) == -5
     assert run(back, **{**ok, "workspace": None}, workspace_bytes=1 << 20) == -5
     assert run(back, stats=6 << 20, grad_input=2 << 20) == -2           # over the residual
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,dtype", [(6140, "fp32"), (6136, "bf16"), (6144, "bf16"), (5640, "fp16"),
+                                     (12280, "fp32"), (768, "bf16")])
+def test_parameters_that_just_fill_shared_memory(H, dtype):
+    """Rows whose parameters take close to 48 KB of a block's shared memory, beside its own arrays."""
+    _check_all(*_inputs(450, H, DT[dtype], True, True, True), 1e-5)
