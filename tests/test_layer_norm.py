@@ -390,3 +390,59 @@ def test_refusals_on_the_host():
 def test_parameters_that_just_fill_shared_memory(H, dtype):
     """Rows whose parameters take close to 48 KB of a block's shared memory, beside its own arrays."""
     _check_all(*_inputs(450, H, DT[dtype], True, True, True), 1e-5)
+
+
+# rows off the 16-byte boundary in tensors on it: every place of a first column in its 16 bytes, rows shorter
+# than 16 bytes, a warp's and a block's rows, more rows than blocks, the longest rows of each variant
+ODD = [(3, 1), (40, 3), (9, 5), (17, 7), (8, 9), (21, 13), (2500, 31), (2399, 255), (700, 506), (601, 1021),
+       (650, 2047), (601, 2046), (599, 4095), (430, 6140), (333, 7001), (300, 8191), (170, 10239),
+       (160, 16369), (150, 16370), (5, 16383)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,H", ODD)
+def test_rows_of_any_length(T, H, dtype):
+    for branch, weight, bias, f32 in ((True, True, True, False), (False, True, False, True)):
+        _check_all(*_inputs(T, H, DT[dtype], branch, weight, bias, f32), 1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,H", [(1, 5), (7, 3), (900, 37), (700, 1023), (500, 3001)])
+def test_rows_of_any_length_write_nothing_else(T, H, dtype):
+    """hidden in place between other values, with NaN before and behind: they are neither used nor changed."""
+    f, x, w, b = _inputs(T, H, DT[dtype], True, True, True)
+    room = 16
+    buf = torch.full((T * H + 2 * room,), float("nan"), device="cuda", dtype=x.dtype)
+    mine = buf[room:-room].view(T, H)
+    assert mine.data_ptr() % 16 == 0
+    mine.copy_(x)
+    h_ref, y_ref = fb.layer_norm(f, x, weight=w, bias=b)
+    h, y = fb.layer_norm(f, mine, weight=w, bias=b, output=mine)
+    assert h is mine and torch.equal(h, h_ref) and torch.equal(y, y_ref)
+    assert bool(torch.isnan(buf[:room]).all()) and bool(torch.isnan(buf[-room:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [37, 1023, 3001])
+def test_a_bad_row_of_any_length_stays_in_its_row(H):
+    """Neighbouring rows share 16 bytes: infinities and NaN at a row's ends reach no other row, forward or
+    backward (but the sums over rows)."""
+    f, x, w, b = _inputs(900, H, torch.bfloat16, True, True, True)
+    clean = x.clone()
+    x[400, 0], x[400, -1], x[402, -1], x[404, 0] = float("inf"), float("nan"), float("inf"), float("nan")
+    dy = torch.randn_like(x)
+    dy[410, 0] = dy[410, -1] = float("nan")
+    good = torch.ones(900, dtype=torch.bool, device="cuda")
+    good[[400, 402, 404]] = False
+    out = []
+    for t in (x, clean):
+        t = t.clone().requires_grad_()
+        h, y = fb.layer_norm(f, t, weight=w, bias=b)
+        out.append((h.detach(), y.detach(), torch.autograd.grad(y, t, dy)[0]))
+    for got, ref in zip(*out):
+        assert torch.equal(got[good].nan_to_num(7.0), ref[good].nan_to_num(7.0))
+    assert bool(torch.isfinite(out[0][2][[399, 401, 403, 405, 409, 411]][:, 1:-1]).any())
+    good[410] = False
+    assert bool(torch.isfinite(out[0][2][good]).all())
