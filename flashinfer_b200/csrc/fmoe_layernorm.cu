@@ -110,8 +110,9 @@ __device__ __forceinline__ Unit<T, V> param(const void* p, int f32, int i) {
 
 // Rows off the 16-byte boundaries (ODD): the units are memory's granules. A row's first column is element `off`
 // of its first unit, the same in every tensor, and in every row of a block: their distance is a multiple of
-// 16 bytes, so that a thread's columns and the block's parameters in shared memory stay what they are. Unit i has columns c .. c + V - 1, c = i * V - off; those below 0 and from H on
-// are another row's: read and not used, and never written.
+// 16 bytes, so that a thread's columns and the block's parameters in shared memory stay what they are. Unit i has
+// columns c .. c + V - 1, c = i * V - off; those below 0 and from H on are another row's: read and not used, and
+// never written.
 template <int V>
 __device__ __forceinline__ bool whole(int c, int H) {
   return c >= 0 && c + V <= H;
@@ -246,24 +247,30 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, ln_blocks(G, U * V))
   T* yo = a.y ? static_cast<T*>(a.y) + at : nullptr;
 
   Pack<T, V> nx[U], nf[U];
-  // `left`: the elements from the row's first to the tensor's end
-  const auto load = [&](const T* p, int u, int left) {
-    const int c = (u * G + g) * V - off;
-    if (ODD && c + V > left) return load_some<T, V>(p + u * G * V, left - c);
-    return load_pack<T, V>(p + u * G * V);
+  // Unit u of a row is loaded as a whole unless it passes the tensor's end, `left` elements behind the row's
+  // first; if it does, by elements and only when it is used, since a branch around loads on their way would
+  // wait for them (4096 x 4095 took 71 us with it).
+  const auto behind = [&](int64_t r) -> int {
+    const int64_t left = (a.T - r) * a.H;
+    return left < (1 << 30) ? static_cast<int>(left) : 1 << 30;
   };
-  const auto behind = [&](int64_t r) { return static_cast<int>(min(static_cast<long long>((a.T - r) * a.H), 1ll << 30)); };
+  const auto here = [&](int u, int left) {
+    return u * G + g < n && (!ODD || (u * G + g + 1) * V - off <= left);
+  };
+  const auto finish = [&](Pack<T, V>& to, const T* p, int u, int left) {
+    if (ODD && !here(u, left)) to = load_some<T, V>(p + u * G * V, left - ((u * G + g) * V - off));
+  };
   const auto fetch = [&](int64_t r) {
     if (r >= a.T) return;
-    const int left = behind(r);
+    const int left = ODD ? behind(r) : 0;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (u * G + g < n) nx[u] = load(x, u, left);
+      if (here(u, left)) nx[u] = load_pack<T, V>(x + u * G * V);
     x += by;
     if (f) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (u * G + g < n) nf[u] = load(f, u, left);
+        if (here(u, left)) nf[u] = load_pack<T, V>(f + u * G * V);
       f += by;
     }
   };
@@ -293,13 +300,16 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, ln_blocks(G, U * V))
 
   for (int flip = 0; row < a.T; row += step, flip ^= 1) {
     if constexpr (!AHEAD) fetch(row);
+    const int now = ODD ? behind(row) : 0;
     Un v[U];
     P two = all<P>(0.0f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u * G + g < n) {
+        finish(nx[u], x - by, u, now);
         v[u] = unit_of(nx[u]);
         if (a.f) {
+          finish(nf[u], f - by, u, now);
           const Un w = unit_of(nf[u]);
 #pragma unroll
           for (int j = 0; j < Un::N; ++j) v[u].p[j] = add(v[u].p[j], w.p[j]);
@@ -449,31 +459,37 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, 1) k_layer_norm_back(const 
     Pack<T, V> x[U], f[U], dy[U];
     float2 stat;
   } next;
-  // `left`: the elements from the row's first to the tensor's end
-  const auto load = [&](const T* p, int u, int left) {
-    const int c = (u * G + g) * V - off;
-    if (ODD && c + V > left) return load_some<T, V>(p + u * G * V, left - c);
-    return load_pack<T, V>(p + u * G * V);
+  // Unit u of a row is loaded as a whole unless it passes the tensor's end, `left` elements behind the row's
+  // first; if it does, by elements and only when it is used, since a branch around loads on their way would
+  // wait for them (4096 x 4095 took 71 us with it).
+  const auto behind = [&](int64_t r) -> int {
+    const int64_t left = (a.T - r) * a.H;
+    return left < (1 << 30) ? static_cast<int>(left) : 1 << 30;
   };
-  const auto behind = [&](int64_t r) { return static_cast<int>(min(static_cast<long long>((a.T - r) * a.H), 1ll << 30)); };
+  const auto here = [&](int u, int left) {
+    return u * G + g < n && (!ODD || (u * G + g + 1) * V - off <= left);
+  };
+  const auto finish = [&](Pack<T, V>& to, const T* p, int u, int left) {
+    if (ODD && !here(u, left)) to = load_some<T, V>(p + u * G * V, left - ((u * G + g) * V - off));
+  };
   const auto fetch = [&](int64_t r) {
     if (r >= a.T) return;
-    const int left = behind(r);
+    const int left = ODD ? behind(r) : 0;
     next.stat = __ldcg(reinterpret_cast<const float2*>(a.stats) + r);
     if (dy_in) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (u * G + g < n) next.x[u] = load(x, u, left);
+        if (here(u, left)) next.x[u] = load_pack<T, V>(x + u * G * V);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (u * G + g < n) next.dy[u] = load(dy, u, left);
+        if (here(u, left)) next.dy[u] = load_pack<T, V>(dy + u * G * V);
       x += by;
       dy += by;
     }
     if (f) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (u * G + g < n) next.f[u] = load(f, u, left);
+        if (here(u, left)) next.f[u] = load_pack<T, V>(f + u * G * V);
       f += by;
     }
   };
@@ -500,15 +516,19 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, 1) k_layer_norm_back(const 
   for (int flip = 0; row < a.T; row += step, flip ^= 1) {
     if constexpr (!AHEAD) fetch(row);
     const float mean = next.stat.x, r = next.stat.y;
+    const int now = ODD ? behind(row) : 0;
     Un v[U], d[U];  // n, and dy and then u
     Pack<T, V> ph[U];
     P t1 = all<P>(0.0f), t2 = t1;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (dh && u * G + g < n) ph[u] = load(dh, u, behind(row));
+      if (dh && here(u, now)) ph[u] = load_pack<T, V>(dh + u * G * V);
       if (dy_in && u * G + g < n) {
+        finish(next.x[u], x - by, u, now);
+        finish(next.dy[u], dy - by, u, now);
         v[u] = unit_of(next.x[u]);
         if (f_in) {
+          finish(next.f[u], f - by, u, now);
           const Un t = unit_of(next.f[u]);
 #pragma unroll
           for (int j = 0; j < N; ++j) v[u].p[j] = add(v[u].p[j], t.p[j]);
@@ -571,6 +591,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, 1) k_layer_norm_back(const 
           for (int j = 0; j < N; ++j) o.p[j] = all<P>(0.0f);
         }
         if (dh) {
+          finish(ph[u], dh - by, u, now);
           const Un t = unit_of(ph[u]);
 #pragma unroll
           for (int j = 0; j < N; ++j) o.p[j] = add(o.p[j], t.p[j]);
@@ -839,8 +860,9 @@ cudaError_t typed(const LayerNorm& p, int sms, cudaStream_t s) {
     wide = wide && on16(q);
   if (wide && p.H % V == 0) return sized<T, V, false>(p, sms, s);
   // Off the boundary, long rows go by memory's 16 bytes and shorter ones by elements: 3001 rows of 7001 bf16
-  // columns take 86 us instead of 205 (with gradients 183 instead of 515), but 500 of 1407 16 instead of 11, and
-  // 4096 of 2047 48 instead of 44 (with gradients 114 instead of 127). The largest variants hold 16384 columns.
+  // columns take 47 us instead of 205 (with gradients 140 instead of 515; 3000 of 7168: 34 and 92), but 500 of
+  // 1407 took 16 instead of 11, for the parameters that each row then gathers by elements. The largest
+  // variants hold 16384 columns.
   if (wide && !p.q && p.H > 2048 && p.H + 2 * V - 2 <= 16384) return sized<T, V, true>(p, sms, s);
   return sized<T, 1, false>(p, sms, s);
 }
