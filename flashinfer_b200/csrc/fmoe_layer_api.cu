@@ -702,8 +702,9 @@ int fmoe_layer_norm_backward(const FmoeLayerNormArgs* a, void* stream) {
   const size_t we = elem(a->weight_dtype), be = elem(a->bias_dtype);
   const bool sums = a->grad_weight || a->grad_bias;
   if ((a->grad_weight && !a->weight) || (a->grad_bias && !a->bias)) return FMOE_ERR_NULL;
+  // the shares of the sums go through the workspace in pairs and fours
   if (!at(a->grad_hidden, e) || !at(a->grad_normed, e) || !at(a->grad_input, e) ||
-      !at(a->workspace, 4) || (a->grad_weight && !at(a->grad_weight, we)) ||
+      !at(a->workspace, sums ? 16 : 4) || (a->grad_weight && !at(a->grad_weight, we)) ||
       (a->grad_bias && !at(a->grad_bias, be)))
     return FMOE_ERR_ALIGN;
   cudaStream_t s = as_stream(stream);

@@ -34,7 +34,7 @@ struct LnArgs {
   // backward
   const void *dh, *dy;        // null: zero
   void* dx;                   // or null
-  float* part;                // [2][blocks][H]: d weight, d bias
+  float* part;                // [2][blocks][H]: d weight, d bias; 16-byte aligned
   int want_w, want_b;
 };
 
@@ -805,7 +805,7 @@ cudaError_t backward(const LayerNorm& p, int sms, cudaStream_t s) {
   cudaError_t e = launch_pdl(k_layer_norm_back<T, V, U, G, WIDE, ODD>, dim3(static_cast<unsigned>(blocks)),
                              dim3(G == 32 ? 256 : G), smem, s, a);
   if (e != cudaSuccess || (!p.dw && !p.db)) return e;
-  const auto sums = p.H % 4 == 0 && on16(p.part) ? k_layer_norm_sums<T, 4> : k_layer_norm_sums<T, 1>;
+  const auto sums = p.H % 4 == 0 ? k_layer_norm_sums<T, 4> : k_layer_norm_sums<T, 1>;
   return launch_pdl(sums, dim3((p.H + 31) / 32, 2), dim3(256), 0, s, static_cast<const float*>(p.part),
                     static_cast<int>(blocks), p.H, p.dw, p.db, a.w_f32, a.b_f32);
 }

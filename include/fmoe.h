@@ -559,8 +559,8 @@ FMOE_API int fmoe_block_norm_backward(const FmoeBlockNormArgs* args, void* cuda_
  * (mean, 1 / sqrt(var + eps)), or NULL: what the backward pass needs.
  * Backward: the forward's inputs and stats, grad_hidden and grad_normed (either may be NULL: zero) and the
  * wanted gradients (NULL: not wanted), each of its input's type. grad_input is the gradient of residual
- * and of branch alike. Workspace of fmoe_layer_norm_workspace_size bytes where the weight's or the
- * bias's gradient is wanted. Sums over tokens run in a fixed order. */
+ * and of branch alike. Workspace of fmoe_layer_norm_workspace_size bytes, on a 16-byte boundary, where the
+ * weight's or the bias's gradient is wanted. Sums over tokens run in a fixed order. */
 typedef struct FmoeLayerNormArgs {
   int64_t num_tokens;
   int32_t hidden_size;
