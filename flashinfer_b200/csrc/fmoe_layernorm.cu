@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, ln_blocks(G, U * V))
       const float2 p = lane < WARPS ? part[flip][lane] : make_float2(0.0f, 0.0f);
       mean = __fdiv_rn(warp_sum_f32(p.x), cols);
       const float2 c = lane < WARPS ? count[lane] : make_float2(0.0f, 0.0f);
-      const float d = p.x * c.y - mean;
+      // without columns there is no mean of its own: 0 * (0 - mean)^2 would be NaN where the square is infinite
+      const float d = c.x > 0.0f ? p.x * c.y - mean : 0.0f;
       dev = warp_sum_f32(fmaf(d * d, c.x, p.y));
     }
     const float r = rsqrtf(fmaf(dev, inv_h, a.eps));

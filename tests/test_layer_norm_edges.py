@@ -2,8 +2,9 @@
 import ctypes
 
 import pytest
-import torch  # noqa: F401  (its libraries before the package's)
+import torch
 
+import flashinfer_b200 as fb
 from flashinfer_b200 import _lib
 
 
@@ -24,3 +25,16 @@ def test_a_workspace_off_the_16_byte_boundary_is_refused(off):
     a.grad_weight = a.grad_bias = None
     a.grad_input = 2 << 20
     assert back(ctypes.byref(a), None) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H", [640, 2048, 3000, 3001, 7168, 16384])
+def test_constant_rows_of_large_values_are_the_bias(H, dtype):
+    """Values whose square passes fp32's range, in rows of a warp and of a block. With eight significant bits and
+    16384 columns at most every sum is exact, so all deviations are zero."""
+    x = torch.tensor([2.0 ** 66, 1e20, -1e20, 3e33, -2.0 ** 64], device="cuda").to(torch.bfloat16)
+    x = x.to(dtype)[:, None].expand(-1, H).contiguous()
+    bias = torch.randn(H, generator=torch.Generator(device="cuda").manual_seed(H), device="cuda").to(dtype)
+    h, y = fb.layer_norm(None, x, bias=bias)
+    assert h is x and torch.equal(y, bias.expand_as(y))
