@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, ln_blocks(G, U * V))
   extern __shared__ float4 ln_smem[];
   float* sw = reinterpret_cast<float*>(ln_smem);
   float* sb = sw + (ODD ? odd_floats(a.H, V) : a.H);
-  __shared__ float2 part[2][32];
+  __shared__ float4 part[2][32];  // a warp's sum, squared deviations and what its mean's rounding left
   __shared__ float2 count[32];
   pdl_begin_in_order();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -338,8 +338,9 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, ln_blocks(G, U * V))
     }
     // the warp's own mean and squared deviations first, then all warps' joined: one barrier a row
     const float sum = warp_sum_f32(total(two));
-    // the mean is divided, not multiplied with a rounded 1 / H: equal values whose sum is exact are their mean
-    float mean = WARP ? __fdiv_rn(sum, own) : sum * own_inv;
+    // the mean is divided, not multiplied with a rounded 1 / H: equal values whose sum is exact are their mean. A
+    // warp's own is rounded before it is used, here and below: `left` is what that rounding left.
+    float mean = WARP ? __fdiv_rn(sum, own) : __fmul_rn(sum, own_inv);
     two = all<P>(0.0f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -353,16 +354,47 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, ln_blocks(G, U * V))
       }
     }
     float dev = warp_sum_f32(total(two));
+    // A mean beyond 2^12 deviations: the rounding of its sum is no longer small beside them (rows of 3000 fp32
+    // values around 10^5 deviations: normed off by 0.015; now by 0.004, half a step of the mean). What is left of
+    // it is the mean of the deviations from it, whose square is taken off theirs. A row of equal values has that value
+    // as its mean.
+    const auto far = [](float m, float var) { return var < m * m * 0x1p-24f; };
+    float left = 0.0f;
+    if (far(mean, dev * own_inv)) {
+      P rest = all<P>(0.0f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u * G + g < n) {
+          Un d;
+#pragma unroll
+          for (int j = 0; j < Un::N; ++j) d.p[j] = add(v[u].p[j], all<P>(-mean));
+          if (ODD && !whole<V>((u * G + g) * V - off, a.H)) keep(d, (u * G + g) * V - off, a.H);
+#pragma unroll
+          for (int j = 0; j < Un::N; ++j) rest = add(rest, d.p[j]);
+        }
+      }
+      const float all_rest = warp_sum_f32(total(rest));
+      left = all_rest * own_inv;
+      dev = fmaxf(dev - all_rest * left, 0.0f);
+      if (WARP) mean += left;
+    }
     if constexpr (!WARP) {
-      if (lane == 0) part[flip][warp] = make_float2(sum, dev);
+      if (lane == 0) part[flip][warp] = make_float4(sum, dev, left, 0.0f);
       __syncthreads();
       // a lane per warp (all of them unrolled took too many registers)
-      const float2 p = lane < WARPS ? part[flip][lane] : make_float2(0.0f, 0.0f);
+      const float4 p = lane < WARPS ? part[flip][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       mean = __fdiv_rn(warp_sum_f32(p.x), cols);
       const float2 c = lane < WARPS ? count[lane] : make_float2(0.0f, 0.0f);
       // without columns there is no mean of its own: 0 * (0 - mean)^2 would be NaN where the square is infinite
-      const float d = c.x > 0.0f ? p.x * c.y - mean : 0.0f;
-      dev = warp_sum_f32(fmaf(d * d, c.x, p.y));
+      const float away = c.x > 0.0f ? __fsub_rn(__fmul_rn(p.x, c.y), mean) + p.z : 0.0f;
+      dev = warp_sum_f32(fmaf(away * away, c.x, p.y));
+      // beside the sum above: 4096 x 2047 takes 49 us, behind a branch 50, the row's correction as a whole behind
+      // one and another barrier 57 (47 without any)
+      left = warp_sum_f32(away * c.x) * inv_h;
+      if (far(mean, dev * inv_h)) {
+        dev = fmaxf(dev - left * left * cols, 0.0f);
+        mean += left;
+      }
     }
     const float r = rsqrtf(fmaf(dev, inv_h, a.eps));
     if (a.stats && g == 0) reinterpret_cast<float2*>(a.stats)[row] = make_float2(mean, r);

@@ -6,6 +6,7 @@ import torch
 
 import flashinfer_b200 as fb
 from flashinfer_b200 import _lib
+from tests import layer_refs as R
 
 
 @pytest.mark.parametrize("off", [4, 8, 12])
@@ -38,3 +39,65 @@ def test_constant_rows_of_large_values_are_the_bias(H, dtype):
     bias = torch.randn(H, generator=torch.Generator(device="cuda").manual_seed(H), device="cuda").to(dtype)
     h, y = fb.layer_norm(None, x, bias=bias)
     assert h is x and torch.equal(y, bias.expand_as(y))
+
+
+def _rows(H, seed, T=24):
+    return torch.randn(T, H, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def _place(x, off):
+    """x at `off` elements past a 16-byte boundary."""
+    buf = torch.zeros(x.numel() + off, dtype=x.dtype, device="cuda")
+    buf[off:] = x.reshape(-1)
+    return buf[off:].view(x.shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("H", [100, 640, 1021, 2048, 3000, 3001, 7168, 16384])
+def test_constant_rows_of_any_value_are_the_bias(H, off):
+    """The sum of equal values rounds, and so does its quotient: by k units of the value's last place, k at most
+    54. The deviations from it are k units exactly, their mean is within 50 * 2^-24 of k units, and added to the
+    first mean it rounds to the value."""
+    v = torch.tensor([1e20, 1234.567, 1e6 + 0.5, -0.1, 1.0 / 3, 77777.7, -1e-3, 16777215.0], device="cuda")
+    x = _place(v[:, None].expand(-1, H), off)
+    bias = _rows(H, H, 1)[0]
+    _, y = fb.layer_norm(None, x, bias=bias)
+    assert torch.equal(y, bias.expand_as(y))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mean", [5e3, -1e5, 1e6])
+@pytest.mark.parametrize("H", [100, 640, 1021, 3000, 3001, 7168, 16384])
+def test_rows_with_a_mean_far_above_their_deviations(H, mean):
+    """The first mean is off by e0 <= 54 U mean|h| (32 values in a thread, 5 + 5 levels, the quotient). The second is
+    rounded once, U |mean|, after a sum of deviations with at most 52 roundings. The squares around the first
+    mean have 56; the square of the deviations' mean is taken off them."""
+    U = 2.0 ** -24
+    x = _rows(H, H) + mean
+    leaf = x.clone().requires_grad_()
+    _, y = fb.layer_norm(None, leaf, eps=1e-5)
+    h = x.double()
+    m = h.mean(1, keepdim=True)
+    c = h - m
+    var = c.square().mean(1, keepdim=True)
+    r = 1 / torch.sqrt(var + 1e-5)
+    e0 = 54 * U * h.abs().mean(1, keepdim=True)
+    dev = c.abs().mean(1, keepdim=True) + e0
+    e_mean = U * (m.abs() + e0) + 52 * U * dev
+    e_var = 56 * U * (var + e0.square()) + 104 * U * e0 * dev + (52 * U * dev).square() + 3 * U * e0.square()
+    rel = e_var / (var + 1e-5) / 2
+    rel = rel + 2 * rel.square() + 5 * U
+    n = c * r
+    en = r * (e_mean + U * (c.abs() + e_mean)) * (1 + rel) + n.abs() * (rel + U)
+    R.check(y.detach(), n, en, "normed")
+    # the backward pass goes from the same mean and 1 / sqrt(var + eps)
+    dy = _rows(H, H + 1)
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    u = dy.double()
+    s1, s2 = u.mean(1, keepdim=True), (u * n).mean(1, keepdim=True)
+    e1 = 61 * U * u.abs().mean(1, keepdim=True)
+    e2 = 62 * U * (u * n).abs().mean(1, keepdim=True) + (u.abs() * en).mean(1, keepdim=True)
+    mag = r * (u.abs() + s1.abs() + (n * s2).abs())
+    ex = r * (e1 + n.abs() * e2 + en * (s2.abs() + e2)) + mag * (rel + 8 * U)
+    R.check(dx, r * (u - s1 - n * s2), ex, "gradient")
