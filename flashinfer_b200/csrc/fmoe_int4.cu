@@ -308,6 +308,9 @@ template <typename T>
 __device__ __forceinline__ float group_scale(const GroupRange& r, bool symmetric) {
   const float amax = __uint_as_float(r.amax);
   float step = symmetric ? __fdiv_rn(amax, 7.0f) : __fdiv_rn(__fsub_rn(r.high, r.low), 15.0f);
+  // finite values further apart than fp32 reaches: from their halves
+  if (!std::is_same<T, __half>::value && step == INFINITY)
+    step = __fdiv_rn(__fsub_rn(0.5f * r.high, 0.5f * r.low), 7.5f);
   const float least = std::is_same<T, __half>::value ? 0x1p-24f : 0x1p-100f;
   step = fmaxf(step, least);
   if (r.amax >= 0x7f800000u) step = __fadd_rn(amax, amax);  // infinite or NaN
