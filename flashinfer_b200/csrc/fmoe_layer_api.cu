@@ -675,7 +675,9 @@ int fmoe_layer_norm(const FmoeLayerNormArgs* a, void* stream) {
       if (!at(q, 16)) return FMOE_ERR_ALIGN;
   }
   const uint64_t n = static_cast<uint64_t>(p.T) * p.H, row = n * e;
-  // hidden may be the residual itself: every element is read by the thread that writes it
+  // hidden may be the residual itself: an element is used by the thread alone that writes it, after it was read.
+  // (Rows off the 16-byte boundaries share 16 bytes with their neighbours: a thread may read a neighbour's elements
+  // while that row's block rewrites them, and puts zeros in their place before their first use.)
   const Span residual{a->hidden == a->residual ? nullptr : a->residual, row};
   if (overlap({{a->hidden, row}, {a->normed, row}, {a->normed_q, n}, {a->normed_scale, n / kBlock * 4},
                {a->stats, static_cast<uint64_t>(p.T) * 8}},

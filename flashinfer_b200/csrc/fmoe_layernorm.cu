@@ -111,8 +111,9 @@ __device__ __forceinline__ Unit<T, V> param(const void* p, int f32, int i) {
 // Rows off the 16-byte boundaries (ODD): the units are memory's granules. A row's first column is element `off`
 // of its first unit, the same in every tensor, and in every row of a block: their distance is a multiple of
 // 16 bytes, so that a thread's columns and the block's parameters in shared memory stay what they are. Unit i has
-// columns c .. c + V - 1, c = i * V - off; those below 0 and from H on are another row's: read and not used, and
-// never written.
+// columns c .. c + V - 1, c = i * V - off; those below 0 and from H on are another row's: read, and never
+// written. With hidden in the residual's place that row's block may be writing them meanwhile, so what was read is
+// of no use: keep() puts zeros in their place before any sum over the row.
 template <int V>
 __device__ __forceinline__ bool whole(int c, int H) {
   return c >= 0 && c + V <= H;

@@ -101,3 +101,18 @@ def test_rows_with_a_mean_far_above_their_deviations(H, mean):
     mag = r * (u.abs() + s1.abs() + (n * s2).abs())
     ex = r * (e1 + n.abs() * e2 + en * (s2.abs() + e2)) + mag * (rel + 8 * U)
     R.check(dx, r * (u - s1 - n * s2), ex, "gradient")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,H", [(3000, 3001), (2999, 2050), (1500, 7001), (5000, 515)])
+def test_in_place_with_many_rows_that_share_16_bytes(T, H, dtype):
+    """hidden over the residual in rows off the 16-byte boundary, far more than there are blocks: neighbouring rows are
+    read by one block while another rewrites them. The same bits as into a new tensor, run after run."""
+    x, f = (_rows(H, s, T).to(dtype) for s in (1, 2))
+    w, b = (_rows(H, s, 1)[0].to(dtype) for s in (3, 4))
+    h_ref, y_ref = fb.layer_norm(f, x, weight=w, bias=b)
+    for _ in range(5):
+        mine = x.clone()
+        h, y = fb.layer_norm(f, mine, weight=w, bias=b, output=mine)
+        assert h is mine and torch.equal(h, h_ref) and torch.equal(y, y_ref)
