@@ -12,8 +12,9 @@
 // by at most half a step of that type, as each output is. (A sum per group, scaled in fp32 as the kernel for
 // few tokens does it, would have to take the accumulator out of tensor memory once per group.) For fp16 the
 // scales of a row are moved by a power of two, such that the largest is in [2^9, 2^10), and the output back:
-// small scales then lose nothing to fp16's range, and a weight cannot overflow. An fp32 scale enters as the
-// sum of two 16-bit values.
+// a row of small scales then loses nothing to fp16's range, and a weight cannot overflow. What is left of the
+// range is 2^-24, fp16's last step: a scale and a product that end in it are off by 2^-25, a weight by 16 or 17 of
+// those, 2^-29 of the row's largest scale. An fp32 scale enters as the sum of two 16-bit values.
 #include <cuda.h>
 
 #include <atomic>

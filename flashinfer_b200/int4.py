@@ -130,6 +130,10 @@ def int4_matmul(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
     fp32) and zero uint8 [N, groups] or None, as ``quantize_int4`` returns them for this ``group``; bias
     fp32 [N]. Sums in fp32. The result is [M, N] of x's type, or is written to ``output``. x and weight
     start on 16-byte boundaries.
+
+    Up to 16 rows multiply the exact 4-bit values and scale each group's sum in fp32. More rows go over the tensor
+    cores, where each ``w`` is rounded to x's type first: off by half a step of that type, or in fp16 by 2^-29 of
+    the largest scale of its row where that is more (scales of one row that are 2^18 and more apart).
     """
     index = first(x, "x", _HALVES, 2)
     need(weight, "weight", index, None, _U8)
@@ -151,7 +155,9 @@ def int4_expert_matmul(rows: torch.Tensor, weights: torch.Tensor, scale: torch.T
     [E, N, groups] (the rows' type or fp32) and zero uint8 [E, N, groups] or None, expert_base int32 [E+1]
     (``ExpertOrder.expert_base``), read on the device: a base smaller than an earlier one counts as that
     one, so a row has one expert at most. Returns [R, N] of the rows' type; rows before ``expert_base[0]``
-    and from ``expert_base[E]`` on are zero in a new tensor and left as they were in a given ``output``.
+    and from ``expert_base[E]`` on are zero in a new tensor and left as they were in a given ``output``. Weights
+    are exact where R is up to 8 E, however many of the rows each expert has, and rounded as in ``int4_matmul``
+    from there on.
     """
     index = first(rows, "rows", _HALVES, 2)
     need(weights, "weights", index, None, _U8)

@@ -458,6 +458,9 @@ FMOE_API int fmoe_dequantize_int4(const void* packed, const void* scale, int32_t
  * expert_base[e] .. expert_base[e + 1] of x times expert e's; bases as in fmoe_int8_expert_matmul, rows of
  * no expert zeroed if zero_tail is set and left as they were otherwise. expert_base NULL: one matrix
  * (num_experts 1). x and weight start on 16-byte boundaries. K up to 131072, num_experts 1..256.
+ * Up to 16 rows (with expert_base: 8 * num_experts) multiply the exact 4-bit values and scale each group's sum
+ * in fp32; with more rows each weight is rounded to `dtype` first: off by half a step of it, or in fp16 by 2^-29
+ * of the largest scale of its row where that is more.
  * workspace of fmoe_int4_workspace_size bytes (may be 0). */
 typedef struct FmoeInt4Args {
   int64_t num_rows;
