@@ -289,8 +289,10 @@ def layer_norm(branch: Optional[torch.Tensor], residual: torch.Tensor, *,
     normed is the pair ``(e4m3 [T, H], fp32 scales [H/128, T])`` that ``run`` takes as
     ``hidden_states`` and ``hidden_states_scale``; that form has no gradient. ``output`` receives
     hidden and may be ``residual`` itself (no gradient either). Otherwise differentiable in every
-    tensor; weight and bias gradients are summed over tokens in a fixed order. Squares are fp32: with
-    eps 0, rows whose deviations are all below 2^-63 are divided by too little.
+    tensor; weight and bias gradients are summed over tokens in a fixed order. A row of equal values has no
+    deviations. Sums and squares are fp32: with eps 0, rows whose deviations are all below 2^-63 are divided
+    by too little, a row with deviations from 2^64 on comes out as the bias, and one whose sum passes fp32's
+    range as NaN.
     """
     index = first(residual, "residual", FLOATS, 2)
     T, H = shape = residual.shape

@@ -554,7 +554,8 @@ FMOE_API int fmoe_block_norm_backward(const FmoeBlockNormArgs* args, void* cuda_
 /* The layer norm of the residual stream in front of a block. Per token:
  *   hidden = residual + branch (branch NULL: the residual)
  *   normed = (hidden - mean) / sqrt(var + eps) * weight + bias
- * with mean and variance (of all hidden_size columns, not corrected) in fp32; weight and bias, each of
+ * with mean and variance (of all hidden_size columns, not corrected) in fp32 (a row with deviations from
+ * 2^64 on is the bias, one whose sum passes fp32's range NaN); weight and bias, each of
  * `dtype` or fp32 and tagged, may be NULL (one, zero). hidden is kept in fp32 up to the norm and rounded
  * once for output. normed leaves as `dtype`, or with normed_q set as e4m3 [T, H] with fp32 scales
  * [H/128, T] (fmoe_block_norm's layout and scale); H is then a multiple of 128 and every pointer 16-byte

@@ -116,3 +116,19 @@ def test_in_place_with_many_rows_that_share_16_bytes(T, H, dtype):
         mine = x.clone()
         h, y = fb.layer_norm(f, mine, weight=w, bias=b, output=mine)
         assert h is mine and torch.equal(h, h_ref) and torch.equal(y, y_ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [128, 640, 3000, 3001, 7168])
+def test_rows_beyond_fp32(H):
+    """Deviations whose square is infinite, a sum that is, and an ordinary row between them."""
+    x = _rows(H, H, 5)
+    x[0] = 2.0 ** 64
+    x[0, ::2] = -2.0 ** 64
+    x[2, 3] = 2.0 ** 65
+    x[4] = torch.finfo(torch.float32).max
+    bias = _rows(H, H + 1, 1)[0]
+    _, y = fb.layer_norm(None, x, bias=bias)
+    assert torch.equal(y[[0, 2]], bias.expand(2, H)) and bool(torch.isnan(y[4]).all())
+    _, alone = fb.layer_norm(None, x[[1, 3]], bias=bias)
+    R.check(y[[1, 3]], alone.double(), 100 * R.U * (alone.double().abs() + 1), "ordinary rows")
